@@ -16,7 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libembla_cuda_attn.so")
 
 BF16, F16 = 0, 1
-KV_INT8, KV_16BIT = 0, 1
+KV_INT8, KV_16BIT, KV_INT4 = 0, 1, 2
 SCALE_F32, SCALE_F16 = 0, 1
 HEAD_DIM, BLOCK, TOPK, RECENT = 128, 128, 1024, 128
 OK, BAD_ARG, OOM, CUDA_ERR, NCCL_ERR, TIMEOUT, UNSUPPORTED = range(7)
@@ -117,15 +117,17 @@ class KVPool:
             pass
 
     def raw(self):
-        """The pool as a uint8 tensor [num_blocks, n_layers, n_kv_heads, page_bytes] aliasing device memory."""
+        """The pool as a uint8 tensor [num_blocks, n_layers, n_kv_heads, page_bytes] aliasing device memory. The tensor (and
+        its views) keep the pool alive; close() frees the memory regardless."""
         base = lib().embla_kv_pool_base(self.handle)
         shape = (self.num_blocks, self.n_layers, self.n_kv_heads, self.page_bytes)
 
         class _Dev:
             __cuda_array_interface__ = {"shape": shape, "typestr": "|u1", "data": (base, False), "version": 3}
 
-        self._keep = _Dev()
-        return torch.as_tensor(self._keep, device="cuda")
+        dev = _Dev()
+        dev.pool = self
+        return torch.as_tensor(dev, device="cuda")
 
     def export_block(self, block, dst):
         _check(lib().embla_kv_block_export(self.handle, block, _ptr(dst), _stream()))
@@ -227,6 +229,23 @@ class Attention:
         _check(lib().embla_kv_append(self.handle, pool.handle, C.byref(view), _ptr(pos0), k.shape[1], _ptr(k), _ptr(v),
                                      C.c_int64(k.stride(1)), C.c_int64(k.stride(0)), int(norm_k), _stream()))
 
+    def kv_read(self, pool, block_table, layer, pos0, k, v):
+        """The inverse of kv_append: k, v [batch, n_tokens, n_kv_heads * 128 (or wider rows)] <- the cached rows of positions
+        pos0[b] + t, dequantised and rounded to the activation dtype. Pools of every type."""
+        if k.dtype != self.torch_dtype or v.dtype != self.torch_dtype or k.shape != v.shape or k.stride() != v.stride() or k.stride(2) != 1:
+            raise ValueError(f"k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} must be alike, rows contiguous, in {self.torch_dtype}")
+        view = self.view(block_table, None, layer)
+        _check(lib().embla_kv_read(self.handle, pool.handle, C.byref(view), _ptr(pos0), k.shape[1], _ptr(k), _ptr(v),
+                                   C.c_int64(k.stride(1)), C.c_int64(k.stride(0)), _stream()))
+
+    def copy_blocks(self, pool, src, dst, rows=None):
+        """Copies block src[i] of the pool to block dst[i] (int32 device tensors), all layers and kv heads, in one launch: the
+        first rows[i] positions of it, or all 128. With a block table edit this forks a sequence or moves its blocks."""
+        for t in (src, dst, rows):
+            if t is not None and (t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous() or t.numel() != src.numel()):
+                raise ValueError("src, dst and rows are contiguous int32 tensors on the device, one entry a copy")
+        _check(lib().embla_kv_copy_blocks(self.handle, pool.handle, _ptr(src), _ptr(dst), _ptr(rows), src.numel(), _stream()))
+
     def full_decode(self, pool, block_table, seq_lens, layer, q, o, gains=None, scores=None, max_seq_len=0):
         view = self.view(block_table, seq_lens, layer, max_seq_len)
         qd = self.query(q, gains)
@@ -260,10 +279,13 @@ class Attention:
                                        scores.shape[0], max_seq_len, _ptr(idx), _stream()))
 
     def sparse_decode(self, pool, block_table, seq_lens, layer, q, o, idx=None, gains=None, max_seq_len=0):
+        """Softmax attention over every key of a sequence of at most 1152, else over its selected rows idx[b][kv head]; over a
+        16-bit pool, or the int8 or 4-bit cache of a full layer."""
         view = self.view(block_table, seq_lens, layer, max_seq_len)
         qd = self.query(q, gains)
-        _check(lib().embla_attn_sparse_decode(self.handle, pool.handle, C.byref(view), C.byref(qd), _ptr(idx), _ptr(o),
-                                              C.c_int64(o.stride(0)), _stream()))
+        fn = {KV_INT8: lib().embla_attn_sparse_decode_int8, KV_INT4: lib().embla_attn_sparse_decode_int4}.get(
+            pool.kv_dtype, lib().embla_attn_sparse_decode)
+        _check(fn(self.handle, pool.handle, C.byref(view), C.byref(qd), _ptr(idx), _ptr(o), C.c_int64(o.stride(0)), _stream()))
 
     def sliding_write(self, ring, pos0, k, v, kgain=None):
         """k, v [batch, n_tokens, n_kv_heads * 128 (or wider rows)] into the rings at positions pos0[b] + t."""

@@ -174,6 +174,7 @@ EmblaStatus embla_attn_check(EmblaAttn* ctx, void* stream) {
     if (err != 0) {
         EMBLA_CUDA_TRY(cudaMemsetAsync(ctx->err_dev, 0, sizeof(int), s));
         EMBLA_CUDA_TRY(cudaStreamSynchronize(s));
+        if (err == ERR_BAD_BLOCK) EMBLA_FAIL(EMBLA_BAD_ARG, "a kernel met a block id or a position outside the pool or the block table");
         EMBLA_FAIL(EMBLA_TIMEOUT, "a kernel gave up a bounded wait (code %d)", err);
     }
     return EMBLA_OK;
@@ -186,10 +187,12 @@ EmblaStatus embla_kv_pool_create(int32_t n_layers, int32_t n_kv_heads, int32_t k
     if (n_layers <= 0 || n_kv_heads <= 0 || num_blocks <= 0)
         EMBLA_FAIL(EMBLA_BAD_ARG, "embla_kv_pool_create: n_layers %d, n_kv_heads %d, num_blocks %d", n_layers, n_kv_heads,
                    num_blocks);
-    if (kv_dtype != EMBLA_KV_INT8 && kv_dtype != EMBLA_KV_16BIT)
+    if (kv_dtype != EMBLA_KV_INT8 && kv_dtype != EMBLA_KV_16BIT && kv_dtype != EMBLA_KV_INT4)
         EMBLA_FAIL(EMBLA_BAD_ARG, "embla_kv_pool_create: kv_dtype %d", kv_dtype);
     if (scale_dtype != EMBLA_SCALE_F32 && scale_dtype != EMBLA_SCALE_F16)
         EMBLA_FAIL(EMBLA_BAD_ARG, "embla_kv_pool_create: scale_dtype %d", scale_dtype);
+    if (kv_dtype == EMBLA_KV_INT4 && scale_dtype != EMBLA_SCALE_F16)
+        EMBLA_FAIL(EMBLA_UNSUPPORTED, "embla_kv_pool_create: a 4-bit pool keeps its scales in fp16 (EMBLA_SCALE_F16)");
     EmblaKVPool* p = new (std::nothrow) EmblaKVPool();
     if (!p) EMBLA_FAIL(EMBLA_OOM, "embla_kv_pool_create: host allocation failed");
     p->n_layers = n_layers;
@@ -198,9 +201,10 @@ EmblaStatus embla_kv_pool_create(int32_t n_layers, int32_t n_kv_heads, int32_t k
     p->scale_dtype = scale_dtype;
     p->num_blocks = num_blocks;
     p->scale_bytes = scale_dtype == EMBLA_SCALE_F32 ? 4 : 2;
-    p->page_bytes = kv_dtype == EMBLA_KV_INT8 ? size_t(2 * CODE_BYTES + 2 * BLK * p->scale_bytes) : size_t(2 * BLK * HD * 2);
-    // tensor-map rows: 128 bytes for int8 pages, 256 bytes (one key) for 16-bit pages
-    const int row_bytes = kv_dtype == EMBLA_KV_INT8 ? 128 : 256;
+    p->page_bytes = kv_dtype == EMBLA_KV_INT8 ? size_t(2 * CODE_BYTES + 2 * BLK * p->scale_bytes)
+                    : kv_dtype == EMBLA_KV_INT4 ? size_t(KV4_PAGE) : size_t(2 * BLK * HD * 2);
+    // tensor-map rows: 128 bytes for int8 pages (one key) and 4-bit pages (two keys), 256 bytes (one key) for 16-bit pages
+    const int row_bytes = kv_dtype == EMBLA_KV_16BIT ? 256 : 128;
     p->rows_per_page = int(p->page_bytes / row_bytes);
     p->block_bytes = p->page_bytes * n_layers * n_kv_heads;
     p->total_bytes = p->block_bytes * num_blocks;
@@ -227,13 +231,14 @@ EmblaStatus embla_kv_pool_create(int32_t n_layers, int32_t n_kv_heads, int32_t k
     // dims 0-63 and 64-127 land in two tiles, each [128 keys][128 B] under the same swizzle.)
     const cuuint64_t dims[2] = {cuuint64_t(row_bytes), cuuint64_t(p->total_bytes / row_bytes)};
     const cuuint64_t strides[1] = {cuuint64_t(row_bytes)};
+    // (4-bit pages: rows of two keys; one box = the 128 code rows, K then V.)
     const cuuint32_t box[2] = {128, kv_dtype == EMBLA_KV_INT8 ? 256u : 128u};
     const cuuint32_t estr[2] = {1, 1};
     CUresult r = enc(&p->tmap_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, p->base, dims, strides, box, estr,
                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r == CUDA_SUCCESS) {
-        const cuuint32_t box_half[2] = {128, 128};
+        const cuuint32_t box_half[2] = {128, kv_dtype == EMBLA_KV_INT4 ? 64u : 128u};
         r = enc(&p->tmap_half, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, p->base, dims, strides, box_half, estr,
                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);

@@ -17,11 +17,18 @@ namespace embla {
 constexpr int HD = EMBLA_HEAD_DIM;       // head dim
 constexpr int BLK = EMBLA_BLOCK;         // positions per KV block
 constexpr int CODE_BYTES = BLK * HD;     // int8 codes of one page side (K or V): 16 KiB
+// 4-bit pages (EMBLA_KV_INT4): K codes [128][64 B] | V codes [128][64 B] | scales fp16 [128][8] (K groups 0-3, V groups 0-3)
+constexpr int KV4_GROUPS = HD / EMBLA_KV4_GROUP;   // scale groups of a row
+constexpr int KV4_ROW = HD / 2;                    // code bytes of a row
+constexpr int KV4_SIDE = BLK * KV4_ROW;            // code bytes of one page side: 8 KiB
+constexpr int KV4_SCALES = BLK * 2 * KV4_GROUPS * 2;   // bytes of a page's scales: 2 KiB
+constexpr int KV4_PAGE = 2 * KV4_SIDE + KV4_SCALES;    // 18,432 bytes
 constexpr float EPS32 = 1.1920929e-07f;  // head-norm epsilon (common.metal:9)
 constexpr float NEG_BIG = -1e30f;        // "-inf" of the running maxima (common.metal:10)
 
 // Device-side error word values (EmblaAttn::err_dev).
 constexpr int ERR_WAIT_FULL = 1, ERR_WAIT_EMPTY = 2, ERR_WAIT_DRAIN = 3;
+constexpr int ERR_BAD_BLOCK = 4;   // a block id or position outside the pool or the block table (4-bit pools, reads, copies)
 // Bounded waits: tries before a kernel gives up, records an error and leaves; and the default bound in SM clocks
 // (about half a second: one try may itself suspend the thread for a while). The clock bound is a launch
 // parameter (KernelCtl::wait_cycles, embla_attn_set_wait_limit).
@@ -85,7 +92,7 @@ struct EmblaKVPool {
     size_t page_bytes, block_bytes, total_bytes;
     uint8_t* base;          // device
     CUtensorMap tmap_codes; // [total rows][128 B] uint8, box 256 rows, 128-byte swizzle
-    CUtensorMap tmap_half;  // the same rows through a 128-row box (one side, K or V, of an int8 page)
+    CUtensorMap tmap_half;  // the same rows through a box of half the height (one side, K or V, of an int8 or 4-bit page)
     int device;
 };
 
@@ -362,5 +369,12 @@ TensorMapEncodeTiledFn tensor_map_encoder();
 // full-layer (ReLU²) decode over a 16-bit pool (attn16_decode.cu), reached from embla_attn_full_decode
 EmblaStatus attn16_full_decode(EmblaAttn* ctx, const EmblaKVPool* pool, const EmblaKVView* view, const EmblaQuery* q, void* o_dev,
                                int64_t o_stride, int max_len, cudaStream_t stream);
+
+// full-layer (ReLU²) decode over a 4-bit pool (kv4_decode.cu), reached from embla_attn_full_decode
+EmblaStatus kv4_full_decode(EmblaAttn* ctx, const EmblaKVPool* pool, const EmblaKVView* view, const EmblaQuery* q, void* o_dev,
+                            int64_t o_stride, float* scores_dev, int64_t scores_stride, int max_len, cudaStream_t stream);
+// the current token's rows (position seq_lens - 1) into a 4-bit pool (kv_append.cu), for embla_attn_full_step
+EmblaStatus kv4_append_token(EmblaAttn* ctx, EmblaKVPool* pool, const EmblaKVView* view, const void* k_dev, const void* v_dev,
+                             int64_t kv_stride, int norm_k, cudaStream_t stream);
 
 }  // namespace embla

@@ -1,0 +1,68 @@
+// Rows of the 4-bit cache (EMBLA_KV_INT4): 128 dims in four groups of 32, a fp16 scale each, codes -7 .. 7 as two's
+// complement nibbles. A 32-bit word holds 8 consecutive dims, nibble n being dim (0, 2, 4, 6, 1, 3, 5, 7)[n]: the nibbles n and
+// n + 4, which one mask takes out of the two halves of the word together, are then the neighbouring dims 2n and 2n + 1, so that
+// widening a word gives fp16 pairs in dim order with no permutation.
+#pragma once
+
+#include "kv_row.cuh"
+
+namespace embla {
+
+__host__ __device__ constexpr int kv4_nibble_of(int d) { return (d >> 1) + 4 * (d & 1); }   // place of dim d (of 8) in its word
+
+// The scale of a group whose largest magnitude is `top` (NaN or infinity: a NaN scale, so that what was not a number does not
+// come back as one), and the code of x under it. x and s have at most 11 significant bits, so x / s never lies within a fp32
+// rounding of a half without being one: the fp32 division gives the code that exact arithmetic gives.
+__device__ __forceinline__ __half kv4_scale(float top) {
+    return top <= 3.4028234e38f ? __float2half_rn(fminf(__fdiv_rn(top, 7.0f), 65504.0f)) : __ushort_as_half(0x7fff);
+}
+__device__ __forceinline__ int kv4_code(float x, float s) {
+    return s > 0.0f ? int(fminf(fmaxf(rintf(__fdiv_rn(x, s)), -7.0f), 7.0f)) : 0;
+}
+// max |x| over the warp that keeps a NaN
+__device__ __forceinline__ float warp_max_abs_nan(float x) {
+    uint32_t m = __float_as_uint(x) & 0x7fffffffu;   // (ordered as the magnitudes are, infinity and NaN on top)
+    return __uint_as_float(__reduce_max_sync(0xffffffffu, m));
+}
+
+// The query row of a head that comes raw: RMS norm over the head with `ng` gains, in the order of the other decode kernels
+// (common.metal:30-41), rounded to the activation dtype. A lane holds dims lane + 32 i.
+template <int DT>
+__device__ __forceinline__ void kv4_query_norm(float (&x)[4], const void* g1, const void* g2, int ng, int lane) {
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) ss = __fadd_rn(ss, __fmul_rn(x[i], x[i]));
+    float tot = 0.0f;
+    for (int l = 0; l < 32; l++) tot = __fadd_rn(tot, __shfl_sync(0xffffffffu, ss, l));
+    const float r = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(tot, float(HD)), EPS32)));
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        float gn = r;
+        if (ng >= 1) gn = __fmul_rn(gn, __fadd_rn(1.0f, Act<DT>::load(g1, lane + 32 * i)));
+        if (ng >= 2) gn = __fmul_rn(gn, __fadd_rn(1.0f, Act<DT>::load(g2, lane + 32 * i)));
+        x[i] = Act<DT>::round(__fmul_rn(x[i], gn));
+    }
+}
+
+// Eight codes of a word -> four half2 (dims 0-1, 2-3, 4-5, 6-7), exactly: a nibble under the exponent of 1024 (low nibble of a
+// byte, 1024 + code + 8 after the sign bit is flipped) or of 64 (high nibble: 64 + code + 8), minus that offset.
+__device__ __forceinline__ uint32_t kv4_lop(uint32_t w, uint32_t mask, uint32_t flip) { return (w & mask) ^ flip; }
+__device__ __forceinline__ uint32_t h2_sub(uint32_t a, uint32_t b) {
+    __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
+    __half2 r = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<uint32_t*>(&r);
+}
+constexpr uint32_t KV4_LO_MASK = 0x000F000Fu, KV4_LO_FLIP = 0x64086408u, KV4_LO_OFF = 0x64086408u;   // half2(1032, 1032)
+constexpr uint32_t KV4_HI_MASK = 0x00F000F0u, KV4_HI_FLIP = 0x54805480u, KV4_HI_OFF = 0x54805480u;   // half2(72, 72)
+__device__ __forceinline__ void kv4_widen(uint32_t w, uint32_t (&h)[4]) {
+    const uint32_t v = w >> 8;
+    h[0] = h2_sub(kv4_lop(w, KV4_LO_MASK, KV4_LO_FLIP), KV4_LO_OFF);
+    h[1] = h2_sub(kv4_lop(w, KV4_HI_MASK, KV4_HI_FLIP), KV4_HI_OFF);
+    h[2] = h2_sub(kv4_lop(v, KV4_LO_MASK, KV4_LO_FLIP), KV4_LO_OFF);
+    h[3] = h2_sub(kv4_lop(v, KV4_HI_MASK, KV4_HI_FLIP), KV4_HI_OFF);
+}
+
+}  // namespace embla

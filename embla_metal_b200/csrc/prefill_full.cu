@@ -961,6 +961,10 @@ __global__ void __launch_bounds__(PF_THREADS, 1) full_prefill_kernel(const __gri
     full_prefill_segment<DT, SB, QK8>(tmap, p, sg);
 }
 
+EmblaStatus kv4_full_prefill(EmblaAttn* ctx, const EmblaKVPool* pool, const EmblaKVView* view, const int32_t* pos0, int n_tokens,
+                             const EmblaQuery* q, int64_t q_token_stride, void* o_dev, int64_t o_token_stride, int64_t o_seq_stride,
+                             cudaStream_t stream);   // kv4_decode.cu
+
 }  // namespace embla
 
 using namespace embla;
@@ -1137,7 +1141,9 @@ static EmblaStatus full_prefill_impl(EmblaAttn* ctx, const EmblaKVPool* pool, co
     if (!ctx || !pool || !view || !pos0_dev || !q || !q->q_dev || !o_dev)
         EMBLA_FAIL(EMBLA_BAD_ARG, "embla_attn_full_prefill: null argument");
     EMBLA_CHECK_DEVICE("embla_attn_full_prefill", ctx, pool);
-    if (pool->kv_dtype != EMBLA_KV_INT8) EMBLA_FAIL(EMBLA_UNSUPPORTED, "embla_attn_full_prefill: the pool is not int8");
+    const bool kv4 = pool->kv_dtype == EMBLA_KV_INT4;
+    if (pool->kv_dtype != EMBLA_KV_INT8 && !kv4) EMBLA_FAIL(EMBLA_UNSUPPORTED, "embla_attn_full_prefill: the pool is neither int8 nor 4-bit");
+    if (kv4 && qk8) EMBLA_FAIL(EMBLA_UNSUPPORTED, "embla_attn_full_prefill_qk8: the pool is not int8");
     if (pool->n_kv_heads != ctx->cfg.n_kv_heads || view->layer < 0 || view->layer >= pool->n_layers)
         EMBLA_FAIL(EMBLA_BAD_ARG, "embla_attn_full_prefill: pool/layer mismatch");
     if (view->batch <= 0 || !view->block_table_dev || n_tokens <= 0)
@@ -1146,6 +1152,7 @@ static EmblaStatus full_prefill_impl(EmblaAttn* ctx, const EmblaKVPool* pool, co
         EMBLA_FAIL(EMBLA_BAD_ARG, "embla_attn_full_prefill: the fused head norm takes both gain vectors (ng = 2)");
     if ((q_token_stride % 8) || (q->q_stride % 8) || (o_token_stride % 8) || (o_seq_stride % 8))
         EMBLA_FAIL(EMBLA_BAD_ARG, "embla_attn_full_prefill: strides must be multiples of 8 elements (16-byte rows)");
+    if (kv4) return kv4_full_prefill(ctx, pool, view, pos0_dev, n_tokens, q, q_token_stride, o_dev, o_token_stride, o_seq_stride, static_cast<cudaStream_t>(stream));
     PrefillParams p;
     p.pool = pool->base;
     p.block_table = view->block_table_dev;

@@ -45,8 +45,8 @@ EmblaStatus embla_stack_create(EmblaAttn* ctx, const EmblaLayerDesc* layers, int
     for (int i = 0; i < n_layers; i++) {
         const EmblaLayerDesc& L = layers[i];
         if (L.kind == EMBLA_LAYER_FULL) {
-            if (!full_pool || full_pool->kv_dtype != EMBLA_KV_INT8 || L.slot < 0 || L.slot >= full_pool->n_layers)
-                EMBLA_FAIL(EMBLA_BAD_ARG, "embla_stack_create: layer %d (full) needs slot %d of an int8 pool", i, L.slot);
+            if (!full_pool || full_pool->kv_dtype == EMBLA_KV_16BIT || L.slot < 0 || L.slot >= full_pool->n_layers)
+                EMBLA_FAIL(EMBLA_BAD_ARG, "embla_stack_create: layer %d (full) needs slot %d of an int8 or 4-bit pool", i, L.slot);
         } else if (L.kind == EMBLA_LAYER_SPARSE) {
             if (!sparse_pool || sparse_pool->kv_dtype != EMBLA_KV_16BIT || L.slot < 0 || L.slot >= sparse_pool->n_layers)
                 EMBLA_FAIL(EMBLA_BAD_ARG, "embla_stack_create: layer %d (sparse) needs slot %d of a 16-bit pool", i, L.slot);
@@ -54,8 +54,9 @@ EmblaStatus embla_stack_create(EmblaAttn* ctx, const EmblaLayerDesc* layers, int
                 EMBLA_FAIL(EMBLA_UNSUPPORTED, "embla_stack_create: layer %d: a sparse layer that scores its own keys takes "
                                               "its queries prenormed", i);
         } else if (L.kind == EMBLA_LAYER_SPARSE_SHARED) {
-            if (!full_pool || full_pool->kv_dtype != EMBLA_KV_INT8 || L.slot < 0 || L.slot >= full_pool->n_layers)
-                EMBLA_FAIL(EMBLA_BAD_ARG, "embla_stack_create: layer %d (sparse, shared cache) needs slot %d of an int8 pool", i, L.slot);
+            if (!full_pool || full_pool->kv_dtype == EMBLA_KV_16BIT || L.slot < 0 || L.slot >= full_pool->n_layers)
+                EMBLA_FAIL(EMBLA_BAD_ARG, "embla_stack_create: layer %d (sparse, shared cache) needs slot %d of an int8 or 4-bit pool", i,
+                           L.slot);
         } else if (L.kind == EMBLA_LAYER_SLIDING) {
             if (!rings || L.slot < 0 || L.slot >= n_rings)
                 EMBLA_FAIL(EMBLA_BAD_ARG, "embla_stack_create: layer %d (sliding) needs ring %d of %d", i, L.slot, n_rings);
@@ -241,9 +242,9 @@ extern "C" EmblaStatus embla_stack_decode_layers(EmblaStack* st, const EmblaStac
             view.block_table_dev = step->full_table_dev;
             view.table_stride = step->full_table_stride;
             const bool selecting = max_len > EMBLA_TOPK + EMBLA_RECENT;
+            auto attend = st->full_pool->kv_dtype == EMBLA_KV_INT4 ? embla_attn_sparse_decode_int4 : embla_attn_sparse_decode_int8;
             EMBLA_STEP(EMBLA_ENTRY_SPARSE_DECODE, TOUCH_NONE, TOUCH_NONE,
-                       embla_attn_sparse_decode_int8(ctx, st->full_pool, &view, &q, selecting ? st->idx : nullptr, op,
-                                                     step->o_stride, stream));
+                       attend(ctx, st->full_pool, &view, &q, selecting ? st->idx : nullptr, op, step->o_stride, stream));
         } else {
             view.block_table_dev = step->sparse_table_dev;
             view.table_stride = step->sparse_table_stride;

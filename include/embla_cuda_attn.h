@@ -52,7 +52,8 @@ typedef enum {
 } EmblaStatus;
 
 enum { EMBLA_BF16 = 0, EMBLA_F16 = 1 };                       /* activation dtype */
-enum { EMBLA_KV_INT8 = 0, EMBLA_KV_16BIT = 1 };               /* cache element type (16BIT = activation dtype) */
+enum { EMBLA_KV_INT8 = 0, EMBLA_KV_16BIT = 1, EMBLA_KV_INT4 = 2 };   /* cache element type (16BIT = activation dtype) */
+enum { EMBLA_KV4_GROUP = 32 };                                /* dims that share a scale in a 4-bit row */
 enum { EMBLA_SCALE_F32 = 0, EMBLA_SCALE_F16 = 1 };            /* int8 row scale dtype */
 enum { EMBLA_HEAD_DIM = 128, EMBLA_BLOCK = 128, EMBLA_TOPK = 1024, EMBLA_RECENT = 128 };
 /* Longest sequence embla_select_keys ranks: a (sequence, kv head) pair's keys are held in the registers of a
@@ -105,7 +106,9 @@ const char* embla_last_error(void);
 EmblaStatus embla_attn_create(const EmblaAttnConfig* cfg, EmblaAttn** out);
 void        embla_attn_destroy(EmblaAttn* ctx);
 /* Reads (and clears) the device-side error word: EMBLA_TIMEOUT if a bounded wait of an earlier
- * kernel ran out. Synchronises the stream. */
+ * kernel ran out, EMBLA_BAD_ARG if a kernel of the 4-bit pool, embla_kv_read or embla_kv_copy_blocks met a block id outside the
+ * pool or a position outside the block table (such rows are neither written nor read: an attention sees zeros there).
+ * Synchronises the stream. */
 EmblaStatus embla_attn_check(EmblaAttn* ctx, void* stream);
 /* Every device-side wait of this library's kernels (on a shared-memory barrier that a TMA copy or
  * another warp completes) is bounded; a wait that runs out makes the kernel record an error code, wait
@@ -164,6 +167,23 @@ EmblaStatus embla_kv_append(EmblaAttn* ctx, EmblaKVPool* pool, const EmblaKVView
                             const void* k_dev, const void* v_dev, int64_t token_stride, int64_t seq_stride,
                             int32_t norm_k, void* stream);
 
+/* The inverse, for callers that need cached rows as activations again (handing a sequence to a pool of another type or to another
+ * engine, recomputing with them): the k and v rows of positions pos0_dev[b] + t, t < n_tokens, of every kv head, code x
+ * scale rounded to the activation dtype (a 16-bit pool: as stored), into k_dev / v_dev [batch][n_tokens][stride] with kv head
+ * h at h * 128. Pools of every type. Strides are multiples of 8 elements, k_dev and v_dev 16-byte aligned. Positions outside
+ * the block table and blocks outside the pool leave their rows of the output untouched (embla_attn_check reports them). */
+EmblaStatus embla_kv_read(EmblaAttn* ctx, const EmblaKVPool* pool, const EmblaKVView* view, const int32_t* pos0_dev,
+                          int32_t n_tokens, void* k_dev, void* v_dev, int64_t token_stride, int64_t seq_stride, void* stream);
+/* Copies blocks inside a pool, one launch for all of them: for i < n, the first rows_dev[i] positions (all 128 when rows_dev is
+ * NULL) of block src_dev[i], in every layer and kv head, to block dst_dev[i]; positions from rows_dev[i] on keep what they
+ * held. With a block table edit this forks a sequence (the full blocks shared, its own copy of the last one's rows) and
+ * moves blocks together (the counterpart of PrefixCache's blits, PrefixCache.swift:200-212, without the store). Pools of
+ * every type. A block must not be written twice or both written and read by one call (its contents are then undefined). A
+ * pair with an id outside the pool is left out (embla_attn_check reports it); rows are clamped to 0 .. 128. n = 0 is
+ * nothing to do. */
+EmblaStatus embla_kv_copy_blocks(EmblaAttn* ctx, EmblaKVPool* pool, const int32_t* src_dev, const int32_t* dst_dev,
+                                 const int32_t* rows_dev, int32_t n, void* stream);
+
 /* ---- the producer of q, k, v: 4-bit stacked GEMV ---------------------------------------------------- */
 /* One 4-bit matrix of the model as the reference stores it (GemvRows, common.metal:105-152; Seg, gemv.metal:21-27):
  * `rows` rows of d_in four-bit values in d_in / 32 words of 16 bytes (word c, 32-bit part k, nibble n: column
@@ -208,7 +228,9 @@ EmblaStatus embla_oproj(EmblaAttn* ctx, const EmblaW4Matrix* wo, int32_t d_in, c
  * rows of `scores_stride` floats, bit-exact against the oracle's summation order.
  * A 16-bit pool is served too: the reference's build without the int8 cache (EMBLA_KV8=0, Engine.swift:163: attn_full,
  * attention.metal:148-220), the rows in the activation dtype and no scales; the scores then come from a scoring pass of
- * their own ahead of the attention (queries prenormed), and embla_attn_full_step is refused (embla_kv_append first). */
+ * their own ahead of the attention (queries prenormed), and embla_attn_full_step is refused (embla_kv_append first).
+ * Over a 4-bit pool the scores come from the same tensor-core products as the attention (fp32 sums, within a few fp32
+ * roundings of exact, the same from run to run), for prenormed queries or not. A sequence of 0 keys gives zeros. */
 EmblaStatus embla_attn_full_decode(EmblaAttn* ctx, const EmblaKVPool* pool, const EmblaKVView* view,
                                    const EmblaQuery* q, void* o_dev, int64_t o_stride,
                                    float* scores_dev, int64_t scores_stride, void* stream);
@@ -216,7 +238,7 @@ EmblaStatus embla_attn_full_decode(EmblaAttn* ctx, const EmblaKVPool* pool, cons
 /* The reference's per-layer pair kv_append + attn_full8 (Engine.swift:756-762, 796-818) in one launch: the current
  * token of every sequence (position seq_lens_dev[b] - 1) is quantised from its raw k and v rows (k_dev, v_dev:
  * [batch][kv_stride] elements, kv head h at h * 128; `norm_k` as embla_kv_append) into the view's layer, and the
- * attention sees it. Same result as embla_kv_append followed by embla_attn_full_decode. */
+ * attention sees it. Same result as embla_kv_append followed by embla_attn_full_decode. (Over a 4-bit pool: two launches.) */
 EmblaStatus embla_attn_full_step(EmblaAttn* ctx, EmblaKVPool* pool, const EmblaKVView* view, const EmblaQuery* q,
                                  const void* k_dev, const void* v_dev, int64_t kv_stride, int32_t norm_k,
                                  void* o_dev, int64_t o_stride, float* scores_dev, int64_t scores_stride, void* stream);
@@ -284,6 +306,12 @@ EmblaStatus embla_attn_sparse_decode_int8(EmblaAttn* ctx, const EmblaKVPool* poo
                                           const EmblaQuery* q, const uint32_t* idx_dev, void* o_dev, int64_t o_stride,
                                           void* stream);
 
+/* The same over a 4-bit cache (EMBLA_KV_INT4; no counterpart in the reference). A sequence of 0 keys gives zeros; a
+ * selected position outside the sequence counts as not selected (embla_attn_check reports it). */
+EmblaStatus embla_attn_sparse_decode_int4(EmblaAttn* ctx, const EmblaKVPool* pool, const EmblaKVView* view,
+                                          const EmblaQuery* q, const uint32_t* idx_dev, void* o_dev, int64_t o_stride,
+                                          void* stream);
+
 /* ---- sliding layers ------------------------------------------------------------------------------------ */
 /* The sliding layers' rings (Engine.swift:269-276; RING = 4096, attention.metal:4-6): per sequence
  * [n_kv_heads][ring][128] keys and the same for values, in the activation dtype, owned by the caller. */
@@ -346,7 +374,7 @@ EmblaStatus embla_attn_sliding_prefill(EmblaAttn* ctx, const EmblaRing* ring, co
  * int8 cache, which must already hold their own keys and values (embla_kv_append first, as the reference
  * runs kv_append_b first). Token t's query head h is at q_dev[b * q->q_stride + t * q_token_stride +
  * h * 128]; out is token-major, o_dev[b * o_seq_stride + t * o_token_stride + h * 128]. Strides are in
- * elements and must be multiples of 8. Runs on tcgen05 tensor cores with fp32 accumulation in TMEM. */
+ * elements and must be multiples of 8. Runs on tcgen05 tensor cores with fp32 accumulation in TMEM. Int8 and 4-bit pools. */
 EmblaStatus embla_attn_full_prefill(EmblaAttn* ctx, const EmblaKVPool* pool, const EmblaKVView* view,
                                     const int32_t* pos0_dev, int32_t n_tokens, const EmblaQuery* q,
                                     int64_t q_token_stride, void* o_dev, int64_t o_token_stride,
