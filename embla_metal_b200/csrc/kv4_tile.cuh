@@ -1,0 +1,180 @@
+// The arithmetic of a 16-key tile of the 4-bit cache on a warp's tensor-core tiles (m16n8k16, fp16 operands, fp32 sums), for up to
+// 8 query heads of a kv head. Rows of 64 code bytes lie in shared memory as TMA puts them there: two rows a 128-byte line, 16-byte
+// chunk c of line l at c ^ (l % 8), which is conflict-free for every access below.
+//
+//   S^T = K Q^T   A = 16 keys x 16 dims. A row's chunk g is its group g: ldmatrix hands lane (r, t) the word of key r that holds
+//                 dims 8t .. 8t + 7 of the group, which widens to the A registers of two products with no permutation. The
+//                 products of a group are summed apart (fp32), times the key's scale of the group into S. The codes enter as
+//                 72 + code (one shift and one logic operation a register, no subtraction); the constant part, 72 x the sum
+//                 of the query over the group, is the accumulator's start value, negated. It costs 2 of the 24 bits.
+//   O^T = V^T P^T A = 16 dims x 16 keys. The transposing ldmatrix, on 16-bit elements of four codes, hands lane (r, t) the
+//                 element r of keys 2t and 2t + 1 side by side: widened, its nibbles are A registers (a dim, two keys). The
+//                 value's scale of the group is multiplied into P (fp16, one more rounding of 2^-11), the codes stay exact.
+#pragma once
+
+#include "kv4.cuh"
+
+namespace embla {
+
+// byte of 16-byte chunk `chunk` (group) of row `row` in a side
+__device__ __forceinline__ int kv4_at(int row, int chunk) { return (row >> 1) * 128 + (((((row & 1) << 2) | chunk) ^ ((row >> 1) & 7)) << 4); }
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t movmatrix4_trans(uint32_t x) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+// 2^(e - 127) for a biased exponent 1 .. 254
+__device__ __forceinline__ float pow2_biased(int e) { return __uint_as_float(uint32_t(e) << 23); }
+
+// The queries of a kv head in shared memory: rows scaled by a power of two that brings their largest element into [1, 2) (exact;
+// fp16 then holds bf16 queries of any size), and what goes with them.
+struct Kv4Queries {
+    __half q[8][HD];
+    float start[8][KV4_GROUPS];   // -72 x the sum of the scaled query over the group
+    int expo[8];                  // biased exponent of the power of two; 0: no such head
+};
+
+// One warp, one head: loads the row (or zeros for a head the kv head does not have), head norm if asked, scales, stores.
+template <int DT>
+__device__ __forceinline__ void kv4_stage_query(Kv4Queries& sq, int hh, bool has, const void* q, size_t off, bool prenormed, const void* g1,
+                                                const void* g2, int ng, int lane) {
+    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (has) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = Act<DT>::load(q, off + lane + 32 * i);
+        if (!prenormed) kv4_query_norm<DT>(x, g1, g2, ng, lane);
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+    top = __reduce_max_sync(0xffffffffu, top);
+    const int e = min(max(int(top >> 23), 1), 253);
+    const float down = pow2_biased(254 - e);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const __half h = __float2half_rn(x[i] * down);
+        sq.q[hh][lane + 32 * i] = h;
+        float sum = __half2float(h);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) sq.start[hh][i] = -72.0f * sum;
+    }
+    if (lane == 0) sq.expo[hh] = has ? e : 0;
+}
+
+// A lane's share of the queries: B registers of head r = lane / 4, start values of heads 2t, 2t + 1 (t = lane % 4).
+struct Kv4Frag {
+    uint32_t b[KV4_GROUPS][4];
+    float start[KV4_GROUPS][2];
+    __device__ __forceinline__ void load(const Kv4Queries& sq, int lane) {
+        const int r = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int g = 0; g < KV4_GROUPS; g++) {
+            const uint4 v = *reinterpret_cast<const uint4*>(&sq.q[r][32 * g + 8 * t]);
+            b[g][0] = v.x;
+            b[g][1] = v.y;
+            b[g][2] = v.z;
+            b[g][3] = v.w;
+            start[g][0] = sq.start[2 * t][g];
+            start[g][1] = sq.start[2 * t + 1][g];
+        }
+    }
+};
+
+// This lane's ldmatrix address in a tile whose row 0 is a multiple of 16 rows into the side: groups 0 and 1; ^ 32 for 2 and 3.
+__device__ __forceinline__ int kv4_lane_at(int lane) { return kv4_at((((lane >> 3) & 1) << 3) | (lane & 7), lane >> 4); }
+
+// S of 16 keys: s[0], s[1] key r, heads 2t, 2t + 1; s[2], s[3] key r + 8. `kaddr`: shared address of the tile's key rows plus
+// kv4_lane_at; `sc`: the tile's scale rows [16][8].
+__device__ __forceinline__ void kv4_tile_scores(uint32_t kaddr, const uint8_t* sc, int lane, const Kv4Frag& f, float (&s)[4]) {
+    const int r = lane >> 2;
+    const uint2 k0 = *reinterpret_cast<const uint2*>(sc + r * 16), k1 = *reinterpret_cast<const uint2*>(sc + (r + 8) * 16);
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        uint32_t w[4];
+        ldmatrix4(w, kaddr ^ (j * 32));
+        const float2 ks0 = __half22float2(*reinterpret_cast<const __half2*>(j ? &k0.y : &k0.x));
+        const float2 ks1 = __half22float2(*reinterpret_cast<const __half2*>(j ? &k1.y : &k1.x));
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int g = 2 * j + h;
+            const uint32_t lo = w[2 * h], hi = w[2 * h + 1];   // keys r and r + 8
+            float a[4] = {f.start[g][0], f.start[g][1], f.start[g][0], f.start[g][1]};
+            mma_16816(a, kv4_lop(lo << 4, KV4_HI_MASK, KV4_HI_FLIP), kv4_lop(hi << 4, KV4_HI_MASK, KV4_HI_FLIP),
+                      kv4_lop(lo, KV4_HI_MASK, KV4_HI_FLIP), kv4_lop(hi, KV4_HI_MASK, KV4_HI_FLIP), f.b[g][0], f.b[g][1]);
+            mma_16816(a, kv4_lop(lo >> 4, KV4_HI_MASK, KV4_HI_FLIP), kv4_lop(hi >> 4, KV4_HI_MASK, KV4_HI_FLIP),
+                      kv4_lop(lo >> 8, KV4_HI_MASK, KV4_HI_FLIP), kv4_lop(hi >> 8, KV4_HI_MASK, KV4_HI_FLIP), f.b[g][2], f.b[g][3]);
+            const float x0 = h ? ks0.y : ks0.x, x1 = h ? ks1.y : ks1.x;
+            if (g == 0) {
+                s[0] = a[0] * x0;
+                s[1] = a[1] * x0;
+                s[2] = a[2] * x1;
+                s[3] = a[3] * x1;
+            } else {
+                s[0] = fmaf(a[0], x0, s[0]);
+                s[1] = fmaf(a[1], x0, s[1]);
+                s[2] = fmaf(a[2], x1, s[2]);
+                s[3] = fmaf(a[3], x1, s[3]);
+            }
+        }
+    }
+}
+
+// The value scales of a lane's keys 2t, 2t + 1, 2t + 8, 2t + 9 as pairs by group: v[g] (keys 2t, 2t + 1), v[4 + g] (2t + 8, 2t + 9).
+__device__ __forceinline__ void kv4_value_scales(const uint8_t* sc, int lane, uint32_t (&v)[8]) {
+    const int t = lane & 3;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const uint2 a = *reinterpret_cast<const uint2*>(sc + (2 * t + 8 * h) * 16 + 8), b = *reinterpret_cast<const uint2*>(sc + (2 * t + 8 * h + 1) * 16 + 8);
+        v[4 * h + 0] = __byte_perm(a.x, b.x, 0x5410);
+        v[4 * h + 1] = __byte_perm(a.x, b.x, 0x7632);
+        v[4 * h + 2] = __byte_perm(a.y, b.y, 0x5410);
+        v[4 * h + 3] = __byte_perm(a.y, b.y, 0x7632);
+    }
+}
+// Some value scale of 2 or more among them (their product with a weight of 2^13 could leave fp16).
+__device__ __forceinline__ bool kv4_scales_large(const uint32_t (&v)[8]) {
+    return (((v[0] | v[1] | v[2]) | (v[3] | v[4] | v[5]) | (v[6] | v[7])) & 0x40004000u) != 0;
+}
+// Zeroes the scales of keys from `lim` (of the tile's 16) on: what lies there may be anything, NaN included.
+__device__ __forceinline__ void kv4_mask_value_scales(uint32_t (&v)[8], int lane, int lim) {
+    const int t = lane & 3;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const uint32_t m = (2 * t + 8 * h < lim ? 0xffffu : 0u) | (2 * t + 8 * h + 1 < lim ? 0xffff0000u : 0u);
+#pragma unroll
+        for (int g = 0; g < 4; g++) v[4 * h + g] &= m;
+    }
+}
+
+// O^T += V^T P^T for the tile: p0, p1 = the weights of head r for keys 2t, 2t + 1 and 2t + 8, 2t + 9. Accumulator tile 2g + p
+// holds, in [0], [1], dim 32 g + 8 (r / 2) + (r % 2) + 4 p of heads 2t, 2t + 1, in [2], [3] that dim + 2.
+__device__ __forceinline__ void kv4_tile_values(uint32_t vaddr, uint32_t p0, uint32_t p1, const uint32_t (&v)[8], float (&O)[8][4]) {
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        uint32_t x[4];
+        ldmatrix4_trans(x, vaddr ^ (j * 32));
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int g = 2 * j + h;
+            uint32_t lo[4], hi[4];
+            kv4_widen(x[2 * h], lo);
+            kv4_widen(x[2 * h + 1], hi);
+            const uint32_t b0 = h2_mul(p0, v[g]), b1 = h2_mul(p1, v[4 + g]);
+            mma_16816(O[2 * g], lo[0], lo[1], hi[0], hi[1], b0, b1);
+            mma_16816(O[2 * g + 1], lo[2], lo[3], hi[2], hi[3], b0, b1);
+        }
+    }
+}
+__device__ __forceinline__ int kv4_dim_of(int tile, int r) { return 32 * (tile >> 1) + 8 * (r >> 1) + (r & 1) + 4 * (tile & 1); }
+
+}  // namespace embla
