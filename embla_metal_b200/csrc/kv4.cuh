@@ -46,7 +46,11 @@ __device__ __forceinline__ void kv4_query_norm(float (&x)[4], const void* g1, co
 
 // Eight codes of a word -> four half2 (dims 0-1, 2-3, 4-5, 6-7), exactly: a nibble under the exponent of 1024 (low nibble of a
 // byte, 1024 + code + 8 after the sign bit is flipped) or of 64 (high nibble: 64 + code + 8), minus that offset.
-__device__ __forceinline__ uint32_t kv4_lop(uint32_t w, uint32_t mask, uint32_t flip) { return (w & mask) ^ flip; }
+__device__ __forceinline__ uint32_t kv4_lop(uint32_t w, uint32_t mask, uint32_t flip) {
+    uint32_t r;   // (w & mask) ^ flip, as one instruction
+    asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(w), "r"(mask), "r"(flip));
+    return r;
+}
 __device__ __forceinline__ uint32_t h2_sub(uint32_t a, uint32_t b) {
     __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
     return *reinterpret_cast<uint32_t*>(&r);

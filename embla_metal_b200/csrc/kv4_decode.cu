@@ -9,7 +9,7 @@
 // Weights. w = relu(q.k / sqrt(128))^2 has no bound, and its product with a value's scale goes through fp16. Each warp
 // therefore keeps its weights as w' = relu(S)^2 f with a power of two f per head: when a weight of a tile passes LIMIT (tested
 // with one vote a tile), f drops so that the tile's largest is TARGET or below, and the sums kept so far are scaled by the same power
-// of two, exactly. Before the first key f is 2^100, so the first tile sets it. Weights between 2^10 and 2^13 at the top of
+// of two, exactly. Before the first key f is 2^120, so the first tile sets it. Weights between 2^10 and 2^13 at the top of
 // their range leave 2^-24 / 2^10 of the largest as the smallest step; scales of 2 and more (values above 14) switch the
 // warp to LIMIT 1/2, which no scale can push out of fp16.
 #include <cstdlib>
@@ -18,10 +18,23 @@
 
 namespace embla {
 
+// The same value, computed here: what hangs on it is not worked out ahead of the loop around it and kept in registers meanwhile.
+__device__ __forceinline__ int here(int x) {
+    asm volatile("" : "+r"(x));
+    return x;
+}
+__device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+
 constexpr int KD_PART = HD + 4;                                    // floats per (range, head): 128 sums, sum of weights
 constexpr float KD_LIMIT = 8192.0f, KD_LIMIT_BIG = 0.5f;           // largest weight kept, usually and with large value scales
 constexpr int KD_TARGET = 10, KD_TARGET_BIG = -4;                  // log2 of the bound a new f puts on the tile's weights
 constexpr int KD_MAX_CLUSTER = 8;
+#ifndef KDCP
+#define KDCP 512
+#define KDMR 3
+#endif
+constexpr long KD_CLUSTER_PAGES = KDCP;   // most pages of a launch whose units are clusters
+constexpr int KD_MIN_RUN = KDMR;          // pages a run has at least
 
 struct Kv4DecodeParams {
     const uint8_t* pool;
@@ -32,25 +45,114 @@ struct Kv4DecodeParams {
     const void* g2;
     void* o;
     float* partials;
-    int* counters;
     KernelCtl ctl;
     float* scores;
     int64_t q_stride, o_stride, scores_stride;
-    int table_stride, layer, n_layers, n_kv_heads, num_blocks, G, nsplit, prenormed, ng;
+    int table_stride, layer, n_layers, n_kv_heads, num_blocks, G, batch, nsplit, n_runs, prenormed, ng;
 };
 
-// shared memory: stages, queries, barriers, then (cluster launches) the rows [sender][head] that other ranges send
+// shared memory: stages, queries, barriers, the warps' sums (cluster launches: over the stages, which are free by then), then
+// (cluster launches) the rows [sender][head] that the other ranges send
 constexpr size_t kd_queries_at(int stages) { return size_t(stages) * KV4_PAGE; }
 constexpr size_t kd_bars_at(int stages) { return kd_queries_at(stages) + sizeof(Kv4Queries); }
-constexpr size_t kd_inbox_at(int stages) { return kd_bars_at(stages) + size_t(stages) * 20 + 12; }
+constexpr size_t kd_sums_at(int stages) { return (kd_bars_at(stages) + size_t(stages) * 20 + 15) / 16 * 16; }
+constexpr size_t kd_smem(int ncons, int stages) { return 1024 + kd_sums_at(stages) + size_t(ncons) * 8 * KD_PART * 4; }
 constexpr size_t kd_inbox_rows(int ranges, int G) { return size_t(ranges) * ((G + ranges - 1) / ranges); }
 
-// NCONS consumer warps share the 8 tiles of every page, the last warp is the producer. CL: the key ranges of a pair are the
+__device__ __forceinline__ int kd_pages(const int32_t* seq_lens, int b) { return max(0, (__ldg(seq_lens + b) + BLK - 1) / BLK); }
+
+// The pages of all units, laid end to end, cut into equal runs (of KD_MIN_RUN pages or more, so that fewer CTAs than launched may
+// have one).
+struct KdRuns {
+    long total;
+    int runs;
+    KdRuns() = default;
+    __device__ __forceinline__ KdRuns(long pages, int most) : total(pages), runs(int(min(long(most), (pages + KD_MIN_RUN - 1) / KD_MIN_RUN))) {}
+    __device__ __forceinline__ long start_of(int c) const { return total * c / runs; }
+    __device__ __forceinline__ int run_of(long x) const { return int(((x + 1) * runs - 1) / total); }   // the run that page x is in
+};
+
+// A piece of work: pages [first, first + n) of a unit (sequence b, kv head kvh) that has `pages` of them.
+struct KdPiece {
+    int b, kvh, first, n, pages;
+};
+
+// The work of a CTA, walked by each of its warps alike. CL: the one range that the launch grid gives it. Else the pages of all
+// units, laid end to end (by sequence, then kv head), are cut into equal runs, one a CTA, whatever the sequences' lengths: a run
+// may end and begin inside a unit, whose pieces then meet in the scratch.
+template <bool CL>
+struct KdWalk {
+    int left, length;               // pages of the run still to come, and of all of it
+    KdPiece at;                     // piece under way (n = 0: none)
+
+    __device__ __forceinline__ void start(const Kv4DecodeParams& p, int lane) {
+        at.n = 0;
+        if (CL) {
+            at.b = blockIdx.z;
+            at.kvh = blockIdx.y;
+            at.pages = kd_pages(p.seq_lens, at.b);
+            const int per = (at.pages + p.nsplit - 1) / p.nsplit;
+            at.first = int(blockIdx.x) * per;
+            left = max(0, min(at.pages, at.first + per) - at.first);
+            length = left;
+            return;
+        }
+        int sum = 0;
+        for (int i = lane; i < p.batch; i += 32) sum += kd_pages(p.seq_lens, i);
+        sum = __reduce_add_sync(0xffffffffu, sum);
+        const KdRuns cut(long(sum) * p.n_kv_heads, p.n_runs);
+        const int c = blockIdx.x;
+        left = length = 0;
+        if (c >= cut.runs) return;
+        const long x0 = cut.start_of(c);
+        left = length = int(cut.start_of(c + 1) - x0);
+        // the sequence that page x0 falls in: the last one whose pages start at or before it (of those that have any)
+        int before = 0;
+        for (int i0 = 0; i0 < p.batch; i0 += 32) {
+            const int n = i0 + lane < p.batch ? kd_pages(p.seq_lens, i0 + lane) : 0;
+            int incl = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += v;
+            }
+            const unsigned here = __ballot_sync(0xffffffffu, long(before + incl) * p.n_kv_heads > x0);
+            if (here) {
+                const int l = __ffs(here) - 1;
+                at.b = i0 + l;
+                at.pages = __shfl_sync(0xffffffffu, n, l);
+                const int in = int(x0 - long(before + __shfl_sync(0xffffffffu, incl, l) - at.pages) * p.n_kv_heads);
+                at.kvh = in / at.pages;
+                at.first = in % at.pages;
+                return;
+            }
+            before += __shfl_sync(0xffffffffu, incl, 31);
+        }
+    }
+    // the next piece of the run; false when it is done
+    __device__ __forceinline__ bool next(const Kv4DecodeParams& p) {
+        if (left <= 0) return false;
+        if (at.n > 0) {   // behind the piece before: a new unit begins
+            at.first = 0;
+            if (++at.kvh == p.n_kv_heads) {
+                at.kvh = 0;
+                do at.pages = kd_pages(p.seq_lens, ++at.b);
+                while (at.pages == 0);   // (the run has pages left: a sequence that has some follows)
+            }
+        }
+        at.n = min(left, at.pages - at.first);
+        left -= at.n;
+        return true;
+    }
+};
+
+// NCONS consumer warps share the 8 tiles of every page, the last warp is the producer. CL: the key ranges of a unit are the
 // CTAs of one thread-block cluster, and each finishes the heads it owns (head h: CTA h % ranges) from its shared memory.
 template <int DT, bool SCORES, int NCONS, int STAGES, int MINB, bool CL>
 __global__ void __launch_bounds__((NCONS + 1) * 32, MINB)
-    kv4_decode_kernel(const __grid_constant__ CUtensorMap tmap, const Kv4DecodeParams p) {
-    constexpr int THREADS = (NCONS + 1) * 32;
+    kv4_decode_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ Kv4DecodeParams p) {
+    constexpr int TILES = 8 / NCONS;   // 16-key tiles of a page a consumer warp takes
+    constexpr int CT = NCONS * 32;     // consumer threads
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* stages = smem;
@@ -58,52 +160,70 @@ __global__ void __launch_bounds__((NCONS + 1) * 32, MINB)
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + kd_bars_at(STAGES));
     uint64_t* empty = full + STAGES;
     volatile int* limits = reinterpret_cast<volatile int*>(empty + STAGES);   // keys of the stage's page that count
-    __shared__ int s_last, s_failed, s_issued;
+    float* sums = reinterpret_cast<float*>(smem + kd_sums_at(STAGES));        // [NCONS][8][KD_PART]
+    __shared__ int s_failed, s_issued, s_more;
+    __shared__ KdWalk<CL> s_walk;   // the consumers' walk (thread 0 moves it on); the producer has its own, some pages ahead
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
     trace_first(p.ctl.trace, 0);
     if (CL) cluster_arrive();   // (every CTA of the cluster has started before any writes into another's shared memory)
-    const int S = p.seq_lens[b];   // (an input of the whole step: read ahead of the wait)
     if (!p.ctl.early) {
         pdl_wait();
         pdl_launch_dependents();
     }
-    const int npages = max(0, (S + BLK - 1) / BLK);
-    const int pps = (npages + p.nsplit - 1) / p.nsplit;
-    const int pg0 = split * pps;
-    const int n = max(0, min(npages, pg0 + pps) - pg0);
+    KdWalk<CL> walk;            // (seq_lens is an input of the whole step: read ahead of the wait)
+    if (warp == 0 || warp == NCONS) walk.start(p, lane);
+    if (tid == 0) s_walk = walk;
 
-    // ---- producer lane: page i of the range into its stage (a block outside the pool: no keys, and the error word set)
-    auto issue = [&](int i, int block) {
-        const int st = i % STAGES, use = i / STAGES;
-        if (i == p.ctl.stall_at) return false;   // diagnostic stall: the consumers' wait for this page runs out
+    // ---- producer: lane 0 keeps the ring of stages full (a block outside the pool: no keys, and the error word set)
+    int issued = 0;
+    bool issuing = true;
+    auto issue = [&](int page, int block, int S) {
+        const int st = issued % STAGES, use = issued / STAGES;
+        if (issued == p.ctl.stall_at) return false;   // diagnostic stall: the consumers' wait for this page runs out
         if (use > 0 && !mbar_wait_bounded(p.ctl.wait_cycles, &empty[st], (use - 1) & 1)) {
             atomicExch(p.ctl.err, ERR_WAIT_EMPTY);
             return false;
         }
-        if (block == -2) block = pg0 + i < p.table_stride ? p.block_table[size_t(b) * p.table_stride + pg0 + i] : -1;
         if (block < 0 || block >= p.num_blocks) {
             atomicExch(p.ctl.err, ERR_BAD_BLOCK);
             limits[st] = 0;
             mbar_arrive(&full[st]);
         } else {
-            const long page = (long(block) * p.n_layers + p.layer) * p.n_kv_heads + kvh;
+            const long pg = (long(block) * p.n_layers + p.layer) * p.n_kv_heads + walk.at.kvh;
             uint8_t* dst = stages + st * KV4_PAGE;
-            limits[st] = min(BLK, S - (pg0 + i) * BLK);
+            limits[st] = min(BLK, S - page * BLK);
             mbar_expect_tx(&full[st], KV4_PAGE);
-            tma_load_2d(dst, &tmap, 0, int(page * (KV4_PAGE / 128)), &full[st]);
-            bulk_load_1d(dst + 2 * KV4_SIDE, p.pool + size_t(page) * KV4_PAGE + 2 * KV4_SIDE, KV4_SCALES, &full[st]);
+            tma_load_2d(dst, &tmap, 0, int(pg * (KV4_PAGE / 128)), &full[st]);
+            bulk_load_1d(dst + 2 * KV4_SIDE, p.pool + size_t(pg) * KV4_PAGE + 2 * KV4_SIDE, KV4_SCALES, &full[st]);
         }
-        *reinterpret_cast<volatile int*>(&s_issued) = i + 1;
+        issued++;
+        *reinterpret_cast<volatile int*>(&s_issued) = issued;
         return true;
     };
-    int next = 0;
-    bool issuing = true;
+    // pages of the walk's pieces until `upto` have been requested or the run is done; block ids are looked up 32 at a time
+    int ahead = 0, blocks = -1, seq_len = 0;   // pages of the piece looked up and not yet requested .. (lane i: its i-th)
+    int done = 0;                              // pages of the piece requested
+    auto produce = [&](int upto) {
+        while (issuing && issued < upto) {
+            if (done == walk.at.n) {
+                if (!walk.next(p)) return;
+                done = 0;
+                seq_len = __ldg(p.seq_lens + walk.at.b);
+            }
+            if (done % 32 == 0) {
+                const int e = walk.at.first + done + lane;
+                blocks = done + lane < walk.at.n && e < p.table_stride ? p.block_table[size_t(walk.at.b) * p.table_stride + e] : -1;
+            }
+            ahead = __shfl_sync(0xffffffffu, blocks, done % 32);
+            bool ok = true;
+            if (lane == 0) ok = issue(walk.at.first + done, ahead, seq_len);
+            issuing = __shfl_sync(0xffffffffu, int(ok), 0) != 0;
+            issued = __shfl_sync(0xffffffffu, issued, 0);
+            done++;
+        }
+    };
     if (warp == NCONS) {
-        const int ahead = min(n, STAGES);
-        int myblock = -1;
-        if (lane < ahead && pg0 + lane < p.table_stride) myblock = p.block_table[size_t(b) * p.table_stride + pg0 + lane];
         if (lane == 0) {
             for (int s = 0; s < STAGES; s++) {
                 mbar_init(&full[s], 1);
@@ -114,205 +234,241 @@ __global__ void __launch_bounds__((NCONS + 1) * 32, MINB)
             fence_barrier_init();
         }
         __syncwarp();
-#pragma unroll
-        for (int s = 0; s < STAGES; s++) {
-            const int blk = __shfl_sync(0xffffffffu, myblock, s);
-            if (lane == 0 && s < n && issuing) {
-                issuing = issue(s, blk < 0 ? -1 : blk);
-                next = s + 1;
-            }
-        }
+        produce(STAGES);   // (the stages start empty: no wait)
     }
     if (p.ctl.early) {
         pdl_wait();
         pdl_launch_dependents();
     }
     trace_first(p.ctl.trace, 1);
-    for (int hh = warp; hh < 8; hh += NCONS + 1)
-        kv4_stage_query<DT>(sq, hh, hh < p.G, p.q, size_t(b) * p.q_stride + size_t(kvh * p.G + hh) * HD, p.prenormed != 0, p.g1, p.g2, p.ng, lane);
     __syncthreads();
 
-    const int r = lane >> 2, t = lane & 3;
-    float O[8][4];
-#pragma unroll
-    for (int i = 0; i < 8; i++) O[i][0] = O[i][1] = O[i][2] = O[i][3] = 0.0f;
-    float ps0 = 0.0f, ps1 = 0.0f;                                   // sums of the kept weights of heads 2t, 2t + 1
-    float f0 = pow2_biased(227), f1 = pow2_biased(227);             // their factors (2^100: nothing seen yet)
-
     if (warp == NCONS) {
-        if (lane == 0)
-            for (; next < n && issuing; next++) issuing = issue(next, -2);
+        produce(0x7fffffff);
     } else {
-        Kv4Frag frag;
-        frag.load(sq, lane);
+        // ---- consumers
+        const int r = lane >> 2, t = lane & 3;
         const uint32_t base = smem_u32(stages) + kv4_lane_at(lane);
-        bool big = false;
-        float limit = KD_LIMIT;
-        // scores: S x the query's power of two; a head that is not there never is the largest
-        float u0 = 0.0f, u1 = 0.0f, n0 = 0.0f, n1 = 0.0f;
-        if (SCORES) {
-            const int e0 = sq.expo[2 * t], e1 = sq.expo[2 * t + 1];
-            if (e0) u0 = pow2_biased(e0);
-            else n0 = __uint_as_float(0xff800000u);
-            if (e1) u1 = pow2_biased(e1);
-            else n1 = __uint_as_float(0xff800000u);
-        }
+        const float sink = sqrtf(float(HD));
         int st = 0, phase = 0;
-        for (int i = 0; i < n; i++) {
-            // (the decision is the warp's: a warp that leaves the loop leaves it whole)
-            if (!__all_sync(0xffffffffu, mbar_wait_bounded(p.ctl.wait_cycles, &full[st], phase))) {
-                atomicExch(p.ctl.err, ERR_WAIT_FULL);
-                *reinterpret_cast<volatile int*>(&s_failed) = 1;
-                break;
+        bool ok = true;                                             // (the warp's: no wait of it has run out)
+        for (int c = blockIdx.x; !CL && c < p.batch; c += gridDim.x)   // sequences without keys have no unit in any run
+            if (__ldg(p.seq_lens + c) <= 0)
+                for (int i = tid; i < p.n_kv_heads * p.G * HD; i += CT) Act<DT>::store(p.o, size_t(c) * p.o_stride + i, 0.0f);
+        while (true) {
+            if (tid == 0) s_more = s_walk.next(p);
+            bar_sync(1, CT);
+            if (!CL && !s_more) break;
+            const KdPiece& pc = s_walk.at;                          // (CL: a range without pages is walked through all the same)
+            const int unit = pc.b * p.n_kv_heads + pc.kvh, n = s_more ? pc.n : 0;
+            const int lane_q = here(lane);
+            for (int hh = here(warp); hh < 8; hh += NCONS)
+                kv4_stage_query<DT>(sq, hh, hh < p.G, p.q, size_t(pc.b) * p.q_stride + size_t(pc.kvh * p.G + hh) * HD, p.prenormed != 0, p.g1, p.g2,
+                                    p.ng, lane_q);
+            bar_sync(1, CT);
+            Kv4Frag frag;
+            frag.load(sq, lane_q);
+            // scores: S x the query's power of two; a head that is not there never is the largest
+            float u0 = 0.0f, u1 = 0.0f, n0 = 0.0f, n1 = 0.0f;
+            if (SCORES) {
+                const int e0 = sq.expo[2 * t], e1 = sq.expo[2 * t + 1];
+                if (e0) u0 = pow2_biased(e0) / KV4_SUBNORMAL;
+                else n0 = __uint_as_float(0xff800000u);
+                if (e1) u1 = pow2_biased(e1) / KV4_SUBNORMAL;
+                else n1 = __uint_as_float(0xff800000u);
             }
-            const int lim = limits[st];
-            const uint8_t* scales = stages + st * KV4_PAGE + 2 * KV4_SIDE;
+            float O[8][4];
 #pragma unroll
-            for (int step = 0; step < 8 / NCONS; step++) {
-                const int R0 = (step * NCONS + warp) * 16;
-                const int left = lim - R0;                          // keys of the tile that count, if under 16
-                if (left <= 0) break;
-                const uint32_t kaddr = base + st * KV4_PAGE + R0 * KV4_ROW;
-                float s[4];
-                kv4_tile_scores(kaddr, scales + R0 * 16, lane, frag, s);
-                if (SCORES) {
-                    float m0 = fmaxf(fmaf(s[0], u0, n0), fmaf(s[1], u1, n1)), m1 = fmaxf(fmaf(s[2], u0, n0), fmaf(s[3], u1, n1));
-                    m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, 1));
-                    m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 1));
-                    m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, 2));
-                    m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 2));
-                    const int key = r + 8 * t;
-                    if (t < 2 && key < left)
-                        p.scores[(size_t(b) * p.n_kv_heads + kvh) * p.scores_stride + (pg0 + i) * BLK + R0 + key] = t ? m1 : m0;
+            for (int i = 0; i < 8; i++) O[i][0] = O[i][1] = O[i][2] = O[i][3] = 0.0f;
+            float ps0 = 0.0f, ps1 = 0.0f;                           // sums of the kept weights of heads 2t, 2t + 1
+            float f0 = pow2_biased(247), f1 = pow2_biased(247);     // their factors (2^120: nothing seen yet)
+            bool big = false;
+            float limit = KD_LIMIT;
+            for (int i = 0; i < n && ok; i++) {
+                // (the decision is the warp's: a warp that leaves the loop leaves it whole)
+                ok = __all_sync(0xffffffffu, mbar_wait_bounded(p.ctl.wait_cycles, &full[st], phase));
+                if (!ok) {
+                    atomicExch(p.ctl.err, ERR_WAIT_FULL);
+                    *reinterpret_cast<volatile int*>(&s_failed) = 1;
+                    break;
                 }
-                uint32_t vs[8];
-                kv4_value_scales(scales + R0 * 16, lane, vs);
+                const int page = pc.first + i;
+                // the warp's tiles of the page together: their products have nothing to wait for in one another
+                const uint32_t kaddr = base + st * KV4_PAGE + warp * (TILES * 16 * KV4_ROW);
+                const uint8_t* sc = stages + st * KV4_PAGE + 2 * KV4_SIDE + warp * (TILES * 16 * 16);
+                const int left = limits[st] - warp * (TILES * 16);   // keys of the tiles that count, if fewer than there are
+                if (left > 0) {
+                    float s[TILES][4];
+                    uint32_t vs[TILES][8];
+                    bool flagged = false;
 #pragma unroll
-                for (int e = 0; e < 4; e++) s[e] = fmaxf(s[e], 0.0f);
-                if (left < 16) {
-                    if (r >= left) s[0] = s[1] = 0.0f;
-                    if (r + 8 >= left) s[2] = s[3] = 0.0f;
-                    kv4_mask_value_scales(vs, lane, left);
+                    for (int k = 0; k < TILES; k++) {
+                        kv4_tile_scores(kaddr + k * 16 * KV4_ROW, sc + k * 256, lane, frag, s[k]);
+                        kv4_value_scales(sc + k * 256, lane, vs[k]);
+                    }
+                    if (SCORES) {
+#pragma unroll
+                        for (int k = 0; k < TILES; k++) {
+                            float m0 = fmaxf(fmaf(s[k][0], u0, n0), fmaf(s[k][1], u1, n1)), m1 = fmaxf(fmaf(s[k][2], u0, n0), fmaf(s[k][3], u1, n1));
+                            m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, 1));
+                            m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 1));
+                            m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, 2));
+                            m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 2));
+                            const int key = k * 16 + r + 8 * t;
+                            if (t < 2 && key < left)
+                                p.scores[size_t(unit) * p.scores_stride + page * BLK + warp * (TILES * 16) + key] = t ? m1 : m0;
+                        }
+                    }
+                    if (left < TILES * 16) {
+#pragma unroll
+                        for (int k = 0; k < TILES; k++) {
+                            if (k * 16 + r >= left) s[k][0] = s[k][1] = 0.0f;
+                            if (k * 16 + r + 8 >= left) s[k][2] = s[k][3] = 0.0f;
+                            kv4_mask_value_scales(vs[k], lane, left - k * 16);
+                        }
+                    }
+                    float w[TILES][4], top = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < TILES; k++) {
+                        flagged |= kv4_scales_large(vs[k]);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            s[k][e] = fmaxf(s[k][e], 0.0f);
+                            w[k][e] = s[k][e] * ((e & 1) ? f1 : f0) * s[k][e];
+                            top = fmaxf(top, w[k][e]);
+                        }
+                    }
+                    if (__any_sync(0xffffffffu, top > limit || (flagged && !big))) {
+                        // (a handful of times a warp) new factors: the tiles' largest weight of a head at most 2^target
+                        if (__any_sync(0xffffffffu, flagged)) {
+                            big = true;
+                            limit = KD_LIMIT_BIG;
+                        }
+                        const int target = big ? KD_TARGET_BIG : KD_TARGET;
+                        float m0 = 0.0f, m1 = 0.0f;
+#pragma unroll
+                        for (int k = 0; k < TILES; k++) {
+                            m0 = fmaxf(m0, fmaxf(s[k][0], s[k][2]));
+                            m1 = fmaxf(m1, fmaxf(s[k][1], s[k][3]));
+                        }
+#pragma unroll
+                        for (int o = 4; o < 32; o <<= 1) {
+                            m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
+                            m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+                        }
+                        // m < 2^(e + 1), so m^2 2^(target - 2 (e + 1)) < 2^target
+                        const int e0 = int(__float_as_uint(m0) >> 23) - 126, e1 = int(__float_as_uint(m1) >> 23) - 126;
+                        const float nf0 = m0 * f0 * m0 > limit ? pow2_biased(min(max(127 + target - 2 * e0, 1), 254)) : f0;
+                        const float nf1 = m1 * f1 * m1 > limit ? pow2_biased(min(max(127 + target - 2 * e1, 1), 254)) : f1;
+                        const float c0 = nf0 / f0, c1 = nf1 / f1;
+                        f0 = nf0;
+                        f1 = nf1;
+                        ps0 *= c0;
+                        ps1 *= c1;
+#pragma unroll
+                        for (int k = 0; k < 8; k++) {
+                            O[k][0] *= c0;
+                            O[k][1] *= c1;
+                            O[k][2] *= c0;
+                            O[k][3] *= c1;
+                        }
+#pragma unroll
+                        for (int k = 0; k < TILES; k++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) w[k][e] = s[k][e] * ((e & 1) ? f1 : f0) * s[k][e];
+                    }
+#pragma unroll
+                    for (int k = 0; k < TILES; k++) {
+                        ps0 += w[k][0] + w[k][2];
+                        ps1 += w[k][1] + w[k][3];
+                        // the weights as fp16 (2^-11), keys across the lanes: the B registers of the sum
+                        kv4_tile_values(kaddr + KV4_SIDE + k * 16 * KV4_ROW, movmatrix4_trans(pack_h2(w[k][0], w[k][1])),
+                                        movmatrix4_trans(pack_h2(w[k][2], w[k][3])), vs[k], O);
+                    }
                 }
-                float w0 = s[0] * f0 * s[0], w1 = s[1] * f1 * s[1], w2 = s[2] * f0 * s[2], w3 = s[3] * f1 * s[3];
-                const bool flagged = kv4_scales_large(vs);
-                if (__any_sync(0xffffffffu, fmaxf(fmaxf(w0, w1), fmaxf(w2, w3)) > limit || (flagged && !big))) {
-                    // (a handful of times a warp) new factors: the tile's largest weight of a head at most 2^target
-                    if (__any_sync(0xffffffffu, flagged)) {
-                        big = true;
-                        limit = KD_LIMIT_BIG;
-                    }
-                    const int target = big ? KD_TARGET_BIG : KD_TARGET;
-                    float m0 = fmaxf(s[0], s[2]), m1 = fmaxf(s[1], s[3]);
-#pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) {
-                        m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
-                        m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
-                    }
-                    // m < 2^(e + 1), so m^2 2^(target - 2 (e + 1)) < 2^target
-                    const int e0 = int(__float_as_uint(m0) >> 23) - 126, e1 = int(__float_as_uint(m1) >> 23) - 126;
-                    const float nf0 = m0 * f0 * m0 > limit ? pow2_biased(min(max(127 + target - 2 * e0, 1), 254)) : f0;
-                    const float nf1 = m1 * f1 * m1 > limit ? pow2_biased(min(max(127 + target - 2 * e1, 1), 254)) : f1;
-                    const float c0 = nf0 / f0, c1 = nf1 / f1;
-                    f0 = nf0;
-                    f1 = nf1;
-                    ps0 *= c0;
-                    ps1 *= c1;
-#pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        O[k][0] *= c0;
-                        O[k][1] *= c1;
-                        O[k][2] *= c0;
-                        O[k][3] *= c1;
-                    }
-                    w0 = s[0] * f0 * s[0];
-                    w1 = s[1] * f1 * s[1];
-                    w2 = s[2] * f0 * s[2];
-                    w3 = s[3] * f1 * s[3];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty[st]);
+                if (++st == STAGES) {
+                    st = 0;
+                    phase ^= 1;
                 }
-                ps0 += w0 + w2;
-                ps1 += w1 + w3;
-                // the weights as fp16 (2^-11), keys across the lanes: the B registers of the sum
-                kv4_tile_values(kaddr + KV4_SIDE, movmatrix4_trans(pack_h2(w0, w1)), movmatrix4_trans(pack_h2(w2, w3)), vs, O);
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&empty[st]);
-            if (++st == STAGES) {
-                st = 0;
-                phase ^= 1;
+            // ---- the warps' sums of the piece into one, in units of the weights themselves
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                ps0 += __shfl_xor_sync(0xffffffffu, ps0, o);
+                ps1 += __shfl_xor_sync(0xffffffffu, ps1, o);
             }
+            // w = w' / f x (the query's power of two x 2^20)^2 / 128, the powers of two multiplied one by one
+            const int lane_s = here(lane), rs = lane_s >> 2, ts = lane_s & 3, tid_s = here(tid);
+            const float q0 = pow2_biased(max(sq.expo[2 * ts], 1)), q1 = pow2_biased(max(sq.expo[2 * ts + 1], 1));
+            const float i0 = (1.0f / 128.0f / KV4_SUBNORMAL / KV4_SUBNORMAL) / f0, i1 = (1.0f / 128.0f / KV4_SUBNORMAL / KV4_SUBNORMAL) / f1;
+            float* mine0 = sums + (warp * 8 + 2 * ts) * KD_PART;
+            float* mine1 = mine0 + KD_PART;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int d = kv4_dim_of(k, rs);
+                mine0[d] = O[k][0] * i0 * q0 * q0;
+                mine1[d] = O[k][1] * i1 * q1 * q1;
+                mine0[d + 2] = O[k][2] * i0 * q0 * q0;
+                mine1[d + 2] = O[k][3] * i1 * q1 * q1;
+            }
+            if (rs == 0) {
+                mine0[HD] = ps0 * i0 * q0 * q0;
+                mine1[HD] = ps1 * i1 * q1 * q1;
+            }
+            bar_sync(1, CT);
+            if (CL) break;   // (the cluster's CTAs meet below, all warps)
+            // A unit inside this run is done: its rows. Else its pieces, one a run, meet in the scratch (a run has at most two pieces
+            // of units that it shares, its first and its last: slots 2 c and 2 c + 1), where kv4_decode_join_kernel adds them.
+            const bool whole = n == pc.pages;
+            float* part = p.partials + size_t(2 * blockIdx.x + (s_walk.length - s_walk.left == n ? 0 : 1)) * p.G * KD_PART;
+            for (int idx = tid_s; idx < p.G * HD; idx += CT) {
+                const int hh = idx >> 7, d = idx & 127;
+                float num = 0.0f, den = 0.0f;
+#pragma unroll
+                for (int w = 0; w < NCONS; w++) {
+                    num += sums[(w * 8 + hh) * KD_PART + d];
+                    den += sums[(w * 8 + hh) * KD_PART + HD];
+                }
+                if (whole) Act<DT>::store(p.o, size_t(pc.b) * p.o_stride + size_t(pc.kvh * p.G + hh) * HD + d, num / (sink + den));
+                else {
+                    part[hh * KD_PART + d] = num;
+                    if (d == 0) part[hh * KD_PART + HD] = den;
+                }
+            }
+            // (the sums and the walk are read before this barrier, written again behind the next piece's)
+            bar_sync(1, CT);
         }
     }
 
     trace_last(p.ctl.trace, 2);
-    // ---- the warps' sums into one partial, in units of the weights themselves. The stages are free: every page that was
-    // requested has been waited for, unless a wait gave up - then wait (bounded) for what is still in flight first.
+    // Every page that was requested has been waited for, unless a wait gave up - then wait (bounded) for what is in flight.
     __syncthreads();
-    if (s_failed) {
-        if (tid == 0) {
-            for (int i = max(0, s_issued - STAGES); i < s_issued; i++)
-                if (!mbar_wait_bounded(p.ctl.wait_cycles, &full[i % STAGES], (i / STAGES) & 1)) atomicExch(p.ctl.err, ERR_WAIT_DRAIN);
-        }
-        __syncthreads();
+    if (s_failed && tid == 0) {
+        for (int i = max(0, s_issued - STAGES); i < s_issued; i++)
+            if (!mbar_wait_bounded(p.ctl.wait_cycles, &full[i % STAGES], (i / STAGES) & 1)) atomicExch(p.ctl.err, ERR_WAIT_DRAIN);
     }
-    float(*red)[8][HD] = reinterpret_cast<float(*)[8][HD]>(stages);
-    float(*redp)[8] = reinterpret_cast<float(*)[8]>(stages + NCONS * 8 * HD * 4);
-    if (warp < NCONS) {
+    if (CL) {
+        // every range's rows go, head by head, to the CTA that finishes the head; it adds them in range order
+        constexpr int THREADS = (NCONS + 1) * 32;
+        const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+        const float sink = sqrtf(float(HD));
+        float* inbox = sums + NCONS * 8 * KD_PART;
+        const int slots = (p.G + p.nsplit - 1) / p.nsplit;
+        cluster_wait();
+        for (int idx = tid; idx < p.G * HD; idx += THREADS) {
+            const int hh = idx >> 7, d = idx & 127;
+            float num = 0.0f, den = 0.0f;
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) {
-            ps0 += __shfl_xor_sync(0xffffffffu, ps0, o);
-            ps1 += __shfl_xor_sync(0xffffffffu, ps1, o);
-        }
-        // w = w' / f x (the query's power of two)^2 / 128, the powers of two multiplied one by one
-        const float q0 = pow2_biased(max(sq.expo[2 * t], 1)), q1 = pow2_biased(max(sq.expo[2 * t + 1], 1));
-        const float i0 = (1.0f / 128.0f) / f0, i1 = (1.0f / 128.0f) / f1;
-        auto real0 = [&](float x) { return x * i0 * q0 * q0; };
-        auto real1 = [&](float x) { return x * i1 * q1 * q1; };
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const int d = kv4_dim_of(k, r);
-            red[warp][2 * t][d] = real0(O[k][0]);
-            red[warp][2 * t + 1][d] = real1(O[k][1]);
-            red[warp][2 * t][d + 2] = real0(O[k][2]);
-            red[warp][2 * t + 1][d + 2] = real1(O[k][3]);
-        }
-        if (r == 0) {
-            redp[warp][2 * t] = real0(ps0);
-            redp[warp][2 * t + 1] = real1(ps1);
-        }
-    }
-    __syncthreads();
-
-    if (CL) cluster_wait();
-    const int pair = b * p.n_kv_heads + kvh;
-    const float sink = sqrtf(float(HD));
-    float* part = p.partials + (size_t(pair) * p.nsplit + split) * p.G * KD_PART;
-    float* inbox = reinterpret_cast<float*>(smem + kd_inbox_at(STAGES));
-    const int slots = CL ? (p.G + p.nsplit - 1) / p.nsplit : 0;     // heads an owner finishes
-    for (int idx = tid; idx < p.G * HD; idx += THREADS) {
-        const int hh = idx >> 7, d = idx & 127;
-        float num = 0.0f, den = 0.0f;
-#pragma unroll
-        for (int w = 0; w < NCONS; w++) {
-            num += red[w][hh][d];
-            den += redp[w][hh];
-        }
-        if (p.nsplit == 1) {
-            Act<DT>::store(p.o, size_t(b) * p.o_stride + size_t(kvh * p.G + hh) * HD + d, num / (sink + den));
-        } else if (CL) {
+            for (int w = 0; w < NCONS; w++) {
+                num += sums[(w * 8 + hh) * KD_PART + d];
+                den += sums[(w * 8 + hh) * KD_PART + HD];
+            }
             const uint32_t row = cluster_map(smem_u32(inbox + (split * slots + hh / p.nsplit) * KD_PART), uint32_t(hh % p.nsplit));
             cluster_st_f32(row + uint32_t(d) * 4u, num);
             if (d == 0) cluster_st_f32(row + HD * 4, den);
-        } else {
-            part[hh * KD_PART + d] = num;
-            if (d == 0) part[hh * KD_PART + HD] = den;
         }
-    }
-    if (p.nsplit == 1) {
-        trace_last(p.ctl.trace, 3);
-        return;
-    }
-    if (CL) {
         cluster_arrive();
         cluster_wait();
         for (int idx = tid; idx < slots * HD; idx += THREADS) {
@@ -327,61 +483,90 @@ __global__ void __launch_bounds__((NCONS + 1) * 32, MINB)
                 Act<DT>::store(p.o, size_t(b) * p.o_stride + size_t(kvh * p.G + hh) * HD + d, num / den);
             }
         }
-        trace_last(p.ctl.trace, 3);
-        return;
-    }
-    // last CTA of the pair to arrive adds the ranges in order (arrive_last, common.metal:88-99)
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) {
-        const int prev = atomicAdd(&p.counters[pair], 1);
-        s_last = prev == p.nsplit - 1;
-        if (s_last) p.counters[pair] = 0;
-    }
-    __syncthreads();
-    if (!s_last) {
-        trace_last(p.ctl.trace, 3);
-        return;
-    }
-    __threadfence();
-    const float* all = p.partials + size_t(pair) * p.nsplit * p.G * KD_PART;
-    const int n4 = p.nsplit * p.G * (KD_PART / 4);
-    const bool staged = n4 * 16 <= STAGES * KV4_PAGE;
-    if (staged) {
-        stage_from_global<THREADS>(reinterpret_cast<float4*>(stages), reinterpret_cast<const float4*>(all), n4, tid);
-        __syncthreads();
-        all = reinterpret_cast<const float*>(stages);
-    }
-    for (int idx = tid; idx < p.G * HD; idx += THREADS) {
-        const int hh = idx >> 7, d = idx & 127;
-        float num = 0.0f, den = sink;
-        for (int k = 0; k < p.nsplit; k++) {
-            const float* row = all + (size_t(k) * p.G + hh) * KD_PART;
-            den += staged ? row[HD] : __ldcg(row + HD);
-            num += staged ? row[d] : __ldcg(row + d);
-        }
-        Act<DT>::store(p.o, size_t(b) * p.o_stride + size_t(kvh * p.G + hh) * HD + d, num / den);
     }
     trace_last(p.ctl.trace, 3);
 }
 
-int choose_full_decode_split(int pairs, int pages, int slots, int max_slots, bool* cluster);   // full_decode.cu
+// Adds the pieces of the units that the runs of a launch cut, in the order of the runs, and writes their rows: one CTA a unit,
+// launched behind the runs (the last run of a unit adding 27 pieces of 8 heads by itself, one query among 132 KB of loads,
+// took longer than this launch). A thread takes four dims of a head.
+template <int DT>
+__global__ void __launch_bounds__(256) kv4_decode_join_kernel(const __grid_constant__ Kv4DecodeParams p) {
+    const int tid = threadIdx.x, lane = tid & 31, unit = blockIdx.x, b = unit / p.n_kv_heads, kvh = unit % p.n_kv_heads;
+    trace_first(p.ctl.trace, 0);
+    int before = 0, sum = 0;
+    for (int i = lane; i < p.batch; i += 32) {
+        const int n = kd_pages(p.seq_lens, i);
+        sum += n;
+        if (i < b) before += n;
+    }
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    before = __reduce_add_sync(0xffffffffu, before);
+    const int pages = kd_pages(p.seq_lens, b);
+    const KdRuns runs(long(sum) * p.n_kv_heads, p.n_runs);
+    const long x = long(before) * p.n_kv_heads + long(kvh) * pages;
+    // (every CTA waits, one with nothing to add too: the launch behind this one takes its end for the end of the runs)
+    pdl_wait();
+    pdl_launch_dependents();
+    trace_first(p.ctl.trace, 1);
+    if (pages == 0) return;
+    const int lo = runs.run_of(x), hi = runs.run_of(x + pages - 1);
+    const int hh = tid >> 5;
+    if (lo == hi || hh >= p.G) return;
+    const int first_slot = runs.start_of(lo) == x ? 2 * lo : 2 * lo + 1;   // (the unit may begin inside run lo)
+    float4 num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float den = sqrtf(float(HD));
+    for (int k = lo; k <= hi; k += 8) {   // eight pieces' loads in flight together
+        float4 v[8];
+        float e[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float* row = p.partials + (size_t(k + j == lo ? first_slot : 2 * (k + j)) * p.G + hh) * KD_PART;
+            v[j] = k + j <= hi ? __ldcg(reinterpret_cast<const float4*>(row) + lane) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            e[j] = k + j <= hi ? __ldcg(row + HD) : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            num.x += v[j].x;
+            num.y += v[j].y;
+            num.z += v[j].z;
+            num.w += v[j].w;
+            den += e[j];
+        }
+    }
+    const float inv = 1.0f / den;
+    const size_t at = size_t(b) * p.o_stride + size_t(kvh * p.G + hh) * HD + 4 * lane;
+    Act<DT>::store(p.o, at, num.x * inv);
+    Act<DT>::store(p.o, at + 1, num.y * inv);
+    Act<DT>::store(p.o, at + 2, num.z * inv);
+    Act<DT>::store(p.o, at + 3, num.w * inv);
+    trace_last(p.ctl.trace, 3);
+}
 
 constexpr int KD_NCONS = 4, KD_STAGES = 3, KD_MINB = 3;
 
+static bool use_pdl() {
+    static const bool on = []() { const char* e = getenv("EMBLA_NO_PDL"); return !(e && e[0] == '1'); }();
+    return on;
+}
+
 template <int DT, bool SCORES, bool CL>
-static EmblaStatus launch_kv4_decode(EmblaAttn* ctx, const EmblaKVPool* pool, const Kv4DecodeParams& p, int batch, cudaStream_t s) {
+static EmblaStatus launch_kv4_decode(EmblaAttn* ctx, const EmblaKVPool* pool, const Kv4DecodeParams& p, int batch, dim3 grid, cudaStream_t s) {
     auto kern = kv4_decode_kernel<DT, SCORES, KD_NCONS, KD_STAGES, KD_MINB, CL>;
-    const size_t smem = 1024 + kd_inbox_at(KD_STAGES) + (CL ? kd_inbox_rows(p.nsplit, p.G) * KD_PART * 4 : 0);
+    const size_t smem = kd_smem(KD_NCONS, KD_STAGES) + (CL ? kd_inbox_rows(p.nsplit, p.G) * KD_PART * 4 : 0);
     static bool configured[64] = {};   // per instantiation and device
     if (!configured[ctx->device & 63]) {
         // (the largest inbox: 7 ranges of 8 heads, two each)
         EMBLA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                            int(1024 + kd_inbox_at(KD_STAGES) + (CL ? 14 * KD_PART * 4 : 0))));
+                                            int(kd_smem(KD_NCONS, KD_STAGES) + (CL ? 14 * KD_PART * 4 : 0))));
         configured[ctx->device & 63] = true;
     }
-    const dim3 grid(p.nsplit, p.n_kv_heads, batch);
     EMBLA_CUDA_TRY(launch_kernel_cluster(ctx->pdl, CL ? p.nsplit : 1, kern, grid, dim3((KD_NCONS + 1) * 32), smem, s, pool->tmap_codes, p));
+    if (!CL && p.n_runs > 1) {
+        Kv4DecodeParams pj = p;
+        pj.ctl = kernel_ctl(ctx);
+        EMBLA_CUDA_TRY(launch_kernel(use_pdl(), kv4_decode_join_kernel<DT>, dim3(unsigned(batch) * p.n_kv_heads), dim3(p.G * 32), 0, s, pj));
+    }
     EMBLA_CUDA_TRY(cudaGetLastError());
     return EMBLA_OK;
 }
@@ -397,7 +582,6 @@ EmblaStatus kv4_full_decode(EmblaAttn* ctx, const EmblaKVPool* pool, const Embla
     p.g2 = q->g2_dev;
     p.o = o_dev;
     p.partials = ctx->partials;
-    p.counters = ctx->counters;
     p.ctl = kernel_ctl(ctx);
     p.scores = scores_dev;
     p.q_stride = q->q_stride;
@@ -409,14 +593,25 @@ EmblaStatus kv4_full_decode(EmblaAttn* ctx, const EmblaKVPool* pool, const Embla
     p.n_kv_heads = pool->n_kv_heads;
     p.num_blocks = pool->num_blocks;
     p.G = ctx->cfg.n_q_heads / ctx->cfg.n_kv_heads;
+    p.batch = view->batch;
     p.prenormed = q->prenormed;
     p.ng = q->ng;
-    const int pairs = view->batch * pool->n_kv_heads, pages = (max_len + BLK - 1) / BLK;
-    bool cluster = false;
-    p.nsplit = choose_full_decode_split(pairs, pages, KD_MINB * ctx->sm_count, ctx->partial_slots, &cluster);
+    const long units = long(view->batch) * pool->n_kv_heads, pages = (max_len + BLK - 1) / BLK;
+    // Few pages: a cluster a unit, one page or a few a CTA. Else equal runs over the resident CTAs (the scratch holds two
+    // pieces a run: embla_attn_create makes it 8 slots an SM and more).
+    const bool cluster = units * pages <= KD_CLUSTER_PAGES && units <= 0xffff;
+    dim3 grid;
+    if (cluster) {
+        p.nsplit = int(pages < KD_MAX_CLUSTER ? pages : KD_MAX_CLUSTER);
+        grid = dim3(p.nsplit, pool->n_kv_heads, view->batch);
+    } else {
+        const long most = (units * pages + KD_MIN_RUN - 1) / KD_MIN_RUN, slots = long(KD_MINB) * ctx->sm_count;
+        p.n_runs = int(most < slots ? most : slots);
+        grid = dim3(p.n_runs);
+    }
     const bool bf = ctx->cfg.act_dtype == EMBLA_BF16;
-#define EMBLA_KD(DT, SC) (cluster ? launch_kv4_decode<DT, SC, true>(ctx, pool, p, view->batch, stream) \
-                                  : launch_kv4_decode<DT, SC, false>(ctx, pool, p, view->batch, stream))
+#define EMBLA_KD(DT, SC) (cluster ? launch_kv4_decode<DT, SC, true>(ctx, pool, p, view->batch, grid, stream) \
+                                  : launch_kv4_decode<DT, SC, false>(ctx, pool, p, view->batch, grid, stream))
     if (scores_dev) return bf ? EMBLA_KD(EMBLA_BF16, true) : EMBLA_KD(EMBLA_F16, true);
     return bf ? EMBLA_KD(EMBLA_BF16, false) : EMBLA_KD(EMBLA_F16, false);
 #undef EMBLA_KD

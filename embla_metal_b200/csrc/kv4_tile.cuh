@@ -4,9 +4,12 @@
 //
 //   S^T = K Q^T   A = 16 keys x 16 dims. A row's chunk g is its group g: ldmatrix hands lane (r, t) the word of key r that holds
 //                 dims 8t .. 8t + 7 of the group, which widens to the A registers of two products with no permutation. The
-//                 products of a group are summed apart (fp32), times the key's scale of the group into S. The codes enter as
-//                 72 + code (one shift and one logic operation a register, no subtraction); the constant part, 72 x the sum
-//                 of the query over the group, is the accumulator's start value, negated. It costs 2 of the 24 bits.
+//                 products of a group are summed apart (fp32), times the key's scale of the group into S. The ALU pipe (two
+//                 instructions a clock and SM) is what a decode runs out of first, so a word costs it one shift and four logic
+//                 operations and no more: a nibble stays where it is, its sign bit flipped, as the fp16 subnormal
+//                 (code + 8) 2^-24 (low nibble of a byte) or (code + 8) 2^-20 (high nibble), exact in the product; the queries
+//                 of the low nibbles' dims carry the missing 2^4. The constant part, 8 x the sum of the query over the group,
+//                 is the accumulator's start value, negated.
 //   O^T = V^T P^T A = 16 dims x 16 keys. The transposing ldmatrix, on 16-bit elements of four codes, hands lane (r, t) the
 //                 element r of keys 2t and 2t + 1 side by side: widened, its nibbles are A registers (a dim, two keys). The
 //                 value's scale of the group is multiplied into P (fp16, one more rounding of 2^-11), the codes stay exact.
@@ -35,11 +38,21 @@ __device__ __forceinline__ uint32_t movmatrix4_trans(uint32_t x) {
 // 2^(e - 127) for a biased exponent 1 .. 254
 __device__ __forceinline__ float pow2_biased(int e) { return __uint_as_float(uint32_t(e) << 23); }
 
+constexpr float KV4_SUBNORMAL = 1.0f / 1048576.0f;   // 2^-20: S comes out of the products scaled by it
+
+// D = A B + C with C apart from D, fp16 operands, fp32 sums (not volatile: the products of two tiles may be interleaved)
+__device__ __forceinline__ void mma_16816_c(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
+                                            const float (&c)[4]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+
 // The queries of a kv head in shared memory: rows scaled by a power of two that brings their largest element into [1, 2) (exact;
 // fp16 then holds bf16 queries of any size), and what goes with them.
 struct Kv4Queries {
     __half q[8][HD];
-    float start[8][KV4_GROUPS];   // -72 x the sum of the scaled query over the group
+    float start[8][KV4_GROUPS];   // -8 x the sum of the scaled query over the group, x 2^-20
     int expo[8];                  // biased exponent of the power of two; 0: no such head
 };
 
@@ -62,11 +75,12 @@ __device__ __forceinline__ void kv4_stage_query(Kv4Queries& sq, int hh, bool has
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const __half h = __float2half_rn(x[i] * down);
-        sq.q[hh][lane + 32 * i] = h;
+        // dims 0, 1, 4, 5 of every 8 lie in low nibbles: 16 x (exact)
+        sq.q[hh][lane + 32 * i] = (lane & 2) ? h : __hmul(h, __float2half_rn(16.0f));
         float sum = __half2float(h);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) sq.start[hh][i] = -72.0f * sum;
+        if (lane == 0) sq.start[hh][i] = -8.0f * KV4_SUBNORMAL * sum;
     }
     if (lane == 0) sq.expo[hh] = has ? e : 0;
 }
@@ -74,7 +88,7 @@ __device__ __forceinline__ void kv4_stage_query(Kv4Queries& sq, int hh, bool has
 // A lane's share of the queries: B registers of head r = lane / 4, start values of heads 2t, 2t + 1 (t = lane % 4).
 struct Kv4Frag {
     uint32_t b[KV4_GROUPS][4];
-    float start[KV4_GROUPS][2];
+    float start[KV4_GROUPS][4];
     __device__ __forceinline__ void load(const Kv4Queries& sq, int lane) {
         const int r = lane >> 2, t = lane & 3;
 #pragma unroll
@@ -84,8 +98,10 @@ struct Kv4Frag {
             b[g][1] = v.y;
             b[g][2] = v.z;
             b[g][3] = v.w;
-            start[g][0] = sq.start[2 * t][g];
-            start[g][1] = sq.start[2 * t + 1][g];
+            // (twice over, through volatile loads: four registers in a row, as the products take them, and no copies)
+            volatile const float(*from)[KV4_GROUPS] = sq.start;
+#pragma unroll
+            for (int e = 0; e < 4; e++) start[g][e] = from[2 * t + (e & 1)][g];
         }
     }
 };
@@ -108,11 +124,13 @@ __device__ __forceinline__ void kv4_tile_scores(uint32_t kaddr, const uint8_t* s
         for (int h = 0; h < 2; h++) {
             const int g = 2 * j + h;
             const uint32_t lo = w[2 * h], hi = w[2 * h + 1];   // keys r and r + 8
-            float a[4] = {f.start[g][0], f.start[g][1], f.start[g][0], f.start[g][1]};
-            mma_16816(a, kv4_lop(lo << 4, KV4_HI_MASK, KV4_HI_FLIP), kv4_lop(hi << 4, KV4_HI_MASK, KV4_HI_FLIP),
-                      kv4_lop(lo, KV4_HI_MASK, KV4_HI_FLIP), kv4_lop(hi, KV4_HI_MASK, KV4_HI_FLIP), f.b[g][0], f.b[g][1]);
-            mma_16816(a, kv4_lop(lo >> 4, KV4_HI_MASK, KV4_HI_FLIP), kv4_lop(hi >> 4, KV4_HI_MASK, KV4_HI_FLIP),
-                      kv4_lop(lo >> 8, KV4_HI_MASK, KV4_HI_FLIP), kv4_lop(hi >> 8, KV4_HI_MASK, KV4_HI_FLIP), f.b[g][2], f.b[g][3]);
+            const uint32_t lo8 = lo >> 8, hi8 = hi >> 8;
+            float a[4];
+            // dims 0, 1 and 4, 5 of the lane's eight, then 2, 3 and 6, 7
+            mma_16816_c(a, kv4_lop(lo, KV4_LO_MASK, 0x00080008u), kv4_lop(hi, KV4_LO_MASK, 0x00080008u), kv4_lop(lo8, KV4_LO_MASK, 0x00080008u),
+                        kv4_lop(hi8, KV4_LO_MASK, 0x00080008u), f.b[g][0], f.b[g][2], f.start[g]);
+            mma_16816_c(a, kv4_lop(lo, KV4_HI_MASK, 0x00800080u), kv4_lop(hi, KV4_HI_MASK, 0x00800080u), kv4_lop(lo8, KV4_HI_MASK, 0x00800080u),
+                        kv4_lop(hi8, KV4_HI_MASK, 0x00800080u), f.b[g][1], f.b[g][3], a);
             const float x0 = h ? ks0.y : ks0.x, x1 = h ? ks1.y : ks1.x;
             if (g == 0) {
                 s[0] = a[0] * x0;
@@ -170,8 +188,8 @@ __device__ __forceinline__ void kv4_tile_values(uint32_t vaddr, uint32_t p0, uin
             kv4_widen(x[2 * h], lo);
             kv4_widen(x[2 * h + 1], hi);
             const uint32_t b0 = h2_mul(p0, v[g]), b1 = h2_mul(p1, v[4 + g]);
-            mma_16816(O[2 * g], lo[0], lo[1], hi[0], hi[1], b0, b1);
-            mma_16816(O[2 * g + 1], lo[2], lo[3], hi[2], hi[3], b0, b1);
+            mma_16816_c(O[2 * g], lo[0], lo[1], hi[0], hi[1], b0, b1, O[2 * g]);
+            mma_16816_c(O[2 * g + 1], lo[2], lo[3], hi[2], hi[3], b0, b1, O[2 * g + 1]);
         }
     }
 }
