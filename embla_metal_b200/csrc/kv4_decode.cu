@@ -26,6 +26,7 @@ __device__ __forceinline__ int here(int x) {
 __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
 constexpr int KD_PART = HD + 4;                                    // floats per (range, head): 128 sums, sum of weights
+constexpr int KD_SUM = HD + 1;   // a row of a warp's sums in shared memory: lanes (r, t) write heads 2t at dims 8 (r / 2) + r % 2: 32 banks
 constexpr float KD_LIMIT = 8192.0f, KD_LIMIT_BIG = 0.5f;           // largest weight kept, usually and with large value scales
 constexpr int KD_TARGET = 10, KD_TARGET_BIG = -4;                  // log2 of the bound a new f puts on the tile's weights
 constexpr int KD_MAX_CLUSTER = 8;
@@ -56,20 +57,25 @@ struct Kv4DecodeParams {
 constexpr size_t kd_queries_at(int stages) { return size_t(stages) * KV4_PAGE; }
 constexpr size_t kd_bars_at(int stages) { return kd_queries_at(stages) + sizeof(Kv4Queries); }
 constexpr size_t kd_sums_at(int stages) { return (kd_bars_at(stages) + size_t(stages) * 20 + 15) / 16 * 16; }
-constexpr size_t kd_smem(int ncons, int stages) { return 1024 + kd_sums_at(stages) + size_t(ncons) * 8 * KD_PART * 4; }
+constexpr size_t kd_smem(int ncons, int stages) { return 1024 + kd_sums_at(stages) + size_t(ncons) * 8 * KD_SUM * 4; }
 constexpr size_t kd_inbox_rows(int ranges, int G) { return size_t(ranges) * ((G + ranges - 1) / ranges); }
 
 __device__ __forceinline__ int kd_pages(const int32_t* seq_lens, int b) { return max(0, (__ldg(seq_lens + b) + BLK - 1) / BLK); }
 
-// The pages of all units, laid end to end, cut into equal runs (of KD_MIN_RUN pages or more, so that fewer CTAs than launched may
-// have one).
+// The pages of all units, laid end to end, cut into `runs` runs whose lengths differ by one at most (and are KD_MIN_RUN or more,
+// so that fewer CTAs than launched may have one).
 struct KdRuns {
-    long total;
-    int runs;
-    KdRuns() = default;
-    __device__ __forceinline__ KdRuns(long pages, int most) : total(pages), runs(int(min(long(most), (pages + KD_MIN_RUN - 1) / KD_MIN_RUN))) {}
-    __device__ __forceinline__ long start_of(int c) const { return total * c / runs; }
-    __device__ __forceinline__ int run_of(long x) const { return int(((x + 1) * runs - 1) / total); }   // the run that page x is in
+    unsigned runs, len, longer;   // the first `longer` runs have len + 1 pages, the others len
+    __device__ __forceinline__ KdRuns(unsigned pages, unsigned most) {
+        runs = max(1u, min(most, (pages + KD_MIN_RUN - 1) / KD_MIN_RUN));
+        len = pages / runs;
+        longer = pages - len * runs;
+    }
+    __device__ __forceinline__ unsigned start_of(unsigned c) const { return c * len + min(c, longer); }
+    __device__ __forceinline__ unsigned run_of(unsigned x) const {   // the run that page x is in
+        const unsigned edge = longer * (len + 1);
+        return x < edge ? x / (len + 1) : longer + (x - edge) / max(len, 1u);
+    }
 };
 
 // A piece of work: pages [first, first + n) of a unit (sequence b, kv head kvh) that has `pages` of them.
@@ -97,33 +103,37 @@ struct KdWalk {
             length = left;
             return;
         }
-        int sum = 0;
-        for (int i = lane; i < p.batch; i += 32) sum += kd_pages(p.seq_lens, i);
-        sum = __reduce_add_sync(0xffffffffu, sum);
-        const KdRuns cut(long(sum) * p.n_kv_heads, p.n_runs);
-        const int c = blockIdx.x;
-        left = length = 0;
-        if (c >= cut.runs) return;
-        const long x0 = cut.start_of(c);
-        left = length = int(cut.start_of(c + 1) - x0);
-        // the sequence that page x0 falls in: the last one whose pages start at or before it (of those that have any)
-        int before = 0;
-        for (int i0 = 0; i0 < p.batch; i0 += 32) {
-            const int n = i0 + lane < p.batch ? kd_pages(p.seq_lens, i0 + lane) : 0;
+        // (up to 32 sequences, the usual case, take one load of their lengths)
+        auto scan = [&](int i0, int& n) {
+            n = i0 + lane < p.batch ? kd_pages(p.seq_lens, i0 + lane) : 0;
             int incl = n;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int v = __shfl_up_sync(0xffffffffu, incl, o);
                 if (lane >= o) incl += v;
             }
-            const unsigned here = __ballot_sync(0xffffffffu, long(before + incl) * p.n_kv_heads > x0);
+            return incl;
+        };
+        int n, incl = scan(0, n), sum = __shfl_sync(0xffffffffu, incl, 31);
+        for (int i = 32 + lane; i < (p.batch + 31) / 32 * 32; i += 32)
+            sum += __reduce_add_sync(0xffffffffu, i < p.batch ? kd_pages(p.seq_lens, i) : 0);
+        const KdRuns cut(unsigned(sum) * p.n_kv_heads, p.n_runs);
+        const unsigned c = blockIdx.x;
+        left = length = 0;
+        if (c >= cut.runs) return;
+        const unsigned x0 = cut.start_of(c);
+        left = length = int(cut.start_of(c + 1) - x0);
+        // the sequence that page x0 falls in: the first one whose pages end behind it
+        for (int i0 = 0, before = 0; i0 < p.batch; i0 += 32) {
+            if (i0 > 0) incl = scan(i0, n);
+            const unsigned here = __ballot_sync(0xffffffffu, unsigned(before + incl) * p.n_kv_heads > x0);
             if (here) {
                 const int l = __ffs(here) - 1;
                 at.b = i0 + l;
                 at.pages = __shfl_sync(0xffffffffu, n, l);
-                const int in = int(x0 - long(before + __shfl_sync(0xffffffffu, incl, l) - at.pages) * p.n_kv_heads);
-                at.kvh = in / at.pages;
-                at.first = in % at.pages;
+                const unsigned in = x0 - unsigned(before + __shfl_sync(0xffffffffu, incl, l) - at.pages) * p.n_kv_heads;
+                at.kvh = int(in / unsigned(at.pages));
+                at.first = int(in - unsigned(at.kvh) * unsigned(at.pages));
                 return;
             }
             before += __shfl_sync(0xffffffffu, incl, 31);
@@ -146,13 +156,18 @@ struct KdWalk {
     }
 };
 
-// NCONS consumer warps share the 8 tiles of every page, the last warp is the producer. CL: the key ranges of a unit are the
-// CTAs of one thread-block cluster, and each finishes the heads it owns (head h: CTA h % ranges) from its shared memory.
-template <int DT, bool SCORES, int NCONS, int STAGES, int MINB, bool CL>
-__global__ void __launch_bounds__((NCONS + 1) * 32, MINB)
+// NCONS consumer warps, the last warp is the producer. WPG warps share the 8 tiles of a page; the NCONS / WPG groups of them take
+// the pages in turn, so that no group gets far ahead of another (three CTAs an SM with a run each did: the warps of the
+// one that the schedulers favoured were done after 0.8 of the time, and the others were left with too few warps for the SM).
+// CL: the key ranges of a unit are the CTAs of one thread-block cluster, and each finishes the heads it owns (head h: CTA h %
+// ranges) from its shared memory.
+template <int DT, bool SCORES, int NCONS, int WPG, int STAGES, bool CL>
+__global__ void __launch_bounds__((NCONS + 1) * 32, 1)
     kv4_decode_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ Kv4DecodeParams p) {
-    constexpr int TILES = 8 / NCONS;   // 16-key tiles of a page a consumer warp takes
-    constexpr int CT = NCONS * 32;     // consumer threads
+    constexpr int TILES = 8 / WPG;          // 16-key tiles of a page a consumer warp takes
+    constexpr int GROUPS = NCONS / WPG;
+    constexpr int CT = NCONS * 32;          // consumer threads
+    static_assert(STAGES >= GROUPS, "a group's stage index advances by GROUPS a page");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* stages = smem;
@@ -160,7 +175,7 @@ __global__ void __launch_bounds__((NCONS + 1) * 32, MINB)
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + kd_bars_at(STAGES));
     uint64_t* empty = full + STAGES;
     volatile int* limits = reinterpret_cast<volatile int*>(empty + STAGES);   // keys of the stage's page that count
-    float* sums = reinterpret_cast<float*>(smem + kd_sums_at(STAGES));        // [NCONS][8][KD_PART]
+    float* sums = reinterpret_cast<float*>(smem + kd_sums_at(STAGES));        // [NCONS][8][KD_SUM]
     __shared__ int s_failed, s_issued, s_more;
     __shared__ KdWalk<CL> s_walk;   // the consumers' walk (thread 0 moves it on); the producer has its own, some pages ahead
 
@@ -175,97 +190,103 @@ __global__ void __launch_bounds__((NCONS + 1) * 32, MINB)
     if (warp == 0 || warp == NCONS) walk.start(p, lane);
     if (tid == 0) s_walk = walk;
 
-    // ---- producer: lane 0 keeps the ring of stages full (a block outside the pool: no keys, and the error word set)
-    int issued = 0;
-    bool issuing = true;
-    auto issue = [&](int page, int block, int S) {
-        const int st = issued % STAGES, use = issued / STAGES;
-        if (issued == p.ctl.stall_at) return false;   // diagnostic stall: the consumers' wait for this page runs out
-        if (use > 0 && !mbar_wait_bounded(p.ctl.wait_cycles, &empty[st], (use - 1) & 1)) {
-            atomicExch(p.ctl.err, ERR_WAIT_EMPTY);
-            return false;
-        }
-        if (block < 0 || block >= p.num_blocks) {
-            atomicExch(p.ctl.err, ERR_BAD_BLOCK);
-            limits[st] = 0;
-            mbar_arrive(&full[st]);
-        } else {
-            const long pg = (long(block) * p.n_layers + p.layer) * p.n_kv_heads + walk.at.kvh;
-            uint8_t* dst = stages + st * KV4_PAGE;
-            limits[st] = min(BLK, S - page * BLK);
-            mbar_expect_tx(&full[st], KV4_PAGE);
-            tma_load_2d(dst, &tmap, 0, int(pg * (KV4_PAGE / 128)), &full[st]);
-            bulk_load_1d(dst + 2 * KV4_SIDE, p.pool + size_t(pg) * KV4_PAGE + 2 * KV4_SIDE, KV4_SCALES, &full[st]);
-        }
-        issued++;
-        *reinterpret_cast<volatile int*>(&s_issued) = issued;
-        return true;
-    };
-    // pages of the walk's pieces until `upto` have been requested or the run is done; block ids are looked up 32 at a time
-    int ahead = 0, blocks = -1, seq_len = 0;   // pages of the piece looked up and not yet requested .. (lane i: its i-th)
-    int done = 0;                              // pages of the piece requested
-    auto produce = [&](int upto) {
-        while (issuing && issued < upto) {
-            if (done == walk.at.n) {
-                if (!walk.next(p)) return;
-                done = 0;
-                seq_len = __ldg(p.seq_lens + walk.at.b);
-            }
-            if (done % 32 == 0) {
-                const int e = walk.at.first + done + lane;
-                blocks = done + lane < walk.at.n && e < p.table_stride ? p.block_table[size_t(walk.at.b) * p.table_stride + e] : -1;
-            }
-            ahead = __shfl_sync(0xffffffffu, blocks, done % 32);
-            bool ok = true;
-            if (lane == 0) ok = issue(walk.at.first + done, ahead, seq_len);
-            issuing = __shfl_sync(0xffffffffu, int(ok), 0) != 0;
-            issued = __shfl_sync(0xffffffffu, issued, 0);
-            done++;
-        }
-    };
     if (warp == NCONS) {
+        // ---- producer: keeps the ring of stages full. The lanes look up 32 pages' blocks and addresses at a time, then each requests
+        // its page when its turn comes (one lane that did it all took 1000 clocks a page, twice what the SM takes to attend one).
+        // A block outside the pool: no keys, and the error word set.
         if (lane == 0) {
             for (int s = 0; s < STAGES; s++) {
                 mbar_init(&full[s], 1);
-                mbar_init(&empty[s], NCONS);
+                mbar_init(&empty[s], WPG);
             }
             s_failed = 0;
-            s_issued = 0;
             fence_barrier_init();
         }
         __syncwarp();
-        produce(STAGES);   // (the stages start empty: no wait)
-    }
-    if (p.ctl.early) {
-        pdl_wait();
-        pdl_launch_dependents();
-    }
-    trace_first(p.ctl.trace, 1);
-    __syncthreads();
-
-    if (warp == NCONS) {
-        produce(0x7fffffff);
+        int count = 0, done = 0, S = 0;   // pages requested, of the run and of the piece; keys of the sequence
+        bool go = true, joined = false;
+        while (true) {
+            if (go && done == walk.at.n) {
+                go = walk.next(p);
+                done = 0;
+                S = go ? __ldg(p.seq_lens + walk.at.b) : 0;
+            }
+            if (!joined && (!go || count >= STAGES)) {
+                // the stages start empty: all of this ran without a wait, in an early launch ahead of the launch before it
+                if (p.ctl.early) {
+                    pdl_wait();
+                    pdl_launch_dependents();
+                }
+                __syncthreads();
+                joined = true;
+            }
+            if (!go) break;
+            const int m = min(min(32, walk.at.n - done), joined ? 32 : STAGES - count);
+            const int page = walk.at.first + done + lane, mine = count + lane, st = mine % STAGES;
+            const int block = lane < m && page < p.table_stride ? p.block_table[size_t(walk.at.b) * p.table_stride + page] : -1;
+            const bool there = block >= 0 && block < p.num_blocks;
+            const long pg = (long(block) * p.n_layers + p.layer) * p.n_kv_heads + walk.at.kvh;
+            const uint8_t* scales = p.pool + size_t(pg) * KV4_PAGE + 2 * KV4_SIDE;
+            uint8_t* dst = stages + st * KV4_PAGE;
+            for (int i = 0; i < m && go; i++) {
+                bool bad = false;
+                if (lane == i) {
+                    if (mine == p.ctl.stall_at) {   // diagnostic stall: the consumers' wait for this page runs out
+                        bad = true;
+                    } else if (mine >= STAGES && !mbar_wait_bounded(p.ctl.wait_cycles, &empty[st], (mine / STAGES - 1) & 1)) {
+                        atomicExch(p.ctl.err, ERR_WAIT_EMPTY);
+                        bad = true;
+                    } else if (there) {
+                        limits[st] = min(BLK, S - page * BLK);
+                        mbar_expect_tx(&full[st], KV4_PAGE);
+                        tma_load_2d(dst, &tmap, 0, int(pg * (KV4_PAGE / 128)), &full[st]);
+                        bulk_load_1d(dst + 2 * KV4_SIDE, scales, KV4_SCALES, &full[st]);
+                    } else {
+                        atomicExch(p.ctl.err, ERR_BAD_BLOCK);
+                        limits[st] = 0;
+                        mbar_arrive(&full[st]);
+                    }
+                }
+                go = !__any_sync(0xffffffffu, bad);
+                count += go ? 1 : 0;
+            }
+            done += m;
+        }
+        if (lane == 0) s_issued = count;
     } else {
+        if (p.ctl.early) {
+            pdl_wait();
+            pdl_launch_dependents();
+        }
+        trace_first(p.ctl.trace, 1);
         // ---- consumers
         const int r = lane >> 2, t = lane & 3;
         const uint32_t base = smem_u32(stages) + kv4_lane_at(lane);
         const float sink = sqrtf(float(HD));
-        int st = 0, phase = 0;
+        const int group = warp / WPG, wg = warp % WPG;
+        int st = group, phase = 0;                                  // stage and phase of the group's next page,
+        int mine = group, piece0 = 0;                               // its number in the run, and of the piece's first page
         bool ok = true;                                             // (the warp's: no wait of it has run out)
+        bool begun = false;
         for (int c = blockIdx.x; !CL && c < p.batch; c += gridDim.x)   // sequences without keys have no unit in any run
             if (__ldg(p.seq_lens + c) <= 0)
                 for (int i = tid; i < p.n_kv_heads * p.G * HD; i += CT) Act<DT>::store(p.o, size_t(c) * p.o_stride + i, 0.0f);
         while (true) {
             if (tid == 0) s_more = s_walk.next(p);
             bar_sync(1, CT);
-            if (!CL && !s_more) break;
+            if (!CL && !s_more) {
+                if (!begun) __syncthreads();
+                break;
+            }
             const KdPiece& pc = s_walk.at;                          // (CL: a range without pages is walked through all the same)
             const int unit = pc.b * p.n_kv_heads + pc.kvh, n = s_more ? pc.n : 0;
             const int lane_q = here(lane);
             for (int hh = here(warp); hh < 8; hh += NCONS)
                 kv4_stage_query<DT>(sq, hh, hh < p.G, p.q, size_t(pc.b) * p.q_stride + size_t(pc.kvh * p.G + hh) * HD, p.prenormed != 0, p.g1, p.g2,
                                     p.ng, lane_q);
-            bar_sync(1, CT);
+            if (begun) bar_sync(1, CT);
+            else __syncthreads();                                   // (with the producer, which has set the barriers up meanwhile)
+            begun = true;
             Kv4Frag frag;
             frag.load(sq, lane_q);
             // scores: S x the query's power of two; a head that is not there never is the largest
@@ -284,7 +305,7 @@ __global__ void __launch_bounds__((NCONS + 1) * 32, MINB)
             float f0 = pow2_biased(247), f1 = pow2_biased(247);     // their factors (2^120: nothing seen yet)
             bool big = false;
             float limit = KD_LIMIT;
-            for (int i = 0; i < n && ok; i++) {
+            for (; mine < piece0 + n && ok; mine += GROUPS) {
                 // (the decision is the warp's: a warp that leaves the loop leaves it whole)
                 ok = __all_sync(0xffffffffu, mbar_wait_bounded(p.ctl.wait_cycles, &full[st], phase));
                 if (!ok) {
@@ -292,11 +313,11 @@ __global__ void __launch_bounds__((NCONS + 1) * 32, MINB)
                     *reinterpret_cast<volatile int*>(&s_failed) = 1;
                     break;
                 }
-                const int page = pc.first + i;
+                const int page = pc.first + mine - piece0;
                 // the warp's tiles of the page together: their products have nothing to wait for in one another
-                const uint32_t kaddr = base + st * KV4_PAGE + warp * (TILES * 16 * KV4_ROW);
-                const uint8_t* sc = stages + st * KV4_PAGE + 2 * KV4_SIDE + warp * (TILES * 16 * 16);
-                const int left = limits[st] - warp * (TILES * 16);   // keys of the tiles that count, if fewer than there are
+                const uint32_t kaddr = base + st * KV4_PAGE + wg * (TILES * 16 * KV4_ROW);
+                const uint8_t* sc = stages + st * KV4_PAGE + 2 * KV4_SIDE + wg * (TILES * 16 * 16);
+                const int left = limits[st] - wg * (TILES * 16);   // keys of the tiles that count, if fewer than there are
                 if (left > 0) {
                     float s[TILES][4];
                     uint32_t vs[TILES][8];
@@ -316,7 +337,7 @@ __global__ void __launch_bounds__((NCONS + 1) * 32, MINB)
                             m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 2));
                             const int key = k * 16 + r + 8 * t;
                             if (t < 2 && key < left)
-                                p.scores[size_t(unit) * p.scores_stride + page * BLK + warp * (TILES * 16) + key] = t ? m1 : m0;
+                                p.scores[size_t(unit) * p.scores_stride + page * BLK + wg * (TILES * 16) + key] = t ? m1 : m0;
                         }
                     }
                     if (left < TILES * 16) {
@@ -388,11 +409,13 @@ __global__ void __launch_bounds__((NCONS + 1) * 32, MINB)
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&empty[st]);
-                if (++st == STAGES) {
-                    st = 0;
+                st += GROUPS;
+                if (st >= STAGES) {
+                    st -= STAGES;
                     phase ^= 1;
                 }
             }
+            piece0 += n;
             // ---- the warps' sums of the piece into one, in units of the weights themselves
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) {
@@ -403,19 +426,21 @@ __global__ void __launch_bounds__((NCONS + 1) * 32, MINB)
             const int lane_s = here(lane), rs = lane_s >> 2, ts = lane_s & 3, tid_s = here(tid);
             const float q0 = pow2_biased(max(sq.expo[2 * ts], 1)), q1 = pow2_biased(max(sq.expo[2 * ts + 1], 1));
             const float i0 = (1.0f / 128.0f / KV4_SUBNORMAL / KV4_SUBNORMAL) / f0, i1 = (1.0f / 128.0f / KV4_SUBNORMAL / KV4_SUBNORMAL) / f1;
-            float* mine0 = sums + (warp * 8 + 2 * ts) * KD_PART;
-            float* mine1 = mine0 + KD_PART;
+            float* row0 = sums + (warp * 8 + 2 * ts) * KD_SUM;
+            float* row1 = row0 + KD_SUM;
+            if (2 * ts < p.G) {
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const int d = kv4_dim_of(k, rs);
-                mine0[d] = O[k][0] * i0 * q0 * q0;
-                mine1[d] = O[k][1] * i1 * q1 * q1;
-                mine0[d + 2] = O[k][2] * i0 * q0 * q0;
-                mine1[d + 2] = O[k][3] * i1 * q1 * q1;
-            }
-            if (rs == 0) {
-                mine0[HD] = ps0 * i0 * q0 * q0;
-                mine1[HD] = ps1 * i1 * q1 * q1;
+                for (int k = 0; k < 8; k++) {
+                    const int d = kv4_dim_of(k, rs);
+                    row0[d] = O[k][0] * i0 * q0 * q0;
+                    row1[d] = O[k][1] * i1 * q1 * q1;
+                    row0[d + 2] = O[k][2] * i0 * q0 * q0;
+                    row1[d + 2] = O[k][3] * i1 * q1 * q1;
+                }
+                if (rs == 0) {
+                    row0[HD] = ps0 * i0 * q0 * q0;
+                    row1[HD] = ps1 * i1 * q1 * q1;
+                }
             }
             bar_sync(1, CT);
             if (CL) break;   // (the cluster's CTAs meet below, all warps)
@@ -428,8 +453,8 @@ __global__ void __launch_bounds__((NCONS + 1) * 32, MINB)
                 float num = 0.0f, den = 0.0f;
 #pragma unroll
                 for (int w = 0; w < NCONS; w++) {
-                    num += sums[(w * 8 + hh) * KD_PART + d];
-                    den += sums[(w * 8 + hh) * KD_PART + HD];
+                    num += sums[(w * 8 + hh) * KD_SUM + d];
+                    den += sums[(w * 8 + hh) * KD_SUM + HD];
                 }
                 if (whole) Act<DT>::store(p.o, size_t(pc.b) * p.o_stride + size_t(pc.kvh * p.G + hh) * HD + d, num / (sink + den));
                 else {
@@ -454,7 +479,7 @@ __global__ void __launch_bounds__((NCONS + 1) * 32, MINB)
         constexpr int THREADS = (NCONS + 1) * 32;
         const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
         const float sink = sqrtf(float(HD));
-        float* inbox = sums + NCONS * 8 * KD_PART;
+        float* inbox = sums + NCONS * 8 * KD_SUM;
         const int slots = (p.G + p.nsplit - 1) / p.nsplit;
         cluster_wait();
         for (int idx = tid; idx < p.G * HD; idx += THREADS) {
@@ -462,8 +487,8 @@ __global__ void __launch_bounds__((NCONS + 1) * 32, MINB)
             float num = 0.0f, den = 0.0f;
 #pragma unroll
             for (int w = 0; w < NCONS; w++) {
-                num += sums[(w * 8 + hh) * KD_PART + d];
-                den += sums[(w * 8 + hh) * KD_PART + HD];
+                num += sums[(w * 8 + hh) * KD_SUM + d];
+                den += sums[(w * 8 + hh) * KD_SUM + HD];
             }
             const uint32_t row = cluster_map(smem_u32(inbox + (split * slots + hh / p.nsplit) * KD_PART), uint32_t(hh % p.nsplit));
             cluster_st_f32(row + uint32_t(d) * 4u, num);
@@ -503,17 +528,17 @@ __global__ void __launch_bounds__(256) kv4_decode_join_kernel(const __grid_const
     sum = __reduce_add_sync(0xffffffffu, sum);
     before = __reduce_add_sync(0xffffffffu, before);
     const int pages = kd_pages(p.seq_lens, b);
-    const KdRuns runs(long(sum) * p.n_kv_heads, p.n_runs);
-    const long x = long(before) * p.n_kv_heads + long(kvh) * pages;
+    const KdRuns runs(unsigned(sum) * p.n_kv_heads, p.n_runs);
+    const unsigned x = unsigned(before) * p.n_kv_heads + unsigned(kvh) * unsigned(pages);
+    const int lo = int(runs.run_of(x)), hi = int(runs.run_of(x + pages - 1));
+    const int first_slot = runs.start_of(lo) == x ? 2 * lo : 2 * lo + 1;   // (the unit may begin inside run lo)
     // (every CTA waits, one with nothing to add too: the launch behind this one takes its end for the end of the runs)
     pdl_wait();
     pdl_launch_dependents();
     trace_first(p.ctl.trace, 1);
     if (pages == 0) return;
-    const int lo = runs.run_of(x), hi = runs.run_of(x + pages - 1);
     const int hh = tid >> 5;
     if (lo == hi || hh >= p.G) return;
-    const int first_slot = runs.start_of(lo) == x ? 2 * lo : 2 * lo + 1;   // (the unit may begin inside run lo)
     float4 num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float den = sqrtf(float(HD));
     for (int k = lo; k <= hi; k += 8) {   // eight pieces' loads in flight together
@@ -543,7 +568,16 @@ __global__ void __launch_bounds__(256) kv4_decode_join_kernel(const __grid_const
     trace_last(p.ctl.trace, 3);
 }
 
-constexpr int KD_NCONS = 4, KD_STAGES = 3, KD_MINB = 3;
+#ifndef KDN
+#define KDN 12
+#define KDW 4
+#define KDS 9
+#endif
+// A CTA an SM: 12 consumer warps (at 128 registers the SM holds no more), four to a page, ten pages in flight. A cluster's CTA:
+// one tile a warp, so that a page or two are done soonest.
+template <bool CL> struct KdShape {
+    static constexpr int ncons = CL ? 8 : KDN, wpg = CL ? 8 : KDW, stages = CL ? 4 : KDS;
+};
 
 static bool use_pdl() {
     static const bool on = []() { const char* e = getenv("EMBLA_NO_PDL"); return !(e && e[0] == '1'); }();
@@ -552,16 +586,17 @@ static bool use_pdl() {
 
 template <int DT, bool SCORES, bool CL>
 static EmblaStatus launch_kv4_decode(EmblaAttn* ctx, const EmblaKVPool* pool, const Kv4DecodeParams& p, int batch, dim3 grid, cudaStream_t s) {
-    auto kern = kv4_decode_kernel<DT, SCORES, KD_NCONS, KD_STAGES, KD_MINB, CL>;
-    const size_t smem = kd_smem(KD_NCONS, KD_STAGES) + (CL ? kd_inbox_rows(p.nsplit, p.G) * KD_PART * 4 : 0);
+    using Shape = KdShape<CL>;
+    auto kern = kv4_decode_kernel<DT, SCORES, Shape::ncons, Shape::wpg, Shape::stages, CL>;
+    constexpr size_t fixed = kd_smem(Shape::ncons, Shape::stages);
+    const size_t smem = fixed + (CL ? kd_inbox_rows(p.nsplit, p.G) * KD_PART * 4 : 0);
     static bool configured[64] = {};   // per instantiation and device
     if (!configured[ctx->device & 63]) {
         // (the largest inbox: 7 ranges of 8 heads, two each)
-        EMBLA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                            int(kd_smem(KD_NCONS, KD_STAGES) + (CL ? 14 * KD_PART * 4 : 0))));
+        EMBLA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(fixed + (CL ? 14 * KD_PART * 4 : 0))));
         configured[ctx->device & 63] = true;
     }
-    EMBLA_CUDA_TRY(launch_kernel_cluster(ctx->pdl, CL ? p.nsplit : 1, kern, grid, dim3((KD_NCONS + 1) * 32), smem, s, pool->tmap_codes, p));
+    EMBLA_CUDA_TRY(launch_kernel_cluster(ctx->pdl, CL ? p.nsplit : 1, kern, grid, dim3((Shape::ncons + 1) * 32), smem, s, pool->tmap_codes, p));
     if (!CL && p.n_runs > 1) {
         Kv4DecodeParams pj = p;
         pj.ctl = kernel_ctl(ctx);
@@ -597,6 +632,8 @@ EmblaStatus kv4_full_decode(EmblaAttn* ctx, const EmblaKVPool* pool, const Embla
     p.prenormed = q->prenormed;
     p.ng = q->ng;
     const long units = long(view->batch) * pool->n_kv_heads, pages = (max_len + BLK - 1) / BLK;
+    if (units * pages > 0x7fffffffL)
+        EMBLA_FAIL(EMBLA_BAD_ARG, "embla_attn_full_decode: %d sequences of up to %d keys are too many pages", view->batch, max_len);
     // Few pages: a cluster a unit, one page or a few a CTA. Else equal runs over the resident CTAs (the scratch holds two
     // pieces a run: embla_attn_create makes it 8 slots an SM and more).
     const bool cluster = units * pages <= KD_CLUSTER_PAGES && units <= 0xffff;
@@ -605,7 +642,7 @@ EmblaStatus kv4_full_decode(EmblaAttn* ctx, const EmblaKVPool* pool, const Embla
         p.nsplit = int(pages < KD_MAX_CLUSTER ? pages : KD_MAX_CLUSTER);
         grid = dim3(p.nsplit, pool->n_kv_heads, view->batch);
     } else {
-        const long most = (units * pages + KD_MIN_RUN - 1) / KD_MIN_RUN, slots = long(KD_MINB) * ctx->sm_count;
+        const long most = (units * pages + KD_MIN_RUN - 1) / KD_MIN_RUN, slots = ctx->sm_count;
         p.n_runs = int(most < slots ? most : slots);
         grid = dim3(p.n_runs);
     }

@@ -52,9 +52,12 @@ __device__ __forceinline__ void mma_16816_c(float (&d)[4], uint32_t a0, uint32_t
 // fp16 then holds bf16 queries of any size), and what goes with them.
 struct Kv4Queries {
     __half q[8][HD];
-    float start[8][KV4_GROUPS];   // -8 x the sum of the scaled query over the group, x 2^-20
     int expo[8];                  // biased exponent of the power of two; 0: no such head
 };
+
+// Dims in the order of the B registers: of every 8, those in low nibbles (0, 1, 4, 5), then those in high ones (2, 3, 6, 7), so that
+// the two registers of a product come out of one load side by side.
+__device__ __forceinline__ int kv4_q_column(int d) { return (d & ~6) | ((d & 4) >> 1) | ((d & 2) << 1); }
 
 // One warp, one head: loads the row (or zeros for a head the kv head does not have), head norm if asked, scales, stores.
 template <int DT>
@@ -76,16 +79,13 @@ __device__ __forceinline__ void kv4_stage_query(Kv4Queries& sq, int hh, bool has
     for (int i = 0; i < 4; i++) {
         const __half h = __float2half_rn(x[i] * down);
         // dims 0, 1, 4, 5 of every 8 lie in low nibbles: 16 x (exact)
-        sq.q[hh][lane + 32 * i] = (lane & 2) ? h : __hmul(h, __float2half_rn(16.0f));
-        float sum = __half2float(h);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) sq.start[hh][i] = -8.0f * KV4_SUBNORMAL * sum;
+        sq.q[hh][kv4_q_column(lane) + 32 * i] = (lane & 2) ? h : __hmul(h, __float2half_rn(16.0f));
     }
     if (lane == 0) sq.expo[hh] = has ? e : 0;
 }
 
-// A lane's share of the queries: B registers of head r = lane / 4, start values of heads 2t, 2t + 1 (t = lane % 4).
+// A lane's share of the queries: B registers of head r = lane / 4, the products' start values of heads
+// 2t, 2t + 1 (t = lane % 4).
 struct Kv4Frag {
     uint32_t b[KV4_GROUPS][4];
     float start[KV4_GROUPS][4];
@@ -98,10 +98,10 @@ struct Kv4Frag {
             b[g][1] = v.y;
             b[g][2] = v.z;
             b[g][3] = v.w;
-            // (twice over, through volatile loads: four registers in a row, as the products take them, and no copies)
-            volatile const float(*from)[KV4_GROUPS] = sq.start;
-#pragma unroll
-            for (int e = 0; e < 4; e++) start[g][e] = from[2 * t + (e & 1)][g];
+            // -8 x the sum over the group, in the products' own way: rows of -8 2^-24 and -8 2^-20
+            const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            mma_16816_c(start[g], 0x80088008u, 0x80088008u, 0x80088008u, 0x80088008u, b[g][0], b[g][1], zero);
+            mma_16816_c(start[g], 0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u, b[g][2], b[g][3], start[g]);
         }
     }
 };
@@ -128,9 +128,9 @@ __device__ __forceinline__ void kv4_tile_scores(uint32_t kaddr, const uint8_t* s
             float a[4];
             // dims 0, 1 and 4, 5 of the lane's eight, then 2, 3 and 6, 7
             mma_16816_c(a, kv4_lop(lo, KV4_LO_MASK, 0x00080008u), kv4_lop(hi, KV4_LO_MASK, 0x00080008u), kv4_lop(lo8, KV4_LO_MASK, 0x00080008u),
-                        kv4_lop(hi8, KV4_LO_MASK, 0x00080008u), f.b[g][0], f.b[g][2], f.start[g]);
+                        kv4_lop(hi8, KV4_LO_MASK, 0x00080008u), f.b[g][0], f.b[g][1], f.start[g]);
             mma_16816_c(a, kv4_lop(lo, KV4_HI_MASK, 0x00800080u), kv4_lop(hi, KV4_HI_MASK, 0x00800080u), kv4_lop(lo8, KV4_HI_MASK, 0x00800080u),
-                        kv4_lop(hi8, KV4_HI_MASK, 0x00800080u), f.b[g][1], f.b[g][3], a);
+                        kv4_lop(hi8, KV4_HI_MASK, 0x00800080u), f.b[g][2], f.b[g][3], a);
             const float x0 = h ? ks0.y : ks0.x, x1 = h ? ks1.y : ks1.x;
             if (g == 0) {
                 s[0] = a[0] * x0;
