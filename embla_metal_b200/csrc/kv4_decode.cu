@@ -320,12 +320,12 @@ __global__ void __launch_bounds__((NCONS + 1) * 32, 1)
                 const int left = limits[st] - wg * (TILES * 16);   // keys of the tiles that count, if fewer than there are
                 if (left > 0) {
                     float s[TILES][4];
-                    uint32_t vs[TILES][8];
+                    Kv4Scales rows[TILES];
                     bool flagged = false;
 #pragma unroll
                     for (int k = 0; k < TILES; k++) {
-                        kv4_tile_scores(kaddr + k * 16 * KV4_ROW, sc + k * 256, lane, frag, s[k]);
-                        kv4_value_scales(sc + k * 256, lane, vs[k]);
+                        rows[k].load(sc + k * 256, lane);
+                        kv4_tile_scores(kaddr + k * 16 * KV4_ROW, rows[k], frag, s[k]);
                     }
                     if (SCORES) {
 #pragma unroll
@@ -345,13 +345,13 @@ __global__ void __launch_bounds__((NCONS + 1) * 32, 1)
                         for (int k = 0; k < TILES; k++) {
                             if (k * 16 + r >= left) s[k][0] = s[k][1] = 0.0f;
                             if (k * 16 + r + 8 >= left) s[k][2] = s[k][3] = 0.0f;
-                            kv4_mask_value_scales(vs[k], lane, left - k * 16);
+                            rows[k].mask(lane, left - k * 16);
                         }
                     }
                     float w[TILES][4], top = 0.0f;
 #pragma unroll
                     for (int k = 0; k < TILES; k++) {
-                        flagged |= kv4_scales_large(vs[k]);
+                        flagged |= rows[k].large();
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             s[k][e] = fmaxf(s[k][e], 0.0f);
@@ -402,9 +402,7 @@ __global__ void __launch_bounds__((NCONS + 1) * 32, 1)
                     for (int k = 0; k < TILES; k++) {
                         ps0 += w[k][0] + w[k][2];
                         ps1 += w[k][1] + w[k][3];
-                        // the weights as fp16 (2^-11), keys across the lanes: the B registers of the sum
-                        kv4_tile_values(kaddr + KV4_SIDE + k * 16 * KV4_ROW, movmatrix4_trans(pack_h2(w[k][0], w[k][1])),
-                                        movmatrix4_trans(pack_h2(w[k][2], w[k][3])), vs[k], O);
+                        kv4_tile_values(kaddr + KV4_SIDE + k * 16 * KV4_ROW, rows[k], w[k], O);
                     }
                 }
                 __syncwarp();

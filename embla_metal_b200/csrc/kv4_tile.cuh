@@ -12,7 +12,9 @@
 //                 is the accumulator's start value, negated.
 //   O^T = V^T P^T A = 16 dims x 16 keys. The transposing ldmatrix, on 16-bit elements of four codes, hands lane (r, t) the
 //                 element r of keys 2t and 2t + 1 side by side: widened, its nibbles are A registers (a dim, two keys). The
-//                 value's scale of the group is multiplied into P (fp16, one more rounding of 2^-11), the codes stay exact.
+//                 value's scale of the group is multiplied into P (a B register a group), the codes stay exact. (As subnormals
+//                 the codes would save the subtraction here too, but the tensor pipe adds products below the largest by their
+//                 exponents, a subnormal's as if it were 2^-14: ten bits of the sums of values were lost.)
 #pragma once
 
 #include "kv4.cuh"
@@ -32,7 +34,7 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr)
 }
 __device__ __forceinline__ uint32_t movmatrix4_trans(uint32_t x) {
     uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
     return r;
 }
 // 2^(e - 127) for a biased exponent 1 .. 254
@@ -109,17 +111,31 @@ struct Kv4Frag {
 // This lane's ldmatrix address in a tile whose row 0 is a multiple of 16 rows into the side: groups 0 and 1; ^ 32 for 2 and 3.
 __device__ __forceinline__ int kv4_lane_at(int lane) { return kv4_at((((lane >> 3) & 1) << 3) | (lane & 7), lane >> 4); }
 
+// The scale rows of a lane's keys r and r + 8 of a tile (`sc`: its rows [16][8]): K groups in x, y, V groups in z, w.
+struct Kv4Scales {
+    uint4 k0, k1;
+    __device__ __forceinline__ void load(const uint8_t* sc, int lane) {
+        k0 = *reinterpret_cast<const uint4*>(sc + (lane >> 2) * 16);
+        k1 = *reinterpret_cast<const uint4*>(sc + ((lane >> 2) + 8) * 16);
+    }
+    // some value scale of 2 or more (its product with a weight of 2^13 could leave fp16)
+    __device__ __forceinline__ bool large() const { return ((k0.z | k0.w | k1.z | k1.w) & 0x40004000u) != 0; }
+    // keys of the tile from `lim` on: their value scales may be anything, NaN included, and become zero
+    __device__ __forceinline__ void mask(int lane, int lim) {
+        if ((lane >> 2) >= lim) k0.z = k0.w = 0;
+        if ((lane >> 2) + 8 >= lim) k1.z = k1.w = 0;
+    }
+};
+
 // S of 16 keys: s[0], s[1] key r, heads 2t, 2t + 1; s[2], s[3] key r + 8. `kaddr`: shared address of the tile's key rows plus
-// kv4_lane_at; `sc`: the tile's scale rows [16][8].
-__device__ __forceinline__ void kv4_tile_scores(uint32_t kaddr, const uint8_t* sc, int lane, const Kv4Frag& f, float (&s)[4]) {
-    const int r = lane >> 2;
-    const uint2 k0 = *reinterpret_cast<const uint2*>(sc + r * 16), k1 = *reinterpret_cast<const uint2*>(sc + (r + 8) * 16);
+// kv4_lane_at.
+__device__ __forceinline__ void kv4_tile_scores(uint32_t kaddr, const Kv4Scales& sc, const Kv4Frag& f, float (&s)[4]) {
 #pragma unroll
     for (int j = 0; j < 2; j++) {
         uint32_t w[4];
         ldmatrix4(w, kaddr ^ (j * 32));
-        const float2 ks0 = __half22float2(*reinterpret_cast<const __half2*>(j ? &k0.y : &k0.x));
-        const float2 ks1 = __half22float2(*reinterpret_cast<const __half2*>(j ? &k1.y : &k1.x));
+        const float2 ks0 = __half22float2(*reinterpret_cast<const __half2*>(j ? &sc.k0.y : &sc.k0.x));
+        const float2 ks1 = __half22float2(*reinterpret_cast<const __half2*>(j ? &sc.k1.y : &sc.k1.x));
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const int g = 2 * j + h;
@@ -147,47 +163,25 @@ __device__ __forceinline__ void kv4_tile_scores(uint32_t kaddr, const uint8_t* s
     }
 }
 
-// The value scales of a lane's keys 2t, 2t + 1, 2t + 8, 2t + 9 as pairs by group: v[g] (keys 2t, 2t + 1), v[4 + g] (2t + 8, 2t + 9).
-__device__ __forceinline__ void kv4_value_scales(const uint8_t* sc, int lane, uint32_t (&v)[8]) {
-    const int t = lane & 3;
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        const uint2 a = *reinterpret_cast<const uint2*>(sc + (2 * t + 8 * h) * 16 + 8), b = *reinterpret_cast<const uint2*>(sc + (2 * t + 8 * h + 1) * 16 + 8);
-        v[4 * h + 0] = __byte_perm(a.x, b.x, 0x5410);
-        v[4 * h + 1] = __byte_perm(a.x, b.x, 0x7632);
-        v[4 * h + 2] = __byte_perm(a.y, b.y, 0x5410);
-        v[4 * h + 3] = __byte_perm(a.y, b.y, 0x7632);
-    }
-}
-// Some value scale of 2 or more among them (their product with a weight of 2^13 could leave fp16).
-__device__ __forceinline__ bool kv4_scales_large(const uint32_t (&v)[8]) {
-    return (((v[0] | v[1] | v[2]) | (v[3] | v[4] | v[5]) | (v[6] | v[7])) & 0x40004000u) != 0;
-}
-// Zeroes the scales of keys from `lim` (of the tile's 16) on: what lies there may be anything, NaN included.
-__device__ __forceinline__ void kv4_mask_value_scales(uint32_t (&v)[8], int lane, int lim) {
-    const int t = lane & 3;
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        const uint32_t m = (2 * t + 8 * h < lim ? 0xffffu : 0u) | (2 * t + 8 * h + 1 < lim ? 0xffff0000u : 0u);
-#pragma unroll
-        for (int g = 0; g < 4; g++) v[4 * h + g] &= m;
-    }
-}
-
-// O^T += V^T P^T for the tile: p0, p1 = the weights of head r for keys 2t, 2t + 1 and 2t + 8, 2t + 9. Accumulator tile 2g + p
-// holds, in [0], [1], dim 32 g + 8 (r / 2) + (r % 2) + 4 p of heads 2t, 2t + 1, in [2], [3] that dim + 2.
-__device__ __forceinline__ void kv4_tile_values(uint32_t vaddr, uint32_t p0, uint32_t p1, const uint32_t (&v)[8], float (&O)[8][4]) {
+// O^T += V^T P^T for the tile: w[0], w[1] the weights of key r for heads 2t, 2t + 1, w[2], w[3] of key r + 8. A weight times
+// the value's scale is rounded once, to fp16 (2^-11, fp32 before); an 8 x 8 transpose makes it the B register of head r, keys 2t,
+// 2t + 1. Accumulator tile 2g + p holds, in [0], [1], dim 32 g + 8 (r / 2) + (r % 2) + 4 p of heads 2t, 2t + 1, in [2], [3]
+// that dim + 2.
+__device__ __forceinline__ void kv4_tile_values(uint32_t vaddr, const Kv4Scales& sc, const float (&w)[4], float (&O)[8][4]) {
 #pragma unroll
     for (int j = 0; j < 2; j++) {
         uint32_t x[4];
         ldmatrix4_trans(x, vaddr ^ (j * 32));
+        const float2 v0 = __half22float2(*reinterpret_cast<const __half2*>(j ? &sc.k0.w : &sc.k0.z));
+        const float2 v1 = __half22float2(*reinterpret_cast<const __half2*>(j ? &sc.k1.w : &sc.k1.z));
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const int g = 2 * j + h;
+            const float x0 = h ? v0.y : v0.x, x1 = h ? v1.y : v1.x;
+            const uint32_t b0 = movmatrix4_trans(pack_h2(w[0] * x0, w[1] * x0)), b1 = movmatrix4_trans(pack_h2(w[2] * x1, w[3] * x1));
             uint32_t lo[4], hi[4];
             kv4_widen(x[2 * h], lo);
             kv4_widen(x[2 * h + 1], hi);
-            const uint32_t b0 = h2_mul(p0, v[g]), b1 = h2_mul(p1, v[4 + g]);
             mma_16816_c(O[2 * g], lo[0], lo[1], hi[0], hi[1], b0, b1, O[2 * g]);
             mma_16816_c(O[2 * g + 1], lo[2], lo[3], hi[2], hi[3], b0, b1, O[2 * g + 1]);
         }
