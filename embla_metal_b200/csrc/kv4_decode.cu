@@ -52,12 +52,15 @@ struct Kv4DecodeParams {
     int table_stride, layer, n_layers, n_kv_heads, num_blocks, G, batch, nsplit, n_runs, prenormed, ng;
 };
 
-// shared memory: stages, queries, barriers, the warps' sums (cluster launches: over the stages, which are free by then), then
-// (cluster launches) the rows [sender][head] that the other ranges send
-constexpr size_t kd_queries_at(int stages) { return size_t(stages) * KV4_PAGE; }
-constexpr size_t kd_bars_at(int stages) { return kd_queries_at(stages) + sizeof(Kv4Queries); }
-constexpr size_t kd_sums_at(int stages) { return (kd_bars_at(stages) + size_t(stages) * 20 + 15) / 16 * 16; }
-constexpr size_t kd_smem(int ncons, int stages) { return 1024 + kd_sums_at(stages) + size_t(ncons) * 8 * KD_SUM * 4; }
+constexpr int KD_HELPERS = 3;
+struct KdSlot;
+constexpr int kd_bufs(bool cl) { return cl ? 1 : 4; }   // pieces staged ahead
+// shared memory: stages, slots, barriers, the warps' sums, then (cluster launches) the rows [sender][head] of the other ranges
+constexpr size_t KD_SLOT_BYTES = sizeof(Kv4Queries) + 16;
+constexpr size_t kd_slots_at(int stages) { return size_t(stages) * KV4_PAGE; }
+constexpr size_t kd_bars_at(int stages, bool cl) { return kd_slots_at(stages) + kd_bufs(cl) * KD_SLOT_BYTES; }
+constexpr size_t kd_sums_at(int stages, bool cl) { return (kd_bars_at(stages, cl) + size_t(stages) * 20 + (2 * kd_bufs(cl) + 4) * 8 + 15) / 16 * 16; }
+constexpr size_t kd_smem(int ncons, int stages, bool cl) { return 1024 + kd_sums_at(stages, cl) + size_t(ncons) * 8 * KD_SUM * 4; }
 constexpr size_t kd_inbox_rows(int ranges, int G) { return size_t(ranges) * ((G + ranges - 1) / ranges); }
 
 __device__ __forceinline__ int kd_pages(const int32_t* seq_lens, int b) { return max(0, (__ldg(seq_lens + b) + BLK - 1) / BLK); }
@@ -156,28 +159,45 @@ struct KdWalk {
     }
 };
 
-// NCONS consumer warps, the last warp is the producer. WPG warps share the 8 tiles of a page; the NCONS / WPG groups of them take
-// the pages in turn, so that no group gets far ahead of another (three CTAs an SM with a run each did: the warps of the
-// one that the schedulers favoured were done after 0.8 of the time, and the others were left with too few warps for the SM).
+// A piece as the helper warps hand it to the consumers: its queries, and what of it is to be done.
+struct KdSlot {
+    Kv4Queries sq;
+    int n;         // pages; -1: there are no more pieces
+    int first;     // its first page in the sequence
+    int unit;      // sequence x kv heads + kv head
+    int out;       // -1: the unit is whole in this run; else the slot of the scratch that its sums go to
+};
+
+// NCONS consumer warps; a producer warp; HELPERS helper warps. WPG consumer warps share the 8 tiles of a page; the NCONS / WPG
+// groups of them take the run's pages in turn, so that no group gets far ahead of another (three CTAs an SM with a run each did:
+// the warps of the one that the schedulers favoured were done after 0.8 of the time, and the others were left with too few warps
+// for the SM). The helpers stage the queries of the next pieces and write out the sums of the last ones, so that a piece costs
+// the consumers a look at its slot, and short pieces (a page or two) are worked on by several groups at a time; with the consumers
+// doing that work between barriers a piece cost 3.7 microseconds beside its pages.
 // CL: the key ranges of a unit are the CTAs of one thread-block cluster, and each finishes the heads it owns (head h: CTA h %
 // ranges) from its shared memory.
+static_assert(sizeof(KdSlot) == KD_SLOT_BYTES && KD_SLOT_BYTES % 16 == 0, "the slots' place in shared memory");
+
 template <int DT, bool SCORES, int NCONS, int WPG, int STAGES, bool CL>
-__global__ void __launch_bounds__((NCONS + 1) * 32, 1)
+__global__ void __launch_bounds__((NCONS + 1 + KD_HELPERS) * 32, 1)
     kv4_decode_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ Kv4DecodeParams p) {
     constexpr int TILES = 8 / WPG;          // 16-key tiles of a page a consumer warp takes
     constexpr int GROUPS = NCONS / WPG;
-    constexpr int CT = NCONS * 32;          // consumer threads
+    constexpr int PRODUCER = NCONS;         // warp roles: consumers, then the producer, then the helpers
+    constexpr int BUFS = kd_bufs(CL);
     static_assert(STAGES >= GROUPS, "a group's stage index advances by GROUPS a page");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* stages = smem;
-    Kv4Queries& sq = *reinterpret_cast<Kv4Queries*>(smem + kd_queries_at(STAGES));
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + kd_bars_at(STAGES));
+    KdSlot* slots = reinterpret_cast<KdSlot*>(smem + kd_slots_at(STAGES));
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + kd_bars_at(STAGES, CL));
     uint64_t* empty = full + STAGES;
-    volatile int* limits = reinterpret_cast<volatile int*>(empty + STAGES);   // keys of the stage's page that count
-    float* sums = reinterpret_cast<float*>(smem + kd_sums_at(STAGES));        // [NCONS][8][KD_SUM]
-    __shared__ int s_failed, s_issued, s_more;
-    __shared__ KdWalk<CL> s_walk;   // the consumers' walk (thread 0 moves it on); the producer has its own, some pages ahead
+    uint64_t* staged = empty + STAGES;      // [BUFS] helpers -> consumers: the slot holds a piece
+    uint64_t* summed = staged + BUFS;       // [BUFS] consumers -> helpers: all are past the slot's piece, its sums written
+    uint64_t* taken = summed + BUFS;        // [GROUPS] helpers -> the group: its sums have been read
+    volatile int* limits = reinterpret_cast<volatile int*>(taken + GROUPS);   // [STAGES] keys of the stage's page that count
+    float* sums = reinterpret_cast<float*>(smem + kd_sums_at(STAGES, CL));    // [NCONS][8][KD_SUM]
+    __shared__ int s_failed, s_issued;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     trace_first(p.ctl.trace, 0);
@@ -186,24 +206,32 @@ __global__ void __launch_bounds__((NCONS + 1) * 32, 1)
         pdl_wait();
         pdl_launch_dependents();
     }
-    KdWalk<CL> walk;            // (seq_lens is an input of the whole step: read ahead of the wait)
-    if (warp == 0 || warp == NCONS) walk.start(p, lane);
-    if (tid == 0) s_walk = walk;
+    auto fail = [&](int code) {
+        atomicExch(p.ctl.err, code);
+        *reinterpret_cast<volatile int*>(&s_failed) = 1;
+    };
 
-    if (warp == NCONS) {
+    if (warp == PRODUCER) {
         // ---- producer: keeps the ring of stages full. The lanes look up 32 pages' blocks and addresses at a time, then each requests
         // its page when its turn comes (one lane that did it all took 1000 clocks a page, twice what the SM takes to attend one).
         // A block outside the pool: no keys, and the error word set.
+        KdWalk<CL> walk;                    // (seq_lens and the table are inputs of the whole step: read ahead of the wait)
+        walk.start(p, lane);
         if (lane == 0) {
             for (int s = 0; s < STAGES; s++) {
                 mbar_init(&full[s], 1);
                 mbar_init(&empty[s], WPG);
             }
+            for (int s = 0; s < BUFS; s++) {
+                mbar_init(&staged[s], KD_HELPERS);
+                mbar_init(&summed[s], NCONS);
+            }
+            for (int s = 0; s < GROUPS; s++) mbar_init(&taken[s], KD_HELPERS);
             s_failed = 0;
             fence_barrier_init();
         }
         __syncwarp();
-        int count = 0, done = 0, S = 0;   // pages requested, of the run and of the piece; keys of the sequence
+        int count = 0, done = 0, S = 0;     // pages requested, of the run and of the piece; keys of the sequence
         bool go = true, joined = false;
         while (true) {
             if (go && done == walk.at.n) {
@@ -253,215 +281,286 @@ __global__ void __launch_bounds__((NCONS + 1) * 32, 1)
             done += m;
         }
         if (lane == 0) s_issued = count;
+    } else if (warp > PRODUCER) {
+        // ---- helpers: warp hw stages heads hw, hw + KD_HELPERS, ..; the sums are shared out by thread
+        const int hw = warp - PRODUCER - 1, ht = hw * 32 + lane;
+        constexpr int HPW = (8 + KD_HELPERS - 1) / KD_HELPERS;      // heads a helper warp takes
+        KdWalk<CL> walk;
+        walk.start(p, lane);
+        bool more = true;
+        if (p.ctl.early) {
+            pdl_wait();
+            pdl_launch_dependents();
+        }
+        auto stage = [&](int j) {
+            KdSlot& slot = slots[j % BUFS];
+            more = walk.next(p) || (CL && j == 0);   // (a range without pages sends its zeros all the same)
+            const KdPiece& at = walk.at;
+            float x[HPW][4];
+            const size_t row = size_t(at.b) * p.q_stride + size_t(at.kvh * p.G) * HD;
+#pragma unroll
+            for (int i = 0; i < HPW; i++) kv4_load_query<DT>(x[i], more && hw + i * KD_HELPERS < p.G, p.q, row + size_t(hw + i * KD_HELPERS) * HD, lane);
+#pragma unroll
+            for (int i = 0; i < HPW; i++) {
+                const int hh = hw + i * KD_HELPERS;
+                if (hh < 8) kv4_stage_query<DT>(slot.sq, hh, hh < p.G, x[i], p.prenormed != 0, p.g1, p.g2, p.ng, lane);
+            }
+            if (ht == 0) {
+                slot.n = more ? at.n : -1;
+                slot.first = at.first;
+                slot.unit = at.b * p.n_kv_heads + at.kvh;
+                // a run has at most two pieces of units that it shares with others, its first and its last
+                slot.out = at.n == at.pages ? -1 : 2 * int(blockIdx.x) + (walk.length - walk.left == at.n ? 0 : 1);
+            }
+        };
+        int ahead = 0;
+        stage(ahead++);
+        __syncthreads();
+        if (lane == 0) mbar_arrive(&staged[0]);
+        if (!CL) {
+            for (int c = blockIdx.x; c < p.batch; c += gridDim.x)   // sequences without keys have no unit in any run
+                if (__ldg(p.seq_lens + c) <= 0)
+                    for (int i = ht; i < p.n_kv_heads * p.G * HD; i += KD_HELPERS * 32) Act<DT>::store(p.o, size_t(c) * p.o_stride + i, 0.0f);
+            const float sink = sqrtf(float(HD));
+            int piece0 = 0;
+#pragma unroll 1
+            for (int j = 0;; j++) {
+                // up to BUFS pieces ahead of the one whose sums come next
+                for (; more && ahead < j + BUFS; ahead++) {
+                    stage(ahead);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&staged[ahead % BUFS]);
+                }
+                const KdSlot& slot = slots[j % BUFS];
+                bar_sync(2, KD_HELPERS * 32);                       // (the slot's words are thread 0's)
+                const int n = slot.n;
+                if (n < 0) break;
+                if (!__all_sync(0xffffffffu, mbar_wait_bounded(p.ctl.wait_cycles, &summed[j % BUFS], (j / BUFS) & 1))) {
+                    fail(ERR_WAIT_FULL);
+                    break;
+                }
+                const int out = slot.out, unit = slot.unit;
+                // the groups that had a page of the piece: those of pages piece0 .. piece0 + n - 1
+                const int g0 = piece0 % GROUPS;
+                auto has = [&](int g) { return (g - g0 + GROUPS) % GROUPS < n; };
+                for (int hh = hw; hh < p.G; hh += KD_HELPERS) {
+                    float num[4] = {0.0f, 0.0f, 0.0f, 0.0f}, den = 0.0f;   // dims lane + 32 i
+#pragma unroll
+                    for (int g = 0; g < GROUPS; g++) {
+                        if (!has(g)) continue;
+#pragma unroll
+                        for (int w = 0; w < WPG; w++) {
+                            const float* from = sums + ((g * WPG + w) * 8 + hh) * KD_SUM;
+#pragma unroll
+                            for (int i = 0; i < 4; i++) num[i] += from[lane + 32 * i];
+                            den += from[HD];
+                        }
+                    }
+                    if (out < 0) {
+                        const size_t at = size_t(unit / p.n_kv_heads) * p.o_stride + size_t(unit % p.n_kv_heads * p.G + hh) * HD + lane;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) Act<DT>::store(p.o, at + 32 * i, num[i] / (sink + den));
+                    } else {
+                        float* part = p.partials + (size_t(out) * p.G + hh) * KD_PART;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) part[lane + 32 * i] = num[i];
+                        if (lane == 0) part[HD] = den;
+                    }
+                }
+                __syncwarp();
+                if (lane == 0)
+                    for (int g = 0; g < GROUPS; g++)
+                        if (has(g)) mbar_arrive(&taken[g]);
+                piece0 += n;
+                bar_sync(2, KD_HELPERS * 32);                       // (all are done with the slot: it may be staged again)
+            }
+        }
     } else {
+        // ---- consumers
         if (p.ctl.early) {
             pdl_wait();
             pdl_launch_dependents();
         }
         trace_first(p.ctl.trace, 1);
-        // ---- consumers
         const int r = lane >> 2, t = lane & 3;
         const uint32_t base = smem_u32(stages) + kv4_lane_at(lane);
-        const float sink = sqrtf(float(HD));
         const int group = warp / WPG, wg = warp % WPG;
         int st = group, phase = 0;                                  // stage and phase of the group's next page,
         int mine = group, piece0 = 0;                               // its number in the run, and of the piece's first page
-        bool ok = true;                                             // (the warp's: no wait of it has run out)
-        bool begun = false;
-        for (int c = blockIdx.x; !CL && c < p.batch; c += gridDim.x)   // sequences without keys have no unit in any run
-            if (__ldg(p.seq_lens + c) <= 0)
-                for (int i = tid; i < p.n_kv_heads * p.G * HD; i += CT) Act<DT>::store(p.o, size_t(c) * p.o_stride + i, 0.0f);
-        while (true) {
-            if (tid == 0) s_more = s_walk.next(p);
-            bar_sync(1, CT);
-            if (!CL && !s_more) {
-                if (!begun) __syncthreads();
+        int given = 0;                                              // pieces that the group has left sums of
+        __syncthreads();
+#pragma unroll 1
+        for (int j = 0;; j++) {
+            const KdSlot& slot = slots[j % BUFS];
+            // (the decision is the warp's, here and below: a warp that leaves a loop leaves it whole)
+            bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(p.ctl.wait_cycles, &staged[j % BUFS], (j / BUFS) & 1));
+            if (!ok) {
+                fail(ERR_WAIT_FULL);
                 break;
             }
-            const KdPiece& pc = s_walk.at;                          // (CL: a range without pages is walked through all the same)
-            const int unit = pc.b * p.n_kv_heads + pc.kvh, n = s_more ? pc.n : 0;
-            const int lane_q = here(lane);
-            for (int hh = here(warp); hh < 8; hh += NCONS)
-                kv4_stage_query<DT>(sq, hh, hh < p.G, p.q, size_t(pc.b) * p.q_stride + size_t(pc.kvh * p.G + hh) * HD, p.prenormed != 0, p.g1, p.g2,
-                                    p.ng, lane_q);
-            if (begun) bar_sync(1, CT);
-            else __syncthreads();                                   // (with the producer, which has set the barriers up meanwhile)
-            begun = true;
-            Kv4Frag frag;
-            frag.load(sq, lane_q);
-            // scores: S x the query's power of two; a head that is not there never is the largest
-            float u0 = 0.0f, u1 = 0.0f, n0 = 0.0f, n1 = 0.0f;
-            if (SCORES) {
-                const int e0 = sq.expo[2 * t], e1 = sq.expo[2 * t + 1];
-                if (e0) u0 = pow2_biased(e0) / KV4_SUBNORMAL;
-                else n0 = __uint_as_float(0xff800000u);
-                if (e1) u1 = pow2_biased(e1) / KV4_SUBNORMAL;
-                else n1 = __uint_as_float(0xff800000u);
-            }
-            float O[8][4];
+            const int n = slot.n;
+            if (n < 0) break;
+            if (CL || mine < piece0 + n) {
+                Kv4Frag frag;
+                frag.load(slot.sq, here(lane));
+                // scores: S x the query's power of two; a head that is not there never is the largest
+                float u0 = 0.0f, u1 = 0.0f, n0 = 0.0f, n1 = 0.0f;
+                float* scores = nullptr;
+                if (SCORES) {
+                    const int e0 = slot.sq.expo[2 * t], e1 = slot.sq.expo[2 * t + 1];
+                    if (e0) u0 = pow2_biased(e0) / KV4_SUBNORMAL;
+                    else n0 = __uint_as_float(0xff800000u);
+                    if (e1) u1 = pow2_biased(e1) / KV4_SUBNORMAL;
+                    else n1 = __uint_as_float(0xff800000u);
+                    scores = p.scores + size_t(slot.unit) * p.scores_stride + long(slot.first - piece0) * BLK + wg * (TILES * 16);
+                }
+                float O[8][4];
 #pragma unroll
-            for (int i = 0; i < 8; i++) O[i][0] = O[i][1] = O[i][2] = O[i][3] = 0.0f;
-            float ps0 = 0.0f, ps1 = 0.0f;                           // sums of the kept weights of heads 2t, 2t + 1
-            float f0 = pow2_biased(247), f1 = pow2_biased(247);     // their factors (2^120: nothing seen yet)
-            bool big = false;
-            float limit = KD_LIMIT;
-            for (; mine < piece0 + n && ok; mine += GROUPS) {
-                // (the decision is the warp's: a warp that leaves the loop leaves it whole)
-                ok = __all_sync(0xffffffffu, mbar_wait_bounded(p.ctl.wait_cycles, &full[st], phase));
+                for (int i = 0; i < 8; i++) O[i][0] = O[i][1] = O[i][2] = O[i][3] = 0.0f;
+                float ps0 = 0.0f, ps1 = 0.0f;                       // sums of the kept weights of heads 2t, 2t + 1
+                float f0 = pow2_biased(247), f1 = pow2_biased(247); // their factors (2^120: nothing seen yet)
+                bool big = false;
+                float limit = KD_LIMIT;
+#pragma unroll 1
+                for (; mine < piece0 + n; mine += GROUPS) {
+                    ok = __all_sync(0xffffffffu, mbar_wait_bounded(p.ctl.wait_cycles, &full[st], phase));
+                    if (!ok) break;
+                    // the warp's tiles of the page together: their products have nothing to wait for in one another
+                    const uint32_t kaddr = base + st * KV4_PAGE + wg * (TILES * 16 * KV4_ROW);
+                    const uint8_t* sc = stages + st * KV4_PAGE + 2 * KV4_SIDE + wg * (TILES * 16 * 16);
+                    const int left = limits[st] - wg * (TILES * 16);   // keys of the tiles that count, if fewer than there are
+                    if (left > 0) {
+                        float s[TILES][4];
+                        Kv4Scales rows[TILES];
+                        bool flagged = false;
+#pragma unroll
+                        for (int k = 0; k < TILES; k++) {
+                            rows[k].load(sc + k * 256, lane);
+                            kv4_tile_scores(kaddr + k * 16 * KV4_ROW, rows[k], frag, s[k]);
+                        }
+                        if (SCORES) {
+#pragma unroll
+                            for (int k = 0; k < TILES; k++) {
+                                float m0 = fmaxf(fmaf(s[k][0], u0, n0), fmaf(s[k][1], u1, n1)), m1 = fmaxf(fmaf(s[k][2], u0, n0), fmaf(s[k][3], u1, n1));
+                                m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, 1));
+                                m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 1));
+                                m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, 2));
+                                m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 2));
+                                const int key = k * 16 + r + 8 * t;
+                                if (t < 2 && key < left)
+                                    scores[long(mine) * BLK + key] = t ? m1 : m0;
+                            }
+                        }
+                        if (left < TILES * 16) {
+#pragma unroll
+                            for (int k = 0; k < TILES; k++) {
+                                if (k * 16 + r >= left) s[k][0] = s[k][1] = 0.0f;
+                                if (k * 16 + r + 8 >= left) s[k][2] = s[k][3] = 0.0f;
+                                rows[k].mask(lane, left - k * 16);
+                            }
+                        }
+                        float w[TILES][4], top = 0.0f;
+#pragma unroll
+                        for (int k = 0; k < TILES; k++) {
+                            flagged |= rows[k].large();
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                s[k][e] = fmaxf(s[k][e], 0.0f);
+                                w[k][e] = s[k][e] * ((e & 1) ? f1 : f0) * s[k][e];
+                                top = fmaxf(top, w[k][e]);
+                            }
+                        }
+                        if (__any_sync(0xffffffffu, top > limit || (flagged && !big))) {
+                            // (a handful of times a warp) new factors: the tiles' largest weight of a head at most 2^target
+                            if (__any_sync(0xffffffffu, flagged)) {
+                                big = true;
+                                limit = KD_LIMIT_BIG;
+                            }
+                            const int target = big ? KD_TARGET_BIG : KD_TARGET;
+                            float m0 = 0.0f, m1 = 0.0f;
+#pragma unroll
+                            for (int k = 0; k < TILES; k++) {
+                                m0 = fmaxf(m0, fmaxf(s[k][0], s[k][2]));
+                                m1 = fmaxf(m1, fmaxf(s[k][1], s[k][3]));
+                            }
+#pragma unroll
+                            for (int o = 4; o < 32; o <<= 1) {
+                                m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
+                                m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+                            }
+                            // m < 2^(e + 1), so m^2 2^(target - 2 (e + 1)) < 2^target
+                            const int e0 = int(__float_as_uint(m0) >> 23) - 126, e1 = int(__float_as_uint(m1) >> 23) - 126;
+                            const float nf0 = m0 * f0 * m0 > limit ? pow2_biased(min(max(127 + target - 2 * e0, 1), 254)) : f0;
+                            const float nf1 = m1 * f1 * m1 > limit ? pow2_biased(min(max(127 + target - 2 * e1, 1), 254)) : f1;
+                            const float c0 = nf0 / f0, c1 = nf1 / f1;
+                            f0 = nf0;
+                            f1 = nf1;
+                            ps0 *= c0;
+                            ps1 *= c1;
+#pragma unroll
+                            for (int k = 0; k < 8; k++) {
+                                O[k][0] *= c0;
+                                O[k][1] *= c1;
+                                O[k][2] *= c0;
+                                O[k][3] *= c1;
+                            }
+#pragma unroll
+                            for (int k = 0; k < TILES; k++)
+#pragma unroll
+                                for (int e = 0; e < 4; e++) w[k][e] = s[k][e] * ((e & 1) ? f1 : f0) * s[k][e];
+                        }
+#pragma unroll
+                        for (int k = 0; k < TILES; k++) {
+                            ps0 += w[k][0] + w[k][2];
+                            ps1 += w[k][1] + w[k][3];
+                            kv4_tile_values(kaddr + KV4_SIDE + k * 16 * KV4_ROW, rows[k], w[k], O);
+                        }
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&empty[st]);
+                    st += GROUPS;
+                    if (st >= STAGES) {
+                        st -= STAGES;
+                        phase ^= 1;
+                    }
+                }
+                // ---- the warp's sums of the piece, in units of the weights themselves, once the helpers have read its last ones
+                if (ok && given > 0) ok = __all_sync(0xffffffffu, mbar_wait_bounded(p.ctl.wait_cycles, &taken[group], (given - 1) & 1));
                 if (!ok) {
-                    atomicExch(p.ctl.err, ERR_WAIT_FULL);
-                    *reinterpret_cast<volatile int*>(&s_failed) = 1;
+                    fail(ERR_WAIT_FULL);
                     break;
                 }
-                const int page = pc.first + mine - piece0;
-                // the warp's tiles of the page together: their products have nothing to wait for in one another
-                const uint32_t kaddr = base + st * KV4_PAGE + wg * (TILES * 16 * KV4_ROW);
-                const uint8_t* sc = stages + st * KV4_PAGE + 2 * KV4_SIDE + wg * (TILES * 16 * 16);
-                const int left = limits[st] - wg * (TILES * 16);   // keys of the tiles that count, if fewer than there are
-                if (left > 0) {
-                    float s[TILES][4];
-                    Kv4Scales rows[TILES];
-                    bool flagged = false;
+                given++;
 #pragma unroll
-                    for (int k = 0; k < TILES; k++) {
-                        rows[k].load(sc + k * 256, lane);
-                        kv4_tile_scores(kaddr + k * 16 * KV4_ROW, rows[k], frag, s[k]);
-                    }
-                    if (SCORES) {
-#pragma unroll
-                        for (int k = 0; k < TILES; k++) {
-                            float m0 = fmaxf(fmaf(s[k][0], u0, n0), fmaf(s[k][1], u1, n1)), m1 = fmaxf(fmaf(s[k][2], u0, n0), fmaf(s[k][3], u1, n1));
-                            m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, 1));
-                            m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 1));
-                            m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, 2));
-                            m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 2));
-                            const int key = k * 16 + r + 8 * t;
-                            if (t < 2 && key < left)
-                                p.scores[size_t(unit) * p.scores_stride + page * BLK + wg * (TILES * 16) + key] = t ? m1 : m0;
-                        }
-                    }
-                    if (left < TILES * 16) {
-#pragma unroll
-                        for (int k = 0; k < TILES; k++) {
-                            if (k * 16 + r >= left) s[k][0] = s[k][1] = 0.0f;
-                            if (k * 16 + r + 8 >= left) s[k][2] = s[k][3] = 0.0f;
-                            rows[k].mask(lane, left - k * 16);
-                        }
-                    }
-                    float w[TILES][4], top = 0.0f;
-#pragma unroll
-                    for (int k = 0; k < TILES; k++) {
-                        flagged |= rows[k].large();
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            s[k][e] = fmaxf(s[k][e], 0.0f);
-                            w[k][e] = s[k][e] * ((e & 1) ? f1 : f0) * s[k][e];
-                            top = fmaxf(top, w[k][e]);
-                        }
-                    }
-                    if (__any_sync(0xffffffffu, top > limit || (flagged && !big))) {
-                        // (a handful of times a warp) new factors: the tiles' largest weight of a head at most 2^target
-                        if (__any_sync(0xffffffffu, flagged)) {
-                            big = true;
-                            limit = KD_LIMIT_BIG;
-                        }
-                        const int target = big ? KD_TARGET_BIG : KD_TARGET;
-                        float m0 = 0.0f, m1 = 0.0f;
-#pragma unroll
-                        for (int k = 0; k < TILES; k++) {
-                            m0 = fmaxf(m0, fmaxf(s[k][0], s[k][2]));
-                            m1 = fmaxf(m1, fmaxf(s[k][1], s[k][3]));
-                        }
-#pragma unroll
-                        for (int o = 4; o < 32; o <<= 1) {
-                            m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
-                            m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
-                        }
-                        // m < 2^(e + 1), so m^2 2^(target - 2 (e + 1)) < 2^target
-                        const int e0 = int(__float_as_uint(m0) >> 23) - 126, e1 = int(__float_as_uint(m1) >> 23) - 126;
-                        const float nf0 = m0 * f0 * m0 > limit ? pow2_biased(min(max(127 + target - 2 * e0, 1), 254)) : f0;
-                        const float nf1 = m1 * f1 * m1 > limit ? pow2_biased(min(max(127 + target - 2 * e1, 1), 254)) : f1;
-                        const float c0 = nf0 / f0, c1 = nf1 / f1;
-                        f0 = nf0;
-                        f1 = nf1;
-                        ps0 *= c0;
-                        ps1 *= c1;
-#pragma unroll
-                        for (int k = 0; k < 8; k++) {
-                            O[k][0] *= c0;
-                            O[k][1] *= c1;
-                            O[k][2] *= c0;
-                            O[k][3] *= c1;
-                        }
-#pragma unroll
-                        for (int k = 0; k < TILES; k++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) w[k][e] = s[k][e] * ((e & 1) ? f1 : f0) * s[k][e];
-                    }
-#pragma unroll
-                    for (int k = 0; k < TILES; k++) {
-                        ps0 += w[k][0] + w[k][2];
-                        ps1 += w[k][1] + w[k][3];
-                        kv4_tile_values(kaddr + KV4_SIDE + k * 16 * KV4_ROW, rows[k], w[k], O);
-                    }
+                for (int o = 4; o < 32; o <<= 1) {
+                    ps0 += __shfl_xor_sync(0xffffffffu, ps0, o);
+                    ps1 += __shfl_xor_sync(0xffffffffu, ps1, o);
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&empty[st]);
-                st += GROUPS;
-                if (st >= STAGES) {
-                    st -= STAGES;
-                    phase ^= 1;
+                // w = w' / f x (the query's power of two x 2^20)^2 / 128, the powers of two multiplied one by one
+                const int lane_s = here(lane), rs = lane_s >> 2, ts = lane_s & 3;
+                const float q0 = pow2_biased(max(slot.sq.expo[2 * ts], 1)), q1 = pow2_biased(max(slot.sq.expo[2 * ts + 1], 1));
+                const float i0 = (1.0f / 128.0f / KV4_SUBNORMAL / KV4_SUBNORMAL) / f0, i1 = (1.0f / 128.0f / KV4_SUBNORMAL / KV4_SUBNORMAL) / f1;
+                float* row0 = sums + (warp * 8 + 2 * ts) * KD_SUM;
+                float* row1 = row0 + KD_SUM;
+                if (2 * ts < p.G) {
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        const int d = kv4_dim_of(k, rs);
+                        row0[d] = O[k][0] * i0 * q0 * q0;
+                        row1[d] = O[k][1] * i1 * q1 * q1;
+                        row0[d + 2] = O[k][2] * i0 * q0 * q0;
+                        row1[d + 2] = O[k][3] * i1 * q1 * q1;
+                    }
+                    if (rs == 0) {
+                        row0[HD] = ps0 * i0 * q0 * q0;
+                        row1[HD] = ps1 * i1 * q1 * q1;
+                    }
                 }
             }
+            if (CL) break;                                          // (the cluster's CTAs meet below, all warps)
             piece0 += n;
-            // ---- the warps' sums of the piece into one, in units of the weights themselves
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) {
-                ps0 += __shfl_xor_sync(0xffffffffu, ps0, o);
-                ps1 += __shfl_xor_sync(0xffffffffu, ps1, o);
-            }
-            // w = w' / f x (the query's power of two x 2^20)^2 / 128, the powers of two multiplied one by one
-            const int lane_s = here(lane), rs = lane_s >> 2, ts = lane_s & 3, tid_s = here(tid);
-            const float q0 = pow2_biased(max(sq.expo[2 * ts], 1)), q1 = pow2_biased(max(sq.expo[2 * ts + 1], 1));
-            const float i0 = (1.0f / 128.0f / KV4_SUBNORMAL / KV4_SUBNORMAL) / f0, i1 = (1.0f / 128.0f / KV4_SUBNORMAL / KV4_SUBNORMAL) / f1;
-            float* row0 = sums + (warp * 8 + 2 * ts) * KD_SUM;
-            float* row1 = row0 + KD_SUM;
-            if (2 * ts < p.G) {
-#pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const int d = kv4_dim_of(k, rs);
-                    row0[d] = O[k][0] * i0 * q0 * q0;
-                    row1[d] = O[k][1] * i1 * q1 * q1;
-                    row0[d + 2] = O[k][2] * i0 * q0 * q0;
-                    row1[d + 2] = O[k][3] * i1 * q1 * q1;
-                }
-                if (rs == 0) {
-                    row0[HD] = ps0 * i0 * q0 * q0;
-                    row1[HD] = ps1 * i1 * q1 * q1;
-                }
-            }
-            bar_sync(1, CT);
-            if (CL) break;   // (the cluster's CTAs meet below, all warps)
-            // A unit inside this run is done: its rows. Else its pieces, one a run, meet in the scratch (a run has at most two pieces
-            // of units that it shares, its first and its last: slots 2 c and 2 c + 1), where kv4_decode_join_kernel adds them.
-            const bool whole = n == pc.pages;
-            float* part = p.partials + size_t(2 * blockIdx.x + (s_walk.length - s_walk.left == n ? 0 : 1)) * p.G * KD_PART;
-            for (int idx = tid_s; idx < p.G * HD; idx += CT) {
-                const int hh = idx >> 7, d = idx & 127;
-                float num = 0.0f, den = 0.0f;
-#pragma unroll
-                for (int w = 0; w < NCONS; w++) {
-                    num += sums[(w * 8 + hh) * KD_SUM + d];
-                    den += sums[(w * 8 + hh) * KD_SUM + HD];
-                }
-                if (whole) Act<DT>::store(p.o, size_t(pc.b) * p.o_stride + size_t(pc.kvh * p.G + hh) * HD + d, num / (sink + den));
-                else {
-                    part[hh * KD_PART + d] = num;
-                    if (d == 0) part[hh * KD_PART + HD] = den;
-                }
-            }
-            // (the sums and the walk are read before this barrier, written again behind the next piece's)
-            bar_sync(1, CT);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&summed[j % BUFS]);
         }
     }
 
@@ -474,11 +573,11 @@ __global__ void __launch_bounds__((NCONS + 1) * 32, 1)
     }
     if (CL) {
         // every range's rows go, head by head, to the CTA that finishes the head; it adds them in range order
-        constexpr int THREADS = (NCONS + 1) * 32;
+        constexpr int THREADS = (NCONS + 1 + KD_HELPERS) * 32;
         const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
         const float sink = sqrtf(float(HD));
         float* inbox = sums + NCONS * 8 * KD_SUM;
-        const int slots = (p.G + p.nsplit - 1) / p.nsplit;
+        const int own = (p.G + p.nsplit - 1) / p.nsplit;
         cluster_wait();
         for (int idx = tid; idx < p.G * HD; idx += THREADS) {
             const int hh = idx >> 7, d = idx & 127;
@@ -488,18 +587,18 @@ __global__ void __launch_bounds__((NCONS + 1) * 32, 1)
                 num += sums[(w * 8 + hh) * KD_SUM + d];
                 den += sums[(w * 8 + hh) * KD_SUM + HD];
             }
-            const uint32_t row = cluster_map(smem_u32(inbox + (split * slots + hh / p.nsplit) * KD_PART), uint32_t(hh % p.nsplit));
+            const uint32_t row = cluster_map(smem_u32(inbox + (split * own + hh / p.nsplit) * KD_PART), uint32_t(hh % p.nsplit));
             cluster_st_f32(row + uint32_t(d) * 4u, num);
             if (d == 0) cluster_st_f32(row + HD * 4, den);
         }
         cluster_arrive();
         cluster_wait();
-        for (int idx = tid; idx < slots * HD; idx += THREADS) {
+        for (int idx = tid; idx < own * HD; idx += THREADS) {
             const int slot = idx >> 7, d = idx & 127, hh = split + slot * p.nsplit;
             if (hh < p.G) {
                 float num = 0.0f, den = sink;
                 for (int k = 0; k < p.nsplit; k++) {
-                    const float* row = inbox + (k * slots + slot) * KD_PART;
+                    const float* row = inbox + (k * own + slot) * KD_PART;
                     den += row[HD];
                     num += row[d];
                 }
@@ -544,17 +643,19 @@ __global__ void __launch_bounds__(256) kv4_decode_join_kernel(const __grid_const
         float e[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float* row = p.partials + (size_t(k + j == lo ? first_slot : 2 * (k + j)) * p.G + hh) * KD_PART;
-            v[j] = k + j <= hi ? __ldcg(reinterpret_cast<const float4*>(row) + lane) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            e[j] = k + j <= hi ? __ldcg(row + HD) : 0.0f;
+            const int piece = min(k + j, hi);   // (behind the last one: loaded again and not added)
+            const float* row = p.partials + (size_t(piece == lo ? first_slot : 2 * piece) * p.G + hh) * KD_PART;
+            v[j] = __ldcg(reinterpret_cast<const float4*>(row) + lane);
+            e[j] = __ldcg(row + HD);
         }
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            num.x += v[j].x;
-            num.y += v[j].y;
-            num.z += v[j].z;
-            num.w += v[j].w;
-            den += e[j];
+            const bool add = k + j <= hi;
+            num.x += add ? v[j].x : 0.0f;
+            num.y += add ? v[j].y : 0.0f;
+            num.z += add ? v[j].z : 0.0f;
+            num.w += add ? v[j].w : 0.0f;
+            den += add ? e[j] : 0.0f;
         }
     }
     const float inv = 1.0f / den;
@@ -586,7 +687,7 @@ template <int DT, bool SCORES, bool CL>
 static EmblaStatus launch_kv4_decode(EmblaAttn* ctx, const EmblaKVPool* pool, const Kv4DecodeParams& p, int batch, dim3 grid, cudaStream_t s) {
     using Shape = KdShape<CL>;
     auto kern = kv4_decode_kernel<DT, SCORES, Shape::ncons, Shape::wpg, Shape::stages, CL>;
-    constexpr size_t fixed = kd_smem(Shape::ncons, Shape::stages);
+    constexpr size_t fixed = kd_smem(Shape::ncons, Shape::stages, CL);
     const size_t smem = fixed + (CL ? kd_inbox_rows(p.nsplit, p.G) * KD_PART * 4 : 0);
     static bool configured[64] = {};   // per instantiation and device
     if (!configured[ctx->device & 63]) {
@@ -594,7 +695,7 @@ static EmblaStatus launch_kv4_decode(EmblaAttn* ctx, const EmblaKVPool* pool, co
         EMBLA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(fixed + (CL ? 14 * KD_PART * 4 : 0))));
         configured[ctx->device & 63] = true;
     }
-    EMBLA_CUDA_TRY(launch_kernel_cluster(ctx->pdl, CL ? p.nsplit : 1, kern, grid, dim3((Shape::ncons + 1) * 32), smem, s, pool->tmap_codes, p));
+    EMBLA_CUDA_TRY(launch_kernel_cluster(ctx->pdl, CL ? p.nsplit : 1, kern, grid, dim3((Shape::ncons + 1 + KD_HELPERS) * 32), smem, s, pool->tmap_codes, p));
     if (!CL && p.n_runs > 1) {
         Kv4DecodeParams pj = p;
         pj.ctl = kernel_ctl(ctx);

@@ -61,16 +61,16 @@ struct Kv4Queries {
 // the two registers of a product come out of one load side by side.
 __device__ __forceinline__ int kv4_q_column(int d) { return (d & ~6) | ((d & 4) >> 1) | ((d & 2) << 1); }
 
-// One warp, one head: loads the row (or zeros for a head the kv head does not have), head norm if asked, scales, stores.
+// One warp, one head: its row as it lies (zeros for a head the kv head does not have); then head norm if asked, scaled and stored.
 template <int DT>
-__device__ __forceinline__ void kv4_stage_query(Kv4Queries& sq, int hh, bool has, const void* q, size_t off, bool prenormed, const void* g1,
-                                                const void* g2, int ng, int lane) {
-    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (has) {
+__device__ __forceinline__ void kv4_load_query(float (&x)[4], bool has, const void* q, size_t off, int lane) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = Act<DT>::load(q, off + lane + 32 * i);
-        if (!prenormed) kv4_query_norm<DT>(x, g1, g2, ng, lane);
-    }
+    for (int i = 0; i < 4; i++) x[i] = has ? Act<DT>::load(q, off + lane + 32 * i) : 0.0f;
+}
+template <int DT>
+__device__ __forceinline__ void kv4_stage_query(Kv4Queries& sq, int hh, bool has, float (&x)[4], bool prenormed, const void* g1, const void* g2,
+                                                int ng, int lane) {
+    if (has && !prenormed) kv4_query_norm<DT>(x, g1, g2, ng, lane);
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < 4; i++) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
