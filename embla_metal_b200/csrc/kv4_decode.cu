@@ -292,20 +292,22 @@ __global__ void __launch_bounds__((NCONS + 1 + KD_HELPERS) * 32, 1)
             pdl_wait();
             pdl_launch_dependents();
         }
-        auto stage = [&](int j) {
-            KdSlot& slot = slots[j % BUFS];
-            more = walk.next(p) || (CL && j == 0);   // (a range without pages sends its zeros all the same)
-            const KdPiece& at = walk.at;
-            float x[HPW][4];
-            const size_t row = size_t(at.b) * p.q_stride + size_t(at.kvh * p.G) * HD;
+        float x[HPW][4];                    // the warp's query rows of the next piece, on their way since the one before it was staged
+        auto fetch = [&]() {
+            more = walk.next(p) || (CL && more);   // (a range without pages sends its zeros all the same)
+            const size_t row = size_t(walk.at.b) * p.q_stride + size_t(walk.at.kvh * p.G) * HD;
 #pragma unroll
             for (int i = 0; i < HPW; i++) kv4_load_query<DT>(x[i], more && hw + i * KD_HELPERS < p.G, p.q, row + size_t(hw + i * KD_HELPERS) * HD, lane);
+        };
+        auto stage = [&](int j) {
+            KdSlot& slot = slots[j % BUFS];
 #pragma unroll
             for (int i = 0; i < HPW; i++) {
                 const int hh = hw + i * KD_HELPERS;
                 if (hh < 8) kv4_stage_query<DT>(slot.sq, hh, hh < p.G, x[i], p.prenormed != 0, p.g1, p.g2, p.ng, lane);
             }
             if (ht == 0) {
+                const KdPiece& at = walk.at;
                 slot.n = more ? at.n : -1;
                 slot.first = at.first;
                 slot.unit = at.b * p.n_kv_heads + at.kvh;
@@ -313,11 +315,14 @@ __global__ void __launch_bounds__((NCONS + 1 + KD_HELPERS) * 32, 1)
                 slot.out = at.n == at.pages ? -1 : 2 * int(blockIdx.x) + (walk.length - walk.left == at.n ? 0 : 1);
             }
         };
+        fetch();
         int ahead = 0;
         stage(ahead++);
         __syncthreads();
         if (lane == 0) mbar_arrive(&staged[0]);
         if (!CL) {
+            bool last = !more;              // the slot without pages has been staged
+            if (!last) fetch();
             for (int c = blockIdx.x; c < p.batch; c += gridDim.x)   // sequences without keys have no unit in any run
                 if (__ldg(p.seq_lens + c) <= 0)
                     for (int i = ht; i < p.n_kv_heads * p.G * HD; i += KD_HELPERS * 32) Act<DT>::store(p.o, size_t(c) * p.o_stride + i, 0.0f);
@@ -326,10 +331,12 @@ __global__ void __launch_bounds__((NCONS + 1 + KD_HELPERS) * 32, 1)
 #pragma unroll 1
             for (int j = 0;; j++) {
                 // up to BUFS pieces ahead of the one whose sums come next
-                for (; more && ahead < j + BUFS; ahead++) {
+                for (; !last && ahead < j + BUFS; ahead++) {
                     stage(ahead);
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&staged[ahead % BUFS]);
+                    last = !more;
+                    if (!last) fetch();
                 }
                 const KdSlot& slot = slots[j % BUFS];
                 bar_sync(2, KD_HELPERS * 32);                       // (the slot's words are thread 0's)
@@ -609,12 +616,15 @@ __global__ void __launch_bounds__((NCONS + 1 + KD_HELPERS) * 32, 1)
     trace_last(p.ctl.trace, 3);
 }
 
-// Adds the pieces of the units that the runs of a launch cut, in the order of the runs, and writes their rows: one CTA a unit,
-// launched behind the runs (the last run of a unit adding 27 pieces of 8 heads by itself, one query among 132 KB of loads,
-// took longer than this launch). A thread takes four dims of a head.
+// Adds the pieces of the units that the runs of a launch cut and writes their rows, launched behind the runs: one CTA a unit and
+// head. What it costs is the latency of its loads, 1.2 to 2.8 microseconds for each round of them: four warps take every fourth
+// piece, four loads in flight each, so that up to 16 pieces are one round, and add up through shared memory in a fixed order.
 template <int DT>
-__global__ void __launch_bounds__(256) kv4_decode_join_kernel(const __grid_constant__ Kv4DecodeParams p) {
-    const int tid = threadIdx.x, lane = tid & 31, unit = blockIdx.x, b = unit / p.n_kv_heads, kvh = unit % p.n_kv_heads;
+__global__ void __launch_bounds__(128) kv4_decode_join_kernel(const __grid_constant__ Kv4DecodeParams p) {
+    __shared__ float4 others[3][32];
+    __shared__ float dens[3];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int hh = blockIdx.x, unit = blockIdx.y, b = unit / p.n_kv_heads, kvh = unit % p.n_kv_heads;
     trace_first(p.ctl.trace, 0);
     int before = 0, sum = 0;
     for (int i = lane; i < p.batch; i += 32) {
@@ -633,24 +643,22 @@ __global__ void __launch_bounds__(256) kv4_decode_join_kernel(const __grid_const
     pdl_wait();
     pdl_launch_dependents();
     trace_first(p.ctl.trace, 1);
-    if (pages == 0) return;
-    const int hh = tid >> 5;
-    if (lo == hi || hh >= p.G) return;
+    if (pages == 0 || lo == hi) return;
     float4 num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float den = sqrtf(float(HD));
-    for (int k = lo; k <= hi; k += 8) {   // eight pieces' loads in flight together
-        float4 v[8];
-        float e[8];
+    float den = 0.0f;
+    for (int k = lo + warp; k <= hi; k += 16) {
+        float4 v[4];
+        float e[4];
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int piece = min(k + j, hi);   // (behind the last one: loaded again and not added)
+        for (int j = 0; j < 4; j++) {
+            const int piece = min(k + 4 * j, hi);   // (behind the last one: loaded again and not added)
             const float* row = p.partials + (size_t(piece == lo ? first_slot : 2 * piece) * p.G + hh) * KD_PART;
             v[j] = __ldcg(reinterpret_cast<const float4*>(row) + lane);
             e[j] = __ldcg(row + HD);
         }
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const bool add = k + j <= hi;
+        for (int j = 0; j < 4; j++) {
+            const bool add = k + 4 * j <= hi;
             num.x += add ? v[j].x : 0.0f;
             num.y += add ? v[j].y : 0.0f;
             num.z += add ? v[j].z : 0.0f;
@@ -658,12 +666,27 @@ __global__ void __launch_bounds__(256) kv4_decode_join_kernel(const __grid_const
             den += add ? e[j] : 0.0f;
         }
     }
-    const float inv = 1.0f / den;
+    if (warp > 0) {
+        others[warp - 1][lane] = num;
+        if (lane == 0) dens[warp - 1] = den;
+    }
+    __syncthreads();
+    if (warp > 0) return;
+    den += sqrtf(float(HD));
+#pragma unroll
+    for (int w = 0; w < 3; w++) {
+        const float4 v = others[w][lane];
+        num.x += v.x;
+        num.y += v.y;
+        num.z += v.z;
+        num.w += v.w;
+        den += dens[w];
+    }
     const size_t at = size_t(b) * p.o_stride + size_t(kvh * p.G + hh) * HD + 4 * lane;
-    Act<DT>::store(p.o, at, num.x * inv);
-    Act<DT>::store(p.o, at + 1, num.y * inv);
-    Act<DT>::store(p.o, at + 2, num.z * inv);
-    Act<DT>::store(p.o, at + 3, num.w * inv);
+    Act<DT>::store(p.o, at, num.x / den);
+    Act<DT>::store(p.o, at + 1, num.y / den);
+    Act<DT>::store(p.o, at + 2, num.z / den);
+    Act<DT>::store(p.o, at + 3, num.w / den);
     trace_last(p.ctl.trace, 3);
 }
 
@@ -699,7 +722,7 @@ static EmblaStatus launch_kv4_decode(EmblaAttn* ctx, const EmblaKVPool* pool, co
     if (!CL && p.n_runs > 1) {
         Kv4DecodeParams pj = p;
         pj.ctl = kernel_ctl(ctx);
-        EMBLA_CUDA_TRY(launch_kernel(use_pdl(), kv4_decode_join_kernel<DT>, dim3(unsigned(batch) * p.n_kv_heads), dim3(p.G * 32), 0, s, pj));
+        EMBLA_CUDA_TRY(launch_kernel(use_pdl(), kv4_decode_join_kernel<DT>, dim3(p.G, unsigned(batch) * p.n_kv_heads), dim3(128), 0, s, pj));
     }
     EMBLA_CUDA_TRY(cudaGetLastError());
     return EMBLA_OK;
@@ -731,11 +754,11 @@ EmblaStatus kv4_full_decode(EmblaAttn* ctx, const EmblaKVPool* pool, const Embla
     p.prenormed = q->prenormed;
     p.ng = q->ng;
     const long units = long(view->batch) * pool->n_kv_heads, pages = (max_len + BLK - 1) / BLK;
-    if (units * pages > 0x7fffffffL)
+    if (units * pages > 0x7fffffffL || units > 0xffff)
         EMBLA_FAIL(EMBLA_BAD_ARG, "embla_attn_full_decode: %d sequences of up to %d keys are too many pages", view->batch, max_len);
     // Few pages: a cluster a unit, one page or a few a CTA. Else equal runs over the resident CTAs (the scratch holds two
     // pieces a run: embla_attn_create makes it 8 slots an SM and more).
-    const bool cluster = units * pages <= KD_CLUSTER_PAGES && units <= 0xffff;
+    const bool cluster = units * pages <= KD_CLUSTER_PAGES;
     dim3 grid;
     if (cluster) {
         p.nsplit = int(pages < KD_MAX_CLUSTER ? pages : KD_MAX_CLUSTER);
