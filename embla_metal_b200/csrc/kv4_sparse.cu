@@ -1,158 +1,320 @@
-// Attention over the 4-bit paged cache (EMBLA_KV_INT4): ReLU² of the full layers (prefill) and softmax of the
-// sparse layers. First form: one CTA of 128 threads per query row; a thread takes one key of a page for the dots (fp32), then
-// one head dim for the sum over the page's keys.
-#include "kv4.cuh"
+// Decode attention of sparse layers over a 4-bit paged cache (EMBLA_KV_INT4): softmax over every key of a sequence with at most
+// 1152, else over the rows idx[kv head][0..1151] that embla_select_keys wrote. No counterpart in the reference, whose cache is
+// int8 (attn_sparse8 / attn_sparse_short, attention.metal:448-645; sparse8_decode.cu).
+//
+// A row is 144 bytes in nine 16-byte pieces at an address that two dependent lookups give (selected position, its block), so this
+// is a matter of latency and of rows in flight. Each warp works alone: 32 rows at a time, lane i looking up row i, the copies
+// (cp.async) of three groups in flight, two 16-key tiles of a group at once on the tensor-core tiles of kv4_tile.cuh. Its
+// softmax keeps a reference score that moves (the sums with it) only when a weight passes 2^13. Up to eight CTAs a (sequence, kv
+// head), as a thread-block cluster, when there are few of them.
+#include "attn16_common.cuh"
+#include "kv4_tile.cuh"
 
 namespace embla {
 
-struct Attend4Params {
+constexpr int KS_WARPS = 4, KS_STAGES = 3, KS_ROWS = 32;
+constexpr int KS_STAGE = KS_ROWS * (2 * KV4_ROW + 4 * KV4_GROUPS);   // a group's rows: K codes, V codes, scales: 4608 bytes
+constexpr int KS_SUM = HD + 1, KS_PART = HD + 4;                     // floats of a row of sums: in shared memory, between CTAs
+constexpr int KS_MAX_CLUSTER = 8;
+// largest weight, and the one a moved reference gives the row's largest score; the second pair with value scales of 2 and more
+constexpr float KS_LIMIT = 8192.0f, KS_LIMIT_BIG = 0.5f, KS_TARGET = 10.0f, KS_TARGET_BIG = -4.0f;
+constexpr float KS_NONE = -1e30f;                                    // a reference before any key
+
+struct Kv4SparseParams {
     const uint8_t* pool;
     const int32_t* block_table;
-    const int32_t* seq_lens;   // decode: keys of a sequence
-    const int32_t* pos0;       // prefill: position of a sequence's first token; token t sees pos0 + t + 1 keys
-    const uint32_t* idx;       // sparse: selected positions of sequences past 1152 keys
+    const uint32_t* idx;
+    const int32_t* seq_lens;
     const void* q;
     const void* g1;
     const void* g2;
     void* o;
-    float* scores;
-    int* err;
-    int64_t q_token_stride, q_seq_stride, o_token_stride, o_seq_stride, scores_stride;
-    int table_stride, layer, n_layers, n_kv_heads, num_blocks, G, prenormed, ng, softmax;
+    KernelCtl ctl;
+    int64_t q_stride, o_stride;
+    int table_stride, layer, n_layers, n_kv_heads, num_blocks, G, prenormed, ng, nsplit;
 };
 
-template <int DT>
-__global__ void __launch_bounds__(128) kv4_attend_kernel(const Attend4Params p) {
+constexpr size_t ks_queries_at() { return size_t(KS_WARPS) * KS_STAGES * KS_STAGE; }
+constexpr size_t ks_inbox_at() { return ks_queries_at() + sizeof(Kv4Queries); }
+constexpr int ks_inbox_rows(int ranges, int G) { return ranges * ((G + ranges - 1) / ranges); }
+constexpr size_t ks_smem(int ranges, int G) { return 1024 + ks_inbox_at() + (ranges > 1 ? size_t(ks_inbox_rows(ranges, G)) * KS_PART * 4 : 0); }
+static_assert(KS_WARPS * 8 * (KS_SUM + 2) * 4 <= KS_WARPS * KS_STAGES * KS_STAGE, "the warps' sums lie over their stages");
+
+__device__ __forceinline__ float ks_exp2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+template <int DT, bool CL>
+__global__ void __launch_bounds__(KS_WARPS * 32, 4) kv4_sparse_kernel(const __grid_constant__ Kv4SparseParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    Kv4Queries& sq = *reinterpret_cast<Kv4Queries*>(smem + ks_queries_at());
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+    trace_first(p.ctl.trace, 0);
+    if (CL) cluster_arrive();   // (every CTA of the cluster has started before any writes into another's shared memory)
+    const int S = max(0, p.seq_lens[b]);   // (read ahead of the wait: nothing on the GPU writes the sequence lengths)
     pdl_wait();
     pdl_launch_dependents();
-    __shared__ float q[HD], w[BLK], red[4];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int head = blockIdx.x, t = blockIdx.y, b = blockIdx.z, kvh = head / p.G;
-    const int S = p.pos0 ? p.pos0[b] + t + 1 : p.seq_lens[b];
-    const bool selecting = p.softmax && S > EMBLA_TOPK + EMBLA_RECENT;
-    const int n = selecting ? EMBLA_TOPK + EMBLA_RECENT : max(S, 0);
-    if (warp == 0) {
-        const size_t off = size_t(b) * p.q_seq_stride + size_t(t) * p.q_token_stride + size_t(head) * HD;
+    trace_first(p.ctl.trace, 1);
+    const bool selecting = S > EMBLA_TOPK + EMBLA_RECENT && p.idx != nullptr;   // (no list given: no sequence is that long, says the caller)
+    const int count = selecting ? EMBLA_TOPK + EMBLA_RECENT : S;
+    // the groups of 32 rows, dealt to the warps of the CTAs in turn
+    const int groups = (count + KS_ROWS - 1) / KS_ROWS;
+    const uint32_t* idx = p.idx + (size_t(b) * p.n_kv_heads + kvh) * (EMBLA_TOPK + EMBLA_RECENT);
+    const int32_t* table = p.block_table + size_t(b) * p.table_stride;
+    uint8_t* stage0 = smem + warp * (KS_STAGES * KS_STAGE);
+    const int step = p.nsplit * KS_WARPS, first = split * KS_WARPS + warp;
+
+    // Lane i's row of a group: where it lies, as (page x 128 + row of the page), or -1 (behind the last one, or nowhere)
+    auto look_up = [&](int grp) {
+        const int j = grp * KS_ROWS + lane;
+        long at = -1;
+        if (grp < groups && j < count) {
+            const uint32_t pos = selecting ? idx[j] : uint32_t(j);
+            const int e = int(pos / BLK);
+            int block = -1;
+            if (pos < uint32_t(S) && e < p.table_stride) block = table[e];
+            if (block >= 0 && block < p.num_blocks) at = ((long(block) * p.n_layers + p.layer) * p.n_kv_heads + kvh) * BLK + long(pos % BLK);
+            else atomicExch(p.ctl.err, ERR_BAD_BLOCK);
+        }
+        return at;
+    };
+    // The copies of a group into stage `st`; rows that are nowhere become zeros. Every call makes one copy group.
+    auto request = [&](int st, long at) {
+        uint8_t* dst = stage0 + st * KS_STAGE;
+#pragma unroll
+        for (int it = 0; it < 4; it++) {
+            const int row = it * 8 + (lane >> 2), ch = lane & 3;
+            const long a = __shfl_sync(0xffffffffu, at, row);
+            const uint8_t* src = p.pool + (a < 0 ? 0 : size_t(a / BLK) * KV4_PAGE + size_t(a % BLK) * KV4_ROW + ch * 16);
+            cp_async16(dst + kv4_at(row, ch), src, a >= 0);
+            cp_async16(dst + KS_ROWS * KV4_ROW + kv4_at(row, ch), src + (a < 0 ? 0 : KV4_SIDE), a >= 0);
+        }
+        const uint8_t* src = p.pool + (at < 0 ? 0 : size_t(at / BLK) * KV4_PAGE + 2 * KV4_SIDE + size_t(at % BLK) * 16);
+        cp_async16(dst + 2 * KS_ROWS * KV4_ROW + lane * 16, src, at >= 0);
+    };
+    auto commit = []() { asm volatile("cp.async.commit_group;" ::: "memory"); };
+
+    // the first two groups' rows on their way, then the queries, then the third's
+    long at[KS_STAGES];
+    unsigned there[KS_STAGES];
+#pragma unroll
+    for (int i = 0; i < KS_STAGES; i++) at[i] = look_up(first + i * step);
+#pragma unroll
+    for (int i = 0; i < KS_STAGES; i++) {
+        there[i] = __ballot_sync(0xffffffffu, at[i] >= 0);
+        if (i < KS_STAGES - 1) {
+            if (first + i * step < groups) request(i, at[i]);
+            commit();
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8 / KS_WARPS; i++) {
+        const int hh = warp + i * KS_WARPS;
         float x[4];
-        kv_row_load<DT>(p.q, off, false, lane, x);
-        if (!p.prenormed) kv4_query_norm<DT>(x, p.g1, p.g2, p.ng, lane);
-        for (int i = 0; i < 4; i++) q[lane + 32 * i] = x[i];
+        kv4_load_query<DT>(x, hh < p.G, p.q, size_t(b) * p.q_stride + size_t(kvh * p.G + hh) * HD, lane);
+        kv4_stage_query<DT>(sq, hh, hh < p.G, x, p.prenormed != 0, p.g1, p.g2, p.ng, lane);
     }
     __syncthreads();
-    const float scale = rsqrtf(float(HD));
-    float m = NEG_BIG, den = 0.0f, acc = 0.0f;
-    for (int j0 = 0; j0 < n; j0 += BLK) {
-        // this thread's key
-        int pos = j0 + tid;
-        bool valid = pos < n;
-        if (selecting && valid) {
-            const uint32_t r = p.idx[(size_t(b) * p.n_kv_heads + kvh) * (EMBLA_TOPK + EMBLA_RECENT) + pos];
-            if (r >= uint32_t(S)) {
-                atomicExch(p.err, ERR_BAD_BLOCK);
-                valid = false;
-            }
-            pos = int(r);
+
+    const int r = lane >> 2, t = lane & 3;
+    Kv4Frag frag;
+    frag.load(sq, lane);
+    // scores in units of log2(e) / sqrt(128) x the query's power of two x 2^20
+    const float u0 = pow2_biased(max(sq.expo[2 * t], 1)) * (1.4426950408889634f * 0.08838834764831845f / KV4_SUBNORMAL);
+    const float u1 = pow2_biased(max(sq.expo[2 * t + 1], 1)) * (1.4426950408889634f * 0.08838834764831845f / KV4_SUBNORMAL);
+    float O[8][4];
+#pragma unroll
+    for (int i = 0; i < 8; i++) O[i][0] = O[i][1] = O[i][2] = O[i][3] = 0.0f;
+    float l0 = 0.0f, l1 = 0.0f, m0 = KS_NONE, m1 = KS_NONE;   // sums of weights, reference scores of heads 2t, 2t + 1
+    bool big = false;
+    float limit = KS_LIMIT;
+    int st = 0;
+#pragma unroll 1
+    for (int grp = first; grp < groups; grp += step) {
+        // the third group behind this one is looked up while this one is attended; the second goes out now
+        const int ahead = (st + KS_STAGES - 1) % KS_STAGES;
+        {
+            long a = at[0];
+            if (ahead == 1) a = at[1];
+            if (ahead == 2) a = at[2];
+            if (grp + (KS_STAGES - 1) * step < groups) request(ahead, a);
+            commit();
         }
-        const uint8_t* page = nullptr;
-        if (valid) {
-            const int e = pos / BLK, block = e < p.table_stride ? p.block_table[size_t(b) * p.table_stride + e] : -1;
-            if (block < 0 || block >= p.num_blocks) {
-                atomicExch(p.err, ERR_BAD_BLOCK);
-                valid = false;
-            } else {
-                page = p.pool + ((size_t(block) * p.n_layers + p.layer) * p.n_kv_heads + kvh) * KV4_PAGE;
-            }
+        const long far = look_up(grp + KS_STAGES * step);
+        unsigned ok = there[0];
+        if (st == 1) ok = there[1];
+        if (st == 2) ok = there[2];
+        asm volatile("cp.async.wait_group %0;" ::"n"(KS_STAGES - 1) : "memory");
+        __syncwarp();
+        const uint8_t* rows = stage0 + st * KS_STAGE;
+        const uint32_t kaddr = smem_u32(rows) + kv4_lane_at(lane);
+        float s[2][4];
+        Kv4Scales sc[2];
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            sc[k].load(rows + 2 * KS_ROWS * KV4_ROW + k * 256, lane);
+            kv4_tile_scores(kaddr + k * 16 * KV4_ROW, sc[k], frag, s[k]);
         }
-        float s = 0.0f;
-        const int row = pos % BLK;
-        if (valid) {
-            const __half* sc = reinterpret_cast<const __half*>(page + 2 * KV4_SIDE) + row * 2 * KV4_GROUPS;
-            for (int g = 0; g < KV4_GROUPS; g++) {
-                float part = 0.0f;
-                for (int c = 0; c < 4; c++) {
-                    const uint32_t word = reinterpret_cast<const uint32_t*>(page + row * KV4_ROW)[g * 4 + c];
-                    for (int d = 0; d < 8; d++) part = fmaf(q[g * 32 + c * 8 + d], float(int(word << (28 - 4 * kv4_nibble_of(d))) >> 28), part);
+        float w[2][4], top = 0.0f;
+        bool flagged = false;
+        auto weigh = [&]() {
+            top = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const bool k0 = (ok >> (16 * k + r)) & 1, k1 = (ok >> (16 * k + r + 8)) & 1;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    // (a NaN score stays one)
+                    w[k][e] = (e < 2 ? k0 : k1) ? ks_exp2(fmaf(s[k][e], (e & 1) ? u1 : u0, -((e & 1) ? m1 : m0))) : 0.0f;
+                    top = fmaxf(top, w[k][e]);
                 }
-                s = fmaf(part, __half2float(sc[g]), s);
             }
-            if (p.scores) {   // max over the kv head's query heads: heads write one after another
-                float* at = p.scores + (size_t(b) * p.n_kv_heads + kvh) * p.scores_stride + pos;
-                if (s >= 0.0f) atomicMax(reinterpret_cast<int*>(at), __float_as_int(s));
-                else atomicMin(reinterpret_cast<unsigned*>(at), __float_as_uint(s));
+        };
+        weigh();
+        flagged = sc[0].large() || sc[1].large();
+        if (__any_sync(0xffffffffu, top > limit || (flagged && !big))) {
+            // new references, no lower than the old: the group's largest score of a head weighs 2^target or less
+            if (__any_sync(0xffffffffu, flagged)) {
+                big = true;
+                limit = KS_LIMIT_BIG;
             }
+            float t0 = KS_NONE, t1 = KS_NONE;
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const bool k0 = (ok >> (16 * k + r)) & 1, k1 = (ok >> (16 * k + r + 8)) & 1;
+                if (k0) t0 = fmaxf(t0, s[k][0] * u0), t1 = fmaxf(t1, s[k][1] * u1);
+                if (k1) t0 = fmaxf(t0, s[k][2] * u0), t1 = fmaxf(t1, s[k][3] * u1);
+            }
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
+                t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
+            }
+            const float target = big ? KS_TARGET_BIG : KS_TARGET;
+            const float n0 = fmaxf(m0, t0 - target), n1 = fmaxf(m1, t1 - target);
+            const float c0 = ks_exp2(m0 - n0), c1 = ks_exp2(m1 - n1);
+            m0 = n0;
+            m1 = n1;
+            l0 *= c0;
+            l1 *= c1;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                O[k][0] *= c0;
+                O[k][1] *= c1;
+                O[k][2] *= c0;
+                O[k][3] *= c1;
+            }
+            weigh();
         }
-        s *= scale;
-        if (p.softmax) {
-            float mt = valid ? s : NEG_BIG;
-            for (int o = 16; o > 0; o >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
-            if (lane == 0) red[warp] = mt;
-            __syncthreads();
-            mt = fmaxf(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), m);
-            const float f = __expf(m - mt);
-            den *= f;
-            acc *= f;
-            m = mt;
-            s = valid ? __expf(s - m) : 0.0f;
-        } else {
-            s = valid ? fmaxf(s, 0.0f) : 0.0f;
-            s *= s;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            l0 += w[k][0] + w[k][2];
+            l1 += w[k][1] + w[k][3];
+            kv4_tile_values(kaddr + KS_ROWS * KV4_ROW + k * 16 * KV4_ROW, sc[k], w[k], O);
         }
-        w[tid] = s;
-        __syncthreads();
-        // this thread's head dim
-        const int word = tid >> 3, nib = kv4_nibble_of(tid & 7), g = tid >> 5;
-        for (int k = 0; k < BLK && j0 + k < n; k++) {
-            int ps = j0 + k;
-            if (selecting) ps = int(p.idx[(size_t(b) * p.n_kv_heads + kvh) * (EMBLA_TOPK + EMBLA_RECENT) + ps]);
-            const float wk = w[k];
-            den += wk;
-            if (wk == 0.0f) continue;   // (invalid keys among them)
-            const int block = p.block_table[size_t(b) * p.table_stride + ps / BLK], r = ps % BLK;
-            const uint8_t* pg = p.pool + ((size_t(block) * p.n_layers + p.layer) * p.n_kv_heads + kvh) * KV4_PAGE;
-            const uint32_t c = reinterpret_cast<const uint32_t*>(pg + KV4_SIDE + r * KV4_ROW)[word];
-            const float vs = __half2float(reinterpret_cast<const __half*>(pg + 2 * KV4_SIDE)[r * 2 * KV4_GROUPS + KV4_GROUPS + g]);
-            acc = fmaf(wk, float(int(c << (28 - 4 * nib)) >> 28) * vs, acc);
-        }
-        __syncthreads();
+        const unsigned ob = __ballot_sync(0xffffffffu, far >= 0);
+        if (st == 0) at[0] = far, there[0] = ob;
+        if (st == 1) at[1] = far, there[1] = ob;
+        if (st == 2) at[2] = far, there[2] = ob;
+        st = st + 1 == KS_STAGES ? 0 : st + 1;
+        __syncwarp();   // (the stage is read: the next turn's copies go into it)
     }
-    const float total = p.softmax ? (den > 0.0f ? den : 1.0f) : sqrtf(float(HD)) + den;
-    Act<DT>::store(p.o, size_t(b) * p.o_seq_stride + size_t(t) * p.o_token_stride + size_t(head) * HD + tid, acc / total);
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    trace_last(p.ctl.trace, 2);
+    __syncthreads();
+    // ---- the warps' sums into one: under the largest reference
+    float* sums = reinterpret_cast<float*>(smem);
+    float* refs = sums + KS_WARPS * 8 * KS_SUM;   // [KS_WARPS][8] references, then as many sums of weights
+    float* wsum = refs + KS_WARPS * 8;
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, o);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, o);
+    }
+    if (2 * t < p.G) {
+        float* row0 = sums + (warp * 8 + 2 * t) * KS_SUM;
+        float* row1 = row0 + KS_SUM;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int d = kv4_dim_of(k, r);
+            row0[d] = O[k][0];
+            row1[d] = O[k][1];
+            row0[d + 2] = O[k][2];
+            row1[d + 2] = O[k][3];
+        }
+        if (r == 0) {
+            refs[warp * 8 + 2 * t] = m0;
+            refs[warp * 8 + 2 * t + 1] = m1;
+            wsum[warp * 8 + 2 * t] = l0;
+            wsum[warp * 8 + 2 * t + 1] = l1;
+        }
+    }
+    if (CL) cluster_wait();
+    __syncthreads();
+    float* inbox = reinterpret_cast<float*>(smem + ks_inbox_at());
+    const int own = (p.G + p.nsplit - 1) / p.nsplit;   // heads that a CTA finishes
+    for (int i = tid; i < p.G * HD; i += KS_WARPS * 32) {
+        const int hh = i >> 7, d = i & 127;
+        float M = KS_NONE;
+#pragma unroll
+        for (int w = 0; w < KS_WARPS; w++) M = fmaxf(M, refs[w * 8 + hh]);
+        float num = 0.0f, den = 0.0f;
+#pragma unroll
+        for (int w = 0; w < KS_WARPS; w++) {
+            const float f = ks_exp2(refs[w * 8 + hh] - M);
+            num += sums[(w * 8 + hh) * KS_SUM + d] * f;
+            den += wsum[w * 8 + hh] * f;
+        }
+        if (!CL) {
+            // (no keys: zeros)
+            Act<DT>::store(p.o, size_t(b) * p.o_stride + size_t(kvh * p.G + hh) * HD + d, den == 0.0f ? 0.0f : num / den);
+        } else {
+            const uint32_t row = cluster_map(smem_u32(inbox + (split * own + hh / p.nsplit) * KS_PART), uint32_t(hh % p.nsplit));
+            cluster_st_f32(row + uint32_t(d) * 4u, num);
+            if (d == 0) {
+                cluster_st_f32(row + HD * 4, den);
+                cluster_st_f32(row + (HD + 1) * 4, M);
+            }
+        }
+    }
+    if (CL) {
+        // one cluster barrier: every range's rows are with their owners; CTA `split` finishes heads split, split + nsplit, ...
+        cluster_arrive();
+        cluster_wait();
+        for (int i = tid; i < own * HD; i += KS_WARPS * 32) {
+            const int slot = i >> 7, d = i & 127, hh = split + slot * p.nsplit;
+            if (hh >= p.G) continue;
+            float M = KS_NONE, num = 0.0f, den = 0.0f;
+            for (int k = 0; k < p.nsplit; k++) M = fmaxf(M, inbox[(k * own + slot) * KS_PART + HD + 1]);
+            for (int k = 0; k < p.nsplit; k++) {
+                const float* row = inbox + (k * own + slot) * KS_PART;
+                const float f = ks_exp2(row[HD + 1] - M);
+                num += row[d] * f;
+                den += row[HD] * f;
+            }
+            Act<DT>::store(p.o, size_t(b) * p.o_stride + size_t(kvh * p.G + hh) * HD + d, den == 0.0f ? 0.0f : num / den);
+        }
+    }
+    trace_last(p.ctl.trace, 3);
 }
 
-static EmblaStatus launch_attend(EmblaAttn* ctx, Attend4Params& p, const EmblaKVPool* pool, const EmblaKVView* view, const EmblaQuery* q,
-                                 int tokens, cudaStream_t s) {
-    p.pool = pool->base;
-    p.block_table = view->block_table_dev;
-    p.seq_lens = view->seq_lens_dev;
-    p.q = q->q_dev;
-    p.g1 = q->g1_dev;
-    p.g2 = q->g2_dev;
-    p.err = ctx->err_dev;
-    p.table_stride = view->table_stride;
-    p.layer = view->layer;
-    p.n_layers = pool->n_layers;
-    p.n_kv_heads = pool->n_kv_heads;
-    p.num_blocks = pool->num_blocks;
-    p.G = ctx->cfg.n_q_heads / ctx->cfg.n_kv_heads;
-    p.prenormed = q->prenormed;
-    p.ng = q->ng;
-    const dim3 grid(ctx->cfg.n_q_heads, tokens, view->batch);
-    if (ctx->cfg.act_dtype == EMBLA_BF16) EMBLA_CUDA_TRY(launch_kernel(ctx->pdl, kv4_attend_kernel<EMBLA_BF16>, grid, dim3(128), 0, s, p));
-    else EMBLA_CUDA_TRY(launch_kernel(ctx->pdl, kv4_attend_kernel<EMBLA_F16>, grid, dim3(128), 0, s, p));
+template <int DT, bool CL>
+static EmblaStatus launch_kv4_sparse(EmblaAttn* ctx, const Kv4SparseParams& p, int batch, cudaStream_t s) {
+    auto kern = kv4_sparse_kernel<DT, CL>;
+    static bool configured[64] = {};   // per instantiation and device
+    if (!configured[ctx->device & 63]) {
+        // (the largest inbox: 7 ranges of 8 heads, two each)
+        EMBLA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(ks_smem(CL ? 7 : 1, 8))));
+        configured[ctx->device & 63] = true;
+    }
+    const dim3 grid(p.nsplit, p.n_kv_heads, batch);
+    EMBLA_CUDA_TRY(launch_kernel_cluster(ctx->pdl, CL ? p.nsplit : 1, kern, grid, dim3(KS_WARPS * 32), ks_smem(p.nsplit, p.G), s, p));
+    EMBLA_CUDA_TRY(cudaGetLastError());
     return EMBLA_OK;
-}
-
-EmblaStatus kv4_full_prefill(EmblaAttn* ctx, const EmblaKVPool* pool, const EmblaKVView* view, const int32_t* pos0, int n_tokens,
-                             const EmblaQuery* q, int64_t q_token_stride, void* o_dev, int64_t o_token_stride, int64_t o_seq_stride,
-                             cudaStream_t stream) {
-    Attend4Params p = {};
-    p.o = o_dev;
-    p.pos0 = pos0;
-    p.q_seq_stride = q->q_stride;
-    p.q_token_stride = q_token_stride;
-    p.o_seq_stride = o_seq_stride;
-    p.o_token_stride = o_token_stride;
-    return launch_attend(ctx, p, pool, view, q, n_tokens, stream);
 }
 
 }  // namespace embla
@@ -175,11 +337,41 @@ extern "C" EmblaStatus embla_attn_sparse_decode_int4(EmblaAttn* ctx, const Embla
     if (max_len > EMBLA_TOPK + EMBLA_RECENT && !idx_dev)
         EMBLA_FAIL(EMBLA_BAD_ARG, "embla_attn_sparse_decode_int4: sequences past %d keys need the selected rows",
                    EMBLA_TOPK + EMBLA_RECENT);
-    Attend4Params p = {};
+    Kv4SparseParams p = {};
+    p.pool = pool->base;
+    p.block_table = view->block_table_dev;
     p.idx = idx_dev;
+    p.seq_lens = view->seq_lens_dev;
+    p.q = q->q_dev;
+    p.g1 = q->g1_dev;
+    p.g2 = q->g2_dev;
     p.o = o_dev;
-    p.q_seq_stride = q->q_stride;
-    p.o_seq_stride = o_stride;
-    p.softmax = 1;
-    return launch_attend(ctx, p, pool, view, q, 1, static_cast<cudaStream_t>(stream));
+    p.ctl = kernel_ctl(ctx);
+    p.q_stride = q->q_stride;
+    p.o_stride = o_stride;
+    p.table_stride = view->table_stride;
+    p.layer = view->layer;
+    p.n_layers = pool->n_layers;
+    p.n_kv_heads = pool->n_kv_heads;
+    p.num_blocks = pool->num_blocks;
+    p.G = ctx->cfg.n_q_heads / ctx->cfg.n_kv_heads;
+    p.prenormed = q->prenormed;
+    p.ng = q->ng;
+    // CTAs a (sequence, kv head): what costs least in groups of rows a warp works through one after another, waves of CTAs
+    // counted (four an SM), plus what a CTA costs beside them
+    const int rows = max_len < EMBLA_TOPK + EMBLA_RECENT ? max_len : EMBLA_TOPK + EMBLA_RECENT;
+    const long units = long(view->batch) * p.n_kv_heads, groups = (rows + KS_ROWS - 1) / KS_ROWS;
+    long best = -1;
+    for (int ns = 1; ns <= KS_MAX_CLUSTER && (ns == 1 || KS_WARPS * (ns - 1) < groups); ns++) {
+        const long waves = (units * ns + 4 * ctx->sm_count - 1) / (4 * ctx->sm_count);
+        const long cost = waves * ((groups + ns * KS_WARPS - 1) / (ns * KS_WARPS) + 4) + (ns > 1 ? 1 : 0);
+        if (best < 0 || cost < best) {
+            best = cost;
+            p.nsplit = ns;
+        }
+    }
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool bf = ctx->cfg.act_dtype == EMBLA_BF16;
+    if (p.nsplit > 1) return bf ? launch_kv4_sparse<EMBLA_BF16, true>(ctx, p, view->batch, s) : launch_kv4_sparse<EMBLA_F16, true>(ctx, p, view->batch, s);
+    return bf ? launch_kv4_sparse<EMBLA_BF16, false>(ctx, p, view->batch, s) : launch_kv4_sparse<EMBLA_F16, false>(ctx, p, view->batch, s);
 }
