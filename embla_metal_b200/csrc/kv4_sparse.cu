@@ -3,8 +3,8 @@
 // int8 (attn_sparse8 / attn_sparse_short, attention.metal:448-645; sparse8_decode.cu).
 //
 // A row is 144 bytes in nine 16-byte pieces at an address that two dependent lookups give (selected position, its block), so this
-// is a matter of latency and of rows in flight. Each warp works alone: 32 rows at a time, lane i looking up row i, the copies
-// (cp.async) of three groups in flight, two 16-key tiles of a group at once on the tensor-core tiles of kv4_tile.cuh. Its
+// is a matter of latency and of rows in flight. Each warp works alone: it looks up all its rows, then takes them 32 at a time, the
+// copies (cp.async) of three groups in flight, two 16-key tiles of a group at once on the tensor-core tiles of kv4_tile.cuh. Its
 // softmax keeps a reference score that moves (the sums with it) only when a weight passes 2^13. Up to eight CTAs a (sequence, kv
 // head), as a thread-block cluster, when there are few of them.
 #include "attn16_common.cuh"
@@ -18,6 +18,8 @@ constexpr int KS_SUM = HD + 1, KS_PART = HD + 4;                     // floats o
 constexpr int KS_MAX_CLUSTER = 8;
 // largest weight, and the one a moved reference gives the row's largest score; the second pair with value scales of 2 and more
 constexpr float KS_LIMIT = 8192.0f, KS_LIMIT_BIG = 0.5f, KS_TARGET = 10.0f, KS_TARGET_BIG = -4.0f;
+constexpr int KS_MAX_GROUPS = (EMBLA_TOPK + EMBLA_RECENT) / KS_ROWS / KS_WARPS;   // of a warp, in a CTA that has all rows to itself
+constexpr uint32_t KS_NOWHERE = 0xffffffffu;
 constexpr float KS_NONE = -1e30f;                                    // a reference before any key
 
 struct Kv4SparseParams {
@@ -35,7 +37,8 @@ struct Kv4SparseParams {
 };
 
 constexpr size_t ks_queries_at() { return size_t(KS_WARPS) * KS_STAGES * KS_STAGE; }
-constexpr size_t ks_inbox_at() { return ks_queries_at() + sizeof(Kv4Queries); }
+constexpr size_t ks_where_at() { return ks_queries_at() + sizeof(Kv4Queries); }
+constexpr size_t ks_inbox_at() { return ks_where_at() + size_t(KS_WARPS) * KS_MAX_GROUPS * KS_ROWS * 4; }
 constexpr int ks_inbox_rows(int ranges, int G) { return ranges * ((G + ranges - 1) / ranges); }
 constexpr size_t ks_smem(int ranges, int G) { return 1024 + ks_inbox_at() + (ranges > 1 ? size_t(ks_inbox_rows(ranges, G)) * KS_PART * 4 : 0); }
 static_assert(KS_WARPS * 8 * (KS_SUM + 2) * 4 <= KS_WARPS * KS_STAGES * KS_STAGE, "the warps' sums lie over their stages");
@@ -59,8 +62,8 @@ __global__ void __launch_bounds__(KS_WARPS * 32, 4) kv4_sparse_kernel(const __gr
     pdl_wait();
     pdl_launch_dependents();
     trace_first(p.ctl.trace, 1);
-    const bool selecting = S > EMBLA_TOPK + EMBLA_RECENT && p.idx != nullptr;   // (no list given: no sequence is that long, says the caller)
-    const int count = selecting ? EMBLA_TOPK + EMBLA_RECENT : S;
+    const bool selecting = S > EMBLA_TOPK + EMBLA_RECENT && p.idx != nullptr;
+    const int count = min(S, EMBLA_TOPK + EMBLA_RECENT);   // (no list given: no sequence is longer, says the caller)
     // the groups of 32 rows, dealt to the warps of the CTAs in turn
     const int groups = (count + KS_ROWS - 1) / KS_ROWS;
     const uint32_t* idx = p.idx + (size_t(b) * p.n_kv_heads + kvh) * (EMBLA_TOPK + EMBLA_RECENT);
@@ -68,49 +71,56 @@ __global__ void __launch_bounds__(KS_WARPS * 32, 4) kv4_sparse_kernel(const __gr
     uint8_t* stage0 = smem + warp * (KS_STAGES * KS_STAGE);
     const int step = p.nsplit * KS_WARPS, first = split * KS_WARPS + warp;
 
-    // Lane i's row of a group: where it lies, as (page x 128 + row of the page), or -1 (behind the last one, or nowhere)
-    auto look_up = [&](int grp) {
-        const int j = grp * KS_ROWS + lane;
-        long at = -1;
-        if (grp < groups && j < count) {
-            const uint32_t pos = selecting ? idx[j] : uint32_t(j);
-            const int e = int(pos / BLK);
-            int block = -1;
-            if (pos < uint32_t(S) && e < p.table_stride) block = table[e];
-            if (block >= 0 && block < p.num_blocks) at = ((long(block) * p.n_layers + p.layer) * p.n_kv_heads + kvh) * BLK + long(pos % BLK);
-            else atomicExch(p.ctl.err, ERR_BAD_BLOCK);
-        }
-        return at;
-    };
-    // The copies of a group into stage `st`; rows that are nowhere become zeros. Every call makes one copy group.
-    auto request = [&](int st, long at) {
-        uint8_t* dst = stage0 + st * KS_STAGE;
+    // Where the rows of all the warp's groups lie, as (page x 128 + row of the page), or KS_NOWHERE (behind the last one, or outside
+    // the pool): the selected positions' loads in flight together, then those of the blocks, so that the chain of lookups is
+    // walked once and not every group.
+    uint32_t* where = reinterpret_cast<uint32_t*>(smem + ks_where_at()) + warp * (KS_MAX_GROUPS * KS_ROWS);
+    {
+        uint32_t pos[KS_MAX_GROUPS];
+        int block[KS_MAX_GROUPS];
 #pragma unroll
-        for (int it = 0; it < 4; it++) {
-            const int row = it * 8 + (lane >> 2), ch = lane & 3;
-            const long a = __shfl_sync(0xffffffffu, at, row);
-            const uint8_t* src = p.pool + (a < 0 ? 0 : size_t(a / BLK) * KV4_PAGE + size_t(a % BLK) * KV4_ROW + ch * 16);
-            cp_async16(dst + kv4_at(row, ch), src, a >= 0);
-            cp_async16(dst + KS_ROWS * KV4_ROW + kv4_at(row, ch), src + (a < 0 ? 0 : KV4_SIDE), a >= 0);
+        for (int i = 0; i < KS_MAX_GROUPS; i++) {
+            const int j = (first + i * step) * KS_ROWS + lane;
+            pos[i] = 0xffffffffu;
+            if (j < count) pos[i] = selecting ? idx[j] : uint32_t(j);
         }
-        const uint8_t* src = p.pool + (at < 0 ? 0 : size_t(at / BLK) * KV4_PAGE + 2 * KV4_SIDE + size_t(at % BLK) * 16);
-        cp_async16(dst + 2 * KS_ROWS * KV4_ROW + lane * 16, src, at >= 0);
-    };
-    auto commit = []() { asm volatile("cp.async.commit_group;" ::: "memory"); };
-
-    // the first two groups' rows on their way, then the queries, then the third's
-    long at[KS_STAGES];
-    unsigned there[KS_STAGES];
 #pragma unroll
-    for (int i = 0; i < KS_STAGES; i++) at[i] = look_up(first + i * step);
-#pragma unroll
-    for (int i = 0; i < KS_STAGES; i++) {
-        there[i] = __ballot_sync(0xffffffffu, at[i] >= 0);
-        if (i < KS_STAGES - 1) {
-            if (first + i * step < groups) request(i, at[i]);
-            commit();
+        for (int i = 0; i < KS_MAX_GROUPS; i++) {
+            block[i] = -1;
+            if (pos[i] < uint32_t(S) && int(pos[i] / BLK) < p.table_stride) block[i] = table[pos[i] / BLK];
         }
+#pragma unroll
+        for (int i = 0; i < KS_MAX_GROUPS; i++) {
+            uint32_t at = KS_NOWHERE;
+            if (block[i] >= 0 && block[i] < p.num_blocks)
+                at = uint32_t((long(block[i]) * p.n_layers + p.layer) * p.n_kv_heads + kvh) * BLK + pos[i] % BLK;
+            else if ((first + i * step) * KS_ROWS + lane < count) atomicExch(p.ctl.err, ERR_BAD_BLOCK);
+            where[i * KS_ROWS + lane] = at;
+        }
+        __syncwarp();
     }
+    // The copies of the warp's group i into its stage; rows that are nowhere become zeros. Every call makes one copy group.
+    auto request = [&](int i) {
+        if (first + i * step < groups) {
+            uint8_t* dst = stage0 + i % KS_STAGES * KS_STAGE;
+            const uint32_t* at = where + i * KS_ROWS;
+#pragma unroll
+            for (int it = 0; it < 4; it++) {
+                const int row = it * 8 + (lane >> 2), ch = lane & 3;
+                const uint32_t a = at[row];
+                const uint8_t* src = p.pool + (a == KS_NOWHERE ? 0 : size_t(a / BLK) * KV4_PAGE + (a % BLK) * KV4_ROW + ch * 16);
+                cp_async16(dst + kv4_at(row, ch), src, a != KS_NOWHERE);
+                cp_async16(dst + KS_ROWS * KV4_ROW + kv4_at(row, ch), src + KV4_SIDE, a != KS_NOWHERE);
+            }
+            const uint32_t a = at[lane];
+            const uint8_t* src = p.pool + (a == KS_NOWHERE ? 0 : size_t(a / BLK) * KV4_PAGE + 2 * KV4_SIDE + (a % BLK) * 16);
+            cp_async16(dst + 2 * KS_ROWS * KV4_ROW + lane * 16, src, a != KS_NOWHERE);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    // the first two groups' rows on their way, then the queries
+#pragma unroll
+    for (int i = 0; i < KS_STAGES - 1; i++) request(i);
 #pragma unroll
     for (int i = 0; i < 8 / KS_WARPS; i++) {
         const int hh = warp + i * KS_WARPS;
@@ -132,25 +142,13 @@ __global__ void __launch_bounds__(KS_WARPS * 32, 4) kv4_sparse_kernel(const __gr
     float l0 = 0.0f, l1 = 0.0f, m0 = KS_NONE, m1 = KS_NONE;   // sums of weights, reference scores of heads 2t, 2t + 1
     bool big = false;
     float limit = KS_LIMIT;
-    int st = 0;
 #pragma unroll 1
-    for (int grp = first; grp < groups; grp += step) {
-        // the third group behind this one is looked up while this one is attended; the second goes out now
-        const int ahead = (st + KS_STAGES - 1) % KS_STAGES;
-        {
-            long a = at[0];
-            if (ahead == 1) a = at[1];
-            if (ahead == 2) a = at[2];
-            if (grp + (KS_STAGES - 1) * step < groups) request(ahead, a);
-            commit();
-        }
-        const long far = look_up(grp + KS_STAGES * step);
-        unsigned ok = there[0];
-        if (st == 1) ok = there[1];
-        if (st == 2) ok = there[2];
+    for (int i = 0; first + i * step < groups; i++) {
+        request(i + KS_STAGES - 1);
+        const unsigned ok = __ballot_sync(0xffffffffu, where[i * KS_ROWS + lane] != KS_NOWHERE);
         asm volatile("cp.async.wait_group %0;" ::"n"(KS_STAGES - 1) : "memory");
         __syncwarp();
-        const uint8_t* rows = stage0 + st * KS_STAGE;
+        const uint8_t* rows = stage0 + i % KS_STAGES * KS_STAGE;
         const uint32_t kaddr = smem_u32(rows) + kv4_lane_at(lane);
         float s[2][4];
         Kv4Scales sc[2];
@@ -216,11 +214,6 @@ __global__ void __launch_bounds__(KS_WARPS * 32, 4) kv4_sparse_kernel(const __gr
             l1 += w[k][1] + w[k][3];
             kv4_tile_values(kaddr + KS_ROWS * KV4_ROW + k * 16 * KV4_ROW, sc[k], w[k], O);
         }
-        const unsigned ob = __ballot_sync(0xffffffffu, far >= 0);
-        if (st == 0) at[0] = far, there[0] = ob;
-        if (st == 1) at[1] = far, there[1] = ob;
-        if (st == 2) at[2] = far, there[2] = ob;
-        st = st + 1 == KS_STAGES ? 0 : st + 1;
         __syncwarp();   // (the stage is read: the next turn's copies go into it)
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
