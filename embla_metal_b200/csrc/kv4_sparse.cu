@@ -4,7 +4,7 @@
 //
 // A row is 144 bytes in nine 16-byte pieces at an address that two dependent lookups give (selected position, its block), so this
 // is a matter of latency and of rows in flight. Each warp works alone: it looks up all its rows, then takes them 32 at a time, the
-// copies (cp.async) of three groups in flight, two 16-key tiles of a group at once on the tensor-core tiles of kv4_tile.cuh. Its
+// copies (cp.async) of two groups in flight, two 16-key tiles of a group at once on the tensor-core tiles of kv4_tile.cuh. Its
 // softmax keeps a reference score that moves (the sums with it) only when a weight passes 2^13. Up to eight CTAs a (sequence, kv
 // head), as a thread-block cluster, when there are few of them.
 #include "attn16_common.cuh"
@@ -12,7 +12,7 @@
 
 namespace embla {
 
-constexpr int KS_WARPS = 4, KS_STAGES = 3, KS_ROWS = 32;
+constexpr int KS_WARPS = 4, KS_STAGES = 2, KS_ROWS = 32;   // (three stages leave room for three CTAs an SM, not four)
 constexpr int KS_STAGE = KS_ROWS * (2 * KV4_ROW + 4 * KV4_GROUPS);   // a group's rows: K codes, V codes, scales: 4608 bytes
 constexpr int KS_SUM = HD + 1, KS_PART = HD + 4;                     // floats of a row of sums: in shared memory, between CTAs
 constexpr int KS_MAX_CLUSTER = 8;
