@@ -22,7 +22,7 @@
 // TMEM (512 columns): per tile S 128 (P aliases its first 64) and O 128. q is converted to fp16 once (bf16 values are exact
 // in fp16 inside its normal range); int8 codes and their products are exact; accumulation is fp32.
 // Every wait is bounded; a wait that runs out sets the context's error word and the CTA winds down.
-#include "kv_row.cuh"
+#include "kv4_tile.cuh"
 #include "tc05.cuh"
 
 namespace embla {
@@ -66,7 +66,7 @@ struct PrefillParams {
     int* counters;        // [2][units]: the unit's ranges that have announced themselves, and those whose partials are written
     int64_t q_token_stride, q_seq_stride, o_token_stride, o_seq_stride;
     size_t page_bytes;
-    int table_stride, layer, n_layers, n_kv_heads, G, scale_bytes, rows_per_page, n_tokens, prenormed, nsplit;
+    int table_stride, layer, n_layers, n_kv_heads, G, scale_bytes, rows_per_page, num_blocks, n_tokens, prenormed, nsplit;
     int cls;              // cluster size (0: none, else = nsplit): the page ranges of a unit are the CTAs of one thread-block
                           // cluster, whose partial sums stay in shared memory
     int heads, pairs;     // query heads and 256-token tile pairs of the launch: unit = (sequence x heads + head) x pairs + pair
@@ -115,6 +115,40 @@ __device__ __forceinline__ void convert_side(const uint8_t* raw, uint8_t* dst, i
     }
 }
 
+// 4-bit pages (EMBLA_KV_INT4, kv4.cuh): the same kernel with other converters. A group's 16 bytes of codes become 32 fp16 values,
+// code x scale rounded once (2^-11); queries enter scaled by 2^-7 and the keys without 1 / sqrt(D), whose square, 2^-7, is exact
+// in the weights: P = relu(s)^2 comes out as the weight x 2^-7 (scores up to 2895 square inside fp16's range), the sink takes
+// the same factor. Weights and their sums stay in fp32 until the one rounding of P to fp16.
+constexpr float PF4_QSCALE = 1.0f / 128.0f, PF4_PSCALE = 1.0f / 128.0f;
+
+// One side of a raw 4-bit page -> fp16 in the UMMA layout; rows from `lim` on (behind the last key, or all of a page that is
+// nowhere) become zeros, whatever lies there. 128 converter threads; the lanes of a quarter warp take 8 consecutive rows of one
+// group, so reads and writes are conflict-free.
+__device__ __forceinline__ void convert_side4(const uint8_t* raw, uint8_t* dst, int ctid, int side, int lim) {
+    const int rl = ctid & 7, g = (ctid >> 3) & 3, rg = ctid >> 5;
+    const __half* scales = reinterpret_cast<const __half*>(raw + KV4_SIDE) + side * KV4_GROUPS + g;
+#pragma unroll
+    for (int it = 0; it < BLK / (8 * PF_CONV_WARPS); it++) {
+        const int row = it * 8 * PF_CONV_WARPS + rg * 8 + rl;
+        uint4 w = *reinterpret_cast<const uint4*>(raw + kv4_at(row, g));
+        __half2 sc = __half2half2(scales[row * 2 * KV4_GROUPS]);
+        if (row >= lim) {
+            w = make_uint4(0, 0, 0, 0);
+            sc = __half2half2(__ushort_as_half(0));
+        }
+        const uint32_t x[4] = {w.x, w.y, w.z, w.w}, s2 = *reinterpret_cast<const uint32_t*>(&sc);
+        // dims 32 g .. 32 g + 31: four 16-byte chunks of the half (dims 0-63 | 64-127) that the group lies in
+        uint8_t* base = dst + (g >> 1) * (BLK * 128) + row * 128;
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            uint32_t h[4];
+            kv4_widen(x[c], h);
+            *reinterpret_cast<uint4*>(base + (((((g & 1) << 2) | c) ^ (row & 7)) << 4)) =
+                make_uint4(h2_mul(h[0], s2), h2_mul(h[1], s2), h2_mul(h[2], s2), h2_mul(h[3], s2));
+        }
+    }
+}
+
 // QK8: the reference's int8 Q Kᵀ variant (attn_nax.metal:14-22, 124-204 with q_prep_b's QK8 branch, prefill.metal:421-422;
 // switched on by EMBLA_ATT8, Prefill.swift:142-144): every query row is quantised like a cache row (write_row8: rounded to
 // the activation dtype, codes rint(x 127 / max|x|), scale max|x| / 127), S = Q8 K8ᵀ runs as tcgen05.mma kind::i8 on the
@@ -137,8 +171,9 @@ struct PfSegment {
     int jb, je;             // the pages
 };
 
-template <int DT, int SB, bool QK8>
+template <int DT, int SB, bool QK8, bool KV4>
 __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, const PrefillParams& p, const PfSegment sg) {
+    constexpr float QSCALE = KV4 ? PF4_QSCALE : PF_QSCALE, PSCALE = KV4 ? PF4_PSCALE : PF_PSCALE;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* Qs = smem;                                               // [2 tiles][32 KiB]
@@ -158,6 +193,7 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
     uint64_t* kf_ready = bars + 17;       // [2 pages] QK8: the page's key factors are set out (converters -> ReLU² warps)
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort, s_last;
+    __shared__ volatile int s_lim[3];     // KV4: keys that count in the page side of each ring slot
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int h = sg.h, b = sg.b, pair_ix = sg.pair_ix, split = sg.split, nparts = sg.nparts, slot0 = sg.slot0;
@@ -195,6 +231,22 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
     // conversion c = 2 j + side takes ring slot c % 3; page j's scales go to scl[j & 1]
     auto request = [&](int c) {
         const int j = jb + (c >> 1), side = c & 1, slot = c % 3;
+        if (KV4) {
+            // codes into the ring slot, the page's scales behind them (with either side: 2 KB more than needed once a page)
+            const int blk = j < p.table_stride ? p.block_table[size_t(b) * p.table_stride + j] : -1;
+            if (blk < 0 || blk >= p.num_blocks) {
+                atomicExch(p.ctl.err, ERR_BAD_BLOCK);
+                s_lim[slot] = 0;
+                mbar_arrive(&raw_full[slot]);
+                return;
+            }
+            const long pg = (long(blk) * p.n_layers + p.layer) * p.n_kv_heads + kvh;
+            s_lim[slot] = p0 + p.n_tokens - j * BLK;
+            mbar_expect_tx(&raw_full[slot], KV4_SIDE + KV4_SCALES);
+            tma_load_2d(raw + slot * CODE_BYTES, &tmap, 0, int(pg * (KV4_PAGE / 128)) + side * (KV4_SIDE / 128), &raw_full[slot]);
+            bulk_load_1d(raw + slot * CODE_BYTES + KV4_SIDE, p.pool + size_t(pg) * KV4_PAGE + 2 * KV4_SIDE, KV4_SCALES, &raw_full[slot]);
+            return;
+        }
         const int block = p.block_table[size_t(b) * p.table_stride + j];
         const long page = (long(block) * p.n_layers + p.layer) * p.n_kv_heads + kvh;
         mbar_expect_tx(&raw_full[slot], CODE_BYTES + (side == 0 ? 2 * BLK * SB : 0));
@@ -237,9 +289,9 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
                 if (DT == EMBLA_BF16) {
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        w[e] = pack_h2(__uint_as_float(w[e] << 16) * PF_QSCALE, __uint_as_float(w[e] & 0xffff0000u) * PF_QSCALE);
+                        w[e] = pack_h2(__uint_as_float(w[e] << 16) * QSCALE, __uint_as_float(w[e] & 0xffff0000u) * QSCALE);
                 } else {
-                    const __half2 qs2 = __float2half2_rn(PF_QSCALE);
+                    const __half2 qs2 = __float2half2_rn(QSCALE);
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const __half2 t = __hmul2(*reinterpret_cast<const __half2*>(&w[e]), qs2);
@@ -329,7 +381,7 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
                     for (int i = 0; i < 4; i++) {
                         const int d = lane + 32 * i, c8 = d >> 3;
                         *reinterpret_cast<__half*>(Qx + (c8 >> 3) * (BLK * 128) + r * 128 + (((c8 & 7) ^ (r & 7)) << 4) + (d & 7) * 2) =
-                            __float2half_rn(xq[k][i] * PF_QSCALE);
+                            __float2half_rn(xq[k][i] * QSCALE);
                     }
                 }
             }
@@ -443,6 +495,8 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
                     kfac[((c >> 1) & 1) * BLK + ctid] =
                         (SB == 4 ? reinterpret_cast<const float*>(ksc)[ctid] : __half2float(reinterpret_cast<const __half*>(ksc)[ctid])) *
                         (rsqrtf(float(HD)) * PF_QK8_C0);
+            } else if (KV4) {
+                convert_side4(raw + slot * CODE_BYTES, kvb + slot * PF_TILE16, ctid, side, s_lim[slot]);
             } else {
                 convert_side<SB>(raw + slot * CODE_BYTES, kvb + slot * PF_TILE16, ctid, scl + ((c >> 1) & 1) * 1024 + side * BLK * SB,
                                  side == 0 ? rsqrtf(float(HD)) : 1.0f);
@@ -508,6 +562,14 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
                         rowsum += w0 + w1;
                         pk[e >> 1] = pack_h2(w0, w1);
                     }
+                } else if (KV4) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        const float m0 = fmaxf(__uint_as_float(s[e]), 0.0f), m1 = fmaxf(__uint_as_float(s[e + 1]), 0.0f);
+                        const float w0 = m0 * m0, w1 = m1 * m1;
+                        rowsum += w0 + w1;
+                        pk[e >> 1] = pack_h2(w0, w1);
+                    }
                 } else {
                     // unmasked pages (all but the last one or two of a tile): ReLU² on packed fp16 pairs. The 16
                     // products a half accumulates stay far inside fp16; their sum joins the fp32 row sum once a chunk.
@@ -563,7 +625,7 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
 #pragma unroll
                         for (int e = 0; e < 32; e++) pcol[size_t(32 * cc + e) * BLK] = nx > 0 ? __uint_as_float(acc[e]) : 0.0f;
                     }
-                    pcol[size_t(HD) * BLK] = split == 0 ? sqrtf(float(HD)) * PF_PSCALE * (QK8 ? qsc[x * BLK + r] : 1.0f) + rowsum : rowsum;
+                    pcol[size_t(HD) * BLK] = split == 0 ? sqrtf(float(HD)) * PSCALE * (QK8 ? qsc[x * BLK + r] : 1.0f) + rowsum : rowsum;
                 }
             } else if (!last) {
                 // the 32 rows of a warp write 32 consecutive floats of a column
@@ -599,7 +661,7 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
                 relu_warps_sync();
                 if (ok && !*reinterpret_cast<volatile int*>(&s_abort)) {
                     const float* pbase = p.partials + (size_t(slot0) * 2 + x) * tstride + r;   // range 0; range s is 2 tstride x s on
-                    float den = sqrtf(float(HD)) * PF_PSCALE * (QK8 ? qsc[x * BLK + r] : 1.0f);
+                    float den = sqrtf(float(HD)) * PSCALE * (QK8 ? qsc[x * BLK + r] : 1.0f);
                     for (int sp = 0; sp < nparts; sp++) den += sp == split ? rowsum : __ldcg(pbase + size_t(sp) * 2 * tstride + size_t(HD) * BLK);
                     const float inv = 1.0f / den;
                     const size_t ooff = size_t(b) * p.o_seq_stride + size_t(t0[x] + r) * p.o_token_stride + size_t(h) * HD;
@@ -663,7 +725,7 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
             prow[HD] = rowsum;
         } else if (nx > 0) {
             tc_fence_after();
-            const float inv = 1.0f / (sqrtf(float(HD)) * PF_PSCALE * (QK8 ? qsc[x * BLK + r] : 1.0f) + rowsum);
+            const float inv = 1.0f / (sqrtf(float(HD)) * PSCALE * (QK8 ? qsc[x * BLK + r] : 1.0f) + rowsum);
             const size_t ooff = size_t(b) * p.o_seq_stride + size_t(t0[x] + r) * p.o_token_stride + size_t(h) * HD;
             uint16_t* orow = static_cast<uint16_t*>(p.o) + ooff;
 #pragma unroll 1
@@ -716,7 +778,7 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
                 float sum = 0.0f;
 #pragma unroll
                 for (int sp = 0; sp < 8; sp++) sum += v[sp];
-                den[i] = sqrtf(float(HD)) * PF_PSCALE * (QK8 ? qsc[x * BLK + r] : 1.0f) + sum;
+                den[i] = sqrtf(float(HD)) * PSCALE * (QK8 ? qsc[x * BLK + r] : 1.0f) + sum;
             }
             __syncthreads();
             for (int it = tid; it < 2 * R * (HD / 2); it += PF_THREADS) {
@@ -927,7 +989,7 @@ __global__ void __launch_bounds__(256) prefill_reduce_kernel(const __grid_consta
     }
 }
 
-template <int DT, int SB, bool QK8>
+template <int DT, int SB, bool QK8, bool KV4>
 __global__ void __launch_bounds__(PF_THREADS, 1) full_prefill_kernel(const __grid_constant__ CUtensorMap tmap,
                                                                      const __grid_constant__ PrefillParams p) {
     PfSegment sg;
@@ -958,12 +1020,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1) full_prefill_kernel(const __gri
         sg.je = min(n_all, sg.jb + pps);
         sg.slot0 = unit * p.nsplit;
     }
-    full_prefill_segment<DT, SB, QK8>(tmap, p, sg);
+    full_prefill_segment<DT, SB, QK8, KV4>(tmap, p, sg);
 }
-
-EmblaStatus kv4_full_prefill(EmblaAttn* ctx, const EmblaKVPool* pool, const EmblaKVView* view, const int32_t* pos0, int n_tokens,
-                             const EmblaQuery* q, int64_t q_token_stride, void* o_dev, int64_t o_token_stride, int64_t o_seq_stride,
-                             cudaStream_t stream);   // kv4_decode.cu
 
 }  // namespace embla
 
@@ -986,9 +1044,9 @@ extern "C" EmblaStatus embla_attn_reserve_prefill(EmblaAttn* ctx, void* stream) 
     return EMBLA_OK;
 }
 
-template <int DT, int SB, bool QK8>
+template <int DT, int SB, bool QK8, bool KV4 = false>
 static EmblaStatus launch_prefill(EmblaAttn* ctx, const EmblaKVPool* pool, PrefillParams& p, int batch, int max_pages, cudaStream_t s) {
-    auto kern = full_prefill_kernel<DT, SB, QK8>;
+    auto kern = full_prefill_kernel<DT, SB, QK8, KV4>;
     static bool configured[64] = {};
     if (!configured[ctx->device & 63]) {
         EMBLA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(PF_SMEM)));
@@ -1152,7 +1210,6 @@ static EmblaStatus full_prefill_impl(EmblaAttn* ctx, const EmblaKVPool* pool, co
         EMBLA_FAIL(EMBLA_BAD_ARG, "embla_attn_full_prefill: the fused head norm takes both gain vectors (ng = 2)");
     if ((q_token_stride % 8) || (q->q_stride % 8) || (o_token_stride % 8) || (o_seq_stride % 8))
         EMBLA_FAIL(EMBLA_BAD_ARG, "embla_attn_full_prefill: strides must be multiples of 8 elements (16-byte rows)");
-    if (kv4) return kv4_full_prefill(ctx, pool, view, pos0_dev, n_tokens, q, q_token_stride, o_dev, o_token_stride, o_seq_stride, static_cast<cudaStream_t>(stream));
     PrefillParams p;
     p.pool = pool->base;
     p.block_table = view->block_table_dev;
@@ -1176,12 +1233,16 @@ static EmblaStatus full_prefill_impl(EmblaAttn* ctx, const EmblaKVPool* pool, co
     p.G = ctx->cfg.n_q_heads / ctx->cfg.n_kv_heads;
     p.scale_bytes = pool->scale_bytes;
     p.rows_per_page = pool->rows_per_page;
+    p.num_blocks = pool->num_blocks;
     p.n_tokens = n_tokens;
     p.prenormed = q->prenormed;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool bf = ctx->cfg.act_dtype == EMBLA_BF16, s4 = pool->scale_bytes == 4;
     // pages a tile may see, from the caller's bound on pos0 + n_tokens (sizes the page split only)
     const int max_pages = ((view->max_seq_len > 0 ? view->max_seq_len : ctx->cfg.max_context) + BLK - 1) / BLK;
+    if (kv4)
+        return bf ? launch_prefill<EMBLA_BF16, 2, false, true>(ctx, pool, p, view->batch, max_pages, s)
+                  : launch_prefill<EMBLA_F16, 2, false, true>(ctx, pool, p, view->batch, max_pages, s);
 #define EMBLA_PF(DT, SB) (qk8 ? launch_prefill<DT, SB, true>(ctx, pool, p, view->batch, max_pages, s) : launch_prefill<DT, SB, false>(ctx, pool, p, view->batch, max_pages, s))
     if (bf) return s4 ? EMBLA_PF(EMBLA_BF16, 4) : EMBLA_PF(EMBLA_BF16, 2);
     return s4 ? EMBLA_PF(EMBLA_F16, 4) : EMBLA_PF(EMBLA_F16, 2);
