@@ -118,7 +118,7 @@ __device__ __forceinline__ void convert_side(const uint8_t* raw, uint8_t* dst, i
 // 4-bit pages (EMBLA_KV_INT4, kv4.cuh): the same kernel with other converters. A group's 16 bytes of codes become 32 fp16 values,
 // code x scale rounded once (2^-11); queries enter scaled by 2^-7 and the keys without 1 / sqrt(D), whose square, 2^-7, is exact
 // in the weights: P = relu(s)^2 comes out as the weight x 2^-7 (scores up to 2895 square inside fp16's range), the sink takes
-// the same factor. Weights and their sums stay in fp32 until the one rounding of P to fp16.
+// the same factor. 2048 tokens at 30720: 431 us, 1236 TFLOP/s (0.75 of the measured burst rate; the int8 pages take 449 us).
 constexpr float PF4_QSCALE = 1.0f / 128.0f, PF4_PSCALE = 1.0f / 128.0f;
 
 // One side of a raw 4-bit page -> fp16 in the UMMA layout; rows from `lim` on (behind the last key, or all of a page that is
@@ -521,6 +521,7 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
         const int pos_r = p0 + t0[x] + r;               // this row's absolute position
         const int nx = max(0, min(je, npg[x]) - jb);     // pages of this CTA's range that the tile sees
         float rowsum = 0.0f;
+        float rowsum1 = 0.0f;   // (KV4: of the odd keys of unmasked pages)
         bool ok = true;
         for (int i = 0; i < nx; i++) {
             const int j = jb + i;
@@ -563,12 +564,17 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
                         pk[e >> 1] = pack_h2(w0, w1);
                     }
                 } else if (KV4) {
+                    // relu(s) rounded to fp16 by the conversion itself, its square once more (2^-11 each); the row sum takes the
+                    // exact squares in fp32 (mixed-precision fma). In fp32 up to P the kernel took 470 microseconds instead of 431
+                    // for 2048 tokens at 30720: these warps bound it, and packed fp32 pairs were no faster.
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
-                        const float m0 = fmaxf(__uint_as_float(s[e]), 0.0f), m1 = fmaxf(__uint_as_float(s[e + 1]), 0.0f);
-                        const float w0 = m0 * m0, w1 = m1 * m1;
-                        rowsum += w0 + w1;
-                        pk[e >> 1] = pack_h2(w0, w1);
+                        uint32_t h;
+                        asm("cvt.rn.relu.f16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(__uint_as_float(s[e + 1])), "f"(__uint_as_float(s[e])));
+                        pk[e >> 1] = h2_mul(h, h);
+                        asm("{\n .reg .b16 lo, hi;\n mov.b32 {lo, hi}, %2;\n fma.rn.f32.f16 %0, lo, lo, %0;\n fma.rn.f32.f16 %1, hi, hi, %1;\n}\n"
+                            : "+f"(rowsum), "+f"(rowsum1)
+                            : "r"(h));
                     }
                 } else {
                     // unmasked pages (all but the last one or two of a tile): ReLU² on packed fp16 pairs. The 16
@@ -594,6 +600,7 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_ready[x]);
         }
+        if (KV4) rowsum += rowsum1;
         if (ok) ok = mbar_wait_bounded(p.ctl.wait_cycles, o_done, 0);
         ok = __all_sync(0xffffffffu, ok);   // (warp-uniform: the TMEM loads below are warp-collective)
         if (!ok) {
