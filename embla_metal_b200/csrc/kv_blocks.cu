@@ -17,26 +17,51 @@ struct CopyParams {
     const int32_t* rows;
     size_t page_bytes, block_bytes;
     int* err;
-    int num_blocks, pages, n_spans;   // pages: layers x kv heads of a block
+    int num_blocks, pages, n_spans, ragged;   // pages: layers x kv heads of a block
     BlockSpan span[4];
 };
 
-__global__ void __launch_bounds__(256) kv_copy_blocks_kernel(const CopyParams p) {
+#ifndef KVB_U
+#define KVB_U 5
+#define KVB_T 256
+#endif
+constexpr int COPY_THREADS = KVB_T, COPY_BATCH = KVB_U;   // 16-byte loads in flight a thread
+
+__global__ void __launch_bounds__(COPY_THREADS) kv_copy_blocks_kernel(const __grid_constant__ CopyParams p) {
     const int i = int(blockIdx.x / unsigned(p.pages)), page = int(blockIdx.x % unsigned(p.pages));
     const int src = p.src[i], dst = p.dst[i];
+    const int rows = p.rows ? max(0, min(BLK, p.rows[i])) : BLK;
     if (src < 0 || src >= p.num_blocks || dst < 0 || dst >= p.num_blocks) {
         if (threadIdx.x == 0) atomicExch(p.err, ERR_BAD_BLOCK);
         return;
     }
-    const int rows = p.rows ? max(0, min(BLK, p.rows[i])) : BLK;
     const uint8_t* from = p.pool + size_t(src) * p.block_bytes + size_t(page) * p.page_bytes;
     uint8_t* to = p.pool + size_t(dst) * p.block_bytes + size_t(page) * p.page_bytes;
-    for (int k = 0; k < p.n_spans; k++) {
-        const int at = p.span[k].offset, bytes = rows * p.span[k].row_bytes, whole = bytes & ~15;
-        for (int o = int(threadIdx.x) * 16; o < whole; o += 256 * 16)
-            *reinterpret_cast<uint4*>(to + at + o) = *reinterpret_cast<const uint4*>(from + at + o);
-        const int o = whole + int(threadIdx.x) * 2;   // (the scales of an odd number of int8 rows)
-        if (o < bytes) *reinterpret_cast<uint16_t*>(to + at + o) = *reinterpret_cast<const uint16_t*>(from + at + o);
+    // the pieces' whole 16-byte words, one piece after another
+    int end[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) end[k] = (k ? end[k - 1] : 0) + (k < p.n_spans ? rows * p.span[k].row_bytes / 16 : 0);
+    for (int base = int(threadIdx.x); base < end[3]; base += COPY_THREADS * COPY_BATCH) {
+        uint4 v[COPY_BATCH];
+        int at[COPY_BATCH];
+#pragma unroll
+        for (int u = 0; u < COPY_BATCH; u++) {
+            const int w = base + u * COPY_THREADS;
+            at[u] = p.span[0].offset + w * 16;
+#pragma unroll
+            for (int k = 1; k < 4; k++)
+                if (w >= end[k - 1]) at[u] = p.span[k].offset + (w - end[k - 1]) * 16;
+            if (w < end[3]) v[u] = __ldcs(reinterpret_cast<const uint4*>(from + at[u]));
+        }
+#pragma unroll
+        for (int u = 0; u < COPY_BATCH; u++)
+            if (base + u * COPY_THREADS < end[3]) __stcs(reinterpret_cast<uint4*>(to + at[u]), v[u]);
+    }
+    if (p.ragged) {   // int8 scales: an odd number of rows ends inside a word
+        for (int k = 2; k < 4; k++) {
+            const int bytes = rows * p.span[k].row_bytes, o = (bytes & ~15) + int(threadIdx.x) * 2;
+            if (o < bytes) *reinterpret_cast<uint16_t*>(to + p.span[k].offset + o) = *reinterpret_cast<const uint16_t*>(from + p.span[k].offset + o);
+        }
     }
 }
 
@@ -67,6 +92,7 @@ extern "C" EmblaStatus embla_kv_copy_blocks(EmblaAttn* ctx, EmblaKVPool* pool, c
         p.span[2] = {2 * KV4_SIDE, 2 * KV4_GROUPS * 2};
     } else if (pool->kv_dtype == EMBLA_KV_INT8) {
         p.n_spans = 4;
+        p.ragged = 1;
         p.span[0] = {0, HD};
         p.span[1] = {CODE_BYTES, HD};
         p.span[2] = {2 * CODE_BYTES, pool->scale_bytes};
@@ -78,7 +104,7 @@ extern "C" EmblaStatus embla_kv_copy_blocks(EmblaAttn* ctx, EmblaKVPool* pool, c
     }
     const long ctas = long(n) * p.pages;
     if (ctas > 0x7fffffffL) EMBLA_FAIL(EMBLA_BAD_ARG, "embla_kv_copy_blocks: %d copies of %d pages are too many", n, p.pages);
-    EMBLA_CUDA_TRY(launch_kernel(false, kv_copy_blocks_kernel, dim3(unsigned(ctas)), dim3(256), 0, static_cast<cudaStream_t>(stream), p));
+    EMBLA_CUDA_TRY(launch_kernel(false, kv_copy_blocks_kernel, dim3(unsigned(ctas)), dim3(COPY_THREADS), 0, static_cast<cudaStream_t>(stream), p));
     EMBLA_CUDA_TRY(cudaGetLastError());
     return EMBLA_OK;
 }
