@@ -11,19 +11,23 @@ namespace embla {
 __host__ __device__ constexpr int kv4_nibble_of(int d) { return (d >> 1) + 4 * (d & 1); }   // place of dim d (of 8) in its word
 
 // The scale of a group whose largest magnitude is `top` (NaN or infinity: a NaN scale, so that what was not a number does not
-// come back as one), and the code of x under it. x and s have at most 11 significant bits, so x / s never lies within a fp32
-// rounding of a half without being one: the fp32 division gives the code that exact arithmetic gives.
+// come back as one).
 __device__ __forceinline__ __half kv4_scale(float top) {
     return top <= 3.4028234e38f ? __float2half_rn(fminf(__fdiv_rn(top, 7.0f), 65504.0f)) : __ushort_as_half(0x7fff);
 }
-__device__ __forceinline__ int kv4_code(float x, float s) {
-    return s > 0.0f ? int(fminf(fmaxf(rintf(__fdiv_rn(x, s)), -7.0f), 7.0f)) : 0;
+// The code of x under the scale s, rint(x / s) clamped, as exact arithmetic gives it, from inv, the fp32 reciprocal of s. x and s
+// have at most 11 significant bits, so x / s is either a half exactly or at least 2^-16 of its size away from one: x inv, off by
+// 2^-23 of its size, lies on the right side of any half that x / s is not. If x / s is a half, x - code s is s / 2 either way
+// (exact: code s has 14 bits), and the even code is taken.
+__device__ __forceinline__ int kv4_code(float x, float s, float inv) {
+    if (!(s > 0.0f)) return 0;
+    float c = rintf(x * inv);
+    const float rest = fmaf(-c, s, x);
+    const int n = int(c);
+    if (fabsf(rest) * 2.0f == s && (n & 1)) c += rest > 0.0f ? 1.0f : -1.0f;
+    return int(fminf(fmaxf(c, -7.0f), 7.0f));
 }
-// max |x| over the warp that keeps a NaN
-__device__ __forceinline__ float warp_max_abs_nan(float x) {
-    uint32_t m = __float_as_uint(x) & 0x7fffffffu;   // (ordered as the magnitudes are, infinity and NaN on top)
-    return __uint_as_float(__reduce_max_sync(0xffffffffu, m));
-}
+__device__ __forceinline__ float fmaxf_nan(float a, float b) { return a != a ? a : b != b ? b : fmaxf(a, b); }
 
 // The query row of a head that comes raw: RMS norm over the head with `ng` gains, in the order of the other decode kernels
 // (common.metal:30-41), rounded to the activation dtype. A lane holds dims lane + 32 i.

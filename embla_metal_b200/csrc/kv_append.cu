@@ -59,157 +59,262 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const AppendParams p) {
     }
 }
 
-// The same for a 4-bit pool: a lane's dims lane + 32 i are one of each group, so a group's largest magnitude is a reduction
-// over the warp; eight lanes put a word's nibbles together. pos0 NULL: one token, at position seq_lens[b] - 1.
-struct Append4Params {
+// ---- 4-bit pools, and reading rows back -------------------------------------------------------------------------------
+// Half a warp takes a row: a lane holds 8 consecutive dims (16 bytes of activations, one word of codes), four lanes a scale
+// group. A warp takes 2 x PASSES consecutive rows of one side (K or V), every load in flight before the first is used; lane i works
+// out where row i lies, the others get it by shuffle. Bound by instructions (about 75 a row and warp to quantise), not by
+// the 784 bytes of a row in, out and back: a warp a row with two-byte loads took 93 us for 8 x 2048 tokens, append and read.
+struct RowsParams {
     uint8_t* pool;
     const int32_t* block_table;
-    const int32_t* pos0;
+    const int32_t* pos0;       // NULL: one token, at position seq_lens[b] - 1
     const int32_t* seq_lens;
-    const void* k;
-    const void* v;
-    int64_t token_stride, seq_stride;
-    int* err;
-    int table_stride, batch, n_tokens, layer, n_layers, n_kv_heads, num_blocks, norm_k;
-};
-
-// The page of a position (block table entry pos / 128), or NULL with the error word set when the position lies outside the
-// table's row or the entry outside the pool.
-__device__ __forceinline__ uint8_t* page_of(uint8_t* pool, const int32_t* table_row, int table_stride, int num_blocks, int pos, int layer,
-                                            int n_layers, int n_kv_heads, int h, size_t page_bytes, int* err) {
-    const int e = pos / BLK;
-    int block = -1;
-    if (pos >= 0 && e < table_stride) block = table_row[e];
-    if (block < 0 || block >= num_blocks) {
-        atomicExch(err, ERR_BAD_BLOCK);
-        return nullptr;
-    }
-    return pool + ((size_t(block) * n_layers + layer) * n_kv_heads + h) * page_bytes;
-}
-
-template <int DT>
-__global__ void __launch_bounds__(128) kv4_append_kernel(const Append4Params p) {
-    pdl_wait();
-    pdl_launch_dependents();
-    const int lane = threadIdx.x & 31;
-    const long warp = (long(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-    const long total = long(p.batch) * p.n_tokens * p.n_kv_heads * 2;
-    if (warp >= total) return;
-    const int is_v = int(warp & 1);
-    const int h = int((warp >> 1) % p.n_kv_heads);
-    const long bt = (warp >> 1) / p.n_kv_heads;
-    const int t = int(bt % p.n_tokens), b = int(bt / p.n_tokens);
-    const int pos = p.pos0 ? p.pos0[b] + t : p.seq_lens[b] - 1;
-    if (!p.pos0 && pos < 0) return;   // (an empty sequence has no current token)
-    uint8_t* page = page_of(p.pool, p.block_table + size_t(b) * p.table_stride, p.table_stride, p.num_blocks, pos, p.layer, p.n_layers,
-                            p.n_kv_heads, h, KV4_PAGE, p.err);
-    if (!page) return;
-    const int row = pos % BLK;
-    float x[4];
-    kv_row_load<DT>(is_v ? p.v : p.k, size_t(b) * p.seq_stride + size_t(t) * p.token_stride + size_t(h) * HD, !is_v && p.norm_k, lane, x);
-    uint32_t word = 0;   // lane: word lane / 8 of group lane % 8 (lanes with lane % 8 < 4)
-    __half scale = __ushort_as_half(0);   // lane g < 4: of group g
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        x[i] = Act<DT>::round(x[i]);
-        const __half s = kv4_scale(warp_max_abs_nan(x[i]));
-        uint32_t w = (uint32_t(kv4_code(x[i], __half2float(s))) & 15u) << (4 * kv4_nibble_of(lane & 7));
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) w |= __shfl_xor_sync(0xffffffffu, w, o);
-        if ((lane & 7) == i) word = w;
-        if (lane == i) scale = s;
-    }
-    if ((lane & 7) < 4)
-        *reinterpret_cast<uint32_t*>(page + is_v * KV4_SIDE + row * KV4_ROW + (lane & 7) * 16 + (lane >> 3) * 4) = word;
-    if (lane < 4) reinterpret_cast<__half*>(page + 2 * KV4_SIDE)[row * 2 * KV4_GROUPS + is_v * KV4_GROUPS + lane] = scale;
-}
-
-// Rows of the cache back as activations: one warp per (sequence, token, kv head, K|V), a lane holds dims 4 lane .. 4 lane + 3.
-struct ReadParams {
-    uint8_t* pool;
-    const int32_t* block_table;
-    const int32_t* pos0;
-    void* k;
+    void* k;                   // rows read (append) or written (read back)
     void* v;
     int64_t token_stride, seq_stride;
     size_t page_bytes;
     int* err;
-    int table_stride, batch, n_tokens, layer, n_layers, n_kv_heads, num_blocks, kv_dtype, scale_bytes;
+    unsigned rows;             // of a side: batch x n_tokens x n_kv_heads
+    int table_stride, n_tokens, layer, n_layers, n_kv_heads, num_blocks, norm_k, kv_dtype, scale_bytes, vec;
 };
 
-template <int DT>
-__global__ void __launch_bounds__(128) kv_read_kernel(const ReadParams p) {
-    pdl_wait();
-    pdl_launch_dependents();
-    const int lane = threadIdx.x & 31;
-    const long warp = (long(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-    const long total = long(p.batch) * p.n_tokens * p.n_kv_heads * 2;
-    if (warp >= total) return;
-    const int is_v = int(warp & 1);
-    const int h = int((warp >> 1) % p.n_kv_heads);
-    const long bt = (warp >> 1) / p.n_kv_heads;
-    const int t = int(bt % p.n_tokens), b = int(bt / p.n_tokens);
-    const int pos = p.pos0[b] + t;
-    const uint8_t* page = page_of(p.pool, p.block_table + size_t(b) * p.table_stride, p.table_stride, p.num_blocks, pos, p.layer,
-                                  p.n_layers, p.n_kv_heads, h, p.page_bytes, p.err);
-    if (!page) return;
-    const int row = pos % BLK;
-    uint2 out;
-    if (p.kv_dtype == EMBLA_KV_16BIT) {
-        out = reinterpret_cast<const uint2*>(page + is_v * (BLK * HD * 2) + row * HD * 2)[lane];
-    } else {
-        float x[4];
-        if (p.kv_dtype == EMBLA_KV_INT4) {
-            const uint32_t w = reinterpret_cast<const uint32_t*>(page + is_v * KV4_SIDE + row * KV4_ROW)[lane >> 1];
-            const float s = __half2float(reinterpret_cast<const __half*>(page + 2 * KV4_SIDE)[row * 2 * KV4_GROUPS + is_v * KV4_GROUPS + (lane >> 3)]);
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int n = kv4_nibble_of(4 * (lane & 1) + i);
-                x[i] = float(int(w << (28 - 4 * n)) >> 28) * s;
-            }
-        } else {
-            const char4 c = reinterpret_cast<const char4*>(page + is_v * CODE_BYTES + row * HD)[lane];
-            const float s = load_scale(page + 2 * CODE_BYTES + is_v * BLK * p.scale_bytes, row, p.scale_bytes);
-            x[0] = float(c.x) * s;
-            x[1] = float(c.y) * s;
-            x[2] = float(c.z) * s;
-            x[3] = float(c.w) * s;
-        }
-        if (DT == EMBLA_F16) out = make_uint2(pack_h2(x[0], x[1]), pack_h2(x[2], x[3]));
-        else {
-            __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), c = __floats2bfloat162_rn(x[2], x[3]);
-            out = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&c));
-        }
+// Where row i of a side lies: elements into k / v, and its page (NULL: nowhere, with the error word set) and row in it.
+struct RowPlace {
+    long at;
+    uint8_t* page;
+    int row;
+};
+__device__ __forceinline__ RowPlace row_place(const RowsParams& p, unsigned i) {
+    RowPlace w = {0, nullptr, 0};
+    if (i >= p.rows) return w;
+    const unsigned bt = i / unsigned(p.n_kv_heads), h = i - bt * unsigned(p.n_kv_heads);
+    const unsigned b = bt / unsigned(p.n_tokens), t = bt - b * unsigned(p.n_tokens);
+    w.at = long(b) * p.seq_stride + long(t) * p.token_stride + long(h) * HD;
+    const int pos = p.pos0 ? p.pos0[b] + int(t) : p.seq_lens[b] - 1;
+    if (!p.pos0 && pos < 0) return w;   // (an empty sequence has no current token)
+    int block = -1;
+    if (pos >= 0 && pos / BLK < p.table_stride) block = p.block_table[size_t(b) * p.table_stride + pos / BLK];
+    if (block < 0 || block >= p.num_blocks) {
+        atomicExch(p.err, ERR_BAD_BLOCK);
+        return w;
     }
-    uint16_t* dst = static_cast<uint16_t*>(is_v ? p.v : p.k) + size_t(b) * p.seq_stride + size_t(t) * p.token_stride + size_t(h) * HD;
-    reinterpret_cast<uint2*>(dst)[lane] = out;
+    w.page = p.pool + ((size_t(block) * p.n_layers + p.layer) * p.n_kv_heads + h) * p.page_bytes;
+    w.row = pos % BLK;
+    return w;
+}
+__device__ __forceinline__ RowPlace shfl_place(const RowPlace& w, int lane) {
+    RowPlace r;
+    r.at = __shfl_sync(0xffffffffu, w.at, lane);
+    r.page = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(w.page), lane));
+    r.row = __shfl_sync(0xffffffffu, w.row, lane);
+    return r;
+}
+template <int DT>
+__device__ __forceinline__ float act_lo(uint32_t w) {
+    return DT == EMBLA_BF16 ? __uint_as_float(w << 16) : __low2float(*reinterpret_cast<const __half2*>(&w));
+}
+template <int DT>
+__device__ __forceinline__ float act_hi(uint32_t w) {
+    return DT == EMBLA_BF16 ? __uint_as_float(w & 0xffff0000u) : __high2float(*reinterpret_cast<const __half2*>(&w));
+}
+template <int DT>
+__device__ __forceinline__ uint32_t act_pack(float lo, float hi) {
+    if (DT == EMBLA_F16) return pack_h2(lo, hi);
+    __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&h);
 }
 
-static EmblaStatus launch_append4(EmblaAttn* ctx, EmblaKVPool* pool, const EmblaKVView* view, const int32_t* pos0, int n_tokens,
-                                  const void* k, const void* v, int64_t token_stride, int64_t seq_stride, int norm_k, cudaStream_t s) {
-    Append4Params p;
+constexpr int ROWS_WARPS = 4;
+
+template <int DT, int PASSES, bool NORM>
+__global__ void __launch_bounds__(ROWS_WARPS * 32) kv4_append_kernel(const __grid_constant__ RowsParams p) {
+    // (keys to be normed: squares of a warp's rows, then their 32 partial sums a row, by the dims' order in the other append kernels)
+    __shared__ float squares[NORM ? ROWS_WARPS : 1][NORM ? 2 * PASSES : 1][HD + 4];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = lane >> 4, col = lane & 15;
+    const unsigned per = 2 * PASSES, groups = (p.rows + per - 1) / per;
+    const unsigned unit = blockIdx.x * ROWS_WARPS + warp;
+    if (unit >= 2 * groups) return;
+    const bool is_v = unit >= groups;
+    const unsigned first = (is_v ? unit - groups : unit) * per;
+    const RowPlace mine = lane < int(per) ? row_place(p, first + lane) : RowPlace{0, nullptr, 0};
+    uint4 x[PASSES];
+    RowPlace w[PASSES];
+#pragma unroll
+    for (int i = 0; i < PASSES; i++) {
+        w[i] = shfl_place(mine, 2 * i + half);
+        const uint16_t* from = static_cast<const uint16_t*>(is_v ? p.v : p.k) + w[i].at + col * 8;
+        x[i] = make_uint4(0, 0, 0, 0);
+        if (w[i].page) {
+            if (p.vec) {
+                x[i] = *reinterpret_cast<const uint4*>(from);
+            } else {
+                uint16_t e[8];
+#pragma unroll
+                for (int d = 0; d < 8; d++) e[d] = from[d];
+                x[i] = make_uint4(e[0] | uint32_t(e[1]) << 16, e[2] | uint32_t(e[3]) << 16, e[4] | uint32_t(e[5]) << 16, e[6] | uint32_t(e[7]) << 16);
+            }
+        }
+    }
+    if (NORM && !is_v) {
+        // RMS norm without gains (common.metal:30-41): dims l, l + 32, l + 64, l + 96 into a partial sum each, then l = 0 .. 31
+        float(*sq)[HD + 4] = squares[warp];
+#pragma unroll
+        for (int i = 0; i < PASSES; i++) {
+            const uint32_t v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+            float* to = &sq[2 * i + half][col * 8];
+#pragma unroll
+            for (int d = 0; d < 4; d++) {
+                const float lo = act_lo<DT>(v[d]), hi = act_hi<DT>(v[d]);
+                to[2 * d] = __fmul_rn(lo, lo);
+                to[2 * d + 1] = __fmul_rn(hi, hi);
+            }
+        }
+        __syncwarp();
+        float part[2 * PASSES];
+#pragma unroll
+        for (int i = 0; i < 2 * PASSES; i++)
+            part[i] = __fadd_rn(__fadd_rn(__fadd_rn(sq[i][lane], sq[i][lane + 32]), sq[i][lane + 64]), sq[i][lane + 96]);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 2 * PASSES; i++) sq[i][lane] = part[i];
+        __syncwarp();
+        float factor = 0.0f;
+        if (lane < 2 * PASSES) {
+            float tot = 0.0f;
+#pragma unroll 8
+            for (int l = 0; l < 32; l++) tot = __fadd_rn(tot, sq[lane][l]);
+            factor = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(tot, float(HD)), EPS32)));
+        }
+#pragma unroll
+        for (int i = 0; i < PASSES; i++) {
+            const float f = __shfl_sync(0xffffffffu, factor, 2 * i + half);
+            uint32_t* v = &x[i].x;
+#pragma unroll
+            for (int d = 0; d < 4; d++) v[d] = act_pack<DT>(__fmul_rn(act_lo<DT>(v[d]), f), __fmul_rn(act_hi<DT>(v[d]), f));
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < PASSES; i++) {
+        const uint32_t v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+        // the group's largest magnitude: the types' bits without the sign are ordered as the magnitudes are, NaN on top
+        uint32_t top = __vmaxu2(__vmaxu2(v[0] & 0x7fff7fffu, v[1] & 0x7fff7fffu), __vmaxu2(v[2] & 0x7fff7fffu, v[3] & 0x7fff7fffu));
+        top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const __half sh = kv4_scale(fmaxf_nan(act_lo<DT>(top), act_hi<DT>(top)));
+        const float s = __half2float(sh), inv = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;
+        uint32_t word = 0;
+#pragma unroll
+        for (int d = 0; d < 8; d++) {
+            const float xv = (d & 1) ? act_hi<DT>(v[d >> 1]) : act_lo<DT>(v[d >> 1]);
+            word |= (uint32_t(kv4_code(xv, s, inv)) & 15u) << (4 * kv4_nibble_of(d));
+        }
+        if (!w[i].page) continue;
+        *reinterpret_cast<uint32_t*>(w[i].page + (is_v ? KV4_SIDE : 0) + w[i].row * KV4_ROW + col * 4) = word;
+        if ((col & 3) == 0)
+            reinterpret_cast<__half*>(w[i].page + 2 * KV4_SIDE)[w[i].row * 2 * KV4_GROUPS + (is_v ? KV4_GROUPS : 0) + (col >> 2)] = sh;
+    }
+}
+
+template <int DT, int PASSES>
+__global__ void __launch_bounds__(ROWS_WARPS * 32) kv_read_kernel(const __grid_constant__ RowsParams p) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = lane >> 4, col = lane & 15;
+    const unsigned per = 2 * PASSES, groups = (p.rows + per - 1) / per;
+    const unsigned unit = blockIdx.x * ROWS_WARPS + warp;
+    if (unit >= 2 * groups) return;
+    const bool is_v = unit >= groups;
+    const unsigned first = (is_v ? unit - groups : unit) * per;
+    const RowPlace mine = lane < int(per) ? row_place(p, first + lane) : RowPlace{0, nullptr, 0};
+    RowPlace w[PASSES];
+    uint4 c[PASSES];   // the lane's 8 codes (or the row's values, 16-bit pools)
+    float s[PASSES];
+#pragma unroll
+    for (int i = 0; i < PASSES; i++) {
+        w[i] = shfl_place(mine, 2 * i + half);
+        const uint8_t* page = w[i].page;
+        const int row = w[i].row;
+        c[i] = make_uint4(0, 0, 0, 0);
+        s[i] = 0.0f;
+        if (!page) continue;
+        if (p.kv_dtype == EMBLA_KV_INT4) {
+            c[i].x = *reinterpret_cast<const uint32_t*>(page + (is_v ? KV4_SIDE : 0) + row * KV4_ROW + col * 4);
+            s[i] = __half2float(reinterpret_cast<const __half*>(page + 2 * KV4_SIDE)[row * 2 * KV4_GROUPS + (is_v ? KV4_GROUPS : 0) + (col >> 2)]);
+        } else if (p.kv_dtype == EMBLA_KV_INT8) {
+            const uint2 t = *reinterpret_cast<const uint2*>(page + (is_v ? CODE_BYTES : 0) + row * HD + col * 8);
+            c[i].x = t.x;
+            c[i].y = t.y;
+            s[i] = load_scale(page + 2 * CODE_BYTES + (is_v ? BLK * p.scale_bytes : 0), row, p.scale_bytes);
+        } else {
+            c[i] = *reinterpret_cast<const uint4*>(page + (is_v ? BLK * HD * 2 : 0) + row * HD * 2 + col * 16);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < PASSES; i++) {
+        if (!w[i].page) continue;
+        uint4 out = c[i];
+        if (p.kv_dtype != EMBLA_KV_16BIT) {
+            float x[8];
+#pragma unroll
+            for (int d = 0; d < 8; d++) {
+                const int code = p.kv_dtype == EMBLA_KV_INT4 ? int(c[i].x << (28 - 4 * kv4_nibble_of(d))) >> 28
+                                                             : int((d < 4 ? c[i].x : c[i].y) << (24 - 8 * (d & 3))) >> 24;
+                x[d] = float(code) * s[i];
+            }
+            out = make_uint4(act_pack<DT>(x[0], x[1]), act_pack<DT>(x[2], x[3]), act_pack<DT>(x[4], x[5]), act_pack<DT>(x[6], x[7]));
+        }
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(is_v ? p.v : p.k) + w[i].at + col * 8) = out;
+    }
+}
+
+// Rows a warp takes: eight, or two while that leaves SMs without a warp.
+static int rows_passes(const EmblaAttn* ctx, unsigned rows) { return rows >= 8u * ROWS_WARPS * unsigned(ctx->sm_count) ? 4 : 1; }
+
+static EmblaStatus rows_params(RowsParams& p, const char* fn, const EmblaKVPool* pool, const EmblaKVView* view, const int32_t* pos0, int n_tokens,
+                               int64_t token_stride, int64_t seq_stride, const EmblaAttn* ctx) {
+    const long rows = long(view->batch) * n_tokens * pool->n_kv_heads;
+    if (rows > 0x3fffffffL) EMBLA_FAIL(EMBLA_BAD_ARG, "%s: %d sequences x %d tokens are too many", fn, view->batch, n_tokens);
     p.pool = pool->base;
     p.block_table = view->block_table_dev;
     p.pos0 = pos0;
     p.seq_lens = view->seq_lens_dev;
-    p.k = k;
-    p.v = v;
     p.token_stride = token_stride;
     p.seq_stride = seq_stride;
+    p.page_bytes = pool->page_bytes;
     p.err = ctx->err_dev;
+    p.rows = unsigned(rows);
     p.table_stride = view->table_stride;
-    p.batch = view->batch;
     p.n_tokens = n_tokens;
     p.layer = view->layer;
     p.n_layers = pool->n_layers;
     p.n_kv_heads = pool->n_kv_heads;
     p.num_blocks = pool->num_blocks;
+    p.kv_dtype = pool->kv_dtype;
+    p.scale_bytes = pool->scale_bytes;
+    return EMBLA_OK;
+}
+static dim3 rows_grid(unsigned rows, int passes) {
+    const unsigned units = 2 * ((rows + 2 * passes - 1) / (2 * passes));
+    return dim3((units + ROWS_WARPS - 1) / ROWS_WARPS);
+}
+
+static EmblaStatus launch_append4(EmblaAttn* ctx, EmblaKVPool* pool, const EmblaKVView* view, const int32_t* pos0, int n_tokens,
+                                  const void* k, const void* v, int64_t token_stride, int64_t seq_stride, int norm_k, cudaStream_t s) {
+    RowsParams p = {};
+    if (EmblaStatus st = rows_params(p, "embla_kv_append", pool, view, pos0, n_tokens, token_stride, seq_stride, ctx)) return st;
+    p.k = const_cast<void*>(k);
+    p.v = const_cast<void*>(v);
     p.norm_k = norm_k;
-    const long warps = long(p.batch) * n_tokens * p.n_kv_heads * 2;
-    if ((warps + 3) / 4 > 0x7fffffffL) EMBLA_FAIL(EMBLA_BAD_ARG, "embla_kv_append: %d sequences x %d tokens are too many", p.batch, n_tokens);
-    const dim3 grid(unsigned((warps + 3) / 4));
-    if (ctx->cfg.act_dtype == EMBLA_BF16) EMBLA_CUDA_TRY(launch_kernel(ctx->pdl, kv4_append_kernel<EMBLA_BF16>, grid, dim3(128), 0, s, p));
-    else EMBLA_CUDA_TRY(launch_kernel(ctx->pdl, kv4_append_kernel<EMBLA_F16>, grid, dim3(128), 0, s, p));
+    p.vec = token_stride % 8 == 0 && seq_stride % 8 == 0 && reinterpret_cast<uintptr_t>(k) % 16 == 0 && reinterpret_cast<uintptr_t>(v) % 16 == 0;
+    const int passes = rows_passes(ctx, p.rows);
+    const bool bf = ctx->cfg.act_dtype == EMBLA_BF16;
+#define EMBLA_A4(DT, P) (norm_k ? launch_kernel(ctx->pdl, kv4_append_kernel<DT, P, true>, rows_grid(p.rows, P), dim3(ROWS_WARPS * 32), 0, s, p) \
+                                : launch_kernel(ctx->pdl, kv4_append_kernel<DT, P, false>, rows_grid(p.rows, P), dim3(ROWS_WARPS * 32), 0, s, p))
+    if (passes == 4) EMBLA_CUDA_TRY(bf ? EMBLA_A4(EMBLA_BF16, 4) : EMBLA_A4(EMBLA_F16, 4));
+    else EMBLA_CUDA_TRY(bf ? EMBLA_A4(EMBLA_BF16, 1) : EMBLA_A4(EMBLA_F16, 1));
+#undef EMBLA_A4
     EMBLA_CUDA_TRY(cudaGetLastError());
     return EMBLA_OK;
 }
@@ -278,31 +383,17 @@ extern "C" EmblaStatus embla_kv_read(EmblaAttn* ctx, const EmblaKVPool* pool, co
         EMBLA_FAIL(EMBLA_BAD_ARG, "embla_kv_read: pool has %d kv heads, context %d", pool->n_kv_heads, ctx->cfg.n_kv_heads);
     if (token_stride % 8 || seq_stride % 8 || reinterpret_cast<uintptr_t>(k_dev) % 16 || reinterpret_cast<uintptr_t>(v_dev) % 16)
         EMBLA_FAIL(EMBLA_BAD_ARG, "embla_kv_read: strides must be multiples of 8 elements and the outputs 16-byte aligned");
-    ReadParams p;
-    p.pool = pool->base;
-    p.block_table = view->block_table_dev;
-    p.pos0 = pos0_dev;
+    RowsParams p = {};
+    if (EmblaStatus st = rows_params(p, "embla_kv_read", pool, view, pos0_dev, n_tokens, token_stride, seq_stride, ctx)) return st;
     p.k = k_dev;
     p.v = v_dev;
-    p.token_stride = token_stride;
-    p.seq_stride = seq_stride;
-    p.page_bytes = pool->page_bytes;
-    p.err = ctx->err_dev;
-    p.table_stride = view->table_stride;
-    p.batch = view->batch;
-    p.n_tokens = n_tokens;
-    p.layer = view->layer;
-    p.n_layers = pool->n_layers;
-    p.n_kv_heads = pool->n_kv_heads;
-    p.num_blocks = pool->num_blocks;
-    p.kv_dtype = pool->kv_dtype;
-    p.scale_bytes = pool->scale_bytes;
-    const long warps = long(p.batch) * n_tokens * p.n_kv_heads * 2;
-    if ((warps + 3) / 4 > 0x7fffffffL) EMBLA_FAIL(EMBLA_BAD_ARG, "embla_kv_read: %d sequences x %d tokens are too many", p.batch, n_tokens);
-    const dim3 grid(unsigned((warps + 3) / 4));
+    const int passes = rows_passes(ctx, p.rows);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (ctx->cfg.act_dtype == EMBLA_BF16) EMBLA_CUDA_TRY(launch_kernel(ctx->pdl, kv_read_kernel<EMBLA_BF16>, grid, dim3(128), 0, s, p));
-    else EMBLA_CUDA_TRY(launch_kernel(ctx->pdl, kv_read_kernel<EMBLA_F16>, grid, dim3(128), 0, s, p));
+    const bool bf = ctx->cfg.act_dtype == EMBLA_BF16;
+#define EMBLA_RD(DT, P) launch_kernel(ctx->pdl, kv_read_kernel<DT, P>, rows_grid(p.rows, P), dim3(ROWS_WARPS * 32), 0, s, p)
+    if (passes == 4) EMBLA_CUDA_TRY(bf ? EMBLA_RD(EMBLA_BF16, 4) : EMBLA_RD(EMBLA_F16, 4));
+    else EMBLA_CUDA_TRY(bf ? EMBLA_RD(EMBLA_BF16, 1) : EMBLA_RD(EMBLA_F16, 1));
+#undef EMBLA_RD
     EMBLA_CUDA_TRY(cudaGetLastError());
     return EMBLA_OK;
 }

@@ -2,7 +2,8 @@
 // block's rows, moving blocks together frees the end of a pool. A page (one layer and kv head of a block) is a handful of
 // arrays with a fixed number of bytes a position, so "the first r positions" are a leading piece of each.
 //
-// Bound by HBM: every byte is read and written once.
+// Bound by HBM: every byte is read and written once. 512 blocks of 442 KB take 71 us, 6.3 TB/s or 0.97 of the measured copy rate (a
+// loop with one load in flight took 101); the last rows of 48 blocks (21 MB moved) 5.4 us.
 #include "common.cuh"
 
 namespace embla {
@@ -21,11 +22,8 @@ struct CopyParams {
     BlockSpan span[4];
 };
 
-#ifndef KVB_U
-#define KVB_U 5
-#define KVB_T 256
-#endif
-constexpr int COPY_THREADS = KVB_T, COPY_BATCH = KVB_U;   // 16-byte loads in flight a thread
+// 16-byte loads in flight a thread: a 4-bit page (1152 words) is one batch of a CTA. 128 x 9, 384 x 3 and 320 x 4 measured the same.
+constexpr int COPY_THREADS = 256, COPY_BATCH = 5;
 
 __global__ void __launch_bounds__(COPY_THREADS) kv_copy_blocks_kernel(const __grid_constant__ CopyParams p) {
     const int i = int(blockIdx.x / unsigned(p.pages)), page = int(blockIdx.x % unsigned(p.pages));
