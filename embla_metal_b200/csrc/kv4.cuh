@@ -29,6 +29,39 @@ __device__ __forceinline__ int kv4_code(float x, float s, float inv) {
 }
 __device__ __forceinline__ float fmaxf_nan(float a, float b) { return a != a ? a : b != b ? b : fmaxf(a, b); }
 
+// The word of eight values under the scale of their group, whose largest magnitude is `top`; `scale` is set to it.
+// Usually without a branch: top / 7 never is half-way between two normal fp16 values (seven times a 12-bit odd number has more
+// than 11 bits), so the product with fp32 1 / 7 rounds to the same scale as the quotient; x inv + 1.5 2^23 rounds to an integer, the
+// four codes of a half are put together as digits of base 16, and 8 is added to each digit and its sign bit flipped at the end.
+// Subnormal scales, groups without one, values beyond 7 scales and quotients that are a half exactly take the long way.
+__device__ __forceinline__ uint32_t kv4_word(const float (&x)[8], float top, __half& scale) {
+    constexpr float MAGIC = 12582912.0f;
+    const float fast = top * (1.0f / 7.0f);
+    scale = __float2half_rn(fast);
+    const float s = __half2float(scale);
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));   // (within an ulp)
+    bool slow = !(fast >= 6.2e-5f && fast <= 65000.0f);       // (normal fp16 with room to round either way; false for NaN)
+    float c[8];
+#pragma unroll
+    for (int d = 0; d < 8; d++) {
+        c[d] = fmaf(x[d], inv, MAGIC) - MAGIC;
+        slow |= fabsf(fmaf(-c[d], s, x[d])) == 0.5f * s;
+    }
+    const float lo = fmaf(fmaf(fmaf(c[6], 16.0f, c[4]), 16.0f, c[2]), 16.0f, c[0]);   // nibbles 3, 2, 1, 0
+    const float hi = fmaf(fmaf(fmaf(c[7], 16.0f, c[5]), 16.0f, c[3]), 16.0f, c[1]);   // nibbles 7, 6, 5, 4
+    const uint32_t l = __float_as_uint(lo + (MAGIC + 34952.0f)), h = __float_as_uint(hi + (MAGIC + 34952.0f));   // 0x8888
+    uint32_t word = __byte_perm(l, h, 0x5410) ^ 0x88888888u;
+    if (slow) {
+        scale = kv4_scale(top);
+        const float sf = __half2float(scale), si = sf > 0.0f ? __fdiv_rn(1.0f, sf) : 0.0f;
+        word = 0;
+#pragma unroll
+        for (int d = 0; d < 8; d++) word |= (uint32_t(kv4_code(x[d], sf, si)) & 15u) << (4 * kv4_nibble_of(d));
+    }
+    return word;
+}
+
 // The query row of a head that comes raw: RMS norm over the head with `ng` gains, in the order of the other decode kernels
 // (common.metal:30-41), rounded to the activation dtype. A lane holds dims lane + 32 i.
 template <int DT>

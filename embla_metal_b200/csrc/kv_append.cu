@@ -62,8 +62,9 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const AppendParams p) {
 // ---- 4-bit pools, and reading rows back -------------------------------------------------------------------------------
 // Half a warp takes a row: a lane holds 8 consecutive dims (16 bytes of activations, one word of codes), four lanes a scale
 // group. A warp takes 2 x PASSES consecutive rows of one side (K or V), every load in flight before the first is used; lane i works
-// out where row i lies, the others get it by shuffle. Bound by instructions (about 75 a row and warp to quantise), not by
-// the 784 bytes of a row in, out and back: a warp a row with two-byte loads took 93 us for 8 x 2048 tokens, append and read.
+// out where row i lies, the others get it by shuffle. Bound by instructions (about 90 a row to quantise, 55 to read back), not by
+// the bytes: 8 x 2048 tokens of 4 kv heads take 17.8 us to append (53 MB; 27 us with the keys normed) and 13.2 us to read
+// back, where a warp a row with two-byte loads took 93 us for the two.
 struct RowsParams {
     uint8_t* pool;
     const int32_t* block_table;
@@ -78,18 +79,20 @@ struct RowsParams {
     int table_stride, n_tokens, layer, n_layers, n_kv_heads, num_blocks, norm_k, kv_dtype, scale_bytes, vec;
 };
 
-// Where row i of a side lies: elements into k / v, and its page (NULL: nowhere, with the error word set) and row in it.
+// Where row i of a side lies: elements into k / v; its page (NULL: nowhere, with the error word set) and row in it.
+__device__ __forceinline__ long row_elements(const RowsParams& p, unsigned i, unsigned& b, unsigned& t, unsigned& h) {
+    const unsigned bt = i / unsigned(p.n_kv_heads);
+    h = i - bt * unsigned(p.n_kv_heads);
+    b = bt / unsigned(p.n_tokens);
+    t = bt - b * unsigned(p.n_tokens);
+    return long(b) * p.seq_stride + long(t) * p.token_stride + long(h) * HD;
+}
 struct RowPlace {
-    long at;
     uint8_t* page;
     int row;
 };
-__device__ __forceinline__ RowPlace row_place(const RowsParams& p, unsigned i) {
-    RowPlace w = {0, nullptr, 0};
-    if (i >= p.rows) return w;
-    const unsigned bt = i / unsigned(p.n_kv_heads), h = i - bt * unsigned(p.n_kv_heads);
-    const unsigned b = bt / unsigned(p.n_tokens), t = bt - b * unsigned(p.n_tokens);
-    w.at = long(b) * p.seq_stride + long(t) * p.token_stride + long(h) * HD;
+__device__ __forceinline__ RowPlace row_place(const RowsParams& p, unsigned b, unsigned t, unsigned h) {
+    RowPlace w = {nullptr, 0};
     const int pos = p.pos0 ? p.pos0[b] + int(t) : p.seq_lens[b] - 1;
     if (!p.pos0 && pos < 0) return w;   // (an empty sequence has no current token)
     int block = -1;
@@ -104,7 +107,6 @@ __device__ __forceinline__ RowPlace row_place(const RowsParams& p, unsigned i) {
 }
 __device__ __forceinline__ RowPlace shfl_place(const RowPlace& w, int lane) {
     RowPlace r;
-    r.at = __shfl_sync(0xffffffffu, w.at, lane);
     r.page = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(w.page), lane));
     r.row = __shfl_sync(0xffffffffu, w.row, lane);
     return r;
@@ -138,15 +140,16 @@ __global__ void __launch_bounds__(ROWS_WARPS * 32) kv4_append_kernel(const __gri
     if (unit >= 2 * groups) return;
     const bool is_v = unit >= groups;
     const unsigned first = (is_v ? unit - groups : unit) * per;
-    const RowPlace mine = lane < int(per) ? row_place(p, first + lane) : RowPlace{0, nullptr, 0};
+    const bool has = lane < int(per) && first + lane < p.rows;
+    unsigned b = 0, t = 0, h = 0;
+    const long elements = has ? row_elements(p, first + lane, b, t, h) : 0;
     uint4 x[PASSES];
-    RowPlace w[PASSES];
 #pragma unroll
     for (int i = 0; i < PASSES; i++) {
-        w[i] = shfl_place(mine, 2 * i + half);
-        const uint16_t* from = static_cast<const uint16_t*>(is_v ? p.v : p.k) + w[i].at + col * 8;
+        const long at = __shfl_sync(0xffffffffu, elements, 2 * i + half);
+        const uint16_t* from = static_cast<const uint16_t*>(is_v ? p.v : p.k) + at + col * 8;
         x[i] = make_uint4(0, 0, 0, 0);
-        if (w[i].page) {
+        if (first + 2 * i + half < p.rows) {
             if (p.vec) {
                 x[i] = *reinterpret_cast<const uint4*>(from);
             } else {
@@ -157,6 +160,8 @@ __global__ void __launch_bounds__(ROWS_WARPS * 32) kv4_append_kernel(const __gri
             }
         }
     }
+    // (the lookups of the rows' pages run beside the loads of the rows)
+    const RowPlace mine = has ? row_place(p, b, t, h) : RowPlace{nullptr, 0};
     if (NORM && !is_v) {
         // RMS norm without gains (common.metal:30-41): dims l, l + 32, l + 64, l + 96 into a partial sum each, then l = 0 .. 31
         float(*sq)[HD + 4] = squares[warp];
@@ -197,23 +202,24 @@ __global__ void __launch_bounds__(ROWS_WARPS * 32) kv4_append_kernel(const __gri
     }
 #pragma unroll
     for (int i = 0; i < PASSES; i++) {
+        const RowPlace w = shfl_place(mine, 2 * i + half);
         const uint32_t v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
         // the group's largest magnitude: the types' bits without the sign are ordered as the magnitudes are, NaN on top
         uint32_t top = __vmaxu2(__vmaxu2(v[0] & 0x7fff7fffu, v[1] & 0x7fff7fffu), __vmaxu2(v[2] & 0x7fff7fffu, v[3] & 0x7fff7fffu));
         top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const __half sh = kv4_scale(fmaxf_nan(act_lo<DT>(top), act_hi<DT>(top)));
-        const float s = __half2float(sh), inv = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;
-        uint32_t word = 0;
+        float xv[8];
 #pragma unroll
-        for (int d = 0; d < 8; d++) {
-            const float xv = (d & 1) ? act_hi<DT>(v[d >> 1]) : act_lo<DT>(v[d >> 1]);
-            word |= (uint32_t(kv4_code(xv, s, inv)) & 15u) << (4 * kv4_nibble_of(d));
+        for (int d = 0; d < 4; d++) {
+            xv[2 * d] = act_lo<DT>(v[d]);
+            xv[2 * d + 1] = act_hi<DT>(v[d]);
         }
-        if (!w[i].page) continue;
-        *reinterpret_cast<uint32_t*>(w[i].page + (is_v ? KV4_SIDE : 0) + w[i].row * KV4_ROW + col * 4) = word;
+        __half sh;
+        const uint32_t word = kv4_word(xv, fmaxf_nan(act_lo<DT>(top), act_hi<DT>(top)), sh);
+        if (!w.page) continue;
+        *reinterpret_cast<uint32_t*>(w.page + (is_v ? KV4_SIDE : 0) + w.row * KV4_ROW + col * 4) = word;
         if ((col & 3) == 0)
-            reinterpret_cast<__half*>(w[i].page + 2 * KV4_SIDE)[w[i].row * 2 * KV4_GROUPS + (is_v ? KV4_GROUPS : 0) + (col >> 2)] = sh;
+            reinterpret_cast<__half*>(w.page + 2 * KV4_SIDE)[w.row * 2 * KV4_GROUPS + (is_v ? KV4_GROUPS : 0) + (col >> 2)] = sh;
     }
 }
 
@@ -227,7 +233,10 @@ __global__ void __launch_bounds__(ROWS_WARPS * 32) kv_read_kernel(const __grid_c
     if (unit >= 2 * groups) return;
     const bool is_v = unit >= groups;
     const unsigned first = (is_v ? unit - groups : unit) * per;
-    const RowPlace mine = lane < int(per) ? row_place(p, first + lane) : RowPlace{0, nullptr, 0};
+    const bool has = lane < int(per) && first + lane < p.rows;
+    unsigned b = 0, t = 0, h = 0;
+    const long elements = has ? row_elements(p, first + lane, b, t, h) : 0;
+    const RowPlace mine = has ? row_place(p, b, t, h) : RowPlace{nullptr, 0};
     RowPlace w[PASSES];
     uint4 c[PASSES];   // the lane's 8 codes (or the row's values, 16-bit pools)
     float s[PASSES];
@@ -253,24 +262,34 @@ __global__ void __launch_bounds__(ROWS_WARPS * 32) kv_read_kernel(const __grid_c
     }
 #pragma unroll
     for (int i = 0; i < PASSES; i++) {
+        const long at = __shfl_sync(0xffffffffu, elements, 2 * i + half);
         if (!w[i].page) continue;
         uint4 out = c[i];
         if (p.kv_dtype != EMBLA_KV_16BIT) {
-            float x[8];
-#pragma unroll
-            for (int d = 0; d < 8; d++) {
-                const int code = p.kv_dtype == EMBLA_KV_INT4 ? int(c[i].x << (28 - 4 * kv4_nibble_of(d))) >> 28
-                                                             : int((d < 4 ? c[i].x : c[i].y) << (24 - 8 * (d & 3))) >> 24;
-                x[d] = float(code) * s[i];
+            uint32_t h[4];   // the codes as fp16 pairs, exactly
+            if (p.kv_dtype == EMBLA_KV_INT4) {
+                kv4_widen(c[i].x, h);
+            } else {
+                const uint32_t x0 = c[i].x ^ 0x80808080u, x1 = c[i].y ^ 0x80808080u;
+                h[0] = h2_from_biased_bytes(x0, 0x4140);
+                h[1] = h2_from_biased_bytes(x0, 0x4342);
+                h[2] = h2_from_biased_bytes(x1, 0x4140);
+                h[3] = h2_from_biased_bytes(x1, 0x4342);
             }
-            out = make_uint4(act_pack<DT>(x[0], x[1]), act_pack<DT>(x[2], x[3]), act_pack<DT>(x[4], x[5]), act_pack<DT>(x[6], x[7]));
+            uint32_t* to = &out.x;
+#pragma unroll
+            for (int d = 0; d < 4; d++) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[d]));
+                to[d] = act_pack<DT>(f.x * s[i], f.y * s[i]);
+            }
         }
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(is_v ? p.v : p.k) + w[i].at + col * 8) = out;
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(is_v ? p.v : p.k) + at + col * 8) = out;
     }
 }
 
-// Rows a warp takes: eight, or two while that leaves SMs without a warp.
-static int rows_passes(const EmblaAttn* ctx, unsigned rows) { return rows >= 8u * ROWS_WARPS * unsigned(ctx->sm_count) ? 4 : 1; }
+// Rows a warp takes: eight (fewer lookups a row), or two while eight would leave an SM fewer than 32 warps (2048 tokens of 4 heads:
+// 7.6 us with eight, 6.3 with four and less with two; 8 x 2048: 17.8 us with eight, 19.1 with four).
+static int rows_passes(const EmblaAttn* ctx, unsigned rows) { return rows >= 128u * unsigned(ctx->sm_count) ? 4 : 1; }
 
 static EmblaStatus rows_params(RowsParams& p, const char* fn, const EmblaKVPool* pool, const EmblaKVView* view, const int32_t* pos0, int n_tokens,
                                int64_t token_stride, int64_t seq_stride, const EmblaAttn* ctx) {
