@@ -1,7 +1,7 @@
 """A stack of attention layers decoding one token per sequence: binding of embla_stack_* (the
 attention half of the reference's Engine.encodeStep loop, Sources/EmblaMetal/Engine.swift:933-991).
 
-`DecodeStack` owns the KV state of a batch of sequences — the int8 pool of the full layers, the
+`DecodeStack` owns the KV state of a batch of sequences — the int8 or 4-bit pool of the full layers, the
 16-bit pool of the sparse layers, the sliding layers' rings, and identity block tables — and runs a
 step from device-resident `qkv` rows or, through `step_host`, from pinned host buffers.
 """
@@ -44,7 +44,8 @@ def cycle_kinds(n_layers):
 
 class DecodeStack:
     def __init__(self, kinds, batch, max_context, n_q_heads=16, n_kv_heads=4, act_dtype=attn.F16, window=1024,
-                 ring=4096, scale_dtype=attn.SCALE_F16, norm_k=False):
+                 ring=4096, scale_dtype=attn.SCALE_F16, norm_k=False, kv_dtype=attn.KV_INT8):
+        """kv_dtype: the full layers' cache, KV_INT8 or KV_INT4 (144 bytes a key and value instead of 260; scales fp16)."""
         self.kinds, self.batch, self.max_context = list(kinds), batch, max_context
         self.Hq, self.Hkv = n_q_heads, n_kv_heads
         self.ctx = attn.Attention(n_q_heads, n_kv_heads, act_dtype, max_batch=batch, max_context=max_context)
@@ -54,7 +55,7 @@ class DecodeStack:
         n_full = sum(k == FULL for k in self.kinds)
         n_sparse = sum(k == SPARSE for k in self.kinds)
         n_sliding = sum(k == SLIDING for k in self.kinds)
-        self.full_pool = attn.KVPool(n_full, n_kv_heads, batch * npages, attn.KV_INT8, scale_dtype) if n_full else None
+        self.full_pool = attn.KVPool(n_full, n_kv_heads, batch * npages, kv_dtype, scale_dtype) if n_full else None
         self.sparse_pool = attn.KVPool(n_sparse, n_kv_heads, batch * npages, attn.KV_16BIT) if n_sparse else None
         self.rings = [attn.Ring(batch, n_kv_heads, ring, window, self.dtype) for _ in range(n_sliding)]
         # sequence b owns blocks b * npages .. of each pool
@@ -106,14 +107,52 @@ class DecodeStack:
         self.seq_lens.copy_(t + 1)
         self.max_seq_len = int(t.max()) + 1
 
+    def fork(self, src, dst):
+        """Sequence `dst` goes on from where `src` stands (its last step or prompt done: keys seen = seq_lens): it shares the blocks
+        that src has filled, gets its own copy of the rows in src's last block and of its rings, and src's position. The
+        blocks dst held itself are used again, which is refused while another sequence shares them. src must not be set
+        back to a position inside the shared blocks while dst lives (its appends would write into them); going on is fine,
+        as is forking again. Reads src's length from the device (synchronises)."""
+        if src == dst or not (0 <= src < self.batch and 0 <= dst < self.batch):
+            raise ValueError(f"fork of sequence {src} into {dst} of {self.batch}")
+        sharers = (self.table // self.npages == dst).any(1)
+        sharers[dst] = False
+        if bool(sharers.any()):
+            raise ValueError(f"fork into sequence {dst}: sequences {sharers.nonzero().flatten().tolist()} share its blocks")
+        n = int(self.seq_lens[src])
+        full, rest = divmod(n, attn.BLOCK)
+        own = torch.arange(dst * self.npages, (dst + 1) * self.npages, dtype=torch.int32, device="cuda")
+        if rest:
+            src_block = self.table[src, full:full + 1].clone()
+            rows = torch.tensor([rest], dtype=torch.int32, device="cuda")
+            for pool in (self.full_pool, self.sparse_pool):
+                if pool is not None:
+                    self.ctx.copy_blocks(pool, src_block, own[full:full + 1], rows)
+        self.table[dst, :full] = self.table[src, :full]
+        self.table[dst, full:] = own[full:]
+        for r in self.rings:
+            r.k[dst].copy_(r.k[src])
+            r.v[dst].copy_(r.v[src])
+        self.pos[dst] = self.pos[src]
+        self.seq_lens[dst] = self.seq_lens[src]
+        self.max_seq_len = max(self.max_seq_len, n)
+
     def fill_random(self, seed=0):
         """Synthetic KV state in the benchmark's distributions: int8 codes uniform in [-127, 127] with fp16
-        scales uniform in [0.005, 0.02]; 16-bit keys/values ~ N(0, 1) with 1 % of the keys scaled x4."""
+        scales uniform in [0.005, 0.02] (4-bit: codes in [-7, 7], scales in [0.1, 0.4]); 16-bit keys/values ~ N(0, 1) with 1 % of the keys scaled x4."""
         g = torch.Generator(device="cuda").manual_seed(seed)
         if self.full_pool is not None:
             raw = self.full_pool.raw()
             flat = raw.view(-1, raw.shape[-1])
             step = max(1, (1 << 28) // flat.shape[1])
+            if self.full_pool.kv_dtype == attn.KV_INT4:
+                for i in range(0, flat.shape[0], step):
+                    part = flat[i:i + step]
+                    codes = torch.randint(-7, 8, (part.shape[0], 2, 16384), dtype=torch.int8, device="cuda", generator=g) & 15
+                    part[:, :16384] = (codes[:, 0] | (codes[:, 1] << 4)).view(torch.uint8)
+                    sc = torch.empty(part.shape[0], 1024, device="cuda").uniform_(0.1, 0.4, generator=g).to(torch.float16)
+                    part[:, 16384:] = sc.view(torch.uint8)
+                flat = flat[:0]
             sdt = torch.float16 if self.full_pool.scale_dtype == attn.SCALE_F16 else torch.float32
             for i in range(0, flat.shape[0], step):
                 part = flat[i:i + step]
@@ -212,7 +251,11 @@ class DecodeStack:
     def launches_per_step(self):
         """Kernels of this library one step launches."""
         selecting = self.max_seq_len > attn.TOPK + attn.RECENT
-        per = {SLIDING: 1, FULL: 1, SPARSE: 3 if selecting else 2, SPARSE_SHARED: 1}
+        # (a 4-bit full layer: the append and the attention; past a few hundred pages a launch that joins their runs as well)
+        four = self.full_pool is not None and self.full_pool.kv_dtype == attn.KV_INT4
+        pages = self.batch * self.Hkv * ((self.max_seq_len + attn.BLOCK - 1) // attn.BLOCK)
+        full = 1 if not four else 2 if pages <= attn.KV4_CLUSTER_PAGES else 3
+        per = {SLIDING: 1, FULL: full, SPARSE: 3 if selecting else 2, SPARSE_SHARED: 1}
         n = sum(per[k] for k in self.kinds)
         if selecting:   # a full layer followed by a shared-cache sparse layer also selects
             n += sum(1 for i, k in enumerate(self.kinds[:-1]) if k == FULL and self.kinds[i + 1] == SPARSE_SHARED)

@@ -415,6 +415,7 @@ enum {   /* Embla.Kind, Engine.swift:14; a sparse layer either owns 16-bit keys 
             reads the preceding full layer's int8 cache (SPARSE_SHARED, Engine.swift:461-462) */
     EMBLA_LAYER_SLIDING = 0, EMBLA_LAYER_FULL = 1, EMBLA_LAYER_SPARSE = 2, EMBLA_LAYER_SPARSE_SHARED = 3
 };
+/* (the full layers' pool may be EMBLA_KV_INT8 or EMBLA_KV_INT4; sparse layers that share it read either) */
 enum {   /* entry points a step launches, for embla_stack_set_probe */
     EMBLA_ENTRY_APPEND = 0, EMBLA_ENTRY_FULL_DECODE = 1, EMBLA_ENTRY_SLIDING_WRITE = 2, EMBLA_ENTRY_SLIDING_DECODE = 3,
     EMBLA_ENTRY_SCORE = 4, EMBLA_ENTRY_SELECT = 5, EMBLA_ENTRY_SPARSE_DECODE = 6
@@ -422,8 +423,8 @@ enum {   /* entry points a step launches, for embla_stack_set_probe */
 
 typedef struct {
     int32_t     kind;        /* EMBLA_LAYER_* */
-    int32_t     slot;        /* full: layer of the int8 pool; sparse: layer of the 16-bit pool; sparse shared: the int8
-                                pool layer of the full layer whose cache it reads; sliding: ring index */
+    int32_t     slot;        /* full: layer of the int8 or 4-bit pool; sparse: layer of the 16-bit pool; sparse shared: that
+                                pool's layer of the full layer whose cache it reads; sliding: ring index */
     int32_t     norm_k;      /* full/sparse: RMS-norm k before it is stored (the reference does) */
     int32_t     emit_scores; /* full: 1 = past 1152 keys also write key scores and select rows for the sparse layers
                                 that follow (Embla.selects, Engine.swift:24-26, 797) */
@@ -440,7 +441,7 @@ typedef struct {
     int64_t        o_stride, o_layer_stride;
     const int32_t* seq_lens_dev;       /* [batch] keys visible, the current token included (pos + 1) */
     const int32_t* pos_dev;            /* [batch] position of the current token */
-    const int32_t* full_table_dev;     /* block table into the int8 pool */
+    const int32_t* full_table_dev;     /* block table into the full layers' pool */
     int32_t        full_table_stride;
     int32_t        sparse_table_stride;
     const int32_t* sparse_table_dev;   /* block table into the 16-bit pool */
@@ -476,7 +477,7 @@ typedef struct {
     void*          o_dev;              /* [n_layers][batch][n_tokens][o_token_stride] */
     int64_t        o_token_stride, o_seq_stride, o_layer_stride;
     const int32_t* pos0_dev;           /* [batch] position of each sequence's first new token */
-    const int32_t* full_table_dev;     /* block table into the int8 pool */
+    const int32_t* full_table_dev;     /* block table into the full layers' pool */
     int32_t        full_table_stride;
     int32_t        batch;
     int32_t        n_tokens;           /* tokens of the chunk, the same for every sequence */
