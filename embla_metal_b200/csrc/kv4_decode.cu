@@ -32,10 +32,16 @@ constexpr int KD_TARGET = 10, KD_TARGET_BIG = -4;                  // log2 of th
 constexpr int KD_MAX_CLUSTER = 8;
 #ifndef KDCP
 #define KDCP 512
-#define KDMR 3
+#endif
+#ifndef KDMR
+#define KDMR 6
+#endif
+#ifndef KDUW
+#define KDUW 4
 #endif
 constexpr long KD_CLUSTER_PAGES = KDCP;   // most pages of a launch whose units are clusters
-constexpr int KD_MIN_RUN = KDMR;          // pages a run has at least
+constexpr int KD_UNIT_COST = KDUW;        // what a unit costs beside its pages, in pages
+constexpr int KD_MIN_RUN = KDMR;          // cost of a run at least
 
 struct Kv4DecodeParams {
     const uint8_t* pool;
@@ -65,17 +71,20 @@ constexpr size_t kd_inbox_rows(int ranges, int G) { return size_t(ranges) * ((G 
 
 __device__ __forceinline__ int kd_pages(const int32_t* seq_lens, int b) { return max(0, (__ldg(seq_lens + b) + BLK - 1) / BLK); }
 
-// The pages of all units, laid end to end, cut into `runs` runs whose lengths differ by one at most (and are KD_MIN_RUN or more,
+// What a unit of that many pages counts for when the work is cut: a unit begins with KD_UNIT_COST counts that stand for no page.
+__device__ __forceinline__ unsigned kd_cost(int pages) { return pages > 0 ? unsigned(pages + KD_UNIT_COST) : 0u; }
+
+// The costs of all units, laid end to end, cut into `runs` runs whose lengths differ by one at most (and are KD_MIN_RUN or more,
 // so that fewer CTAs than launched may have one).
 struct KdRuns {
-    unsigned runs, len, longer;   // the first `longer` runs have len + 1 pages, the others len
-    __device__ __forceinline__ KdRuns(unsigned pages, unsigned most) {
-        runs = max(1u, min(most, (pages + KD_MIN_RUN - 1) / KD_MIN_RUN));
-        len = pages / runs;
-        longer = pages - len * runs;
+    unsigned runs, len, longer;   // the first `longer` runs are len + 1 long, the others len
+    __device__ __forceinline__ KdRuns(unsigned cost, unsigned most) {
+        runs = max(1u, min(most, (cost + KD_MIN_RUN - 1) / KD_MIN_RUN));
+        len = cost / runs;
+        longer = cost - len * runs;
     }
     __device__ __forceinline__ unsigned start_of(unsigned c) const { return c * len + min(c, longer); }
-    __device__ __forceinline__ unsigned run_of(unsigned x) const {   // the run that page x is in
+    __device__ __forceinline__ unsigned run_of(unsigned x) const {   // the run that count x is in
         const unsigned edge = longer * (len + 1);
         return x < edge ? x / (len + 1) : longer + (x - edge) / max(len, 1u);
     }
@@ -86,15 +95,18 @@ struct KdPiece {
     int b, kvh, first, n, pages;
 };
 
-// The work of a CTA, walked by each of its warps alike. CL: the one range that the launch grid gives it. Else the pages of all
-// units, laid end to end (by sequence, then kv head), are cut into equal runs, one a CTA, whatever the sequences' lengths: a run
-// may end and begin inside a unit, whose pieces then meet in the scratch.
+// The work of a CTA, walked by its producer and its helpers alike. CL: the one range that the launch grid gives it. Else the costs
+// of all units, laid end to end (by sequence, then kv head), are cut into equal runs, one a CTA, whatever the sequences'
+// lengths: a run may end and begin inside a unit, whose pieces then meet in the scratch.
 template <bool CL>
 struct KdWalk {
-    int left, length;               // pages of the run still to come, and of all of it
-    KdPiece at;                     // piece under way (n = 0: none)
+    int left;        // cost of the run still to come
+    int into;        // where in the unit `at` stands at its next piece begins, in cost
+    int pieces;      // of the run so far
+    KdPiece at;      // piece under way
 
     __device__ __forceinline__ void start(const Kv4DecodeParams& p, int lane) {
+        left = into = pieces = 0;
         at.n = 0;
         if (CL) {
             at.b = blockIdx.z;
@@ -103,40 +115,44 @@ struct KdWalk {
             const int per = (at.pages + p.nsplit - 1) / p.nsplit;
             at.first = int(blockIdx.x) * per;
             left = max(0, min(at.pages, at.first + per) - at.first);
-            length = left;
             return;
         }
         // (up to 32 sequences, the usual case, take one load of their lengths)
-        auto scan = [&](int i0, int& n) {
-            n = i0 + lane < p.batch ? kd_pages(p.seq_lens, i0 + lane) : 0;
-            int incl = n;
+        auto scan = [&](int i0, unsigned& n, int& pages) {
+            pages = i0 + lane < p.batch ? kd_pages(p.seq_lens, i0 + lane) : 0;
+            n = kd_cost(pages);
+            unsigned incl = n;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, incl, o);
+                const unsigned v = __shfl_up_sync(0xffffffffu, incl, o);
                 if (lane >= o) incl += v;
             }
             return incl;
         };
-        int n, incl = scan(0, n), sum = __shfl_sync(0xffffffffu, incl, 31);
+        unsigned n, incl;
+        int pages;
+        incl = scan(0, n, pages);
+        unsigned sum = __shfl_sync(0xffffffffu, incl, 31);
         for (int i = 32 + lane; i < (p.batch + 31) / 32 * 32; i += 32)
-            sum += __reduce_add_sync(0xffffffffu, i < p.batch ? kd_pages(p.seq_lens, i) : 0);
-        const KdRuns cut(unsigned(sum) * p.n_kv_heads, p.n_runs);
+            sum += __reduce_add_sync(0xffffffffu, i < p.batch ? kd_cost(kd_pages(p.seq_lens, i)) : 0u);
+        const KdRuns cut(sum * p.n_kv_heads, p.n_runs);
         const unsigned c = blockIdx.x;
-        left = length = 0;
         if (c >= cut.runs) return;
         const unsigned x0 = cut.start_of(c);
-        left = length = int(cut.start_of(c + 1) - x0);
-        // the sequence that page x0 falls in: the first one whose pages end behind it
-        for (int i0 = 0, before = 0; i0 < p.batch; i0 += 32) {
-            if (i0 > 0) incl = scan(i0, n);
-            const unsigned here = __ballot_sync(0xffffffffu, unsigned(before + incl) * p.n_kv_heads > x0);
+        left = int(cut.start_of(c + 1) - x0);
+        // the sequence that count x0 falls in: the first one whose units end behind it
+        unsigned before = 0;
+        for (int i0 = 0; i0 < p.batch; i0 += 32) {
+            if (i0 > 0) incl = scan(i0, n, pages);
+            const unsigned here = __ballot_sync(0xffffffffu, (before + incl) * p.n_kv_heads > x0);
             if (here) {
                 const int l = __ffs(here) - 1;
+                const unsigned cost = __shfl_sync(0xffffffffu, n, l);
                 at.b = i0 + l;
-                at.pages = __shfl_sync(0xffffffffu, n, l);
-                const unsigned in = x0 - unsigned(before + __shfl_sync(0xffffffffu, incl, l) - at.pages) * p.n_kv_heads;
-                at.kvh = int(in / unsigned(at.pages));
-                at.first = int(in - unsigned(at.kvh) * unsigned(at.pages));
+                at.pages = __shfl_sync(0xffffffffu, pages, l);
+                const unsigned in = x0 - (before + __shfl_sync(0xffffffffu, incl, l) - cost) * p.n_kv_heads;
+                at.kvh = int(in / cost);
+                into = int(in - unsigned(at.kvh) * cost);
                 return;
             }
             before += __shfl_sync(0xffffffffu, incl, 31);
@@ -144,18 +160,33 @@ struct KdWalk {
     }
     // the next piece of the run; false when it is done
     __device__ __forceinline__ bool next(const Kv4DecodeParams& p) {
-        if (left <= 0) return false;
-        if (at.n > 0) {   // behind the piece before: a new unit begins
-            at.first = 0;
-            if (++at.kvh == p.n_kv_heads) {
-                at.kvh = 0;
-                do at.pages = kd_pages(p.seq_lens, ++at.b);
-                while (at.pages == 0);   // (the run has pages left: a sequence that has some follows)
+        if (CL) {
+            if (left <= 0) return false;
+            at.n = left;
+            left = 0;
+            return true;
+        }
+        while (left > 0) {
+            if (into == at.pages + KD_UNIT_COST) {   // behind the last unit
+                into = 0;
+                if (++at.kvh == p.n_kv_heads) {
+                    at.kvh = 0;
+                    do at.pages = kd_pages(p.seq_lens, ++at.b);
+                    while (at.pages == 0);   // (the run is not done: a sequence that has pages follows)
+                }
+            }
+            const int take = min(left, at.pages + KD_UNIT_COST - into);
+            at.first = max(0, into - KD_UNIT_COST);
+            at.n = max(0, into + take - KD_UNIT_COST) - at.first;
+            into += take;
+            left -= take;
+            if (at.n > 0) {
+                pieces++;
+                return true;
             }
         }
-        at.n = min(left, at.pages - at.first);
-        left -= at.n;
-        return true;
+        at.n = 0;
+        return false;
     }
 };
 
@@ -312,7 +343,7 @@ __global__ void __launch_bounds__((NCONS + 1 + KD_HELPERS) * 32, 1)
                 slot.first = at.first;
                 slot.unit = at.b * p.n_kv_heads + at.kvh;
                 // a run has at most two pieces of units that it shares with others, its first and its last
-                slot.out = at.n == at.pages ? -1 : 2 * int(blockIdx.x) + (walk.length - walk.left == at.n ? 0 : 1);
+                slot.out = at.n == at.pages ? -1 : 2 * int(blockIdx.x) + (walk.pieces == 1 ? 0 : 1);
             }
         };
         fetch();
@@ -626,19 +657,20 @@ __global__ void __launch_bounds__(128) kv4_decode_join_kernel(const __grid_const
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int hh = blockIdx.x, unit = blockIdx.y, b = unit / p.n_kv_heads, kvh = unit % p.n_kv_heads;
     trace_first(p.ctl.trace, 0);
-    int before = 0, sum = 0;
+    unsigned before = 0, sum = 0;
     for (int i = lane; i < p.batch; i += 32) {
-        const int n = kd_pages(p.seq_lens, i);
+        const unsigned n = kd_cost(kd_pages(p.seq_lens, i));
         sum += n;
         if (i < b) before += n;
     }
     sum = __reduce_add_sync(0xffffffffu, sum);
     before = __reduce_add_sync(0xffffffffu, before);
     const int pages = kd_pages(p.seq_lens, b);
-    const KdRuns runs(unsigned(sum) * p.n_kv_heads, p.n_runs);
-    const unsigned x = unsigned(before) * p.n_kv_heads + unsigned(kvh) * unsigned(pages);
-    const int lo = int(runs.run_of(x)), hi = int(runs.run_of(x + pages - 1));
-    const int first_slot = runs.start_of(lo) == x ? 2 * lo : 2 * lo + 1;   // (the unit may begin inside run lo)
+    const KdRuns runs(sum * p.n_kv_heads, p.n_runs);
+    const unsigned x = before * p.n_kv_heads + unsigned(kvh) * kd_cost(pages);
+    const int lo = int(runs.run_of(x + KD_UNIT_COST)), hi = int(runs.run_of(x + KD_UNIT_COST + pages - 1));
+    // (run lo may begin inside the unit, or with the end of one before it, which is a piece: pages come last in a unit's cost)
+    const int first_slot = runs.start_of(lo) >= x ? 2 * lo : 2 * lo + 1;
     // (every CTA waits, one with nothing to add too: the launch behind this one takes its end for the end of the runs)
     pdl_wait();
     pdl_launch_dependents();
@@ -754,7 +786,7 @@ EmblaStatus kv4_full_decode(EmblaAttn* ctx, const EmblaKVPool* pool, const Embla
     p.prenormed = q->prenormed;
     p.ng = q->ng;
     const long units = long(view->batch) * pool->n_kv_heads, pages = (max_len + BLK - 1) / BLK;
-    if (units * pages > 0x7fffffffL || units > 0xffff)
+    if (units * (pages + KD_UNIT_COST) > 0x7fffffffL || units > 0xffff)
         EMBLA_FAIL(EMBLA_BAD_ARG, "embla_attn_full_decode: %d sequences of up to %d keys are too many pages", view->batch, max_len);
     // Few pages: a cluster a unit, one page or a few a CTA. Else equal runs over the resident CTAs (the scratch holds two
     // pieces a run: embla_attn_create makes it 8 slots an SM and more).
@@ -764,7 +796,7 @@ EmblaStatus kv4_full_decode(EmblaAttn* ctx, const EmblaKVPool* pool, const Embla
         p.nsplit = int(pages < KD_MAX_CLUSTER ? pages : KD_MAX_CLUSTER);
         grid = dim3(p.nsplit, pool->n_kv_heads, view->batch);
     } else {
-        const long most = (units * pages + KD_MIN_RUN - 1) / KD_MIN_RUN, slots = ctx->sm_count;
+        const long most = (units * (pages + KD_UNIT_COST) + KD_MIN_RUN - 1) / KD_MIN_RUN, slots = ctx->sm_count;
         p.n_runs = int(most < slots ? most : slots);
         grid = dim3(p.n_runs);
     }
