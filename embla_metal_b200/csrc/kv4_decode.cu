@@ -30,16 +30,12 @@ constexpr int KD_SUM = HD + 1;   // a row of a warp's sums in shared memory: lan
 constexpr float KD_LIMIT = 8192.0f, KD_LIMIT_BIG = 0.5f;           // largest weight kept, usually and with large value scales
 constexpr int KD_TARGET = 10, KD_TARGET_BIG = -4;                  // log2 of the bound a new f puts on the tile's weights
 constexpr int KD_MAX_CLUSTER = 8;
-#ifndef KDCP
-#define KDCP 512
-#endif
 #ifndef KDMR
-#define KDMR 6
+#define KDMR 4
 #endif
 #ifndef KDUW
 #define KDUW 4
 #endif
-constexpr long KD_CLUSTER_PAGES = KDCP;   // most pages of a launch whose units are clusters
 constexpr int KD_UNIT_COST = KDUW;        // what a unit costs beside its pages, in pages
 constexpr int KD_MIN_RUN = KDMR;          // cost of a run at least
 
@@ -760,6 +756,35 @@ static EmblaStatus launch_kv4_decode(EmblaAttn* ctx, const EmblaKVPool* pool, co
     return EMBLA_OK;
 }
 
+// How many clusters of `ns` CTAs of the cluster form the GPU holds at once (all forms of it are alike in what they need).
+static long kd_clusters_at_once(const EmblaAttn* ctx, int ns) {
+    static int known[64][KD_MAX_CLUSTER + 1] = {};   // per device and size; 0: not asked yet, -1: none
+    int& n = known[ctx->device & 63][ns];
+    if (n == 0) {
+        using Shape = KdShape<true>;
+        auto kern = kv4_decode_kernel<EMBLA_BF16, false, Shape::ncons, Shape::wpg, Shape::stages, true>;
+        const size_t smem = kd_smem(Shape::ncons, Shape::stages, true) + 14 * KD_PART * 4;
+        int got = 0;
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) == cudaSuccess) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(ns);
+            cfg.blockDim = dim3((Shape::ncons + 1 + KD_HELPERS) * 32);
+            cfg.dynamicSmemBytes = smem;
+            cudaLaunchAttribute at;
+            at.id = cudaLaunchAttributeClusterDimension;
+            at.val.clusterDim.x = unsigned(ns);
+            at.val.clusterDim.y = 1;
+            at.val.clusterDim.z = 1;
+            cfg.attrs = &at;
+            cfg.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&got, kern, &cfg) != cudaSuccess) got = 0;
+        }
+        (void)cudaGetLastError();
+        n = got > 0 ? got : -1;
+    }
+    return n;
+}
+
 EmblaStatus kv4_full_decode(EmblaAttn* ctx, const EmblaKVPool* pool, const EmblaKVView* view, const EmblaQuery* q, void* o_dev,
                             int64_t o_stride, float* scores_dev, int64_t scores_stride, int max_len, cudaStream_t stream) {
     Kv4DecodeParams p = {};
@@ -788,17 +813,23 @@ EmblaStatus kv4_full_decode(EmblaAttn* ctx, const EmblaKVPool* pool, const Embla
     const long units = long(view->batch) * pool->n_kv_heads, pages = (max_len + BLK - 1) / BLK;
     if (units * (pages + KD_UNIT_COST) > 0x7fffffffL || units > 0xffff)
         EMBLA_FAIL(EMBLA_BAD_ARG, "embla_attn_full_decode: %d sequences of up to %d keys are too many pages", view->batch, max_len);
-    // Few pages: a cluster a unit, one page or a few a CTA. Else equal runs over the resident CTAs (the scratch holds two
-    // pieces a run: embla_attn_create makes it 8 slots an SM and more).
-    const bool cluster = units * pages <= KD_CLUSTER_PAGES;
-    dim3 grid;
-    if (cluster) {
-        p.nsplit = int(pages < KD_MAX_CLUSTER ? pages : KD_MAX_CLUSTER);
-        grid = dim3(p.nsplit, pool->n_kv_heads, view->batch);
-    } else {
-        const long most = (units * (pages + KD_UNIT_COST) + KD_MIN_RUN - 1) / KD_MIN_RUN, slots = ctx->sm_count;
-        p.n_runs = int(most < slots ? most : slots);
-        grid = dim3(p.n_runs);
+    // Two ways, by what they measured, in hundredths of a microsecond: clusters, all at once, 570 + 62 a page of a range (one
+    // sequence of 1000 keys 6.3 us, of 8192 11.2); runs, 1000 + 62 a page or unit cost of a run (11.2 us at the shortest, 8 x 32768
+    // keys of 2 kv heads 27.7). The ranges of a unit are as many as let all clusters be resident (a GPC may hold one cluster of
+    // 8 such CTAs and not two). Runs: the scratch holds two pieces of each (embla_attn_create makes it 8 slots an SM and more).
+    const long cost = units * (pages + KD_UNIT_COST), most = (cost + KD_MIN_RUN - 1) / KD_MIN_RUN;
+    p.n_runs = int(most < ctx->sm_count ? most : ctx->sm_count);
+    long best = 1000 + 62 * ((cost + p.n_runs - 1) / p.n_runs);
+    bool cluster = false;
+    dim3 grid(p.n_runs);
+    for (int ns = 1; ns <= KD_MAX_CLUSTER && ns <= pages; ns++) {
+        const long c = 570 + 62 * ((pages + ns - 1) / ns);
+        if (c < best && units <= kd_clusters_at_once(ctx, ns)) {
+            best = c;
+            cluster = true;
+            p.nsplit = ns;
+            grid = dim3(ns, pool->n_kv_heads, view->batch);
+        }
     }
     const bool bf = ctx->cfg.act_dtype == EMBLA_BF16;
 #define EMBLA_KD(DT, SC) (cluster ? launch_kv4_decode<DT, SC, true>(ctx, pool, p, view->batch, grid, stream) \
