@@ -547,7 +547,7 @@ __global__ void __launch_bounds__((NCONS + 1 + KD_HELPERS) * 32, 1)
                         for (int k = 0; k < TILES; k++) {
                             ps0 += w[k][0] + w[k][2];
                             ps1 += w[k][1] + w[k][3];
-                            kv4_tile_values(kaddr + KV4_SIDE + k * 16 * KV4_ROW, rows[k], w[k], O);
+                            kv4_tile_values<DT>(kaddr + KV4_SIDE + k * 16 * KV4_ROW, rows[k], w[k], O);
                         }
                     }
                     __syncwarp();
@@ -816,7 +816,8 @@ EmblaStatus kv4_full_decode(EmblaAttn* ctx, const EmblaKVPool* pool, const Embla
     // Two ways, by what they measured, in hundredths of a microsecond: clusters, all at once, 570 + 62 a page of a range (one
     // sequence of 1000 keys 6.3 us, of 8192 11.2); runs, 1000 + 62 a page or unit cost of a run (11.2 us at the shortest, 8 x 32768
     // keys of 2 kv heads 27.7). The ranges of a unit are as many as let all clusters be resident (a GPC may hold one cluster of
-    // 8 such CTAs and not two). Runs: the scratch holds two pieces of each (embla_attn_create makes it 8 slots an SM and more).
+    // 8 such CTAs and not two) and no longer than 8 pages: longer ones are read at the pace of the longest sequence, where runs
+    // even uneven lengths out. Runs: the scratch holds two pieces of each (embla_attn_create makes it 8 slots an SM and more).
     const long cost = units * (pages + KD_UNIT_COST), most = (cost + KD_MIN_RUN - 1) / KD_MIN_RUN;
     p.n_runs = int(most < ctx->sm_count ? most : ctx->sm_count);
     long best = 1000 + 62 * ((cost + p.n_runs - 1) / p.n_runs);
@@ -824,7 +825,7 @@ EmblaStatus kv4_full_decode(EmblaAttn* ctx, const EmblaKVPool* pool, const Embla
     dim3 grid(p.n_runs);
     for (int ns = 1; ns <= KD_MAX_CLUSTER && ns <= pages; ns++) {
         const long c = 570 + 62 * ((pages + ns - 1) / ns);
-        if (c < best && units <= kd_clusters_at_once(ctx, ns)) {
+        if (c < best && (pages + ns - 1) / ns <= 8 && units <= kd_clusters_at_once(ctx, ns)) {
             best = c;
             cluster = true;
             p.nsplit = ns;

@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(KS_WARPS * 32, 4) kv4_sparse_kernel(const __gr
         for (int k = 0; k < 2; k++) {
             l0 += w[k][0] + w[k][2];
             l1 += w[k][1] + w[k][3];
-            kv4_tile_values(kaddr + KS_ROWS * KV4_ROW + k * 16 * KV4_ROW, sc[k], w[k], O);
+            kv4_tile_values<DT>(kaddr + KS_ROWS * KV4_ROW + k * 16 * KV4_ROW, sc[k], w[k], O);
         }
         __syncwarp();   // (the stage is read: the next turn's copies go into it)
     }

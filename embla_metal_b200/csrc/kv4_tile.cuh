@@ -164,21 +164,34 @@ __device__ __forceinline__ void kv4_tile_scores(uint32_t kaddr, const Kv4Scales&
 }
 
 // O^T += V^T P^T for the tile: w[0], w[1] the weights of key r for heads 2t, 2t + 1, w[2], w[3] of key r + 8. A weight times
-// the value's scale is rounded once, to fp16 (2^-11, fp32 before); an 8 x 8 transpose makes it the B register of head r, keys 2t,
+// the value's scale is rounded to fp16 once (2^-11, fp32 before) where the output is fp16; where it is bf16, whose own rounding
+// is eight times larger, the weight and the product are rounded both, which saves 22 instructions a tile (64 x 32768 keys: 218 us
+// instead of 230). An 8 x 8 transpose makes it the B register of head r, keys 2t,
 // 2t + 1. Accumulator tile 2g + p holds, in [0], [1], dim 32 g + 8 (r / 2) + (r % 2) + 4 p of heads 2t, 2t + 1, in [2], [3]
 // that dim + 2.
+template <int DT>
 __device__ __forceinline__ void kv4_tile_values(uint32_t vaddr, const Kv4Scales& sc, const float (&w)[4], float (&O)[8][4]) {
+    const uint32_t pw0 = pack_h2(w[0], w[1]), pw1 = pack_h2(w[2], w[3]);   // (bf16)
 #pragma unroll
     for (int j = 0; j < 2; j++) {
         uint32_t x[4];
         ldmatrix4_trans(x, vaddr ^ (j * 32));
-        const float2 v0 = __half22float2(*reinterpret_cast<const __half2*>(j ? &sc.k0.w : &sc.k0.z));
-        const float2 v1 = __half22float2(*reinterpret_cast<const __half2*>(j ? &sc.k1.w : &sc.k1.z));
+        const __half2 s0 = *reinterpret_cast<const __half2*>(j ? &sc.k0.w : &sc.k0.z), s1 = *reinterpret_cast<const __half2*>(j ? &sc.k1.w : &sc.k1.z);
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const int g = 2 * j + h;
-            const float x0 = h ? v0.y : v0.x, x1 = h ? v1.y : v1.x;
-            const uint32_t b0 = movmatrix4_trans(pack_h2(w[0] * x0, w[1] * x0)), b1 = movmatrix4_trans(pack_h2(w[2] * x1, w[3] * x1));
+            uint32_t b0, b1;
+            if (DT == EMBLA_BF16) {
+                const __half2 x0 = h ? __high2half2(s0) : __low2half2(s0), x1 = h ? __high2half2(s1) : __low2half2(s1);
+                b0 = h2_mul(pw0, *reinterpret_cast<const uint32_t*>(&x0));
+                b1 = h2_mul(pw1, *reinterpret_cast<const uint32_t*>(&x1));
+            } else {
+                const float x0 = h ? __high2float(s0) : __low2float(s0), x1 = h ? __high2float(s1) : __low2float(s1);
+                b0 = pack_h2(w[0] * x0, w[1] * x0);
+                b1 = pack_h2(w[2] * x1, w[3] * x1);
+            }
+            b0 = movmatrix4_trans(b0);
+            b1 = movmatrix4_trans(b1);
             uint32_t lo[4], hi[4];
             kv4_widen(x[2 * h], lo);
             kv4_widen(x[2 * h + 1], hi);
