@@ -20,7 +20,6 @@ BF16, F16 = 0, 1
 KV_INT8, KV_16BIT, KV_INT4 = 0, 1, 2
 SCALE_F32, SCALE_F16 = 0, 1
 HEAD_DIM, BLOCK, TOPK, RECENT = 128, 128, 1024, 128
-KV4_CLUSTER_PAGES = 512   # most pages that a 4-bit decode launch attends without a joining launch behind it
 OK, BAD_ARG, OOM, CUDA_ERR, NCCL_ERR, TIMEOUT, UNSUPPORTED = range(7)
 
 _TORCH_DT = {BF16: torch.bfloat16, F16: torch.float16}

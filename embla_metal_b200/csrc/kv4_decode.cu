@@ -4,7 +4,11 @@
 // Bound by HBM: a key and its value are 144 bytes, used once. As in the int8 kernel (full_decode.cu) a CTA streams a range of a
 // sequence's pages through a ring of shared-memory stages filled by TMA and a key's dots and sums run on warp tensor-core
 // tiles (kv4_tile.cuh); per byte there are nearly twice as many codes to widen, so what counts is instructions a key:
-// about 15 issue slots of the 25 that an SM has per key at full bandwidth.
+// 17.7 for fp16 outputs, 16.3 for bf16, of the 25 issue slots that an SM has per key at full bandwidth, 7.5 of them on the ALU
+// pipe, which has 12. 64 sequences of 32768 keys, 4 kv heads: 229 us (fp16, 5.3 TB/s, 0.80 of the measured copy rate) and
+// 217 us (bf16); 16 uneven sequences of up to 9001 keys: 28 us; one of 1000: 5.7 us. What is left of it: half of the issue slots
+// are used, twelve warps being what 128 registers a thread leave room for, and a launch's first 5 microseconds (lengths, block
+// table, queries and first pages one after another, code not yet in the instruction caches).
 //
 // Weights. w = relu(q.k / sqrt(128))^2 has no bound, and its product with a value's scale goes through fp16. Each warp
 // therefore keeps its weights as w' = relu(S)^2 f with a power of two f per head: when a weight of a tile passes LIMIT (tested
@@ -30,14 +34,9 @@ constexpr int KD_SUM = HD + 1;   // a row of a warp's sums in shared memory: lan
 constexpr float KD_LIMIT = 8192.0f, KD_LIMIT_BIG = 0.5f;           // largest weight kept, usually and with large value scales
 constexpr int KD_TARGET = 10, KD_TARGET_BIG = -4;                  // log2 of the bound a new f puts on the tile's weights
 constexpr int KD_MAX_CLUSTER = 8;
-#ifndef KDMR
-#define KDMR 4
-#endif
-#ifndef KDUW
-#define KDUW 4
-#endif
-constexpr int KD_UNIT_COST = KDUW;        // what a unit costs beside its pages, in pages
-constexpr int KD_MIN_RUN = KDMR;          // cost of a run at least
+// What a unit costs beside its pages, in pages (16 uneven sequences of up to 9001 keys: 29.0 us counting 4, 31.7 counting 2, 39 none).
+constexpr int KD_UNIT_COST = 4;
+constexpr int KD_MIN_RUN = 4;   // cost of a run at least
 
 struct Kv4DecodeParams {
     const uint8_t* pool;
@@ -65,7 +64,10 @@ constexpr size_t kd_sums_at(int stages, bool cl) { return (kd_bars_at(stages, cl
 constexpr size_t kd_smem(int ncons, int stages, bool cl) { return 1024 + kd_sums_at(stages, cl) + size_t(ncons) * 8 * KD_SUM * 4; }
 constexpr size_t kd_inbox_rows(int ranges, int G) { return size_t(ranges) * ((G + ranges - 1) / ranges); }
 
-__device__ __forceinline__ int kd_pages(const int32_t* seq_lens, int b) { return max(0, (__ldg(seq_lens + b) + BLK - 1) / BLK); }
+__device__ __forceinline__ int kd_pages(const int32_t* seq_lens, int b) {
+    const int S = __ldg(seq_lens + b);
+    return S > 0 ? (S - 1) / BLK + 1 : 0;
+}
 
 // What a unit of that many pages counts for when the work is cut: a unit begins with KD_UNIT_COST counts that stand for no page.
 __device__ __forceinline__ unsigned kd_cost(int pages) { return pages > 0 ? unsigned(pages + KD_UNIT_COST) : 0u; }
@@ -718,15 +720,11 @@ __global__ void __launch_bounds__(128) kv4_decode_join_kernel(const __grid_const
     trace_last(p.ctl.trace, 3);
 }
 
-#ifndef KDN
-#define KDN 12
-#define KDW 4
-#define KDS 9
-#endif
-// A CTA an SM: 12 consumer warps (at 128 registers the SM holds no more), four to a page, ten pages in flight. A cluster's CTA:
+// A CTA an SM: 12 consumer warps (at 128 registers the SM holds no more beside producer and helpers), four to a page, nine pages in
+// flight. A cluster's CTA:
 // one tile a warp, so that a page or two are done soonest.
 template <bool CL> struct KdShape {
-    static constexpr int ncons = CL ? 8 : KDN, wpg = CL ? 8 : KDW, stages = CL ? 4 : KDS;
+    static constexpr int ncons = CL ? 8 : 12, wpg = CL ? 8 : 4, stages = CL ? 4 : 9;
 };
 
 static bool use_pdl() {

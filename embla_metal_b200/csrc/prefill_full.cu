@@ -1215,6 +1215,8 @@ static EmblaStatus full_prefill_impl(EmblaAttn* ctx, const EmblaKVPool* pool, co
         EMBLA_FAIL(EMBLA_BAD_ARG, "embla_attn_full_prefill: batch %d, n_tokens %d", view->batch, n_tokens);
     if (!q->prenormed && (q->ng != 2 || !q->g1_dev || !q->g2_dev))
         EMBLA_FAIL(EMBLA_BAD_ARG, "embla_attn_full_prefill: the fused head norm takes both gain vectors (ng = 2)");
+    if (kv4 && ((reinterpret_cast<uintptr_t>(q->q_dev) | reinterpret_cast<uintptr_t>(o_dev)) % 16))
+        EMBLA_FAIL(EMBLA_BAD_ARG, "embla_attn_full_prefill: q and o must be 16-byte aligned");
     if ((q_token_stride % 8) || (q->q_stride % 8) || (o_token_stride % 8) || (o_seq_stride % 8))
         EMBLA_FAIL(EMBLA_BAD_ARG, "embla_attn_full_prefill: strides must be multiples of 8 elements (16-byte rows)");
     PrefillParams p;

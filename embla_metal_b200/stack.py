@@ -249,13 +249,11 @@ class DecodeStack:
         return ms.value, n.value
 
     def launches_per_step(self):
-        """Kernels of this library one step launches."""
+        """Kernels of this library one step launches (at least, over a 4-bit cache)."""
         selecting = self.max_seq_len > attn.TOPK + attn.RECENT
-        # (a 4-bit full layer: the append and the attention; past a few hundred pages a launch that joins their runs as well)
+        # (a 4-bit full layer: the append and the attention, and with many pages a third that joins pieces, not counted here)
         four = self.full_pool is not None and self.full_pool.kv_dtype == attn.KV_INT4
-        pages = self.batch * self.Hkv * ((self.max_seq_len + attn.BLOCK - 1) // attn.BLOCK)
-        full = 1 if not four else 2 if pages <= attn.KV4_CLUSTER_PAGES else 3
-        per = {SLIDING: 1, FULL: full, SPARSE: 3 if selecting else 2, SPARSE_SHARED: 1}
+        per = {SLIDING: 1, FULL: 2 if four else 1, SPARSE: 3 if selecting else 2, SPARSE_SHARED: 1}
         n = sum(per[k] for k in self.kinds)
         if selecting:   # a full layer followed by a shared-cache sparse layer also selects
             n += sum(1 for i, k in enumerate(self.kinds[:-1]) if k == FULL and self.kinds[i + 1] == SPARSE_SHARED)

@@ -3,6 +3,7 @@
     python microbench.py full_decode --batch 8 [--scores]
     python microbench.py sparse --batch 8        # score, select, gather-attend, sliding attend
     python microbench.py prefill --tokens 2048 --cached 30720
+    python microbench.py full_decode --kv4; python microbench.py prefill --kv4; python microbench.py copy_blocks    # 4-bit pools
 
 Each case prints one line per kernel with its time per launch and the bandwidth or FLOP rate that follows
 from the algorithmic bytes / FLOPs of the launch.
@@ -33,12 +34,23 @@ def _events(fn, reps=10, warm=3):
     return sorted(ev[i].elapsed_time(ev[i + 1]) for i in range(reps))
 
 
-def full_decode(batch, scores, kv16=False):
+def _fill4(pool):
+    """Codes in [-7, 7] and scales of 0.2 in a 4-bit pool."""
+    raw = pool.raw()
+    codes = torch.randint(-7, 8, (*raw.shape[:-1], 2, 16384), dtype=torch.int8, device="cuda") & 15
+    raw[..., :16384] = (codes[..., 0, :] | (codes[..., 1, :] << 4)).view(torch.uint8)
+    raw[..., 16384:].view(torch.float16).fill_(0.2)
+
+
+def full_decode(batch, scores, kv16=False, kv4=False):
     npg = CTX // 128
     ctx = attn.Attention(HQ, HKV, attn.F16, max_batch=batch, max_context=CTX)
     if kv16:   # the build without the int8 cache: rows in the activation dtype, 512 B a key
         pool = attn.KVPool(1, HKV, batch * npg, attn.KV_16BIT)
         pool.raw().view(torch.float16).normal_()
+    elif kv4:   # 4-bit pages: 144 B a key
+        pool = attn.KVPool(1, HKV, batch * npg, attn.KV_INT4)
+        _fill4(pool)
     else:
         pool = attn.KVPool(1, HKV, batch * npg, attn.KV_INT8, attn.SCALE_F16)
         raw = pool.raw()
@@ -51,8 +63,8 @@ def full_decode(batch, scores, kv16=False):
     sc = torch.zeros(batch, HKV, CTX, device="cuda") if scores else None
     ts = _events(lambda: ctx.full_decode(pool, table, lens, 0, q, o, scores=sc, max_seq_len=CTX))
     ctx.check()
-    nbytes = batch * HKV * CTX * (512 if kv16 else 260)
-    print(f"full_decode{' (16-bit cache)' if kv16 else ''} batch {batch} scores {bool(scores)}: {1e3 * ts[len(ts) // 2]:.1f} us/launch, "
+    nbytes = batch * HKV * CTX * (512 if kv16 else 144 if kv4 else 260)
+    print(f"full_decode{' (16-bit cache)' if kv16 else ' (4-bit cache)' if kv4 else ''} batch {batch} scores {bool(scores)}: {1e3 * ts[len(ts) // 2]:.1f} us/launch, "
           f"{nbytes / ts[len(ts) // 2] / 1e6:.0f} GB/s (min {nbytes / ts[0] / 1e6:.0f})")
 
 
@@ -79,14 +91,17 @@ def sparse(batch):
     st.ctx.check()
 
 
-def prefill(tokens, cached, qk8=False):
+def prefill(tokens, cached, qk8=False, kv4=False):
     S = cached + tokens
     npg = (S + 127) // 128
     ctx = attn.Attention(HQ, HKV, attn.BF16, 1, npg * 128)
-    pool = attn.KVPool(1, HKV, npg, attn.KV_INT8, attn.SCALE_F16)
-    raw = pool.raw()
-    raw.view(-1).random_(0, 256)
-    raw[..., 32768:].view(torch.float16).fill_(0.01)
+    pool = attn.KVPool(1, HKV, npg, attn.KV_INT4 if kv4 else attn.KV_INT8, attn.SCALE_F16)
+    if kv4:
+        _fill4(pool)
+    else:
+        raw = pool.raw()
+        raw.view(-1).random_(0, 256)
+        raw[..., 32768:].view(torch.float16).fill_(0.01)
     tbl = torch.arange(npg, dtype=torch.int32, device="cuda")[None].contiguous()
     q = torch.randn(1, tokens, HQ * 128, device="cuda", dtype=torch.bfloat16)
     o = torch.zeros_like(q)
@@ -95,8 +110,19 @@ def prefill(tokens, cached, qk8=False):
     ctx.check()
     flop = 4 * HQ * 128 * sum(cached + i + 1 for i in range(tokens))
     med = ts[len(ts) // 2]
-    print(f"full_prefill{' (int8 Q K^T)' if qk8 else ''} {tokens} tokens after {cached}: {med:.4f} ms, {flop / med / 1e9:.0f} TFLOP/s "
+    print(f"full_prefill{' (int8 Q K^T)' if qk8 else ' (4-bit cache)' if kv4 else ''} {tokens} tokens after {cached}: {med:.4f} ms, {flop / med / 1e9:.0f} TFLOP/s "
           f"(min-time {flop / ts[0] / 1e9:.0f}), {tokens / med * 1e3:.0f} tok/s")
+
+
+def copy_blocks(n):
+    """`n` whole blocks of a 4-bit pool of six layers moved inside it."""
+    pool = attn.KVPool(6, HKV, 2 * n, attn.KV_INT4)
+    ctx = attn.Attention(HQ, HKV, attn.F16)
+    ids = torch.randperm(2 * n, device="cuda").to(torch.int32)
+    ts = _events(lambda: ctx.copy_blocks(pool, ids[:n], ids[n:]))
+    ctx.check()
+    med = ts[len(ts) // 2]
+    print(f"copy_blocks {n} of {pool.block_bytes} bytes: {1e3 * med:.1f} us, {2 * n * pool.block_bytes / med / 1e6:.0f} GB/s")
 
 
 def sliding_prefill(tokens, cached, window, raw=False):
@@ -154,26 +180,30 @@ def qkv_project(batch, fused):
 
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("case", choices=["full_decode", "sparse", "prefill", "sliding_prefill", "qkv_project"])
+    ap.add_argument("case", choices=["full_decode", "sparse", "prefill", "sliding_prefill", "qkv_project", "copy_blocks"])
     ap.add_argument("--window", type=int, default=1024)
     ap.add_argument("--raw", action="store_true", help="sliding_prefill: queries arrive raw (fused head norm + RoPE)")
     ap.add_argument("--batch", type=int, default=8)
     ap.add_argument("--scores", action="store_true")
     ap.add_argument("--qk8", action="store_true", help="prefill: the int8 Q K^T build")
     ap.add_argument("--kv16", action="store_true", help="full_decode: a 16-bit cache instead of int8")
+    ap.add_argument("--kv4", action="store_true", help="full_decode, prefill: a 4-bit cache instead of int8")
+    ap.add_argument("--blocks", type=int, default=512, help="copy_blocks: how many")
     ap.add_argument("--tokens", type=int, default=2048)
     ap.add_argument("--cached", type=int, default=30720)
     a = ap.parse_args()
     if a.case == "full_decode":
-        full_decode(a.batch, a.scores, a.kv16)
+        full_decode(a.batch, a.scores, a.kv16, a.kv4)
     elif a.case == "sparse":
         sparse(a.batch)
+    elif a.case == "copy_blocks":
+        copy_blocks(a.blocks)
     elif a.case == "qkv_project":
         qkv_project(a.batch, a.scores)
     elif a.case == "sliding_prefill":
         sliding_prefill(a.tokens, a.cached if a.cached != 30720 else 2048, a.window, a.raw)
     else:
-        prefill(a.tokens, a.cached, a.qk8)
+        prefill(a.tokens, a.cached, a.qk8, a.kv4)
 
 
 if __name__ == "__main__":

@@ -513,3 +513,141 @@ def test_refusals():
         ctx.qkv_project_full_step(w, wkv, wkv, torch.zeros(1, 128, dtype=torch.float16, device="cuda"),
                                   torch.zeros(1, 1024, dtype=torch.float16, device="cuda"), pool, table, ln, 1)
     assert e.value.status == attn.BAD_ARG                                               # (as for a 16-bit pool)
+
+
+# ---- blocks taken out and put back, prompts shared, chunks scattered, batches ---------------------------------------
+def test_exported_blocks_decode_the_same():
+    import torch
+    rng, ctx, pool, table, k, v = _setup("bf16", 8, 2, [700], 51, extra=8)
+    q = _queries(rng, 1, 8, "bf16", 0)
+    a, _ = _check_full(ctx, pool, table, k, v, [700], rng, "bf16", 8, q=q)
+    free = [i for i in range(pool.num_blocks) if i not in table[0].tolist()][:6]
+    host = [torch.empty(pool.block_bytes, dtype=torch.uint8).pin_memory() for _ in range(6)]
+    for i in range(6):
+        pool.export_block(int(table[0, i]), host[i])
+    torch.cuda.synchronize()
+    pool.raw()[table[0].long()] = 255
+    for i, f in enumerate(free):
+        pool.import_block(f, host[i])
+    b, _ = _check_full(ctx, pool, torch.tensor([free], dtype=torch.int32, device="cuda"), k, v, [700], rng, "bf16", 8, q=q)
+    assert torch.equal(a, b)
+
+
+def test_prefix_store_keeps_blocks_of_a_4bit_pool():
+    import torch
+    from embla_metal_b200 import attn
+    from embla_metal_b200.prefix import PrefixStore
+    rng = np.random.default_rng(52)
+    ctx = attn.Attention(4, 2, attn.F16, 2, 1024)
+    pool = attn.KVPool(2, 2, 12, attn.KV_INT4)
+    rings = [attn.Ring(2, 2, 1024, 128, torch.float16)]
+    rings[0].k.normal_()
+    rings[0].v.normal_()
+    pool.raw().copy_(torch.from_numpy(rng.integers(0, 256, tuple(pool.raw().shape), dtype=np.uint8)))
+    store = PrefixStore(1 << 28, pool, rings, n_kv_heads=2)
+    tokens = list(range(500))
+    store.save(0, [3, 1, 4, 5], tokens, 500, [500])
+    before = pool.raw()[[3, 1, 4]].clone()
+    start, _ = store.restore(1, [7, 8, 9, 10], tokens + [1, 2, 3])
+    torch.cuda.synchronize()
+    assert start == 384 and torch.equal(pool.raw()[[7, 8, 9]], before)
+
+
+@pytest.mark.parametrize("T,p0,Hq,Hkv", [(64, 300, 8, 2), (300, 5000, 4, 1)])
+def test_prefill_scattered_to_peers(T, p0, Hq, Hkv):
+    import torch
+    from embla_metal_b200 import attn
+    rng, ctx, pool, table, k, v = _setup("bf16", Hq, Hkv, [p0 + T], 53)
+    q = _act(_bits(rng.standard_normal((1, T, Hq * 128)), "bf16"), "bf16")
+    pos0 = torch.tensor([p0], dtype=torch.int32, device="cuda")
+    plain = torch.zeros_like(q)
+    attn.full_prefill(ctx, pool, table, 1, pos0, q, plain)
+    width = Hq * 128 + 256
+    outs = [torch.full((T, width), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(3)]
+    attn.full_prefill_scatter(ctx, pool, table, 1, pos0, q, outs[0][:, 128:128 + Hq * 128].unsqueeze(0),
+                              [o.data_ptr() + 256 for o in outs[1:]], width)
+    ctx.check()
+    for o in outs:
+        assert torch.equal(o[:, 128:128 + Hq * 128], plain[0])
+        assert (o[:, :128] == 7.0).all() and (o[:, 128 + Hq * 128:] == 7.0).all()
+
+
+@pytest.mark.parametrize("batch,n", [(300, 40), (70, 700), (33, 129)])
+def test_full_decode_of_many_sequences(batch, n):
+    """More sequences than a warp has lanes, more units than SMs, lengths from 0 to n."""
+    rng0 = np.random.default_rng(batch)
+    lens = [int(x) for x in rng0.integers(0, n + 1, batch)]
+    lens[0], lens[-1] = n, 0
+    rng, ctx, pool, table, k, v = _setup("f16", 4, 2, lens, 54)
+    _check_full(ctx, pool, table, k, v, lens, rng, "f16", 4, scores=True)
+
+
+def test_all_sequences_empty():
+    import torch
+    from embla_metal_b200 import attn
+    for batch, ctx_len in ((3, 128), (40, 8192)):
+        ctx = attn.Attention(8, 2, attn.BF16, batch, ctx_len)
+        pool = attn.KVPool(1, 2, 4, attn.KV_INT4)
+        table = torch.zeros(batch, ctx_len // 128, dtype=torch.int32, device="cuda")
+        ln = torch.zeros(batch, dtype=torch.int32, device="cuda")
+        q = torch.randn(batch, 1024, device="cuda").bfloat16()
+        for fn in (ctx.full_decode, ctx.sparse_decode):
+            o = torch.full_like(q, 5.0)
+            fn(pool, table, ln, 0, q, o, **({"idx": torch.zeros(batch, 2, 1152, dtype=torch.int32, device="cuda")} if fn == ctx.sparse_decode else {}))
+            ctx.check()
+            assert (o == 0).all()
+
+
+def test_calls_repeat_bit_for_bit_and_in_a_graph():
+    import torch
+    lens = [5000, 300, 1200, 0, 77, 2048]
+    rng, ctx, pool, table, k, v = _setup("bf16", 16, 4, lens, 55)
+    q = _queries(rng, 6, 16, "bf16", 2)
+    ln = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    idx = torch.stack([torch.stack([torch.randperm(max(n, 1152), device="cuda")[:1152] for _ in range(4)]) for n in lens]).to(torch.int32)
+    o, s = torch.zeros(6, 2048, dtype=torch.bfloat16, device="cuda"), torch.zeros(6, 2048, dtype=torch.bfloat16, device="cuda")
+    sc = torch.zeros(6, 4, 5120, device="cuda")
+
+    def calls():
+        ctx.full_decode(pool, table, ln, 1, q[0], o, gains=q[2], scores=sc, max_seq_len=5000)
+        ctx.sparse_decode(pool, table, ln, 1, q[0], s, idx=idx, gains=q[2], max_seq_len=5000)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        calls()
+        side.synchronize()
+        want = [t.clone() for t in (o, s, sc)]
+        for _ in range(5):
+            calls()
+        side.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip((o, s, sc), want))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            calls()
+        for t in (o, s, sc):
+            t.zero_()
+        for _ in range(3):
+            graph.replay()
+        side.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip((o, s, sc), want))
+        ctx.check()
+    del graph
+
+
+def test_append_of_rows_at_any_alignment():
+    """Rows that do not start on 16 bytes, strides that are no multiple of 8 elements."""
+    import torch
+    from embla_metal_b200 import attn
+    ctx = attn.Attention(2, 2, attn.F16, 2, 512)
+    pools = [attn.KVPool(1, 2, 8, attn.KV_INT4) for _ in range(2)]
+    table = torch.arange(8, dtype=torch.int32, device="cuda").view(2, 4)
+    p0 = torch.tensor([3, 250], dtype=torch.int32, device="cuda")
+    x = torch.randn(2, 2, 9, 256, device="cuda").half()
+    odd = torch.zeros(2, 2, 9, 263, device="cuda", dtype=torch.float16)
+    odd[..., 3:259] = x
+    for norm in (False, True):
+        ctx.kv_append(pools[0], table, 0, p0, x[0], x[1], norm_k=norm)
+        ctx.kv_append(pools[1], table, 0, p0, odd[0][..., 3:259], odd[1][..., 3:259], norm_k=norm)
+        ctx.check()
+        assert torch.equal(pools[0].raw(), pools[1].raw())
