@@ -285,6 +285,8 @@ class Attention:
         pos0[b] + t, dequantised and rounded to the activation dtype. Pools of every type."""
         if k.dtype != self.torch_dtype or v.dtype != self.torch_dtype or k.shape != v.shape or k.stride() != v.stride() or k.stride(2) != 1:
             raise ValueError(f"k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} must be alike, rows contiguous, in {self.torch_dtype}")
+        if k.shape[0] != block_table.shape[0] or k.shape[2] < pool.n_kv_heads * HEAD_DIM:
+            raise ValueError(f"k {tuple(k.shape)} does not hold {pool.n_kv_heads} kv heads of {block_table.shape[0]} sequences")
         _check(lib().embla_kv_read(self.handle, pool.handle, self._pack_view(block_table, None, layer), pos0.data_ptr(), k.shape[1],
                                    k.data_ptr(), v.data_ptr(), k.stride(1), k.stride(0), _raw_stream()))
 

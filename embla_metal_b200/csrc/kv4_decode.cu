@@ -29,6 +29,17 @@ __device__ __forceinline__ int here(int x) {
 }
 __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
+// a barrier that tells all its threads whether any of them said yes
+__device__ __forceinline__ bool bar_any(int id, int threads, bool yes) {
+    int any;
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.s32 p, %1, 0;\n bar.red.or.pred q, %2, %3, p;\n selp.s32 %0, 1, 0, q;\n}\n"
+        : "=r"(any)
+        : "r"(int(yes)), "r"(id), "r"(threads)
+        : "memory");
+    return any != 0;
+}
+
 constexpr int KD_PART = HD + 4;                                    // floats per (range, head): 128 sums, sum of weights
 constexpr int KD_SUM = HD + 1;   // a row of a warp's sums in shared memory: lanes (r, t) write heads 2t at dims 8 (r / 2) + r % 2: 32 banks
 constexpr float KD_LIMIT = 8192.0f, KD_LIMIT_BIG = 0.5f;           // largest weight kept, usually and with large value scales
@@ -371,7 +382,8 @@ __global__ void __launch_bounds__((NCONS + 1 + KD_HELPERS) * 32, 1)
                 bar_sync(2, KD_HELPERS * 32);                       // (the slot's words are thread 0's)
                 const int n = slot.n;
                 if (n < 0) break;
-                if (!__all_sync(0xffffffffu, mbar_wait_bounded(p.ctl.wait_cycles, &summed[j % BUFS], (j / BUFS) & 1))) {
+                // (the helpers go on or leave together: the barriers below count all of them)
+                if (bar_any(2, KD_HELPERS * 32, !mbar_wait_bounded(p.ctl.wait_cycles, &summed[j % BUFS], (j / BUFS) & 1))) {
                     fail(ERR_WAIT_FULL);
                     break;
                 }

@@ -501,6 +501,12 @@ def test_refusals():
         ctx.kv_read(pool, table, 2, p0, x, x.clone())                                   # a layer the pool does not have
     with pytest.raises(ValueError):
         ctx.kv_read(pool, table, 1, p0, x.float(), x.float())
+    with pytest.raises(ValueError):                                                     # rows too narrow for two kv heads
+        ctx.kv_read(pool, table, 1, p0, x[..., :128], x[..., :128])
+    shifted = torch.zeros(600, dtype=torch.float16, device="cuda")[1:513].view(1, 1, 512)
+    with pytest.raises(attn.EmblaError) as e:                                           # queries that do not start on 16 bytes
+        attn.full_prefill(ctx, pool, table, 1, p0, shifted, torch.zeros_like(shifted))
+    assert e.value.status == attn.BAD_ARG
     with pytest.raises(ValueError):
         ctx.copy_blocks(pool, p0.long(), p0.long())
     with pytest.raises(ValueError):
