@@ -60,9 +60,10 @@ class KVView(C.Structure):
                 ("batch", C.c_int32), ("layer", C.c_int32), ("max_seq_len", C.c_int32)]
 
 
-# The calls of a serving loop pack their EmblaKVView and EmblaQuery into buffers of the context and pass plain integers to
-# functions that know their argument types: about 4 microseconds of host time less a call than building ctypes objects.
-_VIEW = struct.Struct("@PiPiii")
+# The calls of a serving loop pass their EmblaKVView and EmblaQuery as packed bytes (a call's own, so that threads may share a
+# context for calls that share no scratch) and plain integers to functions that know their argument types: about 4 microseconds
+# of host time less a call than building ctypes objects.
+_VIEW = struct.Struct("@PiPiii4x")
 _QUERY = struct.Struct("@PqiiPP")
 _P, _I, _I64 = C.c_void_p, C.c_int32, C.c_int64
 _ARGTYPES = {
@@ -179,9 +180,6 @@ class Attention:
         self.handle = C.c_void_p()
         _check(lib().embla_attn_create(C.byref(self.cfg), C.byref(self.handle)))
         self.torch_dtype = _TORCH_DT[act_dtype]
-        self._view_buf = C.create_string_buffer(C.sizeof(KVView))
-        self._query_buf = C.create_string_buffer(C.sizeof(Query))
-        self._view_at, self._query_at = C.addressof(self._view_buf), C.addressof(self._query_buf)
 
     def close(self):
         if self.handle:
@@ -221,19 +219,17 @@ class Attention:
         _check(lib().embla_attn_trace_end(self.handle, _stream(), stamps, entries, cap, C.byref(n)))
         return [(entries[i], *[stamps[8 * i + k] for k in range(8)]) for i in range(n.value)]
 
-    def _pack_view(self, block_table, seq_lens, layer, max_seq_len=0):
-        """EmblaKVView of a call into the context's buffer; its address."""
-        _VIEW.pack_into(self._view_buf, 0, block_table.data_ptr(), block_table.stride(0), _addr(seq_lens), block_table.shape[0], layer,
-                        max_seq_len)
-        return self._view_at
+    @staticmethod
+    def _pack_view(block_table, seq_lens, layer, max_seq_len=0):
+        """EmblaKVView of a call, as bytes."""
+        return _VIEW.pack(block_table.data_ptr(), block_table.stride(0), _addr(seq_lens), block_table.shape[0], layer, max_seq_len)
 
-    def _pack_query(self, q, gains):
+    @staticmethod
+    def _pack_query(q, gains):
         if gains is None:
-            _QUERY.pack_into(self._query_buf, 0, q.data_ptr(), q.stride(0), 1, 0, 0, 0)
-        else:
-            g1, g2 = gains
-            _QUERY.pack_into(self._query_buf, 0, q.data_ptr(), q.stride(0), 0, 1 if g2 is None else 2, g1.data_ptr(), _addr(g2))
-        return self._query_at
+            return _QUERY.pack(q.data_ptr(), q.stride(0), 1, 0, 0, 0)
+        g1, g2 = gains
+        return _QUERY.pack(q.data_ptr(), q.stride(0), 0, 1 if g2 is None else 2, g1.data_ptr(), _addr(g2))
 
     @staticmethod
     def view(block_table, seq_lens, layer, max_seq_len=0):

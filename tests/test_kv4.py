@@ -41,3 +41,12 @@ def test_refusals_without_a_gpu():
     assert L.embla_kv_read(None, None, None, None, 1, None, None, C.c_int64(0), C.c_int64(0), None) == attn.BAD_ARG
     assert L.embla_kv_copy_blocks(None, None, None, None, None, 1, None) == attn.BAD_ARG
     assert L.embla_attn_sparse_decode_int4(None, None, None, None, None, None, C.c_int64(0), None) == attn.BAD_ARG
+
+
+def test_packed_records_are_the_header_s_structs():
+    from embla_metal_b200 import attn
+    assert attn._VIEW.size == C.sizeof(attn.KVView) and attn._QUERY.size == C.sizeof(attn.Query)
+    v = attn.KVView.from_buffer_copy(attn._VIEW.pack(2 ** 40 + 1, 7, 2 ** 40 + 2, 3, 4, 5))
+    assert [getattr(v, f[0]) for f in v._fields_] == [2 ** 40 + 1, 7, 2 ** 40 + 2, 3, 4, 5]
+    q = attn.Query.from_buffer_copy(attn._QUERY.pack(2 ** 40 + 1, 2 ** 35, 1, 2, 2 ** 40 + 3, 0))
+    assert [getattr(q, f[0]) for f in q._fields_] == [2 ** 40 + 1, 2 ** 35, 1, 2, 2 ** 40 + 3, None]
