@@ -5,10 +5,12 @@
 // sequence's pages through a ring of shared-memory stages filled by TMA and a key's dots and sums run on warp tensor-core
 // tiles (kv4_tile.cuh); per byte there are nearly twice as many codes to widen, so what counts is instructions a key:
 // 17.7 for fp16 outputs, 16.3 for bf16, of the 25 issue slots that an SM has per key at full bandwidth, 7.5 of them on the ALU
-// pipe, which has 12. 64 sequences of 32768 keys, 4 kv heads: 229 us (fp16, 5.3 TB/s, 0.80 of the measured copy rate) and
-// 217 us (bf16); 16 uneven sequences of up to 9001 keys: 28 us; one of 1000: 5.7 us. What is left of it: half of the issue slots
-// are used, twelve warps being what 128 registers a thread leave room for, and a launch's first 5 microseconds (lengths, block
-// table, queries and first pages one after another, code not yet in the instruction caches).
+// pipe, which has 12. 64 sequences of 32768 keys, 4 kv heads: 224 us (fp16, 5.4 TB/s, 0.82 of the measured copy rate) and
+// 215 us (bf16); 16 uneven sequences of up to 9001 keys: 26 us; one of 1000: 5.6 us. What is left of it: half of the issue slots
+// are used, twelve warps being what 128 registers a thread leave room for; a launch's first 4 microseconds (lengths, block
+// table, first pages one after another) and its last 3 (the pieces' sums, written on one SM and read on another). Adding the
+// pieces up in the CTA that ends last, counted by atomics, took 0.7 to 2 microseconds longer than a second launch that is there
+// and waits; running the page loop once ahead of the first page, for the instruction caches, 1.3 longer than not.
 //
 // Weights. w = relu(q.k / sqrt(128))^2 has no bound, and its product with a value's scale goes through fp16. Each warp
 // therefore keeps its weights as w' = relu(S)^2 f with a power of two f per head: when a weight of a tile passes LIMIT (tested
@@ -28,6 +30,11 @@ __device__ __forceinline__ int here(int x) {
     return x;
 }
 __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+
+__device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+__device__ __forceinline__ void prefetch_l2(const void* at) { asm volatile("prefetch.global.L2 [%0];" ::"l"(at)); }
 
 // a barrier that tells all its threads whether any of them said yes
 __device__ __forceinline__ bool bar_any(int id, int threads, bool yes) {
@@ -225,6 +232,10 @@ __global__ void __launch_bounds__((NCONS + 1 + KD_HELPERS) * 32, 1)
     constexpr int GROUPS = NCONS / WPG;
     constexpr int PRODUCER = NCONS;         // warp roles: consumers, then the producer, then the helpers
     constexpr int BUFS = kd_bufs(CL);
+    // Pages in flight until the first ones are there: the whole ring requested at once by all CTAs is 4 microseconds of the HBM's
+    // time, and the first pages of a CTA come as late as the last (64 sequences of 1000 keys: 20.1 us with three in flight, 21.3
+    // with five, 22.7 with nine; a lone cluster's CTA has few and takes all it can).
+    constexpr int AHEAD = CL ? STAGES : GROUPS;
     static_assert(STAGES >= GROUPS, "a group's stage index advances by GROUPS a page");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -242,10 +253,6 @@ __global__ void __launch_bounds__((NCONS + 1 + KD_HELPERS) * 32, 1)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     trace_first(p.ctl.trace, 0);
     if (CL) cluster_arrive();   // (every CTA of the cluster has started before any writes into another's shared memory)
-    if (!p.ctl.early) {
-        pdl_wait();
-        pdl_launch_dependents();
-    }
     auto fail = [&](int code) {
         atomicExch(p.ctl.err, code);
         *reinterpret_cast<volatile int*>(&s_failed) = 1;
@@ -255,8 +262,9 @@ __global__ void __launch_bounds__((NCONS + 1 + KD_HELPERS) * 32, 1)
         // ---- producer: keeps the ring of stages full. The lanes look up 32 pages' blocks and addresses at a time, then each requests
         // its page when its turn comes (one lane that did it all took 1000 clocks a page, twice what the SM takes to attend one).
         // A block outside the pool: no keys, and the error word set.
-        KdWalk<CL> walk;                    // (seq_lens and the table are inputs of the whole step: read ahead of the wait)
-        walk.start(p, lane);
+        KdWalk<CL> walk;
+        if (lane == 0) prefetch_tensormap(&tmap);
+        walk.start(p, lane);                // (reads the sequence lengths ahead of the wait: nothing on the GPU writes them)
         if (lane == 0) {
             for (int s = 0; s < STAGES; s++) {
                 mbar_init(&full[s], 1);
@@ -270,7 +278,8 @@ __global__ void __launch_bounds__((NCONS + 1 + KD_HELPERS) * 32, 1)
             s_failed = 0;
             fence_barrier_init();
         }
-        __syncwarp();
+        pdl_wait();
+        pdl_launch_dependents();
         int count = 0, done = 0, S = 0;     // pages requested, of the run and of the piece; keys of the sequence
         bool go = true, joined = false;
         while (true) {
@@ -279,17 +288,12 @@ __global__ void __launch_bounds__((NCONS + 1 + KD_HELPERS) * 32, 1)
                 done = 0;
                 S = go ? __ldg(p.seq_lens + walk.at.b) : 0;
             }
-            if (!joined && (!go || count >= STAGES)) {
-                // the stages start empty: all of this ran without a wait, in an early launch ahead of the launch before it
-                if (p.ctl.early) {
-                    pdl_wait();
-                    pdl_launch_dependents();
-                }
+            if (!joined && (!go || count >= AHEAD)) {   // (none of it waited for a barrier so far)
                 __syncthreads();
                 joined = true;
             }
             if (!go) break;
-            const int m = min(min(32, walk.at.n - done), joined ? 32 : STAGES - count);
+            const int m = min(min(32, walk.at.n - done), joined ? 32 : AHEAD - count);
             const int page = walk.at.first + done + lane, mine = count + lane, st = mine % STAGES;
             const int block = lane < m && page < p.table_stride ? p.block_table[size_t(walk.at.b) * p.table_stride + page] : -1;
             const bool there = block >= 0 && block < p.num_blocks;
@@ -303,6 +307,9 @@ __global__ void __launch_bounds__((NCONS + 1 + KD_HELPERS) * 32, 1)
                         bad = true;
                     } else if (mine >= STAGES && !mbar_wait_bounded(p.ctl.wait_cycles, &empty[st], (mine / STAGES - 1) & 1)) {
                         atomicExch(p.ctl.err, ERR_WAIT_EMPTY);
+                        bad = true;
+                    } else if (mine >= AHEAD && mine < STAGES && !mbar_wait_bounded(p.ctl.wait_cycles, &full[mine - AHEAD], 0)) {
+                        atomicExch(p.ctl.err, ERR_WAIT_FULL);
                         bad = true;
                     } else if (there) {
                         limits[st] = min(BLK, S - page * BLK);
@@ -328,10 +335,7 @@ __global__ void __launch_bounds__((NCONS + 1 + KD_HELPERS) * 32, 1)
         KdWalk<CL> walk;
         walk.start(p, lane);
         bool more = true;
-        if (p.ctl.early) {
-            pdl_wait();
-            pdl_launch_dependents();
-        }
+        pdl_wait();
         float x[HPW][4];                    // the warp's query rows of the next piece, on their way since the one before it was staged
         auto fetch = [&]() {
             more = walk.next(p) || (CL && more);   // (a range without pages sends its zeros all the same)
@@ -425,10 +429,12 @@ __global__ void __launch_bounds__((NCONS + 1 + KD_HELPERS) * 32, 1)
         }
     } else {
         // ---- consumers
-        if (p.ctl.early) {
-            pdl_wait();
-            pdl_launch_dependents();
+        if (!CL) {
+            // the block tables on their way to the L2 while the producers look for their runs (16 uneven sequences: 19.5 us instead of 19.9)
+            const long at = (long(blockIdx.x) * NCONS + warp) * 1024 + lane * 32;   // a line of 32 entries a lane
+            if (at <= long(p.batch - 1) * p.table_stride) prefetch_l2(p.block_table + at);
         }
+        pdl_wait();
         trace_first(p.ctl.trace, 1);
         const int r = lane >> 2, t = lane & 3;
         const uint32_t base = smem_u32(stages) + kv4_lane_at(lane);
@@ -824,13 +830,13 @@ EmblaStatus kv4_full_decode(EmblaAttn* ctx, const EmblaKVPool* pool, const Embla
     if (units * (pages + KD_UNIT_COST) > 0x7fffffffL || units > 0xffff)
         EMBLA_FAIL(EMBLA_BAD_ARG, "embla_attn_full_decode: %d sequences of up to %d keys are too many pages", view->batch, max_len);
     // Two ways, by what they measured, in hundredths of a microsecond: clusters, all at once, 570 + 62 a page of a range (one
-    // sequence of 1000 keys 6.3 us, of 8192 11.2); runs, 1000 + 62 a page or unit cost of a run (11.2 us at the shortest, 8 x 32768
-    // keys of 2 kv heads 27.7). The ranges of a unit are as many as let all clusters be resident (a GPC may hold one cluster of
+    // sequence of 1000 keys 5.6 us, of 8192 10.5); runs, 1000 + 50 a page or unit cost of a run (10.0 us at the shortest, 64 sequences
+    // of 1000 keys 20.0, 8 of 32768 37.8). The ranges of a unit are as many as let all clusters be resident (a GPC may hold one cluster of
     // 8 such CTAs and not two) and no longer than 8 pages: longer ones are read at the pace of the longest sequence, where runs
     // even uneven lengths out. Runs: the scratch holds two pieces of each (embla_attn_create makes it 8 slots an SM and more).
     const long cost = units * (pages + KD_UNIT_COST), most = (cost + KD_MIN_RUN - 1) / KD_MIN_RUN;
     p.n_runs = int(most < ctx->sm_count ? most : ctx->sm_count);
-    long best = 1000 + 62 * ((cost + p.n_runs - 1) / p.n_runs);
+    long best = 1000 + 50 * ((cost + p.n_runs - 1) / p.n_runs);
     bool cluster = false;
     dim3 grid(p.n_runs);
     for (int ns = 1; ns <= KD_MAX_CLUSTER && ns <= pages; ns++) {

@@ -43,6 +43,12 @@ constexpr int ks_inbox_rows(int ranges, int G) { return ranges * ((G + ranges - 
 constexpr size_t ks_smem(int ranges, int G) { return 1024 + ks_inbox_at() + (ranges > 1 ? size_t(ks_inbox_rows(ranges, G)) * KS_PART * 4 : 0); }
 static_assert(KS_WARPS * 8 * (KS_SUM + 2) * 4 <= KS_WARPS * KS_STAGES * KS_STAGE, "the warps' sums lie over their stages");
 
+// 16 bytes (zeros if not `valid`) into shared memory; on a miss the L2 fetches the 64 bytes around them and not the 128 that it
+// fetches by itself, since a row's neighbour is no more likely to be selected than any (64 x 32768 keys: 28.8 us instead of 31.0).
+__device__ __forceinline__ void copy16(void* dst, const void* src, bool valid) {
+    const uint32_t bytes = valid ? 16u : 0u;
+    asm volatile("cp.async.cg.shared.global.L2::64B [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ float ks_exp2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -109,12 +115,12 @@ __global__ void __launch_bounds__(KS_WARPS * 32, 4) kv4_sparse_kernel(const __gr
                 const int row = it * 8 + (lane >> 2), ch = lane & 3;
                 const uint32_t a = at[row];
                 const uint8_t* src = p.pool + (a == KS_NOWHERE ? 0 : size_t(a / BLK) * KV4_PAGE + (a % BLK) * KV4_ROW + ch * 16);
-                cp_async16(dst + kv4_at(row, ch), src, a != KS_NOWHERE);
-                cp_async16(dst + KS_ROWS * KV4_ROW + kv4_at(row, ch), src + KV4_SIDE, a != KS_NOWHERE);
+                copy16(dst + kv4_at(row, ch), src, a != KS_NOWHERE);
+                copy16(dst + KS_ROWS * KV4_ROW + kv4_at(row, ch), src + KV4_SIDE, a != KS_NOWHERE);
             }
             const uint32_t a = at[lane];
             const uint8_t* src = p.pool + (a == KS_NOWHERE ? 0 : size_t(a / BLK) * KV4_PAGE + 2 * KV4_SIDE + (a % BLK) * 16);
-            cp_async16(dst + 2 * KS_ROWS * KV4_ROW + lane * 16, src, a != KS_NOWHERE);
+            copy16(dst + 2 * KS_ROWS * KV4_ROW + lane * 16, src, a != KS_NOWHERE);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
