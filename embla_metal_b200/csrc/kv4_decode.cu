@@ -36,6 +36,12 @@ __device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* map) {
 }
 __device__ __forceinline__ void prefetch_l2(const void* at) { asm volatile("prefetch.global.L2 [%0];" ::"l"(at)); }
 
+__device__ __forceinline__ float relu_nan(float x) {   // max(x, 0), NaN of NaN
+    float r;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(x));
+    return r;
+}
+
 // a barrier that tells all its threads whether any of them said yes
 __device__ __forceinline__ bool bar_any(int id, int threads, bool yes) {
     int any;
@@ -519,7 +525,7 @@ __global__ void __launch_bounds__((NCONS + 1 + KD_HELPERS) * 32, 1)
                             flagged |= rows[k].large();
 #pragma unroll
                             for (int e = 0; e < 4; e++) {
-                                s[k][e] = fmaxf(s[k][e], 0.0f);
+                                s[k][e] = relu_nan(s[k][e]);
                                 w[k][e] = s[k][e] * ((e & 1) ? f1 : f0) * s[k][e];
                                 top = fmaxf(top, w[k][e]);
                             }

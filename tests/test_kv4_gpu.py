@@ -657,3 +657,40 @@ def test_append_of_rows_at_any_alignment():
         ctx.kv_append(pools[1], table, 0, p0, odd[0][..., 3:259], odd[1][..., 3:259], norm_k=norm)
         ctx.check()
         assert torch.equal(pools[0].raw(), pools[1].raw())
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("side", ["key", "value"])
+def test_what_is_not_a_number_reaches_its_own_outputs_only(dtype, side):
+    """A row with a NaN, appended at position 200 of the first of three sequences: the outputs of its kv head in that sequence are
+    NaN, and a finite number everywhere else; one key and value that are infinite at a position nobody has reached change nothing."""
+    import torch
+    from embla_metal_b200 import attn
+    Hq, Hkv, lens = 8, 2, [300, 300, 129]
+    rng, ctx, pool, table, k, v = _setup(dtype, Hq, Hkv, lens, 41)
+    tdt = torch.float16 if dtype == "f16" else torch.bfloat16
+    row = torch.zeros(3, 1, Hkv * 128, dtype=tdt, device="cuda")
+    row[0, 0, 128 + 70] = float("nan")
+    row[1, 0, 5] = float("inf")
+    ones = torch.ones_like(row)
+    p0 = torch.tensor([200, 300, 129], dtype=torch.int32, device="cuda")
+    ctx.kv_append(pool, table, 1, p0, row if side == "key" else ones, ones if side == "key" else row, norm_k=False)
+    ln = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    q = torch.from_numpy(rng.standard_normal((3, Hq * 128)).astype(np.float32)).to("cuda", tdt)
+    o = torch.zeros_like(q)
+
+    def check(what):
+        ctx.check()
+        bad = torch.isnan(o.float()).view(3, Hkv, -1)
+        assert not torch.isinf(o).any(), what
+        assert not bad[1:].any() and not bad[0, 0].any(), what
+        # (a value's NaN is in its group of 32 dims; a key's in every dim)
+        own = torch.isnan(o.float()).view(3, Hq, 4, 32)[0, 4:, 70 // 32] if side == "value" else bad[0, 1]
+        assert own.all(), what
+
+    ctx.full_decode(pool, table, ln, 1, q, o)
+    check("full decode")
+    ctx.sparse_decode(pool, table, ln, 1, q, o)
+    check("sparse decode")
+    attn.full_prefill(ctx, pool, table, 1, ln - 1, q.view(3, 1, -1), o.view(3, 1, -1))
+    check("prefill")
