@@ -235,6 +235,9 @@ template <int DT, bool SCORES, int NCONS, int WPG, int STAGES, bool CL>
 __global__ void __launch_bounds__((NCONS + 1 + KD_HELPERS) * 32, 1)
     kv4_decode_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ Kv4DecodeParams p) {
     constexpr int TILES = 8 / WPG;          // 16-key tiles of a page a consumer warp takes
+    // of those, taken together: all (one by one 64 x 32768 keys take 239 us instead of 224), but one by one where scores are written
+    // too, which leaves no registers for two (8 x 32768 keys: 28.8 us instead of 29.8)
+    constexpr int STEP = SCORES ? 1 : TILES;
     constexpr int GROUPS = NCONS / WPG;
     constexpr int PRODUCER = NCONS;         // warp roles: consumers, then the producer, then the helpers
     constexpr int BUFS = kd_bufs(CL);
@@ -485,95 +488,101 @@ __global__ void __launch_bounds__((NCONS + 1 + KD_HELPERS) * 32, 1)
                 for (; mine < piece0 + n; mine += GROUPS) {
                     ok = __all_sync(0xffffffffu, mbar_wait_bounded(p.ctl.wait_cycles, &full[st], phase));
                     if (!ok) break;
-                    // the warp's tiles of the page together: their products have nothing to wait for in one another
-                    const uint32_t kaddr = base + st * KV4_PAGE + wg * (TILES * 16 * KV4_ROW);
-                    const uint8_t* sc = stages + st * KV4_PAGE + 2 * KV4_SIDE + wg * (TILES * 16 * 16);
-                    const int left = limits[st] - wg * (TILES * 16);   // keys of the tiles that count, if fewer than there are
-                    if (left > 0) {
-                        float s[TILES][4];
-                        Kv4Scales rows[TILES];
-                        bool flagged = false;
+                    // the tiles of a step together: their products have nothing to wait for in one another
+                    const uint32_t kaddr0 = base + st * KV4_PAGE + wg * (TILES * 16 * KV4_ROW);
+                    const uint8_t* sc0 = stages + st * KV4_PAGE + 2 * KV4_SIDE + wg * (TILES * 16 * 16);
+                    const int left0 = limits[st] - wg * (TILES * 16);   // keys of the tiles that count, if fewer than there are
 #pragma unroll
-                        for (int k = 0; k < TILES; k++) {
-                            rows[k].load(sc + k * 256, lane);
-                            kv4_tile_scores(kaddr + k * 16 * KV4_ROW, rows[k], frag, s[k]);
-                        }
-                        if (SCORES) {
+                    for (int tile = 0; tile < TILES; tile += STEP) {
+                        const uint32_t kaddr = kaddr0 + tile * 16 * KV4_ROW;
+                        const uint8_t* sc = sc0 + tile * 256;
+                        const int left = left0 - tile * 16;
+                        if (left > 0) {
+                            float s[STEP][4];
+                            Kv4Scales rows[STEP];
+                            bool flagged = false;
 #pragma unroll
-                            for (int k = 0; k < TILES; k++) {
-                                float m0 = fmaxf(fmaf(s[k][0], u0, n0), fmaf(s[k][1], u1, n1)), m1 = fmaxf(fmaf(s[k][2], u0, n0), fmaf(s[k][3], u1, n1));
-                                m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, 1));
-                                m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 1));
-                                m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, 2));
-                                m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 2));
-                                const int key = k * 16 + r + 8 * t;
-                                if (t < 2 && key < left)
-                                    scores[long(mine) * BLK + key] = t ? m1 : m0;
+                            for (int k = 0; k < STEP; k++) {
+                                rows[k].load(sc + k * 256, lane);
+                                kv4_tile_scores(kaddr + k * 16 * KV4_ROW, rows[k], frag, s[k]);
                             }
-                        }
-                        if (left < TILES * 16) {
+                            if (SCORES) {
 #pragma unroll
-                            for (int k = 0; k < TILES; k++) {
-                                if (k * 16 + r >= left) s[k][0] = s[k][1] = 0.0f;
-                                if (k * 16 + r + 8 >= left) s[k][2] = s[k][3] = 0.0f;
-                                rows[k].mask(lane, left - k * 16);
+                                for (int k = 0; k < STEP; k++) {
+                                    float m0 = fmaxf(fmaf(s[k][0], u0, n0), fmaf(s[k][1], u1, n1)), m1 = fmaxf(fmaf(s[k][2], u0, n0), fmaf(s[k][3], u1, n1));
+                                    m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, 1));
+                                    m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 1));
+                                    m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, 2));
+                                    m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 2));
+                                    const int key = k * 16 + r + 8 * t;
+                                    if (t < 2 && key < left)
+                                        scores[long(mine) * BLK + tile * 16 + key] = t ? m1 : m0;
+                                }
                             }
-                        }
-                        float w[TILES][4], top = 0.0f;
+                            if (left < STEP * 16) {
 #pragma unroll
-                        for (int k = 0; k < TILES; k++) {
-                            flagged |= rows[k].large();
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                s[k][e] = relu_nan(s[k][e]);
-                                w[k][e] = s[k][e] * ((e & 1) ? f1 : f0) * s[k][e];
-                                top = fmaxf(top, w[k][e]);
+                                for (int k = 0; k < STEP; k++) {
+                                    if (k * 16 + r >= left) s[k][0] = s[k][1] = 0.0f;
+                                    if (k * 16 + r + 8 >= left) s[k][2] = s[k][3] = 0.0f;
+                                    rows[k].mask(lane, left - k * 16);
+                                }
                             }
-                        }
-                        if (__any_sync(0xffffffffu, top > limit || (flagged && !big))) {
-                            // (a handful of times a warp) new factors: the tiles' largest weight of a head at most 2^target
-                            if (__any_sync(0xffffffffu, flagged)) {
-                                big = true;
-                                limit = KD_LIMIT_BIG;
+                            float w[STEP][4], top = 0.0f;
+#pragma unroll
+                            for (int k = 0; k < STEP; k++) {
+                                flagged |= rows[k].large();
+#pragma unroll
+                                for (int e = 0; e < 4; e++) {
+                                    s[k][e] = relu_nan(s[k][e]);
+                                    w[k][e] = s[k][e] * ((e & 1) ? f1 : f0) * s[k][e];
+                                    top = fmaxf(top, w[k][e]);
+                                }
                             }
-                            const int target = big ? KD_TARGET_BIG : KD_TARGET;
-                            float m0 = 0.0f, m1 = 0.0f;
+                            if (__any_sync(0xffffffffu, top > limit || (flagged && !big))) {
+                                // (a handful of times a warp) new factors: the tiles' largest weight of a head at most 2^target
+                                if (__any_sync(0xffffffffu, flagged)) {
+                                    big = true;
+                                    limit = KD_LIMIT_BIG;
+                                }
+                                const int target = big ? KD_TARGET_BIG : KD_TARGET;
+                                float m0 = 0.0f, m1 = 0.0f;
 #pragma unroll
-                            for (int k = 0; k < TILES; k++) {
-                                m0 = fmaxf(m0, fmaxf(s[k][0], s[k][2]));
-                                m1 = fmaxf(m1, fmaxf(s[k][1], s[k][3]));
+                                for (int k = 0; k < STEP; k++) {
+                                    m0 = fmaxf(m0, fmaxf(s[k][0], s[k][2]));
+                                    m1 = fmaxf(m1, fmaxf(s[k][1], s[k][3]));
+                                }
+#pragma unroll
+                                for (int o = 4; o < 32; o <<= 1) {
+                                    m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
+                                    m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+                                }
+                                // m < 2^(e + 1), so m^2 2^(target - 2 (e + 1)) < 2^target
+                                const int e0 = int(__float_as_uint(m0) >> 23) - 126, e1 = int(__float_as_uint(m1) >> 23) - 126;
+                                const float nf0 = m0 * f0 * m0 > limit ? pow2_biased(min(max(127 + target - 2 * e0, 1), 254)) : f0;
+                                const float nf1 = m1 * f1 * m1 > limit ? pow2_biased(min(max(127 + target - 2 * e1, 1), 254)) : f1;
+                                const float c0 = nf0 / f0, c1 = nf1 / f1;
+                                f0 = nf0;
+                                f1 = nf1;
+                                ps0 *= c0;
+                                ps1 *= c1;
+#pragma unroll
+                                for (int k = 0; k < 8; k++) {
+                                    O[k][0] *= c0;
+                                    O[k][1] *= c1;
+                                    O[k][2] *= c0;
+                                    O[k][3] *= c1;
+                                }
+#pragma unroll
+                                for (int k = 0; k < STEP; k++)
+#pragma unroll
+                                    for (int e = 0; e < 4; e++) w[k][e] = s[k][e] * ((e & 1) ? f1 : f0) * s[k][e];
                             }
 #pragma unroll
-                            for (int o = 4; o < 32; o <<= 1) {
-                                m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
-                                m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+                            for (int k = 0; k < STEP; k++) {
+                                ps0 += w[k][0] + w[k][2];
+                                ps1 += w[k][1] + w[k][3];
+                                kv4_tile_values<DT>(kaddr + KV4_SIDE + k * 16 * KV4_ROW, rows[k], w[k], O);
                             }
-                            // m < 2^(e + 1), so m^2 2^(target - 2 (e + 1)) < 2^target
-                            const int e0 = int(__float_as_uint(m0) >> 23) - 126, e1 = int(__float_as_uint(m1) >> 23) - 126;
-                            const float nf0 = m0 * f0 * m0 > limit ? pow2_biased(min(max(127 + target - 2 * e0, 1), 254)) : f0;
-                            const float nf1 = m1 * f1 * m1 > limit ? pow2_biased(min(max(127 + target - 2 * e1, 1), 254)) : f1;
-                            const float c0 = nf0 / f0, c1 = nf1 / f1;
-                            f0 = nf0;
-                            f1 = nf1;
-                            ps0 *= c0;
-                            ps1 *= c1;
-#pragma unroll
-                            for (int k = 0; k < 8; k++) {
-                                O[k][0] *= c0;
-                                O[k][1] *= c1;
-                                O[k][2] *= c0;
-                                O[k][3] *= c1;
-                            }
-#pragma unroll
-                            for (int k = 0; k < TILES; k++)
-#pragma unroll
-                                for (int e = 0; e < 4; e++) w[k][e] = s[k][e] * ((e & 1) ? f1 : f0) * s[k][e];
-                        }
-#pragma unroll
-                        for (int k = 0; k < TILES; k++) {
-                            ps0 += w[k][0] + w[k][2];
-                            ps1 += w[k][1] + w[k][3];
-                            kv4_tile_values<DT>(kaddr + KV4_SIDE + k * 16 * KV4_ROW, rows[k], w[k], O);
                         }
                     }
                     __syncwarp();
