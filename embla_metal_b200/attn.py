@@ -117,13 +117,15 @@ def _stream():
 
 
 _current_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+# (tensors on the device exist, so torch's CUDA side is up and needs no look at each call)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _raw_stream():
     """The current stream as an integer (for functions that know their argument types)."""
     if _current_raw_stream is None:
         return torch.cuda.current_stream().cuda_stream
-    return _current_raw_stream(torch.cuda.current_device())
+    return _current_raw_stream(_current_device())
 
 
 def _addr(t):
@@ -222,7 +224,8 @@ class Attention:
     @staticmethod
     def _pack_view(block_table, seq_lens, layer, max_seq_len=0):
         """EmblaKVView of a call, as bytes."""
-        return _VIEW.pack(block_table.data_ptr(), block_table.stride(0), _addr(seq_lens), block_table.shape[0], layer, max_seq_len)
+        return _VIEW.pack(block_table.data_ptr(), block_table.stride(0), 0 if seq_lens is None else seq_lens.data_ptr(), block_table.size(0),
+                          layer, max_seq_len)
 
     @staticmethod
     def _pack_query(q, gains):
@@ -273,26 +276,32 @@ class Attention:
 
     def kv_append(self, pool, block_table, layer, pos0, k, v, norm_k=True):
         """k, v [batch, n_tokens, n_kv_heads * 128 (or wider rows)]; pos0 int32 [batch] first position."""
-        _check(lib().embla_kv_append(self.handle, pool.handle, self._pack_view(block_table, None, layer), pos0.data_ptr(), k.shape[1],
-                                     k.data_ptr(), v.data_ptr(), k.stride(1), k.stride(0), int(norm_k), _raw_stream()))
+        strides = k.stride()
+        _check(lib().embla_kv_append(self.handle, pool.handle, self._pack_view(block_table, None, layer), pos0.data_ptr(), k.size(1),
+                                     k.data_ptr(), v.data_ptr(), strides[1], strides[0], int(norm_k), _raw_stream()))
 
     def kv_read(self, pool, block_table, layer, pos0, k, v):
         """The inverse of kv_append: k, v [batch, n_tokens, n_kv_heads * 128 (or wider rows)] <- the cached rows of positions
         pos0[b] + t, dequantised and rounded to the activation dtype. Pools of every type."""
-        if k.dtype != self.torch_dtype or v.dtype != self.torch_dtype or k.shape != v.shape or k.stride() != v.stride() or k.stride(2) != 1:
-            raise ValueError(f"k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} must be alike, rows contiguous, in {self.torch_dtype}")
-        if k.shape[0] != block_table.shape[0] or k.shape[2] < pool.n_kv_heads * HEAD_DIM:
-            raise ValueError(f"k {tuple(k.shape)} does not hold {pool.n_kv_heads} kv heads of {block_table.shape[0]} sequences")
-        _check(lib().embla_kv_read(self.handle, pool.handle, self._pack_view(block_table, None, layer), pos0.data_ptr(), k.shape[1],
-                                   k.data_ptr(), v.data_ptr(), k.stride(1), k.stride(0), _raw_stream()))
+        shape, strides = k.shape, k.stride()
+        if len(shape) != 3:
+            raise ValueError(f"k {tuple(shape)}: batch, tokens, kv heads x {HEAD_DIM}")
+        if k.dtype != self.torch_dtype or v.dtype != self.torch_dtype or shape != v.shape or strides != v.stride() or strides[2] != 1:
+            raise ValueError(f"k {tuple(shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} must be alike, rows contiguous, in {self.torch_dtype}")
+        batch, n_tokens, width = shape
+        if batch != block_table.size(0) or width < pool.n_kv_heads * HEAD_DIM:
+            raise ValueError(f"k {tuple(shape)} does not hold {pool.n_kv_heads} kv heads of {block_table.size(0)} sequences")
+        _check(lib().embla_kv_read(self.handle, pool.handle, self._pack_view(block_table, None, layer), pos0.data_ptr(), n_tokens,
+                                   k.data_ptr(), v.data_ptr(), strides[1], strides[0], _raw_stream()))
 
     def copy_blocks(self, pool, src, dst, rows=None):
         """Copies block src[i] of the pool to block dst[i] (int32 device tensors), all layers and kv heads, in one launch: the
         first rows[i] positions of it, or all 128. With a block table edit this forks a sequence or moves its blocks."""
+        n = src.numel()
         for t in (src, dst, rows):
-            if t is not None and (t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous() or t.numel() != src.numel()):
+            if t is not None and (t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous() or t.numel() != n):
                 raise ValueError("src, dst and rows are contiguous int32 tensors on the device, one entry a copy")
-        _check(lib().embla_kv_copy_blocks(self.handle, pool.handle, src.data_ptr(), dst.data_ptr(), _addr(rows), src.numel(), _raw_stream()))
+        _check(lib().embla_kv_copy_blocks(self.handle, pool.handle, src.data_ptr(), dst.data_ptr(), _addr(rows), n, _raw_stream()))
 
     def full_decode(self, pool, block_table, seq_lens, layer, q, o, gains=None, scores=None, max_seq_len=0):
         _check(lib().embla_attn_full_decode(self.handle, pool.handle, self._pack_view(block_table, seq_lens, layer, max_seq_len),
