@@ -62,9 +62,20 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const AppendParams p) {
 // ---- 4-bit pools, and reading rows back -------------------------------------------------------------------------------
 // Half a warp takes a row: a lane holds 8 consecutive dims (16 bytes of activations, one word of codes), four lanes a scale
 // group. A warp takes 2 x PASSES consecutive rows of one side (K or V), every load in flight before the first is used; lane i works
-// out where row i lies, the others get it by shuffle. Bound by instructions (about 90 a row to quantise, 55 to read back), not by
-// the bytes: 8 x 2048 tokens of 4 kv heads take 17.8 us to append (53 MB; 27 us with the keys normed) and 13.2 us to read
-// back, where a warp a row with two-byte loads took 93 us for the two.
+// out where row i lies, the others get it by shuffle. Bound by instructions (about 90 a row to quantise, 45 to read back), not by
+// the bytes: 8 x 2048 tokens of 4 kv heads take 15.9 us to append (fp16, 17.1 bf16; 43 MB; 19.8 with the keys normed) and 11.5 us to
+// read back, where a warp a row with two-byte loads took 93 us for the two.
+// x / d for x < 2^30: (x mul) >> shift, mul = ceil(2^shift / d), shift = 30 + ceil(log2 d), whose error x (mul d - 2^shift) / (d 2^shift)
+// is below 1 / d (Granlund and Montgomery, "Division by invariant integers using multiplication", 1994).
+struct Divisor {
+    unsigned mul, shift;
+    Divisor() = default;
+    explicit Divisor(unsigned d) : shift(30) {
+        while ((1ull << (shift - 30)) < d) shift++;
+        mul = unsigned(((1ull << shift) + d - 1) / d);
+    }
+    __device__ __forceinline__ unsigned quotient(unsigned x) const { return unsigned((static_cast<unsigned long long>(x) * mul) >> shift); }
+};
 struct RowsParams {
     uint8_t* pool;
     const int32_t* block_table;
@@ -75,42 +86,32 @@ struct RowsParams {
     int64_t token_stride, seq_stride;
     size_t page_bytes;
     int* err;
-    unsigned rows;             // of a side: batch x n_tokens x n_kv_heads
+    unsigned rows;             // of a side: batch x n_tokens x n_kv_heads, below 2^30
+    Divisor by_heads, by_tokens;
     int table_stride, n_tokens, layer, n_layers, n_kv_heads, num_blocks, norm_k, kv_dtype, scale_bytes, vec;
 };
 
-// Where row i of a side lies: elements into k / v; its page (NULL: nowhere, with the error word set) and row in it.
+// Where row i of a side lies: elements into k / v; page x 128 + row of the page (ROW_NOWHERE: no place, with the error word set).
+constexpr unsigned ROW_NOWHERE = 0xffffffffu;
 __device__ __forceinline__ long row_elements(const RowsParams& p, unsigned i, unsigned& b, unsigned& t, unsigned& h) {
-    const unsigned bt = i / unsigned(p.n_kv_heads);
+    const unsigned bt = p.by_heads.quotient(i);
     h = i - bt * unsigned(p.n_kv_heads);
-    b = bt / unsigned(p.n_tokens);
+    b = p.by_tokens.quotient(bt);
     t = bt - b * unsigned(p.n_tokens);
     return long(b) * p.seq_stride + long(t) * p.token_stride + long(h) * HD;
 }
-struct RowPlace {
-    uint8_t* page;
-    int row;
-};
-__device__ __forceinline__ RowPlace row_place(const RowsParams& p, unsigned b, unsigned t, unsigned h) {
-    RowPlace w = {nullptr, 0};
+__device__ __forceinline__ unsigned row_place(const RowsParams& p, unsigned b, unsigned t, unsigned h) {
     const int pos = p.pos0 ? p.pos0[b] + int(t) : p.seq_lens[b] - 1;
-    if (!p.pos0 && pos < 0) return w;   // (an empty sequence has no current token)
+    if (!p.pos0 && pos < 0) return ROW_NOWHERE;   // (an empty sequence has no current token)
     int block = -1;
     if (pos >= 0 && pos / BLK < p.table_stride) block = p.block_table[size_t(b) * p.table_stride + pos / BLK];
     if (block < 0 || block >= p.num_blocks) {
         atomicExch(p.err, ERR_BAD_BLOCK);
-        return w;
+        return ROW_NOWHERE;
     }
-    w.page = p.pool + ((size_t(block) * p.n_layers + p.layer) * p.n_kv_heads + h) * p.page_bytes;
-    w.row = pos % BLK;
-    return w;
+    return unsigned((long(block) * p.n_layers + p.layer) * p.n_kv_heads + long(h)) * BLK + unsigned(pos) % BLK;
 }
-__device__ __forceinline__ RowPlace shfl_place(const RowPlace& w, int lane) {
-    RowPlace r;
-    r.page = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(w.page), lane));
-    r.row = __shfl_sync(0xffffffffu, w.row, lane);
-    return r;
-}
+__device__ __forceinline__ uint8_t* page_of(const RowsParams& p, unsigned place) { return p.pool + size_t(place / BLK) * p.page_bytes; }
 template <int DT>
 __device__ __forceinline__ float act_lo(uint32_t w) {
     return DT == EMBLA_BF16 ? __uint_as_float(w << 16) : __low2float(*reinterpret_cast<const __half2*>(&w));
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(ROWS_WARPS * 32) kv4_append_kernel(const __gri
         }
     }
     // (the lookups of the rows' pages run beside the loads of the rows)
-    const RowPlace mine = has ? row_place(p, b, t, h) : RowPlace{nullptr, 0};
+    const unsigned mine = has ? row_place(p, b, t, h) : ROW_NOWHERE;
     if (NORM && !is_v) {
         // RMS norm without gains (common.metal:30-41): dims l, l + 32, l + 64, l + 96 into a partial sum each, then l = 0 .. 31
         float(*sq)[HD + 4] = squares[warp];
@@ -202,7 +203,7 @@ __global__ void __launch_bounds__(ROWS_WARPS * 32) kv4_append_kernel(const __gri
     }
 #pragma unroll
     for (int i = 0; i < PASSES; i++) {
-        const RowPlace w = shfl_place(mine, 2 * i + half);
+        const unsigned place = __shfl_sync(0xffffffffu, mine, 2 * i + half);
         const uint32_t v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
         // the group's largest magnitude: the types' bits without the sign are ordered as the magnitudes are, NaN on top
         uint32_t top = __vmaxu2(__vmaxu2(v[0] & 0x7fff7fffu, v[1] & 0x7fff7fffu), __vmaxu2(v[2] & 0x7fff7fffu, v[3] & 0x7fff7fffu));
@@ -216,14 +217,16 @@ __global__ void __launch_bounds__(ROWS_WARPS * 32) kv4_append_kernel(const __gri
         }
         __half sh;
         const uint32_t word = kv4_word(xv, fmaxf_nan(act_lo<DT>(top), act_hi<DT>(top)), sh);
-        if (!w.page) continue;
-        *reinterpret_cast<uint32_t*>(w.page + (is_v ? KV4_SIDE : 0) + w.row * KV4_ROW + col * 4) = word;
+        if (place == ROW_NOWHERE) continue;
+        uint8_t* page = page_of(p, place);
+        const int row = place % BLK;
+        *reinterpret_cast<uint32_t*>(page + (is_v ? KV4_SIDE : 0) + row * KV4_ROW + col * 4) = word;
         if ((col & 3) == 0)
-            reinterpret_cast<__half*>(w.page + 2 * KV4_SIDE)[w.row * 2 * KV4_GROUPS + (is_v ? KV4_GROUPS : 0) + (col >> 2)] = sh;
+            reinterpret_cast<__half*>(page + 2 * KV4_SIDE)[row * 2 * KV4_GROUPS + (is_v ? KV4_GROUPS : 0) + (col >> 2)] = sh;
     }
 }
 
-template <int DT, int PASSES>
+template <int DT, int PASSES, bool INT4>
 __global__ void __launch_bounds__(ROWS_WARPS * 32) kv_read_kernel(const __grid_constant__ RowsParams p) {
     pdl_wait();
     pdl_launch_dependents();
@@ -236,19 +239,19 @@ __global__ void __launch_bounds__(ROWS_WARPS * 32) kv_read_kernel(const __grid_c
     const bool has = lane < int(per) && first + lane < p.rows;
     unsigned b = 0, t = 0, h = 0;
     const long elements = has ? row_elements(p, first + lane, b, t, h) : 0;
-    const RowPlace mine = has ? row_place(p, b, t, h) : RowPlace{nullptr, 0};
-    RowPlace w[PASSES];
+    const unsigned mine = has ? row_place(p, b, t, h) : ROW_NOWHERE;
+    unsigned place[PASSES];
     uint4 c[PASSES];   // the lane's 8 codes (or the row's values, 16-bit pools)
     float s[PASSES];
 #pragma unroll
     for (int i = 0; i < PASSES; i++) {
-        w[i] = shfl_place(mine, 2 * i + half);
-        const uint8_t* page = w[i].page;
-        const int row = w[i].row;
+        place[i] = __shfl_sync(0xffffffffu, mine, 2 * i + half);
+        const uint8_t* page = page_of(p, place[i]);
+        const int row = place[i] % BLK;
         c[i] = make_uint4(0, 0, 0, 0);
         s[i] = 0.0f;
-        if (!page) continue;
-        if (p.kv_dtype == EMBLA_KV_INT4) {
+        if (place[i] == ROW_NOWHERE) continue;
+        if (INT4) {
             c[i].x = *reinterpret_cast<const uint32_t*>(page + (is_v ? KV4_SIDE : 0) + row * KV4_ROW + col * 4);
             s[i] = __half2float(reinterpret_cast<const __half*>(page + 2 * KV4_SIDE)[row * 2 * KV4_GROUPS + (is_v ? KV4_GROUPS : 0) + (col >> 2)]);
         } else if (p.kv_dtype == EMBLA_KV_INT8) {
@@ -263,11 +266,11 @@ __global__ void __launch_bounds__(ROWS_WARPS * 32) kv_read_kernel(const __grid_c
 #pragma unroll
     for (int i = 0; i < PASSES; i++) {
         const long at = __shfl_sync(0xffffffffu, elements, 2 * i + half);
-        if (!w[i].page) continue;
+        if (place[i] == ROW_NOWHERE) continue;
         uint4 out = c[i];
         if (p.kv_dtype != EMBLA_KV_16BIT) {
             uint32_t h[4];   // the codes as fp16 pairs, exactly
-            if (p.kv_dtype == EMBLA_KV_INT4) {
+            if (INT4) {
                 kv4_widen(c[i].x, h);
             } else {
                 const uint32_t x0 = c[i].x ^ 0x80808080u, x1 = c[i].y ^ 0x80808080u;
@@ -277,6 +280,12 @@ __global__ void __launch_bounds__(ROWS_WARPS * 32) kv_read_kernel(const __grid_c
                 h[3] = h2_from_biased_bytes(x1, 0x4342);
             }
             uint32_t* to = &out.x;
+            if (DT == EMBLA_F16 && INT4) {
+                // (codes and scales are fp16: their fp16 product is the exact one rounded once, as below)
+                const __half2 s2 = __float2half2_rn(s[i]);
+#pragma unroll
+                for (int d = 0; d < 4; d++) to[d] = h2_mul(h[d], *reinterpret_cast<const uint32_t*>(&s2));
+            } else
 #pragma unroll
             for (int d = 0; d < 4; d++) {
                 const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[d]));
@@ -288,7 +297,7 @@ __global__ void __launch_bounds__(ROWS_WARPS * 32) kv_read_kernel(const __grid_c
 }
 
 // Rows a warp takes: eight (fewer lookups a row), or two while eight would leave an SM fewer than 32 warps (2048 tokens of 4 heads:
-// 7.6 us with eight, 6.3 with four and less with two; 8 x 2048: 17.8 us with eight, 19.1 with four).
+// 7.6 us with eight, 6.3 with four and less with two; 8 x 2048: 7 % less with eight than with four, 6 % less than with sixteen).
 static int rows_passes(const EmblaAttn* ctx, unsigned rows) { return rows >= 128u * unsigned(ctx->sm_count) ? 4 : 1; }
 
 static EmblaStatus rows_params(RowsParams& p, const char* fn, const EmblaKVPool* pool, const EmblaKVView* view, const int32_t* pos0, int n_tokens,
@@ -304,6 +313,8 @@ static EmblaStatus rows_params(RowsParams& p, const char* fn, const EmblaKVPool*
     p.page_bytes = pool->page_bytes;
     p.err = ctx->err_dev;
     p.rows = unsigned(rows);
+    p.by_heads = Divisor(unsigned(pool->n_kv_heads));
+    p.by_tokens = Divisor(unsigned(n_tokens));
     p.table_stride = view->table_stride;
     p.n_tokens = n_tokens;
     p.layer = view->layer;
@@ -409,7 +420,9 @@ extern "C" EmblaStatus embla_kv_read(EmblaAttn* ctx, const EmblaKVPool* pool, co
     const int passes = rows_passes(ctx, p.rows);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool bf = ctx->cfg.act_dtype == EMBLA_BF16;
-#define EMBLA_RD(DT, P) launch_kernel(ctx->pdl, kv_read_kernel<DT, P>, rows_grid(p.rows, P), dim3(ROWS_WARPS * 32), 0, s, p)
+    const bool int4 = pool->kv_dtype == EMBLA_KV_INT4;
+#define EMBLA_RD(DT, P) (int4 ? launch_kernel(ctx->pdl, kv_read_kernel<DT, P, true>, rows_grid(p.rows, P), dim3(ROWS_WARPS * 32), 0, s, p) \
+                              : launch_kernel(ctx->pdl, kv_read_kernel<DT, P, false>, rows_grid(p.rows, P), dim3(ROWS_WARPS * 32), 0, s, p))
     if (passes == 4) EMBLA_CUDA_TRY(bf ? EMBLA_RD(EMBLA_BF16, 4) : EMBLA_RD(EMBLA_F16, 4));
     else EMBLA_CUDA_TRY(bf ? EMBLA_RD(EMBLA_BF16, 1) : EMBLA_RD(EMBLA_F16, 1));
 #undef EMBLA_RD

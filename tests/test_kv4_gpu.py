@@ -694,3 +694,35 @@ def test_what_is_not_a_number_reaches_its_own_outputs_only(dtype, side):
     check("sparse decode")
     attn.full_prefill(ctx, pool, table, 1, ln - 1, q.view(3, 1, -1), o.view(3, 1, -1))
     check("prefill")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n_tokens", [3, 5000])
+def test_append_rounds_halves_to_even(dtype, n_tokens):
+    """Rows whose quotients by their scale are whole numbers and halves, between -7 and 7, with scales down into fp16's subnormals."""
+    import torch
+    from embla_metal_b200 import attn
+    rng = np.random.default_rng(n_tokens)
+    npg = (n_tokens + 127) // 128
+    ctx = attn.Attention(2, 2, DT[dtype], 1, npg * 128)
+    pool = attn.KVPool(1, 2, npg, attn.KV_INT4, attn.SCALE_F16)
+    # scales of 4 significant bits: times 13 / 2 or less they have 8, what bf16 holds
+    s = rng.integers(8, 16, (2, n_tokens, 2, 4, 1)) * 2.0 ** rng.integers(-24, 9, (2, n_tokens, 2, 4, 1))
+    m = rng.integers(-13, 14, (2, n_tokens, 2, 4, 32))
+    m[..., 0] = np.where(rng.random(m[..., 0].shape) < 0.5, 14, -14)
+    x = (np.take_along_axis(m, rng.permuted(np.broadcast_to(np.arange(32), m.shape), axis=-1), -1) * (s / 2)).reshape(2, 1, n_tokens, 2, 128)
+    bits = _bits(x, dtype)
+    keep = np.abs(_val(bits, dtype) - x) == 0            # (fp16: the smallest scales' halves are no numbers of the type)
+    assert keep.mean() > 0.9
+    t = _act(bits.reshape(2, 1, n_tokens, 256), dtype)
+    table = torch.arange(npg, dtype=torch.int32, device="cuda").view(1, -1)
+    ctx.kv_append(pool, table, 0, torch.zeros(1, dtype=torch.int32, device="cuda"), t[0], t[1], norm_k=False)
+    ctx.check()
+    codes, scales = kv4.quantise(_val(bits, dtype))
+    assert (np.abs(x / np.repeat(s.reshape(2, 1, n_tokens, 2, 4), 32, -1)) % 1 == 0.5)[keep].mean() > 0.3
+    raw = pool.raw()[:, 0].cpu().numpy()                 # [page][head][bytes]
+    for side in range(2):
+        got = raw[:, :, side * 8192:side * 8192 + 8192].reshape(npg, 2, 128, 64).transpose(0, 2, 1, 3).reshape(-1, 2, 64)[:n_tokens]
+        assert np.array_equal(got, kv4.pack(codes[side, 0]))
+        sc = raw[:, :, 16384:].copy().view(np.float16).reshape(npg, 2, 128, 8).transpose(0, 2, 1, 3).reshape(-1, 2, 8)[:n_tokens]
+        assert np.array_equal(sc[..., 4 * side:4 * side + 4], scales[side, 0])
