@@ -9,7 +9,7 @@
 // head), as a thread-block cluster, when there are few of them.
 //
 // 64 sequences of 32768 keys, 4 kv heads: 28.8 us for 42 MB of rows (56 MB read: a row's scales are 16 bytes of the 64 that the HBM
-// gives), 4 sequences of 9000: 9.7 us, of which 6 are launch, lookups and one row's way here. 31 instructions a row, 39 % of the
+// gives), 4 sequences of 9000: 9.0 us, of which 6 are launch, lookups and one row's way here. 31 instructions a row, 39 % of the
 // issue slots; the same number of rows side by side instead of scattered take 17.6 us.
 #include "attn16_common.cuh"
 #include "kv4_tile.cuh"
@@ -260,8 +260,10 @@ __global__ void __launch_bounds__(KS_WARPS * 32, 4) kv4_sparse_kernel(const __gr
     __syncthreads();
     float* inbox = reinterpret_cast<float*>(smem + ks_inbox_at());
     const int own = (p.G + p.nsplit - 1) / p.nsplit;   // heads that a CTA finishes
-    for (int i = tid; i < p.G * HD; i += KS_WARPS * 32) {
-        const int hh = i >> 7, d = i & 127;
+    static_assert(KS_WARPS * 32 == HD, "a thread a dim");   // (heads and ranges unrolled: 4 x 9000 keys 9.0 us instead of 9.7)
+    const int d = tid;
+#pragma unroll 4
+    for (int hh = 0; hh < p.G; hh++) {
         float M = KS_NONE;
 #pragma unroll
         for (int w = 0; w < KS_WARPS; w++) M = fmaxf(M, refs[w * 8 + hh]);
@@ -288,14 +290,21 @@ __global__ void __launch_bounds__(KS_WARPS * 32, 4) kv4_sparse_kernel(const __gr
         // one cluster barrier: every range's rows are with their owners; CTA `split` finishes heads split, split + nsplit, ...
         cluster_arrive();
         cluster_wait();
-        for (int i = tid; i < own * HD; i += KS_WARPS * 32) {
-            const int slot = i >> 7, d = i & 127, hh = split + slot * p.nsplit;
-            if (hh >= p.G) continue;
+        for (int slot = 0; slot < own; slot++) {
+            const int hh = split + slot * p.nsplit;
+            if (hh >= p.G) break;
             float M = KS_NONE, num = 0.0f, den = 0.0f;
-            for (int k = 0; k < p.nsplit; k++) M = fmaxf(M, inbox[(k * own + slot) * KS_PART + HD + 1]);
-            for (int k = 0; k < p.nsplit; k++) {
+            float refs_of[KS_MAX_CLUSTER];
+#pragma unroll
+            for (int k = 0; k < KS_MAX_CLUSTER; k++) {
+                refs_of[k] = k < p.nsplit ? inbox[(k * own + slot) * KS_PART + HD + 1] : KS_NONE;
+                M = fmaxf(M, refs_of[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < KS_MAX_CLUSTER; k++) {
+                if (k >= p.nsplit) break;
                 const float* row = inbox + (k * own + slot) * KS_PART;
-                const float f = ks_exp2(row[HD + 1] - M);
+                const float f = ks_exp2(refs_of[k] - M);
                 num += row[d] * f;
                 den += row[HD] * f;
             }
