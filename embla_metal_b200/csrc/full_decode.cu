@@ -700,11 +700,8 @@ static EmblaStatus full_decode_impl(EmblaAttn* ctx, const EmblaKVPool* pool, con
     }
     if (pool->kv_dtype == EMBLA_KV_INT4) {
         cudaStream_t s4 = static_cast<cudaStream_t>(stream);
-        if (k_new) {
-            // two launches; the second reads the pages that the first writes, so it must not fetch them ahead of its wait
+        if (k_new)   // (a launch of its own; the decode kernel reads no page ahead of its wait for it)
             if (EmblaStatus st = kv4_append_token(ctx, const_cast<EmblaKVPool*>(pool), view, k_new, v_new, kv_stride, norm_k, s4)) return st;
-            ctx->early = 0;
-        }
         return kv4_full_decode(ctx, pool, view, q, o_dev, o_stride, scores_dev, scores_stride, max_len, s4);
     }
     if (pool->kv_dtype != EMBLA_KV_INT8) EMBLA_FAIL(EMBLA_UNSUPPORTED, "embla_attn_full_decode: unknown pool dtype %d", pool->kv_dtype);

@@ -567,8 +567,9 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
                     // relu(s) rounded to fp16 by the conversion itself, its square once more (2^-11 each); the row sum takes the
                     // exact squares in fp32 (mixed-precision fma). In fp32 up to P the kernel took 470 microseconds instead of 431
                     // for 2048 tokens at 30720: these warps bound it, and packed fp32 pairs were no faster. (fp16 outputs of 333 tokens, error
-                    // relative to their size: 5.4e-4, with weights in fp32 rounded once 4.1e-4 and 7 % slower; 2.1e-4 is the
-                    // outputs' own rounding, the rest that of code x scale.)
+                    // relative to their size: 5.4e-4, with weights in fp32 rounded once 4.1e-4 and 7 to 12 % slower, whether as the
+                    // square of relu(s) or as s |s| with the conversion's relu; 2.1e-4 is the outputs' own rounding, the rest
+                    // that of code x scale.)
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
                         uint32_t h;
