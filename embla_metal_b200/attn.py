@@ -288,9 +288,11 @@ class Attention:
             raise ValueError(f"k {tuple(shape)}: batch, tokens, kv heads x {HEAD_DIM}")
         if k.dtype != self.torch_dtype or v.dtype != self.torch_dtype or shape != v.shape or strides != v.stride() or strides[2] != 1:
             raise ValueError(f"k {tuple(shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} must be alike, rows contiguous, in {self.torch_dtype}")
+        if not (k.is_cuda and v.is_cuda and pos0.is_cuda and block_table.is_cuda) or pos0.dtype != torch.int32 or block_table.dtype != torch.int32:
+            raise ValueError("k, v, pos0 and block_table are on the device, the last two int32")
         batch, n_tokens, width = shape
-        if batch != block_table.size(0) or width < pool.n_kv_heads * HEAD_DIM:
-            raise ValueError(f"k {tuple(shape)} does not hold {pool.n_kv_heads} kv heads of {block_table.size(0)} sequences")
+        if batch != block_table.size(0) or pos0.numel() < batch or width < pool.n_kv_heads * HEAD_DIM:
+            raise ValueError(f"k {tuple(shape)} does not hold {pool.n_kv_heads} kv heads of {block_table.size(0)} sequences with a position each")
         _check(lib().embla_kv_read(self.handle, pool.handle, self._pack_view(block_table, None, layer), pos0.data_ptr(), n_tokens,
                                    k.data_ptr(), v.data_ptr(), strides[1], strides[0], _raw_stream()))
 

@@ -501,6 +501,10 @@ def test_refusals():
         ctx.kv_read(pool, table, 2, p0, x, x.clone())                                   # a layer the pool does not have
     with pytest.raises(ValueError):
         ctx.kv_read(pool, table, 1, p0, x.float(), x.float())
+    for args in ((table, 1, p0, x.cpu(), x.cpu()), (table, 1, p0.cpu(), x, x.clone()), (table.long(), 1, p0, x, x.clone()), (table, 1, p0[:0], x, x.clone()),
+                 (table, 1, p0, x.view(1, 1, 2, -1), x.view(1, 1, 2, -1))):
+        with pytest.raises(ValueError):
+            ctx.kv_read(pool, *args)
     with pytest.raises(ValueError):                                                     # rows too narrow for two kv heads
         ctx.kv_read(pool, table, 1, p0, x[..., :128], x[..., :128])
     shifted = torch.zeros(600, dtype=torch.float16, device="cuda")[1:513].view(1, 1, 512)
