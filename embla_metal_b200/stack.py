@@ -60,6 +60,7 @@ class DecodeStack:
         self.rings = [attn.Ring(batch, n_kv_heads, ring, window, self.dtype) for _ in range(n_sliding)]
         # sequence b owns blocks b * npages .. of each pool
         self.table = torch.arange(batch * npages, dtype=torch.int32, device="cuda").view(batch, npages).contiguous()
+        self._owner = [[b] * npages for b in range(batch)]   # whose blocks a row of the table holds (fork)
         descs = (LayerDesc * len(self.kinds))()
         slots = {SLIDING: 0, FULL: 0, SPARSE: 0}
         for i, k in enumerate(self.kinds):
@@ -103,22 +104,46 @@ class DecodeStack:
     def set_positions(self, pos):
         """pos: int or list — position of the token each sequence decodes next (keys seen = pos + 1)."""
         t = torch.as_tensor([pos] * self.batch if isinstance(pos, int) else list(pos), dtype=torch.int32)
+        if any(o[0] != b for b, o in enumerate(self._owner)):   # (blocks are shared from the first on)
+            for b, p in enumerate(t.tolist()):
+                if p < self._shared(b) * attn.BLOCK:
+                    raise ValueError(f"position {p} of sequence {b} lies in blocks that it shares with another (fork)")
         self.pos.copy_(t)
         self.seq_lens.copy_(t + 1)
         self.max_seq_len = int(t.max()) + 1
 
+    def _shared(self, b):
+        """Blocks at the head of sequence b that it shares with another."""
+        mine, n = self._owner[b], 0
+        while n < self.npages and (mine[n] != b or any(o[n] == b for i, o in enumerate(self._owner) if i != b)):
+            n += 1
+        return n
+
+    def _lent_to(self, b):
+        return [i for i, o in enumerate(self._owner) if i != b and b in o]
+
+    def restart(self, b):
+        """Sequence b starts anew at position 0 in blocks of its own, giving back those it shares (fork); refused while another
+        sequence shares b's."""
+        if not 0 <= b < self.batch:
+            raise ValueError(f"restart of sequence {b} of {self.batch}")
+        if self._lent_to(b):
+            raise ValueError(f"restart of sequence {b}: sequences {self._lent_to(b)} share its blocks")
+        self.table[b] = torch.arange(b * self.npages, (b + 1) * self.npages, dtype=torch.int32, device="cuda")
+        self._owner[b] = [b] * self.npages
+        self.pos[b] = 0
+        self.seq_lens[b] = 1
+
     def fork(self, src, dst):
         """Sequence `dst` goes on from where `src` stands (its last step or prompt done: keys seen = seq_lens): it shares the blocks
         that src has filled, gets its own copy of the rows in src's last block and of its rings, and src's position. The
-        blocks dst held itself are used again, which is refused while another sequence shares them. src must not be set
-        back to a position inside the shared blocks while dst lives (its appends would write into them); going on is fine,
-        as is forking again. Reads src's length from the device (synchronises)."""
+        blocks dst held itself are used again, which is refused while another sequence shares them. Both go on from there and may be
+        forked again; neither is set back to a position inside the shared blocks (set_positions refuses it, a prefill chunk must not
+        start there) until dst is restarted. Reads src's length from the device (synchronises)."""
         if src == dst or not (0 <= src < self.batch and 0 <= dst < self.batch):
             raise ValueError(f"fork of sequence {src} into {dst} of {self.batch}")
-        sharers = (self.table // self.npages == dst).any(1)
-        sharers[dst] = False
-        if bool(sharers.any()):
-            raise ValueError(f"fork into sequence {dst}: sequences {sharers.nonzero().flatten().tolist()} share its blocks")
+        if self._lent_to(dst):
+            raise ValueError(f"fork into sequence {dst}: sequences {self._lent_to(dst)} share its blocks")
         n = int(self.seq_lens[src])
         full, rest = divmod(n, attn.BLOCK)
         own = torch.arange(dst * self.npages, (dst + 1) * self.npages, dtype=torch.int32, device="cuda")
@@ -130,6 +155,7 @@ class DecodeStack:
                     self.ctx.copy_blocks(pool, src_block, own[full:full + 1], rows)
         self.table[dst, :full] = self.table[src, :full]
         self.table[dst, full:] = own[full:]
+        self._owner[dst] = self._owner[src][:full] + [dst] * (self.npages - full)
         for r in self.rings:
             r.k[dst].copy_(r.k[src])
             r.v[dst].copy_(r.v[src])

@@ -272,3 +272,33 @@ def test_a_stalled_producer_is_reported_and_the_next_call_is_right(batch, n):
     ctx.full_decode(pool, table, ln, 1, q, o)
     ctx.check()
     assert torch.equal(o, good)
+
+
+def test_shared_blocks_are_not_written_and_are_given_back():
+    import torch
+    from embla_metal_b200 import stack as stk
+    st = _stack([stk.FULL, stk.SPARSE], 4, 1024, seed=8)
+    st.set_positions([299, 5, 5, 5])
+    st.fork(0, 1)
+    st.fork(1, 2)                          # shares blocks of sequence 0 through sequence 1, and has its own last one
+    for pos in ([255, 300, 300, 5], [300, 0, 300, 5], [300, 300, 255, 5]):
+        with pytest.raises(ValueError):
+            st.set_positions(pos)
+    st.set_positions([300, 256, 299, 0])   # inside the blocks that each has to itself
+    for b in (0, 4, -1):
+        with pytest.raises(ValueError):
+            st.restart(b)                  # others share its blocks; no such sequence
+    before = st.full_pool.raw()[:2].clone()
+    st.restart(1)
+    st.set_positions([300, 0, 300, 0])
+    st.qkv.normal_()
+    st.step()
+    st.ctx.check()
+    assert torch.equal(st.full_pool.raw()[:2], before)
+    assert st.table[1].tolist() == list(range(st.npages, 2 * st.npages))
+    with pytest.raises(ValueError):
+        st.restart(0)                      # sequence 2 still does
+    st.restart(2)
+    st.restart(0)
+    st.set_positions(0)
+    st.close()
