@@ -61,6 +61,7 @@ class DecodeStack:
         # sequence b owns blocks b * npages .. of each pool
         self.table = torch.arange(batch * npages, dtype=torch.int32, device="cuda").view(batch, npages).contiguous()
         self._owner = [[b] * npages for b in range(batch)]   # whose blocks a row of the table holds (fork)
+        self._standing = []   # (sequence, block) of forks that still stand on the last row of a block they share
         descs = (LayerDesc * len(self.kinds))()
         slots = {SLIDING: 0, FULL: 0, SPARSE: 0}
         for i, k in enumerate(self.kinds):
@@ -104,13 +105,14 @@ class DecodeStack:
     def set_positions(self, pos):
         """pos: int or list — position of the token each sequence decodes next (keys seen = pos + 1)."""
         t = torch.as_tensor([pos] * self.batch if isinstance(pos, int) else list(pos), dtype=torch.int32)
-        if any(o[0] != b for b, o in enumerate(self._owner)):   # (blocks are shared from the first on)
-            for b, p in enumerate(t.tolist()):
-                if p < self._shared(b) * attn.BLOCK:
-                    raise ValueError(f"position {p} of sequence {b} lies in blocks that it shares with another (fork)")
+        if self._shares():
+            self._claim(t.tolist())
         self.pos.copy_(t)
         self.seq_lens.copy_(t + 1)
         self.max_seq_len = int(t.max()) + 1
+
+    def _shares(self):
+        return any(o[0] != b for b, o in enumerate(self._owner))   # (blocks are shared from the first on)
 
     def _shared(self, b):
         """Blocks at the head of sequence b that it shares with another."""
@@ -122,6 +124,31 @@ class DecodeStack:
     def _lent_to(self, b):
         return [i for i, o in enumerate(self._owner) if i != b and b in o]
 
+    def _claim(self, at):
+        """Every sequence goes on at its position in `at`: those that a fork left in a block of their source and that write there, or whose
+        source does, get a copy of it; positions in blocks that stay shared are refused."""
+        for dst, block in list(self._standing):
+            owner = self._owner[dst][block]
+            if any(p // attn.BLOCK == block and self._owner[b][block] == owner for b, p in enumerate(at)):
+                self._part(dst, block)
+        for b, p in enumerate(at):
+            if p < self._shared(b) * attn.BLOCK:
+                raise ValueError(f"position {p} of sequence {b} lies in blocks that it shares with another (fork)")
+        self._standing = []
+
+    def _part(self, dst, block):
+        """Sequence dst's own copy of a block that it shares."""
+        own = torch.full((1,), dst * self.npages + block, dtype=torch.int32, device=self.table.device)
+        self._copy_block(self.table[dst, block:block + 1].clone(), own)
+        self.table[dst, block:block + 1] = own
+        self._owner[dst][block] = dst
+        self._standing.remove((dst, block))
+
+    def _copy_block(self, src, dst, rows=None):
+        for pool in (self.full_pool, self.sparse_pool):
+            if pool is not None:
+                self.ctx.copy_blocks(pool, src, dst, rows)
+
     def restart(self, b):
         """Sequence b starts anew at position 0 in blocks of its own, giving back those it shares (fork); refused while another
         sequence shares b's."""
@@ -129,8 +156,9 @@ class DecodeStack:
             raise ValueError(f"restart of sequence {b} of {self.batch}")
         if self._lent_to(b):
             raise ValueError(f"restart of sequence {b}: sequences {self._lent_to(b)} share its blocks")
-        self.table[b] = torch.arange(b * self.npages, (b + 1) * self.npages, dtype=torch.int32, device="cuda")
+        self.table[b] = torch.arange(b * self.npages, (b + 1) * self.npages, dtype=torch.int32, device=self.table.device)
         self._owner[b] = [b] * self.npages
+        self._standing = [e for e in self._standing if e[0] != b]
         self.pos[b] = 0
         self.seq_lens[b] = 1
 
@@ -139,23 +167,23 @@ class DecodeStack:
         that src has filled, gets its own copy of the rows in src's last block and of its rings, and src's position. The
         blocks dst held itself are used again, which is refused while another sequence shares them. Both go on from there and may be
         forked again; neither is set back to a position inside the shared blocks (set_positions refuses it, a prefill chunk must not
-        start there) until dst is restarted. Reads src's length from the device (synchronises)."""
+        start there) until dst is restarted. Where src stands on the last row of a block, that block is shared until one of the two
+        writes into it, and the call that does so copies it first (a graph captured before cannot: set_positions, then replay). Reads
+        src's length from the device (synchronises)."""
         if src == dst or not (0 <= src < self.batch and 0 <= dst < self.batch):
             raise ValueError(f"fork of sequence {src} into {dst} of {self.batch}")
         if self._lent_to(dst):
             raise ValueError(f"fork into sequence {dst}: sequences {self._lent_to(dst)} share its blocks")
         n = int(self.seq_lens[src])
         full, rest = divmod(n, attn.BLOCK)
-        own = torch.arange(dst * self.npages, (dst + 1) * self.npages, dtype=torch.int32, device="cuda")
+        own = torch.arange(dst * self.npages, (dst + 1) * self.npages, dtype=torch.int32, device=self.table.device)
         if rest:
-            src_block = self.table[src, full:full + 1].clone()
-            rows = torch.tensor([rest], dtype=torch.int32, device="cuda")
-            for pool in (self.full_pool, self.sparse_pool):
-                if pool is not None:
-                    self.ctx.copy_blocks(pool, src_block, own[full:full + 1], rows)
+            rows = torch.full((1,), rest, dtype=torch.int32, device=self.table.device)
+            self._copy_block(self.table[src, full:full + 1].clone(), own[full:full + 1], rows)
         self.table[dst, :full] = self.table[src, :full]
         self.table[dst, full:] = own[full:]
         self._owner[dst] = self._owner[src][:full] + [dst] * (self.npages - full)
+        self._standing = [e for e in self._standing if e[0] != dst] + ([(dst, full - 1)] if full and not rest else [])
         for r in self.rings:
             r.k[dst].copy_(r.k[src])
             r.v[dst].copy_(r.v[src])
@@ -202,6 +230,11 @@ class DecodeStack:
             r.v.copy_(torch.randn(r.v.shape, device="cuda", generator=g).to(self.dtype))
 
     def _step_struct(self):
+        if self._standing:
+            if self.table.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise ValueError("a step straight after a fork copies a block: set_positions (or one step) before the capture")
+            for dst, block in list(self._standing):
+                self._part(dst, block)
         return StackStep(self.qkv.data_ptr(), self.qkv.stride(1), self.qkv.stride(0), self.o.data_ptr(),
                          self.o.stride(1), self.o.stride(0), self.seq_lens.data_ptr(), self.pos.data_ptr(),
                          self.table.data_ptr(), self.table.stride(0), self.table.stride(0), self.table.data_ptr(),

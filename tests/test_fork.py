@@ -1,0 +1,118 @@
+"""DecodeStack's forks without a GPU: whose blocks a table holds, and what each call refuses or copies. The pool is a tensor of row marks, a step
+writes the mark of its token where the table points."""
+import pytest
+import torch
+
+from embla_metal_b200 import stack as stk
+
+PAGES = 4
+
+
+class _Pool:
+    def __init__(self, blocks):
+        self.rows = torch.full((blocks, 128), -1)
+
+
+class _Ctx:
+    def copy_blocks(self, pool, src, dst, rows=None):
+        for i in range(src.numel()):
+            n = 128 if rows is None else int(rows[i])
+            pool.rows[int(dst[i]), :n] = pool.rows[int(src[i]), :n]
+
+
+def _stack(batch):
+    st = stk.DecodeStack.__new__(stk.DecodeStack)
+    st.batch, st.npages, st.max_context, st.max_seq_len = batch, PAGES, PAGES * 128, PAGES * 128
+    st.ctx, st.full_pool, st.sparse_pool, st.rings = _Ctx(), _Pool(batch * PAGES), None, []
+    st.table = torch.arange(batch * PAGES, dtype=torch.int32).view(batch, PAGES).contiguous()
+    st._owner, st._standing = [[b] * PAGES for b in range(batch)], []
+    st.pos, st.seq_lens = torch.zeros(batch, dtype=torch.int32), torch.zeros(batch, dtype=torch.int32)
+    st.qkv = st.o = torch.zeros(1, batch, 1)
+    st.handle = None
+    return st
+
+
+def _step(st, marks):
+    """What a step writes: the token's row of every sequence, all of them before any is read."""
+    st._step_struct()
+    at = [(int(st.table[b, int(st.pos[b]) // 128]), int(st.pos[b]) % 128) for b in range(st.batch)]
+    assert len(set(at)) == st.batch, "two sequences write one row"
+    for (block, row), m in zip(at, marks):
+        st.full_pool.rows[block, row] = m
+
+
+def _rows(st, b, n):
+    return st.full_pool.rows[st.table[b].long()].flatten()[:n].tolist()
+
+
+def _fill(st, n):
+    """n steps, sequence b marking position t with 1000 b + t."""
+    for t in range(n):
+        st.set_positions(t)
+        _step(st, [1000 * b + t for b in range(st.batch)])
+
+
+@pytest.mark.parametrize("n", [1, 127, 128, 129, 256, 300])
+@pytest.mark.parametrize("ahead", [False, True])
+def test_fork_then_steps_keep_the_sequences_apart(n, ahead):
+    """Forked behind a step that wrote position n - 1, or with the positions moved on to it already: the next steps, with or without
+    set_positions, write rows of each sequence's own."""
+    st = _stack(3)
+    _fill(st, n - 1 if ahead else n)
+    if ahead:
+        st.set_positions(n - 1)
+    st.fork(0, 2)
+    _step(st, [1, 2, 3])                                   # no set_positions: position n - 1 (again)
+    for i in range(3):
+        st.set_positions(n + i)
+        _step(st, [10 + i, 20 + i, 30 + i])
+    head = list(range(n - 1))
+    assert _rows(st, 0, n + 3) == head + [1, 10, 11, 12]
+    assert _rows(st, 2, n + 3) == head + [3, 30, 31, 32]
+    assert _rows(st, 1, n + 3) == [1000 + t for t in head] + [2, 20, 21, 22]
+
+
+@pytest.mark.parametrize("who", [0, 1, 2])
+def test_a_chain_of_forks_on_the_last_row(who):
+    """0 -> 1 -> 2, all at 256 keys; one of them writes position 255 once more, the others go on behind it."""
+    st = _stack(3)
+    _fill(st, 256)
+    st.fork(0, 1)
+    st.fork(1, 2)
+    at = [256] * 3
+    at[who] = 255
+    st.set_positions(at)
+    _step(st, [1, 2, 3])
+    for b in range(3):
+        assert _rows(st, b, at[b] + 1) == list(range(at[b])) + [b + 1]
+    assert all(int(st.table[b, 0]) == 0 for b in range(3))
+
+
+def test_moved_on_positions_stay_shared_and_are_refused_later():
+    st = _stack(2)
+    _fill(st, 128)
+    st.fork(0, 1)
+    st.set_positions(128)
+    assert int(st.table[1, 0]) == 0
+    for p in ([127, 128], [128, 127]):
+        with pytest.raises(ValueError):
+            st.set_positions(p)
+    with pytest.raises(ValueError):
+        st.restart(0)
+    st.restart(1)
+    st.set_positions([127, 0])
+    assert int(st.table[1, 0]) == PAGES
+
+
+def test_restart_and_another_fork_forget_the_first():
+    st = _stack(3)
+    _fill(st, 128)
+    st.fork(0, 1)
+    st.restart(1)
+    _step(st, [1, 2, 3])
+    assert _rows(st, 0, 128)[-1] == 1 and _rows(st, 1, 1) == [2]
+    st.set_positions([127, 100, 127])
+    st.fork(0, 1)
+    st.fork(2, 1)                                          # dst again, of another source
+    _step(st, [4, 5, 6])
+    assert _rows(st, 0, 128)[-1] == 4 and _rows(st, 1, 128) == [2000 + t for t in range(127)] + [5] and _rows(st, 2, 128)[-1] == 6
