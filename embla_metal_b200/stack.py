@@ -163,8 +163,8 @@ class DecodeStack:
         self.seq_lens[b] = 1
 
     def fork(self, src, dst):
-        """Sequence `dst` goes on from where `src` stands (its last step or prompt done: keys seen = seq_lens): it shares the blocks
-        that src has filled, gets its own copy of the rows in src's last block and of its rings, and src's position. The
+        """Sequence `dst` goes on from where `src` stands (its last step or prompt chunk done: keys seen = seq_lens): it shares the
+        blocks that src has filled, gets its own copy of the rows in src's last block and of its rings, and src's position. The
         blocks dst held itself are used again, which is refused while another sequence shares them. Both go on from there and may be
         forked again; neither is set back to a position inside the shared blocks (set_positions refuses it, a prefill chunk must not
         start there) until dst is restarted. Where src stands on the last row of a block, that block is shared until one of the two
@@ -248,7 +248,9 @@ class DecodeStack:
     def prefill_chunk(self, qkv, o, pos0, kv_only_layers=0, max_seq_len=0):
         """A chunk of new tokens through every layer (sliding and full layers only): qkv [n_layers, batch, T, qkv_width],
         o [n_layers, batch, T, o_width] on the device, pos0 int32 [batch] the position of each sequence's first new token.
-        The last `kv_only_layers` layers only store their keys and values."""
+        The last `kv_only_layers` layers only store their keys and values. The stack's positions are then those behind the chunk: a
+        step decodes the token after it, a fork goes on from it. (A sequence whose context the chunk has filled has no such
+        position: it stays on its last one.) max_seq_len: a bound on pos0 + T where the host knows one."""
         n, b, t, _ = qkv.shape
         if (n, b) != (len(self.kinds), self.batch) or tuple(o.shape[:3]) != (n, b, t):
             raise ValueError(f"qkv {tuple(qkv.shape)} / o {tuple(o.shape)} do not fit {len(self.kinds)} layers x {self.batch} sequences")
@@ -257,6 +259,9 @@ class DecodeStack:
         ck = StackChunk(qkv.data_ptr(), qkv.stride(2), qkv.stride(1), qkv.stride(0), o.data_ptr(), o.stride(2), o.stride(1),
                         o.stride(0), pos0.data_ptr(), self.table.data_ptr(), self.table.stride(0), b, t, max_seq_len, kv_only_layers)
         attn._check(attn.lib().embla_stack_prefill_chunk(self.handle, C.byref(ck), attn._stream()))
+        torch.add(pos0[:b], t, out=self.pos).clamp_(max=self.max_context - 1)
+        torch.add(self.pos, 1, out=self.seq_lens)
+        self.max_seq_len = max(self.max_seq_len, min(max_seq_len + 1, self.max_context) if max_seq_len else self.max_context)
 
     def step_layers(self, first, count):
         """The step for layers first .. first + count - 1 only."""

@@ -116,3 +116,52 @@ def test_restart_and_another_fork_forget_the_first():
     st.fork(2, 1)                                          # dst again, of another source
     _step(st, [4, 5, 6])
     assert _rows(st, 0, 128)[-1] == 4 and _rows(st, 1, 128) == [2000 + t for t in range(127)] + [5] and _rows(st, 2, 128)[-1] == 6
+
+
+def _chunk(st, monkeypatch, pos0, T, mark=0, **kw):
+    """prefill_chunk with a library that writes the rows' marks: 1000 b + position + mark."""
+    class Lib:
+        @staticmethod
+        def embla_stack_prefill_chunk(handle, ck, stream):
+            for b, p0 in enumerate(pos0):
+                for t in range(p0, p0 + T):
+                    st.full_pool.rows[int(st.table[b, t // 128]), t % 128] = 1000 * b + t + mark
+            return 0
+    monkeypatch.setattr(stk.attn, "lib", lambda: Lib)
+    monkeypatch.setattr(stk.attn, "_stream", lambda: None)
+    st.kinds = [stk.FULL]
+    x = torch.zeros(1, st.batch, T, 1)
+    st.prefill_chunk(x, x, torch.tensor(pos0, dtype=torch.int32), **kw)
+
+
+@pytest.mark.parametrize("n", [1, 127, 128, 129, 256, 300])
+@pytest.mark.parametrize("used", [0, 400])
+@pytest.mark.parametrize("positions", [False, True])
+def test_fork_after_a_chunk_has_the_prompt(n, used, positions, monkeypatch):
+    """A prompt of n tokens, on a new stack or behind other work, forked; the next tokens are those at n, whether or not the caller says so."""
+    st = _stack(3)
+    if used:
+        _fill(st, used)
+    _chunk(st, monkeypatch, [0, 0, 0], n, max_seq_len=n)
+    st.fork(0, 2)
+    for i in range(3):
+        if i or positions:
+            st.set_positions(n + i)
+        _step(st, [10 + i, 20 + i, 30 + i])
+    head = list(range(n))
+    assert _rows(st, 0, n + 3) == head + [10, 11, 12]
+    assert _rows(st, 2, n + 3) == head + [30, 31, 32]
+    assert _rows(st, 1, n + 3) == [1000 + t for t in head] + [20, 21, 22]
+
+
+def test_positions_behind_a_chunk(monkeypatch):
+    st = _stack(2)
+    st.set_positions([3, 9])
+    _chunk(st, monkeypatch, [4, 200], 100, max_seq_len=300)
+    assert st.pos.tolist() == [104, 300] and st.seq_lens.tolist() == [105, 301] and st.max_seq_len == 301
+    _chunk(st, monkeypatch, [0, PAGES * 128 - 100], 100, max_seq_len=PAGES * 128)   # the second sequence's context is full
+    assert st.pos.tolist() == [100, PAGES * 128 - 1] and st.seq_lens.tolist() == [101, PAGES * 128]
+    assert st.max_seq_len == PAGES * 128
+    st.set_positions([1, 1])
+    _chunk(st, monkeypatch, [0, 0], 100)                   # no bound given
+    assert st.max_seq_len == PAGES * 128

@@ -45,3 +45,43 @@ def test_a_step_straight_after_a_fork(n):
         assert torch.equal(st.o, whole.o), i
     st.close()
     whole.close()
+
+
+@pytest.mark.parametrize("kv", ["int4", "int8"])
+@pytest.mark.parametrize("n", [1, 127, 128, 256, 300])
+@pytest.mark.parametrize("positions", [False, True])
+def test_a_fork_after_a_prompt_chunk(n, kv, positions):
+    """A prompt of n tokens, forked, then steps with different tokens: bit-equal to sequences that went through the prompt themselves."""
+    import torch
+    from embla_metal_b200 import attn, stack as stk
+    from oracle import oracle as orc
+    kinds = [stk.FULL, stk.SLIDING, stk.FULL]
+    both = []
+    for _ in range(2):
+        st = stk.DecodeStack(kinds, 3, 1024, n_q_heads=8, n_kv_heads=2, act_dtype=orc.F16, window=128, ring=1024,
+                             kv_dtype=attn.KV_INT4 if kv == "int4" else attn.KV_INT8)
+        st.fill_random(3)                                  # what earlier sequences left behind
+        st.set_positions([700, 5, 900])
+        both.append(st)
+    st, whole = both
+    g = torch.Generator("cuda").manual_seed(n)
+    qkv = torch.randn(3, 3, n, st.qkv_width, device="cuda", generator=g).to(st.dtype)
+    qkv[:, 2] = qkv[:, 0]
+    o = torch.zeros(3, 3, n, st.o_width, dtype=st.dtype, device="cuda")
+    pos0 = torch.zeros(3, dtype=torch.int32, device="cuda")
+    whole.prefill_chunk(qkv, o, pos0, max_seq_len=n)
+    qkv[:, 2].normal_()                                    # (the forked stack's sequence 2 had another prompt)
+    st.prefill_chunk(qkv, o, pos0, max_seq_len=n)
+    st.fork(0, 2)
+    assert (st.table[2, :n // 128] == st.table[0, :n // 128]).all()
+    for i in range(3):
+        q = _tokens(st, i)
+        for s in (st, whole):
+            s.qkv.copy_(q)
+            if i or positions:
+                s.set_positions(n + i)
+            s.step()
+            s.ctx.check()
+        assert torch.equal(st.o, whole.o), i
+    st.close()
+    whole.close()
