@@ -166,8 +166,8 @@ class DecodeStack:
         """Sequence `dst` goes on from where `src` stands (its last step or prompt chunk done: keys seen = seq_lens): it shares the
         blocks that src has filled, gets its own copy of the rows in src's last block and of its rings, and src's position. The
         blocks dst held itself are used again, which is refused while another sequence shares them. Both go on from there and may be
-        forked again; neither is set back to a position inside the shared blocks (set_positions refuses it, a prefill chunk must not
-        start there) until dst is restarted. Where src stands on the last row of a block, that block is shared until one of the two
+        forked again; neither is set back to a position inside the shared blocks (set_positions and prefill_chunk refuse it) until
+        dst is restarted. Where src stands on the last row of a block, that block is shared until one of the two
         writes into it, and the call that does so copies it first (a graph captured before cannot: set_positions, then replay). Reads
         src's length from the device (synchronises)."""
         if src == dst or not (0 <= src < self.batch and 0 <= dst < self.batch):
@@ -250,12 +250,17 @@ class DecodeStack:
         o [n_layers, batch, T, o_width] on the device, pos0 int32 [batch] the position of each sequence's first new token.
         The last `kv_only_layers` layers only store their keys and values. The stack's positions are then those behind the chunk: a
         step decodes the token after it, a fork goes on from it. (A sequence whose context the chunk has filled has no such
-        position: it stays on its last one.) max_seq_len: a bound on pos0 + T where the host knows one."""
+        position: it stays on its last one.) Where sequences share blocks (fork) pos0 is read on the host, and a chunk that starts inside
+        them is refused, as set_positions refuses it. max_seq_len: a bound on pos0 + T where the host knows one."""
         n, b, t, _ = qkv.shape
         if (n, b) != (len(self.kinds), self.batch) or tuple(o.shape[:3]) != (n, b, t):
             raise ValueError(f"qkv {tuple(qkv.shape)} / o {tuple(o.shape)} do not fit {len(self.kinds)} layers x {self.batch} sequences")
         if qkv.stride(3) != 1 or o.stride(3) != 1:
             raise ValueError("rows must be contiguous")
+        if self._shares():
+            if self.table.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise ValueError("a chunk over sequences that share blocks (fork) reads its positions: not while a graph is captured")
+            self._claim(pos0[:b].tolist())
         ck = StackChunk(qkv.data_ptr(), qkv.stride(2), qkv.stride(1), qkv.stride(0), o.data_ptr(), o.stride(2), o.stride(1),
                         o.stride(0), pos0.data_ptr(), self.table.data_ptr(), self.table.stride(0), b, t, max_seq_len, kv_only_layers)
         attn._check(attn.lib().embla_stack_prefill_chunk(self.handle, C.byref(ck), attn._stream()))

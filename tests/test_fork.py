@@ -165,3 +165,30 @@ def test_positions_behind_a_chunk(monkeypatch):
     st.set_positions([1, 1])
     _chunk(st, monkeypatch, [0, 0], 100)                   # no bound given
     assert st.max_seq_len == PAGES * 128
+
+
+def test_a_chunk_does_not_write_shared_blocks(monkeypatch):
+    st = _stack(3)
+    _chunk(st, monkeypatch, [0, 0, 0], 300, max_seq_len=300)
+    st.fork(0, 2)
+    before, at = st.full_pool.rows.clone(), st.pos.tolist()
+    for pos0 in ([0, 0, 300], [300, 0, 255], [255, 300, 256], [0, 0, 0]):
+        with pytest.raises(ValueError):
+            _chunk(st, monkeypatch, pos0, 100, mark=5, max_seq_len=400)
+    assert torch.equal(st.full_pool.rows, before) and st.pos.tolist() == at
+    _chunk(st, monkeypatch, [256, 0, 300], 100, mark=5, max_seq_len=400)   # behind them
+    head = list(range(256))
+    assert _rows(st, 0, 356) == head + [t + 5 for t in range(256, 356)]
+    assert _rows(st, 2, 400) == head + list(range(256, 300)) + [2000 + t + 5 for t in range(300, 400)]
+    st.restart(2)                                          # a new prompt for all of them
+    _chunk(st, monkeypatch, [0, 0, 0], 10, mark=7, max_seq_len=10)
+    assert [_rows(st, b, 10) for b in range(3)] == [[1000 * b + t + 7 for t in range(10)] for b in range(3)]
+
+
+def test_a_chunk_from_the_last_row_of_a_shared_block(monkeypatch):
+    st = _stack(2)
+    _fill(st, 256)
+    st.fork(0, 1)
+    _chunk(st, monkeypatch, [255, 255], 3, mark=5, max_seq_len=258)
+    assert _rows(st, 0, 258) == list(range(255)) + [260, 261, 262]
+    assert _rows(st, 1, 258) == list(range(255)) + [1260, 1261, 1262]

@@ -85,3 +85,34 @@ def test_a_fork_after_a_prompt_chunk(n, kv, positions):
         assert torch.equal(st.o, whole.o), i
     st.close()
     whole.close()
+
+
+def test_a_chunk_into_shared_blocks_is_refused():
+    import torch
+    from embla_metal_b200 import stack as stk
+    st = _stack([stk.FULL], 2, 1024, seed=3)
+    st.set_positions([299, 5])
+    st.fork(0, 1)
+    qkv = torch.zeros(1, 2, 4, st.qkv_width, dtype=st.dtype, device="cuda")
+    o = torch.zeros(1, 2, 4, st.o_width, dtype=st.dtype, device="cuda")
+    before = st.full_pool.raw().clone()
+    at = lambda *p: torch.tensor(p, dtype=torch.int32, device="cuda")
+    for p in (at(0, 300), at(300, 255)):
+        with pytest.raises(ValueError):
+            st.prefill_chunk(qkv, o, p, max_seq_len=304)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        graph = torch.cuda.CUDAGraph()
+        p = at(300, 300)
+        stream.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            with pytest.raises(ValueError):                # (the positions cannot be looked at)
+                st.prefill_chunk(qkv, o, p, max_seq_len=304)
+            o.zero_()                                      # (a graph of something)
+    torch.cuda.synchronize()
+    assert torch.equal(st.full_pool.raw(), before)
+    st.prefill_chunk(qkv, o, p, max_seq_len=304)
+    st.ctx.check()
+    assert torch.equal(st.full_pool.raw()[:2], before[:2])
+    del graph
+    st.close()
