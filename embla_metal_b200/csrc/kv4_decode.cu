@@ -36,12 +36,6 @@ __device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* map) {
 }
 __device__ __forceinline__ void prefetch_l2(const void* at) { asm volatile("prefetch.global.L2 [%0];" ::"l"(at)); }
 
-__device__ __forceinline__ float relu_nan(float x) {   // max(x, 0), NaN of NaN
-    float r;
-    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(x));
-    return r;
-}
-
 // a barrier that tells all its threads whether any of them said yes
 __device__ __forceinline__ bool bar_any(int id, int threads, bool yes) {
     int any;

@@ -37,6 +37,11 @@ __device__ __forceinline__ uint32_t movmatrix4_trans(uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
     return r;
 }
+__device__ __forceinline__ float relu_nan(float x) {   // max(x, 0), NaN of NaN
+    float r;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(x));
+    return r;
+}
 // 2^(e - 127) for a biased exponent 1 .. 254
 __device__ __forceinline__ float pow2_biased(int e) { return __uint_as_float(uint32_t(e) << 23); }
 

@@ -555,7 +555,9 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
                 if (diag) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
-                        const float m0 = fmaxf(__uint_as_float(s[e]), 0.0f), m1 = fmaxf(__uint_as_float(s[e + 1]), 0.0f);
+                        // (KV4: a key that is not a number stays one here too, as in the unmasked pages and in the decode)
+                        const float s0 = __uint_as_float(s[e]), s1 = __uint_as_float(s[e + 1]);
+                        const float m0 = KV4 ? relu_nan(s0) : fmaxf(s0, 0.0f), m1 = KV4 ? relu_nan(s1) : fmaxf(s1, 0.0f);
                         float w0 = m0 * m0, w1 = m1 * m1;
                         const int kb = j * BLK + 32 * cc + e;
                         if (kb > pos_r) w0 = 0.0f;
