@@ -48,6 +48,7 @@ constexpr float PF_QK8_C0 = 1.0f / 256.0f;
 // alignment slack, 2 Q tiles, 3 converted sides, 3 raw int8 sides, 2 pages' scales, barriers
 constexpr size_t PF_SMEM = 1024 + 2 * PF_TILE16 + PF_KVBUFS * PF_TILE16 + PF_KVBUFS * CODE_BYTES + 2 * 1024 + 256 + 2 * 1024;
 
+__device__ __forceinline__ int pick(const int (&a)[2], int x) { return x ? a[1] : a[0]; }   // (an array indexed at run time would lie in memory)
 struct PfPiece;
 struct PrefillParams {
     const uint8_t* pool;
@@ -119,12 +120,19 @@ __device__ __forceinline__ void convert_side(const uint8_t* raw, uint8_t* dst, i
 // code x scale rounded once (2^-11); queries enter scaled by 2^-7 and the keys without 1 / sqrt(D), whose square, 2^-7, is exact
 // in the weights: P = relu(s)^2 comes out as the weight x 2^-7 (scores up to 2895 square inside fp16's range), the sink takes
 // the same factor. 2048 tokens at 30720: 431 us, 1236 TFLOP/s (0.75 of the measured burst rate; the int8 pages take 449 us).
+// What does not fit in fp16 so (a score above 2895, a scale of 8192 or more, a bf16 query above 8.4e6) is seen once the range's products are
+// done, and the CTA then takes its pages twice more: with every query row scaled by a power of two that brings its largest element into
+// [1, 2), once for the largest score of each row and once with the scores under the power of two that brings that one into [64, 128).
+// Sums and outputs leave in the usual units, so what the other ranges of a unit did makes no difference. Three times the time, for rows
+// that fp16 would have made infinite; all others pay one barrier.
 constexpr float PF4_QSCALE = 1.0f / 128.0f, PF4_PSCALE = 1.0f / 128.0f;
+constexpr float PF4_FULL = 65504.0f;   // a row sum below it has no weight that fp16 does not hold
 
 // One side of a raw 4-bit page -> fp16 in the UMMA layout; rows from `lim` on (behind the last key, or all of a page that is
 // nowhere) become zeros, whatever lies there. 128 converter threads; the lanes of a quarter warp take 8 consecutive rows of one
-// group, so reads and writes are conflict-free.
-__device__ __forceinline__ void convert_side4(const uint8_t* raw, uint8_t* dst, int ctid, int side, int lim) {
+// group, so reads and writes are conflict-free. A scale whose products may leave fp16 sets *large; values an eighth of their size with
+// `eighth`.
+__device__ __forceinline__ void convert_side4(const uint8_t* raw, uint8_t* dst, int ctid, int side, int lim, bool eighth, volatile int* large) {
     const int rl = ctid & 7, g = (ctid >> 3) & 3, rg = ctid >> 5;
     const __half* scales = reinterpret_cast<const __half*>(raw + KV4_SIDE) + side * KV4_GROUPS + g;
 #pragma unroll
@@ -136,6 +144,9 @@ __device__ __forceinline__ void convert_side4(const uint8_t* raw, uint8_t* dst, 
             w = make_uint4(0, 0, 0, 0);
             sc = __half2half2(__ushort_as_half(0));
         }
+        const uint32_t bits = __half_as_ushort(__low2half(sc)) & 0x7fffu;
+        if (bits >= 0x7000u && bits < 0x7c00u) *large = 1;   // 8192 .. 65504
+        if (eighth) sc = __hmul2(sc, __float2half2_rn(0.125f));
         const uint32_t x[4] = {w.x, w.y, w.z, w.w}, s2 = *reinterpret_cast<const uint32_t*>(&sc);
         // dims 32 g .. 32 g + 31: four 16-byte chunks of the half (dims 0-63 | 64-127) that the group lies in
         uint8_t* base = dst + (g >> 1) * (BLK * 128) + row * 128;
@@ -171,45 +182,69 @@ struct PfSegment {
     int jb, je;             // the pages
 };
 
-template <int DT, int SB, bool QK8, bool KV4>
-__device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, const PrefillParams& p, const PfSegment sg) {
-    constexpr float QSCALE = KV4 ? PF4_QSCALE : PF_QSCALE, PSCALE = KV4 ? PF4_PSCALE : PF_PSCALE;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* Qs = smem;                                               // [2 tiles][32 KiB]
-    uint8_t* kvb = smem + 2 * PF_TILE16;                              // [3][32 KiB] converted K / V sides
-    uint8_t* raw = kvb + PF_KVBUFS * PF_TILE16;                       // [3][16 KiB] int8 sides as loaded
-    uint8_t* scl = raw + PF_KVBUFS * CODE_BYTES;                      // [2 pages][K scales | V scales], 1 KiB each
-    uint64_t* bars = reinterpret_cast<uint64_t*>(scl + 2 * 1024);
-    float* qsc = reinterpret_cast<float*>(scl + 2 * 1024 + 256);     // QK8: [2 tiles][128] 1 / rho^2 of the int8 query rows
-    float* kfac = qsc + 2 * BLK;                                      // QK8: [2 pages][128] kscale / sqrt(D) x 2^-8 of the page's keys
-    uint64_t* raw_full = bars;            // [3]
-    uint64_t* raw_empty = bars + 3;       // [3]
-    uint64_t* kv_ready = bars + 6;        // [3]
-    uint64_t* kv_free = bars + 9;         // [3]
-    uint64_t* s_full = bars + 12;         // [2 tiles]
-    uint64_t* p_ready = bars + 14;        // [2 tiles]
-    uint64_t* o_done = bars + 16;
-    uint64_t* kf_ready = bars + 17;       // [2 pages] QK8: the page's key factors are set out (converters -> ReLU² warps)
-    __shared__ uint32_t s_tmem;
-    __shared__ int s_abort, s_last;
-    __shared__ volatile int s_lim[3];     // KV4: keys that count in the page side of each ring slot
+// A CTA's shared memory, and what follows from its segment.
+struct PfPlace {
+    uint8_t *smem, *Qs, *kvb, *raw, *scl;
+    uint64_t* bars;
+    float *qsc, *kfac;
+    int unit, kvh, p0, n;   // n: pages of the range
+    int t0[2], rows[2], npg[2];
+
+    __device__ __forceinline__ PfPlace(const PrefillParams& p, const PfSegment& sg) {
+        extern __shared__ uint8_t smem_raw[];
+        smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+        Qs = smem;                                               // [2 tiles][32 KiB]
+        kvb = smem + 2 * PF_TILE16;                              // [3][32 KiB] converted K / V sides
+        raw = kvb + PF_KVBUFS * PF_TILE16;                       // [3][16 KiB] int8 sides as loaded
+        scl = raw + PF_KVBUFS * CODE_BYTES;                      // [2 pages][K scales | V scales], 1 KiB each
+        bars = reinterpret_cast<uint64_t*>(scl + 2 * 1024);
+        qsc = reinterpret_cast<float*>(scl + 2 * 1024 + 256);    // QK8: [2 tiles][128] 1 / rho^2 of the int8 query rows
+        kfac = qsc + 2 * BLK;                                    // QK8: [2 pages][128] kscale / sqrt(D) x 2^-8 of the page's keys
+        unit = (sg.b * p.heads + sg.h) * p.pairs + sg.pair_ix;
+        kvh = sg.h / p.G;
+        p0 = p.pos0[sg.b];
+        // two query tiles of 128 consecutive tokens each share every converted page
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            t0[x] = (2 * sg.pair_ix + x) * BLK;
+            rows[x] = max(0, min(BLK, p.n_tokens - t0[x]));
+            npg[x] = rows[x] > 0 ? (p0 + t0[x] + rows[x] - 1) / BLK + 1 : 0;
+        }
+        n = max(0, sg.je - sg.jb);
+    }
+};
+struct PfShared {
+    uint32_t tmem;
+    int abort, last;
+    PfSegment sg;           // KV4: for prefill_wide
+    volatile int lim[3];    // KV4: keys that count in the page side of each ring slot
+    volatile int large;     // KV4: a scale of 8192 or more
+};
+constexpr int PF_BARS = 19;
+
+// The pages of a segment through the products: afterwards O of the tiles is in TMEM, and `rowsum` in the ReLU² warps; `ok`: no wait of
+// theirs ran out. WIDE (KV4): the second form of the rows that do not fit in fp16, run twice; the first time it only looks for the
+// rows' largest scores and leaves the factors that bring them into [64, 128).
+template <int DT, int SB, bool QK8, bool KV4, bool WIDE>
+__device__ __forceinline__ void prefill_pages(const CUtensorMap& tmap, const PrefillParams& p, const PfSegment& sg, const PfPlace& at, PfShared& sh,
+                                              bool measure, float& rowsum, bool& ok) {
+    constexpr float QSCALE = KV4 ? PF4_QSCALE : PF_QSCALE;
+    uint8_t *const Qs = at.Qs, *const kvb = at.kvb, *const raw = at.raw, *const scl = at.scl;
+    float *const qsc = at.qsc, *const kfac = at.kfac;
+    uint64_t* raw_full = at.bars;            // [3]
+    uint64_t* raw_empty = at.bars + 3;       // [3]
+    uint64_t* kv_ready = at.bars + 6;        // [3]
+    uint64_t* kv_free = at.bars + 9;         // [3]
+    uint64_t* s_full = at.bars + 12;         // [2 tiles]
+    uint64_t* p_ready = at.bars + 14;        // [2 tiles]
+    uint64_t* o_done = at.bars + 16;
+    uint64_t* kf_ready = at.bars + 17;       // [2 pages] QK8: the page's key factors are set out (converters -> ReLU² warps)
+    int* qexp = reinterpret_cast<int*>(qsc);   // WIDE: [2 tiles][128] exponents of the query rows,
+    float* factor = kfac;                      // and factors of their scores (each set and read by the row's thread)
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int h = sg.h, b = sg.b, pair_ix = sg.pair_ix, split = sg.split, nparts = sg.nparts, slot0 = sg.slot0;
-    const int jb = sg.jb, je = sg.je;
-    const int unit = (b * p.heads + h) * p.pairs + pair_ix;
-    const int kvh = h / p.G;
-    const int p0 = p.pos0[b];
-    // two query tiles of 128 consecutive tokens each share every converted page
-    int t0[2], rows[2], npg[2];
-#pragma unroll
-    for (int x = 0; x < 2; x++) {
-        t0[x] = (2 * pair_ix + x) * BLK;
-        rows[x] = max(0, min(BLK, p.n_tokens - t0[x]));
-        npg[x] = rows[x] > 0 ? (p0 + t0[x] + rows[x] - 1) / BLK + 1 : 0;
-    }
-    const int n = max(0, je - jb);
+    const int h = sg.h, b = sg.b, jb = sg.jb, je = sg.je, kvh = at.kvh, p0 = at.p0, n = at.n;
+    const int(&t0)[2] = at.t0, (&rows)[2] = at.rows, (&npg)[2] = at.npg;
     // The producer lane sets the barriers up and requests the first pages while the other warps stage the query tiles.
     if (warp == PF_PRODUCER && lane == 0) {
         for (int i = 0; i < 3; i++) {
@@ -225,7 +260,10 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
         mbar_init(o_done, 1);
         mbar_init(&kf_ready[0], PF_CONV_WARPS);
         mbar_init(&kf_ready[1], PF_CONV_WARPS);
-        s_abort = 0;
+        if (!WIDE) {
+            sh.abort = 0;
+            if (KV4) sh.large = 0;
+        }
         fence_barrier_init();
     }
     // conversion c = 2 j + side takes ring slot c % 3; page j's scales go to scl[j & 1]
@@ -236,12 +274,12 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
             const int blk = j < p.table_stride ? p.block_table[size_t(b) * p.table_stride + j] : -1;
             if (blk < 0 || blk >= p.num_blocks) {
                 atomicExch(p.ctl.err, ERR_BAD_BLOCK);
-                s_lim[slot] = 0;
+                sh.lim[slot] = 0;
                 mbar_arrive(&raw_full[slot]);
                 return;
             }
             const long pg = (long(blk) * p.n_layers + p.layer) * p.n_kv_heads + kvh;
-            s_lim[slot] = p0 + p.n_tokens - j * BLK;
+            sh.lim[slot] = p0 + p.n_tokens - j * BLK;
             mbar_expect_tx(&raw_full[slot], KV4_SIDE + KV4_SCALES);
             tma_load_2d(raw + slot * CODE_BYTES, &tmap, 0, int(pg * (KV4_PAGE / 128)) + side * (KV4_SIDE / 128), &raw_full[slot]);
             bulk_load_1d(raw + slot * CODE_BYTES + KV4_SIDE, p.pool + size_t(pg) * KV4_PAGE + 2 * KV4_SIDE, KV4_SCALES, &raw_full[slot]);
@@ -257,13 +295,35 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
     int requested = 0;        // (producer lane) conversions requested so far
     if (warp == PF_PRODUCER && lane == 0)
         for (; requested < min(3, 2 * n) && requested != p.ctl.stall_at; requested++) request(requested);
-    if (warp == PF_MMA) tmem_alloc(&s_tmem, 512);
+    if (warp == PF_MMA && !WIDE) tmem_alloc(&sh.tmem, 512);
     // the staging warps: every warp but the producer
     constexpr int SW = PF_THREADS / 32 - 1;
     const int swarp = warp < PF_PRODUCER ? warp : warp - 1, stid = swarp * 32 + lane;
 
     // ---- Q tiles: [128 tokens][128 dims] of head h as fp16 in the K-major swizzled layout
-    if (!QK8 && p.prenormed && warp != PF_PRODUCER) {
+    if (WIDE) {
+        // one warp a row: head norm if asked, then the row by a power of two
+        for (int i = swarp; i < 2 * BLK && warp != PF_PRODUCER; i += SW) {
+            const int x = i >> 7, r = i & 127;
+            const bool has = r < pick(rows, x);
+            float xq[4];
+            kv4_load_query<DT>(xq, has, p.q, size_t(b) * p.q_seq_stride + size_t(pick(t0, x) + r) * p.q_token_stride + size_t(h) * HD, lane);
+            if (has && !p.prenormed) kv4_query_norm<DT>(xq, p.g1, p.g2, 2, lane);
+            uint32_t top = 0;
+#pragma unroll
+            for (int k = 0; k < 4; k++) top = max(top, __float_as_uint(xq[k]) & 0x7fffffffu);
+            top = __reduce_max_sync(0xffffffffu, top);
+            const int e = min(max(int(top >> 23), 1), 253);
+            const float down = pow2_biased(254 - e);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int d = lane + 32 * k, c8 = d >> 3;
+                *reinterpret_cast<__half*>(Qs + x * PF_TILE16 + (c8 >> 3) * (BLK * 128) + r * 128 + (((c8 & 7) ^ (r & 7)) << 4) + (d & 7) * 2) =
+                    __float2half_rn(xq[k] * down);
+            }
+            if (lane == 0) qexp[i] = e - 127;
+        }
+    } else if (!QK8 && p.prenormed && warp != PF_PRODUCER) {
         // rows as they are, times the query scale: 16 bytes a thread and trip, every load of a thread (both tiles) in flight
         // before the first store
         constexpr int TRIPS = (BLK * 16 + SW * 32 - 1) / (SW * 32);
@@ -301,7 +361,7 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
                 *reinterpret_cast<uint4*>(Qs + x * PF_TILE16 + (c8 >> 3) * (BLK * 128) + r * 128 + (((c8 & 7) ^ (r & 7)) << 4)) = v[x][k];
             }
     }
-    for (int x = 0; x < 2 && warp != PF_PRODUCER && (QK8 || !p.prenormed); x++) {
+    for (int x = 0; x < 2 && warp != PF_PRODUCER && (QK8 || !p.prenormed) && !WIDE; x++) {
         uint8_t* Qx = Qs + x * PF_TILE16;
         if (QK8) {
             // one warp a row, four rows a trip with their loads in flight together: head norm (unless the rows come normed),
@@ -311,14 +371,14 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     const int r = r4 + k;
-                    const size_t off = size_t(b) * p.q_seq_stride + size_t(t0[x] + r) * p.q_token_stride + size_t(h) * HD;
+                    const size_t off = size_t(b) * p.q_seq_stride + size_t(pick(t0, x) + r) * p.q_token_stride + size_t(h) * HD;
 #pragma unroll
-                    for (int i = 0; i < 4; i++) xq[k][i] = r < rows[x] ? Act<DT>::load(p.q, off + lane + 32 * i) : 0.0f;
+                    for (int i = 0; i < 4; i++) xq[k][i] = r < pick(rows, x) ? Act<DT>::load(p.q, off + lane + 32 * i) : 0.0f;
                 }
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     const int r = r4 + k;
-                    if (r < rows[x] && !p.prenormed) {
+                    if (r < pick(rows, x) && !p.prenormed) {
                         float ss = 0.0f;
 #pragma unroll
                         for (int i = 0; i < 4; i++) ss = __fadd_rn(ss, __fmul_rn(xq[k][i], xq[k][i]));
@@ -355,14 +415,14 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     const int r = r4 + k;
-                    const size_t off = size_t(b) * p.q_seq_stride + size_t(t0[x] + r) * p.q_token_stride + size_t(h) * HD;
+                    const size_t off = size_t(b) * p.q_seq_stride + size_t(pick(t0, x) + r) * p.q_token_stride + size_t(h) * HD;
 #pragma unroll
-                    for (int i = 0; i < 4; i++) xq[k][i] = r < rows[x] ? Act<DT>::load(p.q, off + lane + 32 * i) : 0.0f;
+                    for (int i = 0; i < 4; i++) xq[k][i] = r < pick(rows, x) ? Act<DT>::load(p.q, off + lane + 32 * i) : 0.0f;
                 }
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     const int r = r4 + k;
-                    if (r < rows[x]) {
+                    if (r < pick(rows, x)) {
                         float ss = 0.0f;
 #pragma unroll
                         for (int i = 0; i < 4; i++) ss = __fadd_rn(ss, __fmul_rn(xq[k][i], xq[k][i]));
@@ -391,7 +451,7 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = sh.tmem;
     // TMEM columns: S/P of tile 0 at 0, of tile 1 at 128 (P overwrites the first 64 columns of its S); O at 256, 384
 
     if (warp == PF_PRODUCER) {
@@ -404,7 +464,7 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
                     atomicExch(p.ctl.err, ERR_WAIT_EMPTY);
                     break;
                 }
-                if (*reinterpret_cast<volatile int*>(&s_abort)) break;
+                if (*reinterpret_cast<volatile int*>(&sh.abort)) break;
                 request(c);
             }
         }
@@ -469,7 +529,7 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
             }
             if (!ok) {
                 atomicExch(p.ctl.err, ERR_WAIT_FULL);
-                *reinterpret_cast<volatile int*>(&s_abort) = 1;
+                *reinterpret_cast<volatile int*>(&sh.abort) = 1;
             }
             tc_commit(o_done);
         }
@@ -496,7 +556,7 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
                         (SB == 4 ? reinterpret_cast<const float*>(ksc)[ctid] : __half2float(reinterpret_cast<const __half*>(ksc)[ctid])) *
                         (rsqrtf(float(HD)) * PF_QK8_C0);
             } else if (KV4) {
-                convert_side4(raw + slot * CODE_BYTES, kvb + slot * PF_TILE16, ctid, side, s_lim[slot]);
+                convert_side4(raw + slot * CODE_BYTES, kvb + slot * PF_TILE16, ctid, side, sh.lim[slot], WIDE && sh.large, &sh.large);
             } else {
                 convert_side<SB>(raw + slot * CODE_BYTES, kvb + slot * PF_TILE16, ctid, scl + ((c >> 1) & 1) * 1024 + side * BLK * SB,
                                  side == 0 ? rsqrtf(float(HD)) : 1.0f);
@@ -511,25 +571,26 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
         }
         if (!ok) {
             atomicExch(p.ctl.err, ERR_WAIT_FULL);
-            *reinterpret_cast<volatile int*>(&s_abort) = 1;
+            *reinterpret_cast<volatile int*>(&sh.abort) = 1;
         }
     } else {
         // ---- ReLU² warps: warpgroup x (warps 4x .. 4x+3) owns tile x, one query row a thread
         const int x = warp >> 2, r = tid & 127;
         const uint32_t lane_sel = uint32_t((warp & 3) * 32) << 16;
-        const uint32_t tS = tmem + 128 * x, tO = tmem + 256 + 128 * x;
-        const int pos_r = p0 + t0[x] + r;               // this row's absolute position
-        const int nx = max(0, min(je, npg[x]) - jb);     // pages of this CTA's range that the tile sees
-        float rowsum = 0.0f;
+        const uint32_t tS = tmem + 128 * x;
+        const int pos_r = p0 + pick(t0, x) + r;               // this row's absolute position
+        const int nx = max(0, min(je, pick(npg, x)) - jb);     // pages of this CTA's range that the tile sees
+        rowsum = 0.0f;
         float rowsum1 = 0.0f;   // (KV4: of the odd keys of unmasked pages)
-        bool ok = true;
+        float smax = 0.0f;      // WIDE: the row's largest score
+        const float g = WIDE && !measure ? factor[x * BLK + r] : 1.0f;
         for (int i = 0; i < nx; i++) {
             const int j = jb + i;
             ok = __all_sync(0xffffffffu, mbar_wait_bounded(p.ctl.wait_cycles, &s_full[x], i & 1) &&
                                              (!QK8 || mbar_wait_bounded(p.ctl.wait_cycles, &kf_ready[i & 1], (i >> 1) & 1)));
             if (!ok) break;   // (warp-uniform: the TMEM loads below are warp-collective)
             tc_fence_after();
-            const bool diag = j * BLK + BLK - 1 > p0 + t0[x];   // some (row, key) of this page is masked
+            const bool diag = j * BLK + BLK - 1 > p0 + pick(t0, x);   // some (row, key) of this page is masked
             // chunk cc + 1 of the row is on its way from TMEM while chunk cc is squared and packed
             uint32_t sbuf[2][32];
             tmem_ld32(tS + lane_sel, sbuf[0]);
@@ -552,7 +613,17 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
                     }
                 }
                 uint32_t pk[16];
-                if (diag) {
+                if (WIDE) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        const int kb = j * BLK + 32 * cc + e;
+                        const float m0 = kb > pos_r ? 0.0f : relu_nan(__uint_as_float(s[e])), m1 = kb + 1 > pos_r ? 0.0f : relu_nan(__uint_as_float(s[e + 1]));
+                        smax = fmaxf(smax, fmaxf(m0, m1));
+                        const float w0 = (m0 * g) * (m0 * g), w1 = (m1 * g) * (m1 * g);
+                        rowsum += w0 + w1;
+                        pk[e >> 1] = pack_h2(w0, w1);
+                    }
+                } else if (diag) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
                         // (KV4: a key that is not a number stays one here too, as in the unmasked pages and in the decode)
@@ -610,8 +681,37 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
         ok = __all_sync(0xffffffffu, ok);   // (warp-uniform: the TMEM loads below are warp-collective)
         if (!ok) {
             atomicExch(p.ctl.err, ERR_WAIT_FULL);
-            *reinterpret_cast<volatile int*>(&s_abort) = 1;
+            *reinterpret_cast<volatile int*>(&sh.abort) = 1;
         }
+        if (WIDE && measure) factor[x * BLK + r] = smax > 0.0f ? pow2_biased(min(max(127 + 6 - (int(__float_as_uint(smax) >> 23) - 127), 1), 254)) : 1.0f;
+    }
+}
+
+// The segment's rows out of TMEM: written, or left for the unit's other ranges.
+template <int DT, bool QK8, bool KV4, bool WIDE>
+__device__ __forceinline__ void prefill_rows(const PrefillParams& p, const PfSegment& sg, const PfPlace& at, PfShared& sh, float rowsum, bool ok) {
+    constexpr float PSCALE = KV4 ? PF4_PSCALE : PF_PSCALE;
+    uint8_t* const smem = at.smem;
+    float* const qsc = at.qsc;
+    const uint32_t tmem = sh.tmem;
+    const int tid = threadIdx.x, warp = tid >> 5;
+    const int h = sg.h, b = sg.b, split = sg.split, nparts = sg.nparts, slot0 = sg.slot0, jb = sg.jb, je = sg.je, unit = at.unit;
+    const int(&t0)[2] = at.t0, (&rows)[2] = at.rows, (&npg)[2] = at.npg;
+    if (warp < 8) {
+        const int x = warp >> 2, r = tid & 127;
+        const uint32_t lane_sel = uint32_t((warp & 3) * 32) << 16;
+        const uint32_t tO = tmem + 256 + 128 * x;
+        const int nx = max(0, min(je, pick(npg, x)) - jb);
+        float unit_of = 1.0f, vunit = 1.0f;   // WIDE: the weights' unit in usual ones, and the products'
+        if (WIDE) {
+            // weights (S g)^2 where the usual ones are (q.k)^2 2^-14; S = q.k 2^-(the row's exponent), 2^-3 with scales an eighth, whose
+            // values are an eighth too
+            const int e = (-14 + 2 * reinterpret_cast<const int*>(qsc)[x * BLK + r] + (sh.large ? 6 : 0)) - 2 * (int(__float_as_uint(at.kfac[x * BLK + r]) >> 23) - 127);
+            unit_of = pow2_biased(min(max(127 + e, 1), 204));   // (fp32 then holds the sums; the sink is nothing beside weights of 2^90)
+            vunit = sh.large ? 8.0f * unit_of : unit_of;
+        }
+        if (WIDE) rowsum *= unit_of;
+        auto from_acc = [&](uint32_t a) { return WIDE ? __uint_as_float(a) * vunit : __uint_as_float(a); };   // in usual units
         if (nparts > 1 && !p.cls) {
             // The page ranges of the unit meet in the scratch (common.metal:88-99). Each range's CTA announces itself on the
             // unit's first counter when its products are complete; all but the last to do so leave their unnormalised O and
@@ -623,9 +723,9 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
             tc_fence_after();
             int* arrived = p.counters + unit;
             int* written = p.counters + p.units + unit;
-            if (tid == 0 && !p.reduce_later) s_last = atomicAdd(arrived, 1) == nparts - 1;
+            if (tid == 0 && !p.reduce_later) sh.last = atomicAdd(arrived, 1) == nparts - 1;
             if (!p.reduce_later) relu_warps_sync();
-            const bool last = !p.reduce_later && s_last != 0;
+            const bool last = !p.reduce_later && sh.last != 0;
             const size_t tstride = size_t(BLK) * (HD + 1);   // floats of a tile's partial: column-major [128 + 1][128 rows]
             if (p.reduce_later) {
                 float* pcol = p.partials + (size_t(slot0 + split) * 2 + x) * tstride + r;
@@ -635,7 +735,7 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
                         uint32_t acc[32];
                         if (nx > 0) tmem_ld32(tO + 32 * cc + lane_sel, acc);
 #pragma unroll
-                        for (int e = 0; e < 32; e++) pcol[size_t(32 * cc + e) * BLK] = nx > 0 ? __uint_as_float(acc[e]) : 0.0f;
+                        for (int e = 0; e < 32; e++) pcol[size_t(32 * cc + e) * BLK] = nx > 0 ? from_acc(acc[e]) : 0.0f;
                     }
                     pcol[size_t(HD) * BLK] = split == 0 ? sqrtf(float(HD)) * PSCALE * (QK8 ? qsc[x * BLK + r] : 1.0f) + rowsum : rowsum;
                 }
@@ -648,7 +748,7 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
                         uint32_t acc[32];
                         if (nx > 0) tmem_ld32(tO + 32 * cc + lane_sel, acc);
 #pragma unroll
-                        for (int e = 0; e < 32; e++) pcol[size_t(32 * cc + e) * BLK] = nx > 0 ? __uint_as_float(acc[e]) : 0.0f;
+                        for (int e = 0; e < 32; e++) pcol[size_t(32 * cc + e) * BLK] = nx > 0 ? from_acc(acc[e]) : 0.0f;
                     }
                     pcol[size_t(HD) * BLK] = rowsum;
                 }
@@ -665,18 +765,18 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
                     }
                     if (!seen) {
                         atomicExch(p.ctl.err, ERR_WAIT_FULL);
-                        *reinterpret_cast<volatile int*>(&s_abort) = 1;
+                        *reinterpret_cast<volatile int*>(&sh.abort) = 1;
                     }
                     *arrived = 0;    // (every range of the unit has been at both counters: they are left at zero for the next launch)
                     *written = 0;
                 }
                 relu_warps_sync();
-                if (ok && !*reinterpret_cast<volatile int*>(&s_abort)) {
+                if (ok && !*reinterpret_cast<volatile int*>(&sh.abort)) {
                     const float* pbase = p.partials + (size_t(slot0) * 2 + x) * tstride + r;   // range 0; range s is 2 tstride x s on
                     float den = sqrtf(float(HD)) * PSCALE * (QK8 ? qsc[x * BLK + r] : 1.0f);
                     for (int sp = 0; sp < nparts; sp++) den += sp == split ? rowsum : __ldcg(pbase + size_t(sp) * 2 * tstride + size_t(HD) * BLK);
                     const float inv = 1.0f / den;
-                    const size_t ooff = size_t(b) * p.o_seq_stride + size_t(t0[x] + r) * p.o_token_stride + size_t(h) * HD;
+                    const size_t ooff = size_t(b) * p.o_seq_stride + size_t(pick(t0, x) + r) * p.o_token_stride + size_t(h) * HD;
                     uint16_t* orow = static_cast<uint16_t*>(p.o) + ooff;
 #pragma unroll 1
                     for (int cc = 0; cc < 4; cc++) {
@@ -687,8 +787,13 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
                         for (int sp = 0; sp < nparts; sp++) {
                             uint32_t v[32];
                             if (sp == split) {
-                                if (nx > 0) tmem_ld32(tO + 32 * cc + lane_sel, v);
-                                else {
+                                if (nx > 0) {
+                                    tmem_ld32(tO + 32 * cc + lane_sel, v);
+                                    if (WIDE) {
+#pragma unroll
+                                        for (int e = 0; e < 32; e++) v[e] = __float_as_uint(from_acc(v[e]));
+                                    }
+                                } else {
 #pragma unroll
                                     for (int e = 0; e < 32; e++) v[e] = 0u;
                                 }
@@ -700,7 +805,7 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
 #pragma unroll
                             for (int e = 0; e < 32; e++) tot[e] += __uint_as_float(v[e]);
                         }
-                        if (r < rows[x]) {
+                        if (r < pick(rows, x)) {
                             uint32_t outw[16];
 #pragma unroll
                             for (int e = 0; e < 32; e += 2) {
@@ -732,23 +837,23 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
                 uint32_t acc[32];
                 if (nx > 0) tmem_ld32(tO + 32 * cc + lane_sel, acc);
 #pragma unroll
-                for (int e = 0; e < 32; e++) prow[32 * cc + e] = nx > 0 ? __uint_as_float(acc[e]) : 0.0f;
+                for (int e = 0; e < 32; e++) prow[32 * cc + e] = nx > 0 ? from_acc(acc[e]) : 0.0f;
             }
             prow[HD] = rowsum;
         } else if (nx > 0) {
             tc_fence_after();
             const float inv = 1.0f / (sqrtf(float(HD)) * PSCALE * (QK8 ? qsc[x * BLK + r] : 1.0f) + rowsum);
-            const size_t ooff = size_t(b) * p.o_seq_stride + size_t(t0[x] + r) * p.o_token_stride + size_t(h) * HD;
+            const size_t ooff = size_t(b) * p.o_seq_stride + size_t(pick(t0, x) + r) * p.o_token_stride + size_t(h) * HD;
             uint16_t* orow = static_cast<uint16_t*>(p.o) + ooff;
 #pragma unroll 1
             for (int cc = 0; cc < 4; cc++) {
                 uint32_t acc[32];
                 tmem_ld32(tO + 32 * cc + lane_sel, acc);
-                if (r < rows[x]) {
+                if (r < pick(rows, x)) {
                     uint32_t outw[16];
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
-                        const float a0 = __uint_as_float(acc[e]) * inv, a1 = __uint_as_float(acc[e + 1]) * inv;
+                        const float a0 = from_acc(acc[e]) * inv, a1 = from_acc(acc[e + 1]) * inv;
                         if (DT == EMBLA_F16) outw[e >> 1] = pack_h2(a0, a1);
                         else {
                             __nv_bfloat162 t = __floats2bfloat162_rn(a0, a1);
@@ -796,7 +901,7 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
             for (int it = tid; it < 2 * R * (HD / 2); it += PF_THREADS) {
                 const int i = it / (HD / 2), c = 2 * (it % (HD / 2));
                 const int x = i / R, r = rank * R + i % R;
-                if (r >= rows[x]) continue;
+                if (r >= pick(rows, x)) continue;
                 const uint32_t at = part0 + uint32_t((x * BLK + r) * (HD + 1) + c) * 4u;
                 float v0[8], v1[8];
 #pragma unroll
@@ -818,7 +923,7 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
                     __nv_bfloat162 t = __floats2bfloat162_rn(a0 * inv, a1 * inv);
                     w = *reinterpret_cast<uint32_t*>(&t);
                 }
-                const size_t off = size_t(b) * p.o_seq_stride + size_t(t0[x] + r) * p.o_token_stride + size_t(h) * HD + c;
+                const size_t off = size_t(b) * p.o_seq_stride + size_t(pick(t0, x) + r) * p.o_token_stride + size_t(h) * HD + c;
                 *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.o) + off) = w;
                 for (int pr = 0; pr < p.n_peers; pr++) *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.o_peer[pr]) + off) = w;
             }
@@ -826,11 +931,75 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
             cluster_wait();
         }
     }
+}
+
+// A segment in the second form, once the first has found that it is needed: out of line, so that the first one's loops are compiled as if
+// it were not there (in one loop with it, 333 tokens of 3 sequences took 32.8 microseconds instead of 26.6).
+template <int DT>
+__device__ __noinline__ void prefill_wide(const CUtensorMap& tmap, const PrefillParams& p, PfShared& sh) {
+    const PfSegment sg = sh.sg;
+    const PfPlace at(p, sg);
+    float rowsum = 0.0f;
+    bool ok = true;
+#pragma unroll 1
+    for (int pass = 0; pass < 2; pass++) {
+        if (threadIdx.x == PF_PRODUCER * 32) {
+            // (every wait of the pass before has ended, so nothing of it is in flight but arrivals on kv_free)
+            for (int i = 0; i < min(3, 2 * at.n); i++)
+                if (!mbar_wait_bounded(p.ctl.wait_cycles, &at.bars[9 + i], ((2 * at.n - i + 2) / 3 - 1) & 1)) atomicExch(p.ctl.err, ERR_WAIT_EMPTY);
+            for (int i = 0; i < PF_BARS; i++) mbar_inval(&at.bars[i]);
+        }
+        prefill_pages<DT, 2, false, true, true>(tmap, p, sg, at, sh, pass == 0, rowsum, ok);
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+        if (*reinterpret_cast<volatile int*>(&sh.abort)) {   // (a wait ran out, and what is in flight is not known)
+            ok = false;
+            break;
+        }
+    }
+    prefill_rows<DT, false, true, true>(p, sg, at, sh, rowsum, ok);
+}
+
+template <int DT, int SB, bool QK8, bool KV4>
+__device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, const PrefillParams& p, const PfSegment sg) {
+    __shared__ PfShared sh;
+    const PfPlace at(p, sg);
+    const int warp = threadIdx.x >> 5;
+    float rowsum = 0.0f;    // (ReLU² warps) the row's sum of weights
+    bool ok = true, wide = false;
+    prefill_pages<DT, SB, QK8, KV4, false>(tmap, p, sg, at, sh, false, rowsum, ok);
+    if (KV4) {
+        bool again = false;
+        if (warp < 8 && ok) {
+            // a weight that fp16 did not hold leaves a large row sum, and an output that is no number (infinity times a zero code, or infinity)
+            again = !(rowsum < PF4_FULL);
+            if (__any_sync(0xffffffffu, again)) {
+                tc_fence_after();
+                bool odd = false;
+#pragma unroll 1
+                for (int cc = 0; cc < 4; cc++) {
+                    uint32_t acc[32];
+                    tmem_ld32(sh.tmem + 256 + 128 * (warp >> 2) + 32 * cc + (uint32_t((warp & 3) * 32) << 16), acc);
+#pragma unroll
+                    for (int e = 0; e < 32; e++) odd |= (acc[e] & 0x7f800000u) == 0x7f800000u;
+                }
+                again &= odd;
+            }
+        }
+        if (threadIdx.x == 0) sh.sg = sg;
+        tc_fence_before();
+        __syncwarp();
+        wide = __syncthreads_or(again) || sh.large;
+        wide = wide && !*reinterpret_cast<volatile int*>(&sh.abort);
+        if (wide) prefill_wide<DT>(tmap, p, sh);
+    }
+    if (!wide) prefill_rows<DT, QK8, KV4, false>(p, sg, at, sh, rowsum, ok);
     tc_fence_before();
     __syncthreads();
     if (warp == PF_MMA) {
         tc_fence_after();
-        tmem_dealloc(tmem, 512);
+        tmem_dealloc(sh.tmem, 512);
     }
 }
 

@@ -36,3 +36,102 @@ def test_prefill_a_key_that_is_not_a_number(dtype, T, at):
     ctx.full_decode(pool, table, torch.tensor([n], dtype=torch.int32, device="cuda"), 1, q[:, -1].contiguous(), d)
     ctx.check()
     assert torch.equal(torch.isnan(d), torch.isnan(o[0, -1:]))
+
+
+# ---- rows of every size, in prefill ------------------------------------------------------------------------------
+def _prefill_case(dtype, Hq, Hkv, pos0, T, seed, kf=None, vf=None, qf=None, gains=False):
+    """A chunk of T tokens at pos0 over rows ~ N(0, 1) times kf / vf [keys] (any size that bf16 holds), queries times qf [T]. Returns outputs [B, T, Hq,
+    128], their values in 64 bits and the bounds."""
+    import torch
+    from embla_metal_b200 import attn
+    rng = np.random.default_rng(seed)
+    B, G = len(pos0), Hq // Hkv
+    S = [p + T for p in pos0]
+    npg = [(s + 127) // 128 for s in S]
+    ctx = attn.Attention(Hq, Hkv, DT[dtype], B, max(npg) * 128)
+    pool = attn.KVPool(1, Hkv, sum(npg), attn.KV_INT4)
+    table = torch.zeros(B, max(npg), dtype=torch.int32, device="cuda")
+    ids = rng.permutation(sum(npg)).astype(np.int32)
+    k, v, at = [], [], 0
+    for b in range(B):
+        pages = np.zeros((Hkv, npg[b], kv4.PAGE), np.uint8)
+        rows = []
+        for side, f in ((0, kf), (1, vf)):
+            x = rng.standard_normal((Hkv, npg[b] * 128, 128))
+            if f is not None:
+                x *= np.broadcast_to(f(np.arange(npg[b] * 128), S[b]), (npg[b] * 128,))[None, :, None]
+            c, s = kv4.quantise(_val(_bits(x, dtype), dtype))
+            rows.append(kv4.values(c, s)[:, :S[b]])
+            pages[..., side * kv4.SIDE:(side + 1) * kv4.SIDE] = kv4.pack(c).reshape(Hkv, npg[b], kv4.SIDE)
+            sc = pages[..., 2 * kv4.SIDE:].reshape(Hkv, npg[b], 128, 16)
+            sc[..., 8 * side:8 * side + 8] = s.view(np.uint8).reshape(Hkv, npg[b], 128, 8)
+            pages[..., 2 * kv4.SIDE:] = sc.reshape(Hkv, npg[b], 2048)
+        blocks = ids[at:at + npg[b]]
+        at += npg[b]
+        table[b, :npg[b]] = torch.from_numpy(blocks)
+        pool.raw()[torch.from_numpy(blocks.astype(np.int64)).cuda(), 0] = torch.from_numpy(pages.transpose(1, 0, 2)).cuda()
+        k.append(rows[0])
+        v.append(rows[1])
+    x = rng.standard_normal((B, T, Hq, 128))
+    if qf is not None:
+        x *= np.broadcast_to(qf(np.arange(T)), (T,))[None, :, None, None]
+    bits = _bits(x, dtype)
+    x, gt = _val(bits, dtype), None
+    if gains:
+        f = kv4.norm_rows32(x)
+        g = [_bits(rng.standard_normal(128) * 0.1 + 3, dtype) for _ in range(2)]
+        for gb in g:
+            f = f * (np.float32(1) + _val(gb, dtype).astype(np.float32))
+        x, gt = _val(_bits(x.astype(np.float32) * f, dtype), dtype), tuple(_act(gb, dtype) for gb in g)
+    o = torch.full((B, T, Hq * 128), 3.0, dtype=ctx.torch_dtype, device="cuda")
+    attn.full_prefill(ctx, pool, table, 0, torch.tensor(pos0, dtype=torch.int32, device="cuda"), _act(bits, dtype).view(B, T, Hq * 128), o, gains=gt)
+    ctx.check()
+    got = _out(o, dtype).reshape(B, T, Hq, 128)
+    want, bound = np.zeros_like(got), np.zeros_like(got)
+    for b in range(B):
+        seen = np.arange(S[b])[None] <= pos0[b] + np.arange(T)[:, None]
+        for h in range(Hq):
+            want[b, :, h], bound[b, :, h] = kv4.relu2(x[b, :, h], k[b][h // G], v[b][h // G], seen, kv4.U16[dtype], wround=4, dot=2.0 ** -11)
+    return got, want, bound
+
+
+SIZES = {
+    "scores past fp16": dict(kf=lambda t, S: 30.0, qf=lambda t: 60.0),
+    "scores of 1e8": dict(kf=lambda t, S: 3000.0, qf=lambda t: 3000.0),
+    "one large query row": dict(kf=lambda t, S: 8.0, qf=lambda t: np.where(t == 100, 3000.0, 1.0)),
+    "one large key in the chunk": dict(kf=lambda t, S: np.where(t == S - 30, 10000.0, 1.0), qf=lambda t: 8.0),
+    "one large key ahead of it": dict(kf=lambda t, S: np.where(t == 3, 10000.0, 1.0), qf=lambda t: 8.0),
+    "values near the type's largest": dict(vf=lambda t, S: 12000.0),
+    "small queries beside large ones": dict(kf=lambda t, S: 100.0, qf=lambda t: np.where(t % 2, 1000.0, 1e-3)),
+}
+SIZES_BF16 = {
+    "queries past fp16": dict(qf=lambda t: 1e8),
+    "keys and values past fp16": dict(kf=lambda t, S: 1e5, vf=lambda t, S: 1e5),
+    "one value past fp16 in the chunk": dict(vf=lambda t, S: np.where(t == S - 2, 1e5, 1.0)),
+    "all of it": dict(kf=lambda t, S: 1e5, vf=lambda t, S: 1e5, qf=lambda t: 1e6),
+}
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("what", list(SIZES) + list(SIZES_BF16))
+@pytest.mark.parametrize("Hq,Hkv,pos0,T", [(2, 1, [300, 0], 333), (8, 2, [3000], 200), (4, 1, [9000], 40)])
+def test_prefill_rows_of_every_size(dtype, what, Hq, Hkv, pos0, T):
+    """Scores whose squares, and rows that fp16 does not hold, with whole chunks, and page ranges in clusters and through the scratch."""
+    if dtype == "f16" and what in SIZES_BF16:
+        return
+    got, want, bound = _prefill_case(dtype, Hq, Hkv, pos0, T, 5, **{**SIZES, **SIZES_BF16}[what])
+    keep = np.abs(want) < 65504.0 * (1 - 2.0 ** -9) if dtype == "f16" else np.ones(want.shape, bool)   # (what the output type holds)
+    assert keep.mean() > 0.9
+    _within(np.where(keep, got, 0), np.where(keep, want, 0), bound, what)
+    # as a whole: 2^-11 for each of key, value, weight and output (the weight's key twice), at most doubled, and bf16's own half step
+    some = np.abs(want).max(-1) > 0                        # (a token at position 0 whose only score is negative has zeros)
+    rms = np.sqrt((np.where(keep, got - want, 0)[some] ** 2).sum(-1) / (np.where(keep, want, 0)[some] ** 2).sum(-1))
+    assert np.median(rms) < (2.0 ** -10 if dtype == "f16" else 2.0 ** -8.5), np.median(rms)
+
+
+@pytest.mark.parametrize("Hq,Hkv,pos0,T", [(8, 2, [6000], 1024), (2, 1, [12000], 700)])
+def test_prefill_large_rows_shared_among_ctas(Hq, Hkv, pos0, T):
+    """Large keys in some page ranges of a unit and none in others, and gains that make large queries."""
+    got, want, bound = _prefill_case("bf16", Hq, Hkv, pos0, T, 6, kf=lambda t, S: np.where(t % 1500 == 77, 3000.0, 1.0),
+                                     vf=lambda t, S: np.where(t == S - 1000, 1e5, 1.0), gains=True)
+    _within(got, want, bound, "rows")
