@@ -117,15 +117,16 @@ __device__ __forceinline__ void convert_side(const uint8_t* raw, uint8_t* dst, i
 }
 
 // 4-bit pages (EMBLA_KV_INT4, kv4.cuh): the same kernel with other converters. A group's 16 bytes of codes become 32 fp16 values,
-// code x scale rounded once (2^-11); queries enter scaled by 2^-7 and the keys without 1 / sqrt(D), whose square, 2^-7, is exact
-// in the weights: P = relu(s)^2 comes out as the weight x 2^-7 (scores up to 2895 square inside fp16's range), the sink takes
-// the same factor. 2048 tokens at 30720: 431 us, 1236 TFLOP/s (0.75 of the measured burst rate; the int8 pages take 449 us).
-// What does not fit in fp16 so (a score above 2895, a scale of 8192 or more, a bf16 query above 8.4e6) is seen once the range's products are
+// code x scale rounded once (2^-11); queries enter scaled by 2^-5 and the keys without 1 / sqrt(D), whose square, 2^-7, is exact
+// in the weights: P = relu(s)^2 comes out as the weight x 2^-3 (scores up to 724 square inside fp16's range, and fp16's smallest step keeps
+// the weights to 2^-22: with 2^-7 for the queries it was 2895 and 2^-18, and rows whose scores are all about 0.01 came out 1.2 % off), the
+// sink takes the same factor. 2048 tokens at 30720: 431 us, 1236 TFLOP/s (0.75 of the measured burst rate; the int8 pages take 449 us).
+// What does not fit in fp16 so (a score above 724, a scale of 8192 or more, a bf16 query above 2e6) is seen once the range's products are
 // done, and the CTA then takes its pages twice more: with every query row scaled by a power of two that brings its largest element into
 // [1, 2), once for the largest score of each row and once with the scores under the power of two that brings that one into [64, 128).
 // Sums and outputs leave in the usual units, so what the other ranges of a unit did makes no difference. Three times the time, for rows
 // that fp16 would have made infinite; all others pay one barrier.
-constexpr float PF4_QSCALE = 1.0f / 128.0f, PF4_PSCALE = 1.0f / 128.0f;
+constexpr float PF4_QSCALE = 1.0f / 32.0f, PF4_PSCALE = 1.0f / 8.0f;
 constexpr float PF4_FULL = 65504.0f;   // a row sum below it has no weight that fp16 does not hold
 
 // One side of a raw 4-bit page -> fp16 in the UMMA layout; rows from `lim` on (behind the last key, or all of a page that is
@@ -704,9 +705,9 @@ __device__ __forceinline__ void prefill_rows(const PrefillParams& p, const PfSeg
         const int nx = max(0, min(je, pick(npg, x)) - jb);
         float unit_of = 1.0f, vunit = 1.0f;   // WIDE: the weights' unit in usual ones, and the products'
         if (WIDE) {
-            // weights (S g)^2 where the usual ones are (q.k)^2 2^-14; S = q.k 2^-(the row's exponent), 2^-3 with scales an eighth, whose
+            // weights (S g)^2 where the usual ones are (q.k)^2 2^-10; S = q.k 2^-(the row's exponent), 2^-3 with scales an eighth, whose
             // values are an eighth too
-            const int e = (-14 + 2 * reinterpret_cast<const int*>(qsc)[x * BLK + r] + (sh.large ? 6 : 0)) - 2 * (int(__float_as_uint(at.kfac[x * BLK + r]) >> 23) - 127);
+            const int e = (-10 + 2 * reinterpret_cast<const int*>(qsc)[x * BLK + r] + (sh.large ? 6 : 0)) - 2 * (int(__float_as_uint(at.kfac[x * BLK + r]) >> 23) - 127);
             unit_of = pow2_biased(min(max(127 + e, 1), 204));   // (fp32 then holds the sums; the sink is nothing beside weights of 2^90)
             vunit = sh.large ? 8.0f * unit_of : unit_of;
         }

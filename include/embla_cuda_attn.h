@@ -377,8 +377,8 @@ EmblaStatus embla_attn_sliding_prefill(EmblaAttn* ctx, const EmblaRing* ring, co
  * elements and must be multiples of 8. Runs on tcgen05 tensor cores with fp32 accumulation in TMEM. Int8 and 4-bit
  * pools; over a 4-bit one q_dev and o_dev must be 16-byte aligned, and a cached value that is not a number reaches every
  * token of the chunk, those ahead of it among them (masked weights are zeros, and zero times it is not one). Over a 4-bit pool rows
- * of any size are served, scores to 2^48; where one passes 2895, a scale 8192 or a query 8.4e6, the 256 tokens of the head take three times
- * as long. (Int8: scores to 2047.) */
+ * of any size are served, scores to 2^48, weights (scores squared) kept to 2^-22; where a score passes 724, a scale 8192 or a query 2e6,
+ * the 256 tokens of the head take three times as long. (Int8: scores to 2047, weights to 2^-19.) */
 EmblaStatus embla_attn_full_prefill(EmblaAttn* ctx, const EmblaKVPool* pool, const EmblaKVView* view,
                                     const int32_t* pos0_dev, int32_t n_tokens, const EmblaQuery* q,
                                     int64_t q_token_stride, void* o_dev, int64_t o_token_stride,

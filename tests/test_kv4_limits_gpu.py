@@ -135,3 +135,17 @@ def test_prefill_large_rows_shared_among_ctas(Hq, Hkv, pos0, T):
     got, want, bound = _prefill_case("bf16", Hq, Hkv, pos0, T, 6, kf=lambda t, S: np.where(t % 1500 == 77, 3000.0, 1.0),
                                      vf=lambda t, S: np.where(t == S - 1000, 1e5, 1.0), gains=True)
     _within(got, want, bound, "rows")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("Hq,Hkv,pos0,T", [(2, 1, [300, 0], 333), (8, 2, [3000], 200)])
+def test_prefill_small_rows(dtype, Hq, Hkv, pos0, T):
+    """Scores of about 0.01, all of them: the weights, of 1e-4, keep their leading bits."""
+    got, want, bound = _prefill_case(dtype, Hq, Hkv, pos0, T, 5, kf=lambda t, S: 1e-2)
+    # beside the other roundings a weight is off by half of fp16's smallest step, 2^-25 x 2^3, times a value of 6 or less and the keys seen
+    seen = np.stack([p + 1 + np.arange(T) for p in pos0])[:, :, None, None]
+    _within(got, want, bound + seen * 6 * 2.0 ** -22 / np.sqrt(128.0), "small rows")
+    # as a whole, for the tokens that see many: 2^-22 of 1e-4 at random is 2^-9.5 at most, halved by the rounding's distribution
+    late = np.arange(T) > T // 2
+    rms = np.sqrt(((got - want)[:, late] ** 2).mean() / (want[:, late] ** 2).mean())
+    assert rms < (2.0 ** -9 if dtype == "f16" else 2.0 ** -8), rms
