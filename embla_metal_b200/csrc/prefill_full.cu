@@ -132,8 +132,10 @@ constexpr float PF4_FULL = 65504.0f;   // a row sum below it has no weight that 
 // One side of a raw 4-bit page -> fp16 in the UMMA layout; rows from `lim` on (behind the last key, or all of a page that is
 // nowhere) become zeros, whatever lies there. 128 converter threads; the lanes of a quarter warp take 8 consecutive rows of one
 // group, so reads and writes are conflict-free. A scale whose products may leave fp16 sets *large; values an eighth of their size with
-// `eighth`.
-__device__ __forceinline__ void convert_side4(const uint8_t* raw, uint8_t* dst, int ctid, int side, int lim, bool eighth, volatile int* large) {
+// `eighth`. A value group that is not a number becomes zeros, with its position left in nan_from[group] if it is the first (`first`: that of
+// the page's row 0): a token that does not see it would have zero times it, a NaN, in its sum.
+__device__ __forceinline__ void convert_side4(const uint8_t* raw, uint8_t* dst, int ctid, int side, int lim, bool eighth, volatile int* large,
+                                              int* nan_from, int first) {
     const int rl = ctid & 7, g = (ctid >> 3) & 3, rg = ctid >> 5;
     const __half* scales = reinterpret_cast<const __half*>(raw + KV4_SIDE) + side * KV4_GROUPS + g;
 #pragma unroll
@@ -146,7 +148,14 @@ __device__ __forceinline__ void convert_side4(const uint8_t* raw, uint8_t* dst, 
             sc = __half2half2(__ushort_as_half(0));
         }
         const uint32_t bits = __half_as_ushort(__low2half(sc)) & 0x7fffu;
-        if (bits >= 0x7000u && bits < 0x7c00u) *large = 1;   // 8192 .. 65504
+        if (bits >= 0x7000u) {
+            if (bits < 0x7c00u) {
+                *large = 1;   // 8192 .. 65504
+            } else if (side == 1) {
+                atomicMin(&nan_from[g], first + row);
+                sc = __half2half2(__ushort_as_half(0));
+            }
+        }
         if (eighth) sc = __hmul2(sc, __float2half2_rn(0.125f));
         const uint32_t x[4] = {w.x, w.y, w.z, w.w}, s2 = *reinterpret_cast<const uint32_t*>(&sc);
         // dims 32 g .. 32 g + 31: four 16-byte chunks of the half (dims 0-63 | 64-127) that the group lies in
@@ -220,6 +229,7 @@ struct PfShared {
     PfSegment sg;           // KV4: for prefill_wide
     volatile int lim[3];    // KV4: keys that count in the page side of each ring slot
     volatile int large;     // KV4: a scale of 8192 or more
+    int nan_from[KV4_GROUPS];   // KV4: the first position whose value group is not a number
 };
 constexpr int PF_BARS = 19;
 
@@ -263,7 +273,10 @@ __device__ __forceinline__ void prefill_pages(const CUtensorMap& tmap, const Pre
         mbar_init(&kf_ready[1], PF_CONV_WARPS);
         if (!WIDE) {
             sh.abort = 0;
-            if (KV4) sh.large = 0;
+            if (KV4) {
+                sh.large = 0;
+                for (int i = 0; i < KV4_GROUPS; i++) sh.nan_from[i] = 0x7fffffff;
+            }
         }
         fence_barrier_init();
     }
@@ -557,7 +570,8 @@ __device__ __forceinline__ void prefill_pages(const CUtensorMap& tmap, const Pre
                         (SB == 4 ? reinterpret_cast<const float*>(ksc)[ctid] : __half2float(reinterpret_cast<const __half*>(ksc)[ctid])) *
                         (rsqrtf(float(HD)) * PF_QK8_C0);
             } else if (KV4) {
-                convert_side4(raw + slot * CODE_BYTES, kvb + slot * PF_TILE16, ctid, side, sh.lim[slot], WIDE && sh.large, &sh.large);
+                convert_side4(raw + slot * CODE_BYTES, kvb + slot * PF_TILE16, ctid, side, sh.lim[slot], WIDE && sh.large, &sh.large, sh.nan_from,
+                              (jb + (c >> 1)) * BLK);
             } else {
                 convert_side<SB>(raw + slot * CODE_BYTES, kvb + slot * PF_TILE16, ctid, scl + ((c >> 1) & 1) * 1024 + side * BLK * SB,
                                  side == 0 ? rsqrtf(float(HD)) : 1.0f);
@@ -712,7 +726,11 @@ __device__ __forceinline__ void prefill_rows(const PrefillParams& p, const PfSeg
             vunit = sh.large ? 8.0f * unit_of : unit_of;
         }
         if (WIDE) rowsum *= unit_of;
-        auto from_acc = [&](uint32_t a) { return WIDE ? __uint_as_float(a) * vunit : __uint_as_float(a); };   // in usual units
+// O of group cc of the row in usual units; NaN from its first value on that is one
+        auto from_acc = [&](uint32_t a, int cc) {
+            if (!KV4) return __uint_as_float(a);
+            return __uint_as_float(a) * (at.p0 + pick(t0, x) + r >= sh.nan_from[cc] ? __uint_as_float(0x7fffffffu) : vunit);
+        };
         if (nparts > 1 && !p.cls) {
             // The page ranges of the unit meet in the scratch (common.metal:88-99). Each range's CTA announces itself on the
             // unit's first counter when its products are complete; all but the last to do so leave their unnormalised O and
@@ -736,7 +754,7 @@ __device__ __forceinline__ void prefill_rows(const PrefillParams& p, const PfSeg
                         uint32_t acc[32];
                         if (nx > 0) tmem_ld32(tO + 32 * cc + lane_sel, acc);
 #pragma unroll
-                        for (int e = 0; e < 32; e++) pcol[size_t(32 * cc + e) * BLK] = nx > 0 ? from_acc(acc[e]) : 0.0f;
+                        for (int e = 0; e < 32; e++) pcol[size_t(32 * cc + e) * BLK] = nx > 0 ? from_acc(acc[e], cc) : 0.0f;
                     }
                     pcol[size_t(HD) * BLK] = split == 0 ? sqrtf(float(HD)) * PSCALE * (QK8 ? qsc[x * BLK + r] : 1.0f) + rowsum : rowsum;
                 }
@@ -749,7 +767,7 @@ __device__ __forceinline__ void prefill_rows(const PrefillParams& p, const PfSeg
                         uint32_t acc[32];
                         if (nx > 0) tmem_ld32(tO + 32 * cc + lane_sel, acc);
 #pragma unroll
-                        for (int e = 0; e < 32; e++) pcol[size_t(32 * cc + e) * BLK] = nx > 0 ? from_acc(acc[e]) : 0.0f;
+                        for (int e = 0; e < 32; e++) pcol[size_t(32 * cc + e) * BLK] = nx > 0 ? from_acc(acc[e], cc) : 0.0f;
                     }
                     pcol[size_t(HD) * BLK] = rowsum;
                 }
@@ -790,9 +808,9 @@ __device__ __forceinline__ void prefill_rows(const PrefillParams& p, const PfSeg
                             if (sp == split) {
                                 if (nx > 0) {
                                     tmem_ld32(tO + 32 * cc + lane_sel, v);
-                                    if (WIDE) {
+                                    if (KV4) {
 #pragma unroll
-                                        for (int e = 0; e < 32; e++) v[e] = __float_as_uint(from_acc(v[e]));
+                                        for (int e = 0; e < 32; e++) v[e] = __float_as_uint(from_acc(v[e], cc));
                                     }
                                 } else {
 #pragma unroll
@@ -838,7 +856,7 @@ __device__ __forceinline__ void prefill_rows(const PrefillParams& p, const PfSeg
                 uint32_t acc[32];
                 if (nx > 0) tmem_ld32(tO + 32 * cc + lane_sel, acc);
 #pragma unroll
-                for (int e = 0; e < 32; e++) prow[32 * cc + e] = nx > 0 ? from_acc(acc[e]) : 0.0f;
+                for (int e = 0; e < 32; e++) prow[32 * cc + e] = nx > 0 ? from_acc(acc[e], cc) : 0.0f;
             }
             prow[HD] = rowsum;
         } else if (nx > 0) {
@@ -854,7 +872,7 @@ __device__ __forceinline__ void prefill_rows(const PrefillParams& p, const PfSeg
                     uint32_t outw[16];
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
-                        const float a0 = from_acc(acc[e]) * inv, a1 = from_acc(acc[e + 1]) * inv;
+                        const float a0 = from_acc(acc[e], cc) * inv, a1 = from_acc(acc[e + 1], cc) * inv;
                         if (DT == EMBLA_F16) outw[e >> 1] = pack_h2(a0, a1);
                         else {
                             __nv_bfloat162 t = __floats2bfloat162_rn(a0, a1);

@@ -375,9 +375,8 @@ EmblaStatus embla_attn_sliding_prefill(EmblaAttn* ctx, const EmblaRing* ring, co
  * runs kv_append_b first). Token t's query head h is at q_dev[b * q->q_stride + t * q_token_stride +
  * h * 128]; out is token-major, o_dev[b * o_seq_stride + t * o_token_stride + h * 128]. Strides are in
  * elements and must be multiples of 8. Runs on tcgen05 tensor cores with fp32 accumulation in TMEM. Int8 and 4-bit
- * pools; over a 4-bit one q_dev and o_dev must be 16-byte aligned, and a cached value that is not a number reaches every
- * token of the chunk, those ahead of it among them (masked weights are zeros, and zero times it is not one). Over a 4-bit pool rows
- * of any size are served, scores to 2^48, weights (scores squared) kept to 2^-22; where a score passes 724, a scale 8192 or a query 2e6,
+ * pools; over a 4-bit one q_dev and o_dev must be 16-byte aligned. Over a 4-bit pool a cached key or value that is not a
+ * number reaches the tokens from its position on, as in the decode, and none ahead of it; rows of any size are served, scores to 2^48, weights (scores squared) kept to 2^-22; where a score passes 724, a scale 8192 or a query 2e6,
  * the 256 tokens of the head take three times as long. (Int8: scores to 2047, weights to 2^-19.) */
 EmblaStatus embla_attn_full_prefill(EmblaAttn* ctx, const EmblaKVPool* pool, const EmblaKVView* view,
                                     const int32_t* pos0_dev, int32_t n_tokens, const EmblaQuery* q,

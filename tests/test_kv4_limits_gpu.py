@@ -38,6 +38,35 @@ def test_prefill_a_key_that_is_not_a_number(dtype, T, at):
     assert torch.equal(torch.isnan(d), torch.isnan(o[0, -1:]))
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("T,at,p0", [(1, 299, 299), (40, 259, 260), (40, 259, 230), (40, 128, 260), (300, 0, 0), (300, 130, 0), (300, 255, 0),
+                                     (300, 299, 0), (200, 3100, 3000), (600, 3300, 2900)])
+def test_prefill_a_value_that_is_not_a_number(dtype, T, at, p0):
+    """A NaN in one value row of the second kv head: its group of 32 dims is NaN in every token from that position on, and in nothing else: not in the
+    tokens ahead of it, whose masked weights are zeros, and not in what the rest of the row gives."""
+    import torch
+    from embla_metal_b200 import attn
+    Hq, Hkv, n = 4, 2, p0 + T
+    rng, ctx, pool, table, k, v = _setup(dtype, Hq, Hkv, [n], at + T)
+    row = torch.ones(1, 1, Hkv * 128, dtype=ctx.torch_dtype, device="cuda")
+    bad = row.clone()
+    bad[0, 0, 128 + 70] = float("nan")
+    q = _act(_bits(rng.standard_normal((1, T, Hq * 128)), dtype), dtype)
+    pos = torch.tensor([p0], dtype=torch.int32, device="cuda")
+    outs = []
+    for x in (row, bad):
+        ctx.kv_append(pool, table, 1, torch.tensor([at], dtype=torch.int32, device="cuda"), row, x, norm_k=False)
+        o = torch.zeros_like(q)
+        attn.full_prefill(ctx, pool, table, 1, pos, q, o)
+        ctx.check()
+        outs.append(o[0].float().view(T, Hkv, Hq // Hkv, 4, 32).cpu().numpy())
+    want = np.zeros(outs[0].shape, bool)
+    want[np.arange(p0, n) >= at, 1, :, 70 // 32] = True
+    assert np.isfinite(outs[0]).all()
+    assert np.array_equal(np.isnan(outs[1]), want)
+    assert np.array_equal(outs[0][~want], outs[1][~want])
+
+
 # ---- rows of every size, in prefill ------------------------------------------------------------------------------
 def _prefill_case(dtype, Hq, Hkv, pos0, T, seed, kf=None, vf=None, qf=None, gains=False):
     """A chunk of T tokens at pos0 over rows ~ N(0, 1) times kf / vf [keys] (any size that bf16 holds), queries times qf [T]. Returns outputs [B, T, Hq,
