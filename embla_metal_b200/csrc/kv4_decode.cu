@@ -16,8 +16,8 @@
 // therefore keeps its weights as w' = relu(S)^2 f with a power of two f per head: when a weight of a tile passes LIMIT (tested
 // with one vote a tile), f drops so that the tile's largest is TARGET or below, and the sums kept so far are scaled by the same power
 // of two, exactly. Before the first key f is 2^120, so the first tile sets it. Weights between 2^10 and 2^13 at the top of
-// their range leave 2^-24 / 2^10 of the largest as the smallest step; scales of 2 and more (values above 14) switch the
-// warp to LIMIT 1/2, which no scale can push out of fp16.
+// their range leave 2^-24 / 2^10 of the largest as the smallest step. A tile with a value scale of 8 or more (values above 56), whose
+// product with a weight fp16 may not hold, takes its products in two bf16 parts (kv4_tile_values_wide).
 #include <cstdlib>
 
 #include "kv4_tile.cuh"
@@ -49,8 +49,8 @@ __device__ __forceinline__ bool bar_any(int id, int threads, bool yes) {
 
 constexpr int KD_PART = HD + 4;                                    // floats per (range, head): 128 sums, sum of weights
 constexpr int KD_SUM = HD + 1;   // a row of a warp's sums in shared memory: lanes (r, t) write heads 2t at dims 8 (r / 2) + r % 2: 32 banks
-constexpr float KD_LIMIT = 8192.0f, KD_LIMIT_BIG = 0.5f;           // largest weight kept, usually and with large value scales
-constexpr int KD_TARGET = 10, KD_TARGET_BIG = -4;                  // log2 of the bound a new f puts on the tile's weights
+constexpr float KD_LIMIT = 8192.0f;                                // largest weight kept
+constexpr int KD_TARGET = 10;                                      // log2 of the bound a new f puts on the tile's weights
 constexpr int KD_MAX_CLUSTER = 8;
 // What a unit costs beside its pages, in pages (16 uneven sequences of up to 9001 keys: 29.0 us counting 4, 31.7 counting 2, 39 none).
 constexpr int KD_UNIT_COST = 4;
@@ -476,8 +476,6 @@ __global__ void __launch_bounds__((NCONS + 1 + KD_HELPERS) * 32, 1)
                 for (int i = 0; i < 8; i++) O[i][0] = O[i][1] = O[i][2] = O[i][3] = 0.0f;
                 float ps0 = 0.0f, ps1 = 0.0f;                       // sums of the kept weights of heads 2t, 2t + 1
                 float f0 = pow2_biased(247), f1 = pow2_biased(247); // their factors (2^120: nothing seen yet)
-                bool big = false;
-                float limit = KD_LIMIT;
 #pragma unroll 1
                 for (; mine < piece0 + n; mine += GROUPS) {
                     ok = __all_sync(0xffffffffu, mbar_wait_bounded(p.ctl.wait_cycles, &full[st], phase));
@@ -532,50 +530,52 @@ __global__ void __launch_bounds__((NCONS + 1 + KD_HELPERS) * 32, 1)
                                     top = fmaxf(top, w[k][e]);
                                 }
                             }
-                            if (__any_sync(0xffffffffu, top > limit || (flagged && !big))) {
-                                // (a handful of times a warp) new factors: the tiles' largest weight of a head at most 2^target
-                                if (__any_sync(0xffffffffu, flagged)) {
-                                    big = true;
-                                    limit = KD_LIMIT_BIG;
+                            bool wide = false;
+                            if (__any_sync(0xffffffffu, top > KD_LIMIT || flagged)) {
+#pragma unroll
+                                for (int k = 0; k < STEP; k++) wide |= rows[k].wide();
+                                wide = __any_sync(0xffffffffu, wide);
+                                if (__any_sync(0xffffffffu, top > KD_LIMIT)) {
+                                    // (a handful of times a warp) new factors: the tiles' largest weight of a head at most 2^target
+                                    float m0 = 0.0f, m1 = 0.0f;
+#pragma unroll
+                                    for (int k = 0; k < STEP; k++) {
+                                        m0 = fmaxf(m0, fmaxf(s[k][0], s[k][2]));
+                                        m1 = fmaxf(m1, fmaxf(s[k][1], s[k][3]));
+                                    }
+#pragma unroll
+                                    for (int o = 4; o < 32; o <<= 1) {
+                                        m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
+                                        m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+                                    }
+                                    // m < 2^(e + 1), so m^2 2^(target - 2 (e + 1)) < 2^target
+                                    const int e0 = int(__float_as_uint(m0) >> 23) - 126, e1 = int(__float_as_uint(m1) >> 23) - 126;
+                                    const float nf0 = m0 * f0 * m0 > KD_LIMIT ? pow2_biased(min(max(127 + KD_TARGET - 2 * e0, 1), 254)) : f0;
+                                    const float nf1 = m1 * f1 * m1 > KD_LIMIT ? pow2_biased(min(max(127 + KD_TARGET - 2 * e1, 1), 254)) : f1;
+                                    const float c0 = nf0 / f0, c1 = nf1 / f1;
+                                    f0 = nf0;
+                                    f1 = nf1;
+                                    ps0 *= c0;
+                                    ps1 *= c1;
+#pragma unroll
+                                    for (int k = 0; k < 8; k++) {
+                                        O[k][0] *= c0;
+                                        O[k][1] *= c1;
+                                        O[k][2] *= c0;
+                                        O[k][3] *= c1;
+                                    }
+#pragma unroll
+                                    for (int k = 0; k < STEP; k++)
+#pragma unroll
+                                        for (int e = 0; e < 4; e++) w[k][e] = s[k][e] * ((e & 1) ? f1 : f0) * s[k][e];
                                 }
-                                const int target = big ? KD_TARGET_BIG : KD_TARGET;
-                                float m0 = 0.0f, m1 = 0.0f;
-#pragma unroll
-                                for (int k = 0; k < STEP; k++) {
-                                    m0 = fmaxf(m0, fmaxf(s[k][0], s[k][2]));
-                                    m1 = fmaxf(m1, fmaxf(s[k][1], s[k][3]));
-                                }
-#pragma unroll
-                                for (int o = 4; o < 32; o <<= 1) {
-                                    m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
-                                    m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
-                                }
-                                // m < 2^(e + 1), so m^2 2^(target - 2 (e + 1)) < 2^target
-                                const int e0 = int(__float_as_uint(m0) >> 23) - 126, e1 = int(__float_as_uint(m1) >> 23) - 126;
-                                const float nf0 = m0 * f0 * m0 > limit ? pow2_biased(min(max(127 + target - 2 * e0, 1), 254)) : f0;
-                                const float nf1 = m1 * f1 * m1 > limit ? pow2_biased(min(max(127 + target - 2 * e1, 1), 254)) : f1;
-                                const float c0 = nf0 / f0, c1 = nf1 / f1;
-                                f0 = nf0;
-                                f1 = nf1;
-                                ps0 *= c0;
-                                ps1 *= c1;
-#pragma unroll
-                                for (int k = 0; k < 8; k++) {
-                                    O[k][0] *= c0;
-                                    O[k][1] *= c1;
-                                    O[k][2] *= c0;
-                                    O[k][3] *= c1;
-                                }
-#pragma unroll
-                                for (int k = 0; k < STEP; k++)
-#pragma unroll
-                                    for (int e = 0; e < 4; e++) w[k][e] = s[k][e] * ((e & 1) ? f1 : f0) * s[k][e];
                             }
 #pragma unroll
                             for (int k = 0; k < STEP; k++) {
                                 ps0 += w[k][0] + w[k][2];
                                 ps1 += w[k][1] + w[k][3];
-                                kv4_tile_values<DT>(kaddr + KV4_SIDE + k * 16 * KV4_ROW, rows[k], w[k], O);
+                                if (!wide) kv4_tile_values<DT>(kaddr + KV4_SIDE + k * 16 * KV4_ROW, rows[k], w[k], O);
+                                else kv4_tile_values_wide(kaddr + KV4_SIDE + k * 16 * KV4_ROW, rows[k], w[k], O);
                             }
                         }
                     }

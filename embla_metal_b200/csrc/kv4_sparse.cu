@@ -20,8 +20,8 @@ constexpr int KS_WARPS = 4, KS_STAGES = 2, KS_ROWS = 32;   // (three stages leav
 constexpr int KS_STAGE = KS_ROWS * (2 * KV4_ROW + 4 * KV4_GROUPS);   // a group's rows: K codes, V codes, scales: 4608 bytes
 constexpr int KS_SUM = HD + 1, KS_PART = HD + 4;                     // floats of a row of sums: in shared memory, between CTAs
 constexpr int KS_MAX_CLUSTER = 8;
-// largest weight, and the one a moved reference gives the row's largest score; the second pair with value scales of 2 and more
-constexpr float KS_LIMIT = 8192.0f, KS_LIMIT_BIG = 0.5f, KS_TARGET = 10.0f, KS_TARGET_BIG = -4.0f;
+// largest weight, and the log2 of the one a moved reference gives the row's largest score (large value scales: kv4_tile_values_wide)
+constexpr float KS_LIMIT = 8192.0f, KS_TARGET = 10.0f;
 constexpr int KS_MAX_GROUPS = (EMBLA_TOPK + EMBLA_RECENT) / KS_ROWS / KS_WARPS;   // of a warp, in a CTA that has all rows to itself
 constexpr uint32_t KS_NOWHERE = 0xffffffffu;
 constexpr float KS_NONE = -1e30f;                                    // a reference before any key
@@ -150,8 +150,6 @@ __global__ void __launch_bounds__(KS_WARPS * 32, 4) kv4_sparse_kernel(const __gr
 #pragma unroll
     for (int i = 0; i < 8; i++) O[i][0] = O[i][1] = O[i][2] = O[i][3] = 0.0f;
     float l0 = 0.0f, l1 = 0.0f, m0 = KS_NONE, m1 = KS_NONE;   // sums of weights, reference scores of heads 2t, 2t + 1
-    bool big = false;
-    float limit = KS_LIMIT;
 #pragma unroll 1
     for (int i = 0; first + i * step < groups; i++) {
         request(i + KS_STAGES - 1);
@@ -184,12 +182,10 @@ __global__ void __launch_bounds__(KS_WARPS * 32, 4) kv4_sparse_kernel(const __gr
         };
         weigh();
         flagged = sc[0].large() || sc[1].large();
-        if (__any_sync(0xffffffffu, top > limit || (flagged && !big))) {
+        bool wide = false;
+        if (__any_sync(0xffffffffu, flagged)) wide = __any_sync(0xffffffffu, sc[0].wide() || sc[1].wide());
+        if (__any_sync(0xffffffffu, top > KS_LIMIT)) {
             // new references, no lower than the old: the group's largest score of a head weighs 2^target or less
-            if (__any_sync(0xffffffffu, flagged)) {
-                big = true;
-                limit = KS_LIMIT_BIG;
-            }
             float t0 = KS_NONE, t1 = KS_NONE;
 #pragma unroll
             for (int k = 0; k < 2; k++) {
@@ -202,8 +198,7 @@ __global__ void __launch_bounds__(KS_WARPS * 32, 4) kv4_sparse_kernel(const __gr
                 t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
                 t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
             }
-            const float target = big ? KS_TARGET_BIG : KS_TARGET;
-            const float n0 = fmaxf(m0, t0 - target), n1 = fmaxf(m1, t1 - target);
+            const float n0 = fmaxf(m0, t0 - KS_TARGET), n1 = fmaxf(m1, t1 - KS_TARGET);
             const float c0 = ks_exp2(m0 - n0), c1 = ks_exp2(m1 - n1);
             m0 = n0;
             m1 = n1;
@@ -222,7 +217,8 @@ __global__ void __launch_bounds__(KS_WARPS * 32, 4) kv4_sparse_kernel(const __gr
         for (int k = 0; k < 2; k++) {
             l0 += w[k][0] + w[k][2];
             l1 += w[k][1] + w[k][3];
-            kv4_tile_values<DT>(kaddr + KS_ROWS * KV4_ROW + k * 16 * KV4_ROW, sc[k], w[k], O);
+            if (!wide) kv4_tile_values<DT>(kaddr + KS_ROWS * KV4_ROW + k * 16 * KV4_ROW, sc[k], w[k], O);
+            else kv4_tile_values_wide(kaddr + KS_ROWS * KV4_ROW + k * 16 * KV4_ROW, sc[k], w[k], O);
         }
         __syncwarp();   // (the stage is read: the next turn's copies go into it)
     }

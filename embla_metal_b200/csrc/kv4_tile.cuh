@@ -123,8 +123,12 @@ struct Kv4Scales {
         k0 = *reinterpret_cast<const uint4*>(sc + (lane >> 2) * 16);
         k1 = *reinterpret_cast<const uint4*>(sc + ((lane >> 2) + 8) * 16);
     }
-    // some value scale of 2 or more (its product with a weight of 2^13 could leave fp16)
+    // some value scale of 2 or more (one test of a bit), and of 8 or more or NaN: its product with a weight of 2^13 could leave fp16
     __device__ __forceinline__ bool large() const { return ((k0.z | k0.w | k1.z | k1.w) & 0x40004000u) != 0; }
+    __device__ __forceinline__ bool wide() const {
+        const uint32_t top = __vmaxu2(__vmaxu2(k0.z, k0.w), __vmaxu2(k1.z, k1.w));
+        return (top & 0xffffu) >= 0x4800u || (top >> 16) >= 0x4800u;
+    }
     // keys of the tile from `lim` on: their value scales may be anything, NaN included, and become zero
     __device__ __forceinline__ void mask(int lane, int lim) {
         if ((lane >> 2) >= lim) k0.z = k0.w = 0;
@@ -202,6 +206,51 @@ __device__ __forceinline__ void kv4_tile_values(uint32_t vaddr, const Kv4Scales&
             kv4_widen(x[2 * h + 1], hi);
             mma_16816_c(O[2 * g], lo[0], lo[1], hi[0], hi[1], b0, b1, O[2 * g]);
             mma_16816_c(O[2 * g + 1], lo[2], lo[3], hi[2], hi[3], b0, b1, O[2 * g + 1]);
+        }
+    }
+}
+
+// The same where a weight times a scale may leave fp16 (Kv4Scales::wide): the product in fp32, as the sum of two bf16 numbers (2^-17), so
+// that groups of any size keep their bits beside one another; two products a tile, codes widened to bf16.
+__device__ __forceinline__ void mma_16816_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// four codes of a word's low nibbles (of the bytes 0 and 2) -> bf16 pairs: 128 + code + 8 under the exponent of 128, minus 136
+__device__ __forceinline__ uint32_t kv4_low_bf16(uint32_t w) {
+    const uint32_t x = (w & KV4_LO_MASK) ^ 0x43084308u, off = 0x43084308u;
+    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&off));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 r = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ void kv4_tile_values_wide(uint32_t vaddr, const Kv4Scales& sc, const float (&w)[4], float (&O)[8][4]) {
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        uint32_t x[4];
+        ldmatrix4_trans(x, vaddr ^ (j * 32));
+        const float2 s0 = __half22float2(*reinterpret_cast<const __half2*>(j ? &sc.k0.w : &sc.k0.z));
+        const float2 s1 = __half22float2(*reinterpret_cast<const __half2*>(j ? &sc.k1.w : &sc.k1.z));
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int g = 2 * j + h;
+            float b[4] = {w[0] * (h ? s0.y : s0.x), w[1] * (h ? s0.y : s0.x), w[2] * (h ? s1.y : s1.x), w[3] * (h ? s1.y : s1.x)};
+#pragma unroll
+            for (int part = 0; part < 2; part++) {
+                uint32_t b0 = pack_bf16(b[0], b[1]), b1 = pack_bf16(b[2], b[3]);
+                b[0] -= __uint_as_float(b0 << 16);
+                b[1] -= __uint_as_float(b0 & 0xffff0000u);
+                b[2] -= __uint_as_float(b1 << 16);
+                b[3] -= __uint_as_float(b1 & 0xffff0000u);
+                b0 = movmatrix4_trans(b0);
+                b1 = movmatrix4_trans(b1);
+                const uint32_t lo = x[2 * h], hi = x[2 * h + 1];
+                mma_16816_bf16(O[2 * g], kv4_low_bf16(lo), kv4_low_bf16(lo >> 4), kv4_low_bf16(hi), kv4_low_bf16(hi >> 4), b0, b1);
+                mma_16816_bf16(O[2 * g + 1], kv4_low_bf16(lo >> 8), kv4_low_bf16(lo >> 12), kv4_low_bf16(hi >> 8), kv4_low_bf16(hi >> 12), b0, b1);
+            }
         }
     }
 }

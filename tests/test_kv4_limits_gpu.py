@@ -178,3 +178,77 @@ def test_prefill_small_rows(dtype, Hq, Hkv, pos0, T):
     late = np.arange(T) > T // 2
     rms = np.sqrt(((got - want)[:, late] ** 2).mean() / (want[:, late] ** 2).mean())
     assert rms < (2.0 ** -9 if dtype == "f16" else 2.0 ** -8), rms
+
+
+# ---- value groups of different sizes, in the decodes -------------------------------------------------------------
+def _group_pages(rng, pool, table, b, lens, Hkv, layer, vf):
+    """Pages of sequence b: keys ~ N(0, 1), values ~ N(0, 1) x vf [4] by group; returns their values."""
+    import torch
+    npg = (lens[b] + 127) // 128
+    pages = np.zeros((Hkv, npg, kv4.PAGE), np.uint8)
+    out = []
+    for side, f in ((0, np.ones(4)), (1, np.asarray(vf, float))):
+        x = (rng.standard_normal((Hkv, npg * 128, 4, 32)) * f[:, None]).astype(np.float16).astype(np.float64).reshape(Hkv, npg * 128, 128)
+        c, s = kv4.quantise(x)
+        out.append(kv4.values(c, s)[:, :lens[b]])
+        pages[..., side * kv4.SIDE:(side + 1) * kv4.SIDE] = kv4.pack(c).reshape(Hkv, npg, kv4.SIDE)
+        sc = pages[..., 2 * kv4.SIDE:].reshape(Hkv, npg, 128, 16)
+        sc[..., 8 * side:8 * side + 8] = s.view(np.uint8).reshape(Hkv, npg, 128, 8)
+        pages[..., 2 * kv4.SIDE:] = sc.reshape(Hkv, npg, 2048)
+    pool.raw()[table[b, :npg].long(), layer] = torch.from_numpy(pages.transpose(1, 0, 2)).cuda()
+    return out
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("vf", [[100.0, 1e-3, 1.0, 1e-2], [12000.0, 1e-3, 1e-3, 1e-2], [5.0, 1e-3, 15.0, 1e-2]])
+@pytest.mark.parametrize("Hq,Hkv,lens", [(8, 2, [1000, 37]), (16, 2, [9000] * 3 + [300] * 8)])
+def test_decodes_keep_small_groups_beside_large_ones(dtype, vf, Hq, Hkv, lens):
+    """A group of values far above the others changes nothing for them: full decode (as a cluster and in runs, with key scores and without) and
+    sparse decode."""
+    import torch
+    from embla_metal_b200 import attn
+    rng = np.random.default_rng(len(lens))
+    B, G, width = len(lens), Hq // Hkv, (max(lens) + 127) // 128
+    ctx = attn.Attention(Hq, Hkv, DT[dtype], B, width * 128)
+    pool = attn.KVPool(1, Hkv, B * width, attn.KV_INT4)
+    table = torch.from_numpy(rng.permutation(B * width).reshape(B, width).astype(np.int32)).cuda()
+    kv = [_group_pages(rng, pool, table, b, lens, Hkv, 0, vf) for b in range(B)]
+    qt, qv, _ = _queries(rng, B, Hq, dtype, 0)
+    ln = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    o = torch.zeros(B, Hq * 128, dtype=ctx.torch_dtype, device="cuda")
+    sc = torch.zeros(B, Hkv, width * 128, device="cuda")
+    idx = np.zeros((B, Hkv, 1152), np.int32)
+    for b in range(B):
+        if lens[b] > 1152:
+            for h in range(Hkv):
+                idx[b, h, :1024] = np.sort(rng.permutation(lens[b] - 128)[:1024])
+            idx[b, :, 1024:] = np.arange(lens[b] - 128, lens[b])
+
+    def check(what, form):
+        ctx.check()
+        got = _out(o, dtype).reshape(B, Hq, 128)
+        rms = []
+        for b in range(B):
+            for h in range(Hkv):
+                k, v = (x[h] for x in kv[b])
+                if form == "sparse" and lens[b] > 1152:
+                    k, v = k[idx[b, h]], v[idx[b, h]]
+                qb = qv[b, h * G:(h + 1) * G]
+                if form == "sparse":
+                    want, bound = kv4.softmax(qb, k, v, kv4.U16[dtype])
+                else:
+                    want, bound = kv4.relu2(qb, k, v, np.ones((G, len(k)), bool), kv4.U16[dtype])
+                _within(got[b, h * G:(h + 1) * G], want, bound, f"{what}, sequence {b}, kv head {h}")
+                d = (got[b, h * G:(h + 1) * G] - want).reshape(G, 4, 32)
+                rms.append(np.sqrt((d ** 2).sum((0, 2)) / (want.reshape(G, 4, 32) ** 2).sum((0, 2))))
+        # each group as a whole: a weight's and an output's rounding (2^-11 each; bf16 2^-8; fp16 outputs of 1e-4 are subnormal: 2^-25)
+        worst = np.max(rms, 0)
+        limit = np.array([2.0 ** -10 if f > 5e-3 else 2.0 ** -8 for f in vf]) if dtype == "f16" else 2.0 ** -8
+        assert (worst < limit).all(), (what, worst)
+
+    ctx.full_decode(pool, table, ln, 0, qt, o)
+    check("full decode", "full")
+    ctx.full_decode(pool, table, ln, 0, qt, o, scores=sc)
+    check("full decode with scores", "full")
+    ctx.sparse_decode(pool, table, ln, 0, qt, o, idx=torch.from_numpy(idx).cuda())
+    check("sparse decode", "sparse")
