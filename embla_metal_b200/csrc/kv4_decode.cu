@@ -322,6 +322,10 @@ __global__ void __launch_bounds__((NCONS + 1 + KD_HELPERS) * 32, 1)
                     } else {
                         atomicExch(p.ctl.err, ERR_BAD_BLOCK);
                         limits[st] = 0;
+                        if (SCORES) {   // (its scores are zeros, not an earlier call's)
+                            float* row = p.scores + size_t(walk.at.b * p.n_kv_heads + walk.at.kvh) * p.scores_stride + long(page) * BLK;
+                            for (int key = min(BLK, S - page * BLK) - 1; key >= 0; key--) row[key] = 0.0f;
+                        }
                         mbar_arrive(&full[st]);
                     }
                 }

@@ -211,7 +211,9 @@ __device__ __forceinline__ void kv4_tile_values(uint32_t vaddr, const Kv4Scales&
 }
 
 // The same where a weight times a scale may leave fp16 (Kv4Scales::wide): the product in fp32, as the sum of two bf16 numbers (2^-17), so
-// that groups of any size keep their bits beside one another; two products a tile, codes widened to bf16.
+// that groups of any size keep their bits beside one another; two products a tile, codes widened to bf16 (64 x 32768 keys with every value
+// scale above 8: 318 us, without 228 in fp16 and 216 in bf16; a warp that kept its weights below 1/2 instead left groups of 0.01
+// beside one of 100 a few bits).
 __device__ __forceinline__ void mma_16816_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])

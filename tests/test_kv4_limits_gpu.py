@@ -252,3 +252,30 @@ def test_decodes_keep_small_groups_beside_large_ones(dtype, vf, Hq, Hkv, lens):
     check("full decode with scores", "full")
     ctx.sparse_decode(pool, table, ln, 0, qt, o, idx=torch.from_numpy(idx).cuda())
     check("sparse decode", "sparse")
+
+
+# ---- pages that are not there ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("bad", [-1, 10 ** 6])
+@pytest.mark.parametrize("lens,page", [([400], 1), ([400], 3), ([9000] * 6 + [300] * 9, 2), ([9000] * 6 + [300] * 9, 70)])
+def test_scores_of_a_bad_block_are_zeros(bad, lens, page):
+    """The call is reported, and leaves no score of an earlier one behind: those of the positions in the bad block are 0, all others right."""
+    import torch
+    from embla_metal_b200 import attn
+    rng, ctx, pool, table, k, v = _setup("bf16", 8, 2, lens, 19)
+    qt, qv, _ = _queries(rng, len(lens), 8, "bf16", 0)
+    table[0, page] = bad
+    o = torch.zeros(len(lens), 1024, dtype=torch.bfloat16, device="cuda")
+    sc = torch.full((len(lens), 2, table.shape[1] * 128 + 5), -7.0, device="cuda")
+    ctx.full_decode(pool, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), 1, qt, o, scores=sc)
+    with pytest.raises(attn.EmblaError) as e:
+        ctx.check()
+    assert e.value.status == attn.BAD_ARG
+    for b, n in enumerate(lens):
+        for h in range(2):
+            row = sc[b, h].cpu().numpy().astype(np.float64)
+            qb = qv[b, 4 * h:4 * h + 4]
+            want, err = (qb @ k[b][h].T).max(0), kv4.DOT * (np.abs(qb) @ np.abs(k[b][h]).T).max(0)
+            if b == 0:
+                want[128 * page:128 * page + 128] = err[128 * page:128 * page + 128] = 0.0
+            assert (row[n:] == -7.0).all()
+            _within(row[:n], want, err, f"scores of sequence {b}, kv head {h}")
