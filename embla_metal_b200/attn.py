@@ -277,7 +277,7 @@ class Attention:
     def kv_append(self, pool, block_table, layer, pos0, k, v, norm_k=True):
         """k, v [batch, n_tokens, n_kv_heads * 128 (or wider rows)]; pos0 int32 [batch] first position."""
         strides = k.stride()
-        _check(lib().embla_kv_append(self.handle, pool.handle, self._pack_view(block_table, None, layer), pos0.data_ptr(), k.size(1),
+        _check(lib().embla_kv_append(self.handle, pool.handle, self._pack_view(block_table, None, layer), _addr(pos0), k.size(1),
                                      k.data_ptr(), v.data_ptr(), strides[1], strides[0], int(norm_k), _raw_stream()))
 
     def kv_read(self, pool, block_table, layer, pos0, k, v):
@@ -377,7 +377,7 @@ def full_prefill(ctx, pool, block_table, layer, pos0, q, o, gains=None, qk8=Fals
         _check(lib().embla_attn_reserve_prefill(ctx.handle, _stream()))
         ctx._prefill_reserved = True
     fn = lib().embla_attn_full_prefill_qk8 if qk8 else lib().embla_attn_full_prefill
-    _check(fn(ctx.handle, pool.handle, ctx._pack_view(block_table, None, layer), pos0.data_ptr(), q.shape[1], ctx._pack_query(q, gains),
+    _check(fn(ctx.handle, pool.handle, ctx._pack_view(block_table, None, layer), _addr(pos0), q.shape[1], ctx._pack_query(q, gains),
               q.stride(1), o.data_ptr(), o.stride(1), o.stride(0), _raw_stream()))
 
 
