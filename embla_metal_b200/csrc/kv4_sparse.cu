@@ -174,8 +174,9 @@ __global__ void __launch_bounds__(KS_WARPS * 32, 4) kv4_sparse_kernel(const __gr
                 const bool k0 = (ok >> (16 * k + r)) & 1, k1 = (ok >> (16 * k + r + 8)) & 1;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    // (a NaN score stays one)
-                    w[k][e] = (e < 2 ? k0 : k1) ? ks_exp2(fmaf(s[k][e], (e & 1) ? u1 : u0, -((e & 1) ? m1 : m0))) : 0.0f;
+                    // (a NaN score stays one; the product is rounded before the reference is taken off, as the reference was when it was taken: what a
+                    // fused operation would keep of a score of 2^31 is more than exp2 can take)
+                    w[k][e] = (e < 2 ? k0 : k1) ? ks_exp2(__fsub_rn(__fmul_rn(s[k][e], (e & 1) ? u1 : u0), (e & 1) ? m1 : m0)) : 0.0f;
                     top = fmaxf(top, w[k][e]);
                 }
             }
@@ -190,15 +191,15 @@ __global__ void __launch_bounds__(KS_WARPS * 32, 4) kv4_sparse_kernel(const __gr
 #pragma unroll
             for (int k = 0; k < 2; k++) {
                 const bool k0 = (ok >> (16 * k + r)) & 1, k1 = (ok >> (16 * k + r + 8)) & 1;
-                if (k0) t0 = fmaxf(t0, s[k][0] * u0), t1 = fmaxf(t1, s[k][1] * u1);
-                if (k1) t0 = fmaxf(t0, s[k][2] * u0), t1 = fmaxf(t1, s[k][3] * u1);
+                if (k0) t0 = fmaxf(t0, __fmul_rn(s[k][0], u0)), t1 = fmaxf(t1, __fmul_rn(s[k][1], u1));
+                if (k1) t0 = fmaxf(t0, __fmul_rn(s[k][2], u0)), t1 = fmaxf(t1, __fmul_rn(s[k][3], u1));
             }
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) {
                 t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
                 t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
             }
-            const float n0 = fmaxf(m0, t0 - KS_TARGET), n1 = fmaxf(m1, t1 - KS_TARGET);
+            const float n0 = fmaxf(m0, __fsub_ru(t0, KS_TARGET)), n1 = fmaxf(m1, __fsub_ru(t1, KS_TARGET));   // (no lower, whatever the scores' size)
             const float c0 = ks_exp2(m0 - n0), c1 = ks_exp2(m1 - n1);
             m0 = n0;
             m1 = n1;

@@ -279,3 +279,47 @@ def test_scores_of_a_bad_block_are_zeros(bad, lens, page):
                 want[128 * page:128 * page + 128] = err[128 * page:128 * page + 128] = 0.0
             assert (row[n:] == -7.0).all()
             _within(row[:n], want, err, f"scores of sequence {b}, kv head {h}")
+
+
+# ---- queries of any size -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("size", [1e4, 1e7, 1e8, 1e10, 1e25])
+def test_sparse_decode_of_large_queries(size):
+    """Softmax over scores that far apart: the value of the largest."""
+    import torch
+    lens = [900, 64]
+    rng, ctx, pool, table, k, v = _setup("bf16", 4, 2, lens, 3)
+    q, qv, _ = _queries(rng, 2, 4, "bf16", 0, factor=size)
+    o = torch.zeros(2, 512, dtype=torch.bfloat16, device="cuda")
+    ctx.sparse_decode(pool, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), 1, q, o)
+    ctx.check()
+    got = _out(o, "bf16").reshape(2, 4, 128)
+    for b in range(2):
+        for h in range(4):
+            best = np.argmax(k[b][h // 2] @ qv[b, h])
+            want = v[b][h // 2][best]
+            # the weight and its product with the scale in fp16, the sum of weights, the output
+            _within(got[b, h], want, np.abs(want) * (3 * 2.0 ** -11 + 2.0 ** -8), f"sequence {b}, head {h}")
+
+
+@pytest.mark.parametrize("scores", [False, True])
+@pytest.mark.parametrize("size", [1e4, 1e10, 1e15])
+@pytest.mark.parametrize("lens", [[900, 64], [9000] * 5])
+def test_full_decode_of_large_queries(size, lens, scores):
+    """Weights up to 1e31: the same bounds as for small ones."""
+    import torch
+    rng, ctx, pool, table, k, v = _setup("bf16", 4, 2, lens, 3)
+    B = len(lens)
+    q, qv, _ = _queries(rng, B, 4, "bf16", 0, factor=size)
+    o = torch.zeros(B, 512, dtype=torch.bfloat16, device="cuda")
+    sc = torch.zeros(B, 2, table.shape[1] * 128, device="cuda") if scores else None
+    ctx.full_decode(pool, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), 1, q, o, scores=sc)
+    ctx.check()
+    got = _out(o, "bf16").reshape(B, 2, 2, 128)
+    for b in range(B):
+        for h in range(2):
+            qb = qv[b].reshape(2, 2, 128)[h]
+            want, bound = kv4.relu2(qb, k[b][h], v[b][h], np.ones((2, lens[b]), bool), kv4.U16["bf16"])
+            _within(got[b, h], want, bound, f"sequence {b}, kv head {h}")
+            if scores:
+                _within(sc[b, h, :lens[b]].cpu().numpy().astype(np.float64), (qb @ k[b][h].T).max(0), kv4.DOT * (np.abs(qb) @ np.abs(k[b][h]).T).max(0),
+                        f"scores of sequence {b}, kv head {h}")
