@@ -143,9 +143,10 @@ __global__ void __launch_bounds__(KS_WARPS * 32, 4) kv4_sparse_kernel(const __gr
     const int r = lane >> 2, t = lane & 3;
     Kv4Frag frag;
     frag.load(sq, lane);
-    // scores in units of log2(e) / sqrt(128) x the query's power of two x 2^20
-    const float u0 = pow2_biased(max(sq.expo[2 * t], 1)) * (1.4426950408889634f * 0.08838834764831845f / KV4_SUBNORMAL);
-    const float u1 = pow2_biased(max(sq.expo[2 * t + 1], 1)) * (1.4426950408889634f * 0.08838834764831845f / KV4_SUBNORMAL);
+    // scores in units of log2(e) / sqrt(128) x the query's power of two x 2^20. (Queries above 2^60 as if they were that large: the scores stay
+    // inside fp32, and any two of them that differ already leave the smaller one no weight.)
+    const float u0 = pow2_biased(min(max(sq.expo[2 * t], 1), 187)) * (1.4426950408889634f * 0.08838834764831845f / KV4_SUBNORMAL);
+    const float u1 = pow2_biased(min(max(sq.expo[2 * t + 1], 1), 187)) * (1.4426950408889634f * 0.08838834764831845f / KV4_SUBNORMAL);
     float O[8][4];
 #pragma unroll
     for (int i = 0; i < 8; i++) O[i][0] = O[i][1] = O[i][2] = O[i][3] = 0.0f;

@@ -282,7 +282,7 @@ def test_scores_of_a_bad_block_are_zeros(bad, lens, page):
 
 
 # ---- queries of any size -----------------------------------------------------------------------------------------
-@pytest.mark.parametrize("size", [1e4, 1e7, 1e8, 1e10, 1e25])
+@pytest.mark.parametrize("size", [1e4, 1e7, 1e8, 1e10, 1e25, 1e33, 1e37])
 def test_sparse_decode_of_large_queries(size):
     """Softmax over scores that far apart: the value of the largest."""
     import torch
