@@ -9,7 +9,9 @@
 //                 operations and no more: a nibble stays where it is, its sign bit flipped, as the fp16 subnormal
 //                 (code + 8) 2^-24 (low nibble of a byte) or (code + 8) 2^-20 (high nibble), exact in the product; the queries
 //                 of the low nibbles' dims carry the missing 2^4. The constant part, 8 x the sum of the query over the group,
-//                 is the accumulator's start value, negated.
+//                 is the accumulator's start value, negated. What that costs, against 64 bits: 2^-20.8 of sum |q| |k| for rows of
+//                 even size (bf16 queries 2^-24), at most 2^-18.5 of max |q| sum |k| for any (queries that span 2^24, keys of
+//                 one code a group): the offset's terms are up to 15 max |q| in size, whatever the key.
 //   O^T = V^T P^T A = 16 dims x 16 keys. The transposing ldmatrix, on 16-bit elements of four codes, hands lane (r, t) the
 //                 element r of keys 2t and 2t + 1 side by side: widened, its nibbles are A registers (a dim, two keys). The
 //                 value's scale of the group is multiplied into P (a B register a group), the codes stay exact. (As subnormals
@@ -55,8 +57,8 @@ __device__ __forceinline__ void mma_16816_c(float (&d)[4], uint32_t a0, uint32_t
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
-// The queries of a kv head in shared memory: rows scaled by a power of two that brings their largest element into [1, 2) (exact;
-// fp16 then holds bf16 queries of any size), and what goes with them.
+// The queries of a kv head in shared memory: rows scaled by a power of two that brings their largest element into [1, 2), so that fp16
+// holds bf16 rows of any size, elements below 2^-14 of the largest to 2^-25 of it; and what goes with them.
 struct Kv4Queries {
     __half q[8][HD];
     int expo[8];                  // biased exponent of the power of two; 0: no such head

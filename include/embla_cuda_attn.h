@@ -229,8 +229,9 @@ EmblaStatus embla_oproj(EmblaAttn* ctx, const EmblaW4Matrix* wo, int32_t d_in, c
  * A 16-bit pool is served too: the reference's build without the int8 cache (EMBLA_KV8=0, Engine.swift:163: attn_full,
  * attention.metal:148-220), the rows in the activation dtype and no scales; the scores then come from a scoring pass of
  * their own ahead of the attention (queries prenormed), and embla_attn_full_step is refused (embla_kv_append first).
- * Over a 4-bit pool the scores come from the same tensor-core products as the attention (fp32 sums, within a few fp32
- * roundings of exact, the same from run to run), for prenormed queries or not. A sequence of 0 keys gives zeros. */
+ * Over a 4-bit pool the scores come from the same tensor-core products as the attention, for prenormed queries or not, the
+ * same from run to run and off by at most 2^-16 of max |q| x sum |k| (queries are rounded to fp16 under a power of two that
+ * brings their largest element into [1, 2); queries above 2^108 give infinite scores). A sequence of 0 keys gives zeros. */
 EmblaStatus embla_attn_full_decode(EmblaAttn* ctx, const EmblaKVPool* pool, const EmblaKVView* view,
                                    const EmblaQuery* q, void* o_dev, int64_t o_stride,
                                    float* scores_dev, int64_t scores_stride, void* stream);

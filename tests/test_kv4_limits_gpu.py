@@ -301,6 +301,44 @@ def test_sparse_decode_of_large_queries(size):
             _within(got[b, h], want, np.abs(want) * (3 * 2.0 ** -11 + 2.0 ** -8), f"sequence {b}, head {h}")
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("kind", ["even", "one 2^8", "one 2^16", "wide", "sparse"])
+def test_scores_of_uneven_rows(dtype, kind):
+    """Key scores where one query element is far above the rest, where they span 2^24, and for keys of one code a group: off by at most 2^-16 of
+    max |q| x sum |k|. A group's products are fp32 sums of 32 terms and a start value, of either sign and up to 15 max |q| s in size, where the
+    pipe may truncate: 34 steps of 2^-24 of a partial sum that is 15 sqrt(32) max |q| s at most as a rule, at random 2^-15.1 max |q| s, and sum
+    |k| of the group is 7 s or more: 2^-17.9. A query element is off by 2^-25 max |q|."""
+    import torch
+    from embla_metal_b200 import attn
+    n = 4096
+    for seed in range(2):
+        rng = np.random.default_rng(seed)
+        ctx = attn.Attention(2, 2, DT[dtype], 1, n)
+        pool = attn.KVPool(1, 2, n // 128, attn.KV_INT4)
+        pages = kv4.make_pages(rng, (n // 128, 1, 2))
+        if kind == "sparse":
+            codes = np.zeros((n // 128, 1, 2, 128, 4, 32), np.int8)
+            np.put_along_axis(codes, rng.integers(0, 32, codes.shape[:-1])[..., None], 7, -1)
+            pages[..., :8192] = kv4.pack(codes.reshape(*codes.shape[:-2], 128)).reshape(n // 128, 1, 2, 8192)
+        pool.raw().copy_(torch.from_numpy(pages))
+        x = rng.standard_normal((1, 2, 128))
+        if kind in ("wide", "sparse"):
+            x *= np.exp2(rng.uniform(-24, 0, x.shape))
+        if kind.startswith("one"):
+            x *= 2.0 ** -3
+            x[:, :, 5] *= 2.0 ** float(kind[6:])
+        bits = _bits(x, dtype)
+        q = _val(bits, dtype)[0]
+        o = torch.zeros(1, 256, dtype=ctx.torch_dtype, device="cuda")
+        sc = torch.zeros(1, 2, n, device="cuda")
+        ctx.full_decode(pool, torch.arange(n // 128, dtype=torch.int32, device="cuda")[None], torch.tensor([n], dtype=torch.int32, device="cuda"), 0,
+                        _act(bits, dtype).view(1, -1), o, scores=sc)
+        ctx.check()
+        k = kv4.page_values(pages[:, 0].transpose(1, 0, 2))[0].reshape(2, n, 128)
+        bound = 2.0 ** -16 * np.abs(q).max(-1)[:, None] * np.abs(k).sum(-1)
+        _within(sc[0].cpu().numpy().astype(np.float64), np.einsum("hd,hnd->hn", q, k), bound + 1e-30, kind)
+
+
 @pytest.mark.parametrize("scores", [False, True])
 @pytest.mark.parametrize("size", [1e4, 1e10, 1e15])
 @pytest.mark.parametrize("lens", [[900, 64], [9000] * 5])
