@@ -192,3 +192,67 @@ def test_a_chunk_from_the_last_row_of_a_shared_block(monkeypatch):
     _chunk(st, monkeypatch, [255, 255], 3, mark=5, max_seq_len=258)
     assert _rows(st, 0, 258) == list(range(255)) + [260, 261, 262]
     assert _rows(st, 1, 258) == list(range(255)) + [1260, 1261, 1262]
+
+
+@pytest.mark.parametrize("seed", range(60))
+def test_random_forks_chunks_and_steps(seed, monkeypatch):
+    """Any order of calls: what each sequence's table holds is what that sequence wrote, or has from where it was forked; a call that is refused
+    changes nothing."""
+    import random
+    rng = random.Random(seed)
+    B, cap = 4, PAGES * 128
+    st = _stack(B)
+    st.set_positions(0)
+    rows = [[] for _ in range(B)]                          # what sequence b has written: its positions 0 .. len - 1
+    near = lambda n: min(cap - 3, max(0, rng.choice([n, n, n, n - 1, n // 128 * 128 - 1, n // 128 * 128, rng.randint(0, n)])))
+    done = 0
+    for turn in range(150):
+        kind = rng.choice(["step", "step", "chunk", "fork", "fork", "restart"])
+        if kind == "step":
+            at = [near(len(r)) for r in rows]
+            if rng.random() < 0.7:
+                try:
+                    st.set_positions(at)
+                except ValueError:
+                    assert any(st._shared(b) for b in range(B))
+                    continue
+            at = st.pos.tolist()
+            if any(p > len(r) for p, r in zip(at, rows)):
+                continue                                   # (positions behind what is there: not after a refusal)
+            marks = [10 ** 6 * turn + b for b in range(B)]
+            _step(st, marks)
+            for b, p in enumerate(at):
+                rows[b][p:] = [marks[b]]
+        elif kind == "chunk":
+            T = rng.choice([1, 2, 100, 128, 129])
+            at = [min(near(len(r)), cap - T) for r in rows]
+            try:
+                _chunk(st, monkeypatch, at, T, mark=10 ** 6 * turn, max_seq_len=max(at) + T)
+            except ValueError:
+                assert any(st._shared(b) for b in range(B))
+                continue
+            for b, p in enumerate(at):
+                rows[b][p:] = [1000 * b + t + 10 ** 6 * turn for t in range(p, p + T)]
+        elif kind == "fork":
+            src, dst = rng.sample(range(B), 2)
+            n = int(st.seq_lens[src])
+            if n > len(rows[src]) + 1:
+                continue
+            try:
+                st.fork(src, dst)
+            except ValueError:
+                assert st._lent_to(dst)
+                continue
+            rows[dst] = rows[src][:n]
+        else:
+            b = rng.randrange(B)
+            try:
+                st.restart(b)
+            except ValueError:
+                assert st._lent_to(b)
+                continue
+            rows[b] = []
+        done += 1
+        for b in range(B):
+            assert _rows(st, b, len(rows[b])) == rows[b], (turn, kind, b)
+    assert done > 40
