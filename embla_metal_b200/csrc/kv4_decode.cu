@@ -4,9 +4,10 @@
 // Bound by HBM: a key and its value are 144 bytes, used once. As in the int8 kernel (full_decode.cu) a CTA streams a range of a
 // sequence's pages through a ring of shared-memory stages filled by TMA and a key's dots and sums run on warp tensor-core
 // tiles (kv4_tile.cuh); per byte there are nearly twice as many codes to widen, so what counts is instructions a key:
-// 17.7 for fp16 outputs, 16.3 for bf16, of the 25 issue slots that an SM has per key at full bandwidth, 7.5 of them on the ALU
-// pipe, which has 12. 64 sequences of 32768 keys, 4 kv heads: 224 us (fp16, 5.4 TB/s, 0.82 of the measured copy rate) and
-// 215 us (bf16); 16 uneven sequences of up to 9001 keys: 26 us; one of 1000: 5.6 us. What is left of it: half of the issue slots
+// about 17.8 for fp16 outputs, 16.4 for bf16, of the 25 issue slots that an SM has per key at full bandwidth, 7.5 of them on the ALU
+// pipe, which has 12. 64 sequences of 32768 keys, 4 kv heads: 224 to 260 us (fp16, 4.6 to 5.4 TB/s, 0.71 to 0.82 of the measured copy rate;
+// it differs from GPU to GPU and with the values that the cache holds) and 9 to 12 us less in bf16; 16 uneven sequences of up to 9001 keys: 26 to 28 us;
+// one of 1000: 6.6 us. What is left of it: half of the issue slots
 // are used, twelve warps being what 128 registers a thread leave room for; a launch's first 4 microseconds (lengths, block
 // table, first pages one after another) and its last 3 (the pieces' sums, written on one SM and read on another). Adding the
 // pieces up in the CTA that ends last, counted by atomics, took 0.7 to 2 microseconds longer than a second launch that is there
@@ -52,7 +53,8 @@ constexpr int KD_SUM = HD + 1;   // a row of a warp's sums in shared memory: lan
 constexpr float KD_LIMIT = 8192.0f;                                // largest weight kept
 constexpr int KD_TARGET = 10;                                      // log2 of the bound a new f puts on the tile's weights
 constexpr int KD_MAX_CLUSTER = 8;
-// What a unit costs beside its pages, in pages (16 uneven sequences of up to 9001 keys: 29.0 us counting 4, 31.7 counting 2, 39 none).
+// What a unit costs beside its pages, in pages (16 uneven sequences of up to 9001 keys, where 4 take 26 to 28 us: 2.7 us more counting 2, 10 more
+// counting none).
 constexpr int KD_UNIT_COST = 4;
 constexpr int KD_MIN_RUN = 4;   // cost of a run at least
 
@@ -229,8 +231,8 @@ template <int DT, bool SCORES, int NCONS, int WPG, int STAGES, bool CL>
 __global__ void __launch_bounds__((NCONS + 1 + KD_HELPERS) * 32, 1)
     kv4_decode_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ Kv4DecodeParams p) {
     constexpr int TILES = 8 / WPG;          // 16-key tiles of a page a consumer warp takes
-    // of those, taken together: all (one by one 64 x 32768 keys take 239 us instead of 224), but one by one where scores are written
-    // too, which leaves no registers for two (8 x 32768 keys: 28.8 us instead of 29.8)
+    // of those, taken together: all (one by one 64 x 32768 keys take 7 % longer), but one by one where scores are written
+    // too, which leaves no registers for two (8 x 32768 keys, where one by one takes 28.8 to 30.8 us: 1 us more)
     constexpr int STEP = SCORES ? 1 : TILES;
     constexpr int GROUPS = NCONS / WPG;
     constexpr int PRODUCER = NCONS;         // warp roles: consumers, then the producer, then the helpers
@@ -437,7 +439,8 @@ __global__ void __launch_bounds__((NCONS + 1 + KD_HELPERS) * 32, 1)
     } else {
         // ---- consumers
         if (!CL) {
-            // the block tables on their way to the L2 while the producers look for their runs (16 uneven sequences: 19.5 us instead of 19.9)
+            // the block tables on their way to the L2 while the producers look for their runs (16 uneven sequences of up to 9001 keys, 26 to 28 us:
+            // 0.4 us less)
             const long at = (long(blockIdx.x) * NCONS + warp) * 1024 + lane * 32;   // a line of 32 entries a lane
             if (at <= long(p.batch - 1) * p.table_stride) prefetch_l2(p.block_table + at);
         }
@@ -843,7 +846,7 @@ EmblaStatus kv4_full_decode(EmblaAttn* ctx, const EmblaKVPool* pool, const Embla
     if (units * (pages + KD_UNIT_COST) > 0x7fffffffL || units > 0xffff)
         EMBLA_FAIL(EMBLA_BAD_ARG, "embla_attn_full_decode: %d sequences of up to %d keys are too many pages", view->batch, max_len);
     // Two ways, by what they measured, in hundredths of a microsecond: clusters, all at once, 570 + 62 a page of a range (one
-    // sequence of 1000 keys 5.6 us, of 8192 10.5); runs, 1000 + 50 a page or unit cost of a run (10.0 us at the shortest, 64 sequences
+    // sequence of 1000 keys 5.6 us when it was fitted, 6.6 with kv4_tile_values_wide in the kernel, of 8192 10.5); runs, 1000 + 50 a page or unit cost of a run (10.0 us at the shortest, 64 sequences
     // of 1000 keys 20.0, 8 of 32768 37.8). The ranges of a unit are as many as let all clusters be resident (a GPC may hold one cluster of
     // 8 such CTAs and not two) and no longer than 8 pages: longer ones are read at the pace of the longest sequence, where runs
     // even uneven lengths out. Runs: the scratch holds two pieces of each (embla_attn_create makes it 8 slots an SM and more).

@@ -8,8 +8,8 @@
 // softmax keeps a reference score that moves (the sums with it) only when a weight passes 2^13. Up to eight CTAs a (sequence, kv
 // head), as a thread-block cluster, when there are few of them.
 //
-// 64 sequences of 32768 keys, 4 kv heads: 28.8 us for 42 MB of rows (56 MB read: a row's scales are 16 bytes of the 64 that the HBM
-// gives), 4 sequences of 9000: 9.0 us, of which 6 are launch, lookups and one row's way here. 31 instructions a row, 39 % of the
+// 64 sequences of 32768 keys, 4 kv heads: 27 to 29 us for 42 MB of rows (56 MB read: a row's scales are 16 bytes of the 64 that the HBM
+// gives), 4 sequences of 9000: 9.0 to 10.3 us, of which 6 are launch, lookups and one row's way here. 31 instructions a row, 39 % of the
 // issue slots; the same number of rows side by side instead of scattered take 17.6 us.
 #include "attn16_common.cuh"
 #include "kv4_tile.cuh"

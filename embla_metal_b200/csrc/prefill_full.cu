@@ -120,12 +120,13 @@ __device__ __forceinline__ void convert_side(const uint8_t* raw, uint8_t* dst, i
 // code x scale rounded once (2^-11); queries enter scaled by 2^-5 and the keys without 1 / sqrt(D), whose square, 2^-7, is exact
 // in the weights: P = relu(s)^2 comes out as the weight x 2^-3 (scores up to 724 square inside fp16's range, and fp16's smallest step keeps
 // the weights to 2^-22: with 2^-7 for the queries it was 2895 and 2^-18, and rows whose scores are all about 0.01 came out 1.2 % off), the
-// sink takes the same factor. 2048 tokens at 30720: 431 us, 1236 TFLOP/s (0.75 of the measured burst rate; the int8 pages take 449 us).
+// sink takes the same factor. 2048 tokens at 30720: 425 to 490 us, 1090 to 1250 TFLOP/s (0.66 to 0.76 of the measured burst rate; the int8
+// pages take 445 us where these take 440).
 // What does not fit in fp16 so (a score above 724, a scale of 8192 or more, a bf16 query above 2e6) is seen once the range's products are
 // done, and the CTA then takes its pages twice more: with every query row scaled by a power of two that brings its largest element into
 // [1, 2), once for the largest score of each row and once with the scores under the power of two that brings that one into [64, 128).
-// Sums and outputs leave in the usual units, so what the other ranges of a unit did makes no difference. Three times the time, for rows
-// that fp16 would have made infinite; all others pay one barrier.
+// Sums and outputs leave in the usual units, so what the other ranges of a unit did makes no difference. Four times the time (2048 tokens at
+// 30720, all in this form: 1850 us), for rows that fp16 would have made infinite; all others pay one barrier.
 constexpr float PF4_QSCALE = 1.0f / 32.0f, PF4_PSCALE = 1.0f / 8.0f;
 constexpr float PF4_FULL = 65504.0f;   // a row sum below it has no weight that fp16 does not hold
 
