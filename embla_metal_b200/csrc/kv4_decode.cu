@@ -4,7 +4,7 @@
 // Bound by HBM: a key and its value are 144 bytes, used once. As in the int8 kernel (full_decode.cu) a CTA streams a range of a
 // sequence's pages through a ring of shared-memory stages filled by TMA and a key's dots and sums run on warp tensor-core
 // tiles (kv4_tile.cuh); per byte there are nearly twice as many codes to widen, so what counts is instructions a key:
-// about 17.8 for fp16 outputs, 16.4 for bf16, of the 25 issue slots that an SM has per key at full bandwidth, 7.5 of them on the ALU
+// about 17.9 for fp16 outputs, 16.5 for bf16, of the 25 issue slots that an SM has per key at full bandwidth, 7.5 of them on the ALU
 // pipe, which has 12. 64 sequences of 32768 keys, 4 kv heads: 224 to 260 us (fp16, 4.6 to 5.4 TB/s, 0.71 to 0.82 of the measured copy rate;
 // it differs from GPU to GPU and with the values that the cache holds) and 9 to 12 us less in bf16; 16 uneven sequences of up to 9001 keys: 26 to 28 us;
 // one of 1000: 6.6 us. What is left of it: half of the issue slots

@@ -230,6 +230,7 @@ struct PfShared {
     PfSegment sg;           // KV4: for prefill_wide
     volatile int lim[3];    // KV4: keys that count in the page side of each ring slot
     volatile int large;     // KV4: a scale of 8192 or more
+    int odd_query;          // KV4: a query element that is infinite in fp16
     int nan_from[KV4_GROUPS];   // KV4: the first position whose value group is not a number
 };
 constexpr int PF_BARS = 19;
@@ -275,7 +276,7 @@ __device__ __forceinline__ void prefill_pages(const CUtensorMap& tmap, const Pre
         if (!WIDE) {
             sh.abort = 0;
             if (KV4) {
-                sh.large = 0;
+                sh.large = sh.odd_query = 0;
                 for (int i = 0; i < KV4_GROUPS; i++) sh.nan_from[i] = 0x7fffffff;
             }
         }
@@ -315,6 +316,7 @@ __device__ __forceinline__ void prefill_pages(const CUtensorMap& tmap, const Pre
     constexpr int SW = PF_THREADS / 32 - 1;
     const int swarp = warp < PF_PRODUCER ? warp : warp - 1, stid = swarp * 32 + lane;
 
+    uint32_t qtop = 0;   // KV4: largest magnitude (bits) of the staged bf16 queries, halves apart
     // ---- Q tiles: [128 tokens][128 dims] of head h as fp16 in the K-major swizzled layout
     if (WIDE) {
         // one warp a row: head norm if asked, then the row by a power of two
@@ -363,8 +365,10 @@ __device__ __forceinline__ void prefill_pages(const CUtensorMap& tmap, const Pre
                 uint32_t* w = &v[x][k].x;
                 if (DT == EMBLA_BF16) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
+                    for (int e = 0; e < 4; e++) {
                         w[e] = pack_h2(__uint_as_float(w[e] << 16) * QSCALE, __uint_as_float(w[e] & 0xffff0000u) * QSCALE);
+                        if (KV4) qtop = __vmaxu2(qtop, w[e] & 0x7fff7fffu);
+                    }
                 } else {
                     const __half2 qs2 = __float2half2_rn(QSCALE);
 #pragma unroll
@@ -455,8 +459,9 @@ __device__ __forceinline__ void prefill_pages(const CUtensorMap& tmap, const Pre
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const int d = lane + 32 * i, c8 = d >> 3;
-                        *reinterpret_cast<__half*>(Qx + (c8 >> 3) * (BLK * 128) + r * 128 + (((c8 & 7) ^ (r & 7)) << 4) + (d & 7) * 2) =
-                            __float2half_rn(xq[k][i] * QSCALE);
+                        const __half hq = __float2half_rn(xq[k][i] * QSCALE);
+                        if (KV4) qtop = max(qtop, __half_as_ushort(hq) & 0x7fffu);
+                        *reinterpret_cast<__half*>(Qx + (c8 >> 3) * (BLK * 128) + r * 128 + (((c8 & 7) ^ (r & 7)) << 4) + (d & 7) * 2) = hq;
                     }
                 }
             }
@@ -464,7 +469,13 @@ __device__ __forceinline__ void prefill_pages(const CUtensorMap& tmap, const Pre
     }
     fence_proxy_async();      // Q was written by ordinary stores; the tensor pipe reads it through the async proxy
     tc_fence_before();
-    __syncthreads();
+    if (KV4 && DT == EMBLA_BF16 && !WIDE) {
+        // (a query that is infinite in fp16 need not show in its row's sum: scores of minus infinity weigh nothing)
+        __syncwarp();
+        if (__syncthreads_or((qtop & 0xffffu) >= 0x7c00u || (qtop >> 16) >= 0x7c00u)) sh.odd_query = 1;
+    } else {
+        __syncthreads();
+    }
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
     // TMEM columns: S/P of tile 0 at 0, of tile 1 at 128 (P overwrites the first 64 columns of its S); O at 256, 384
@@ -1010,7 +1021,7 @@ __device__ __forceinline__ void full_prefill_segment(const CUtensorMap& tmap, co
         if (threadIdx.x == 0) sh.sg = sg;
         tc_fence_before();
         __syncwarp();
-        wide = __syncthreads_or(again) || sh.large;
+        wide = __syncthreads_or(again) || sh.large || sh.odd_query;
         wide = wide && !*reinterpret_cast<volatile int*>(&sh.abort);
         if (wide) prefill_wide<DT>(tmap, p, sh);
     }

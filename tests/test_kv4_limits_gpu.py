@@ -180,6 +180,48 @@ def test_prefill_small_rows(dtype, Hq, Hkv, pos0, T):
     assert rms < (2.0 ** -9 if dtype == "f16" else 2.0 ** -8), rms
 
 
+@pytest.mark.parametrize("gains", [False, True])
+def test_prefill_one_query_element_past_fp16(gains):
+    """Every key has a negative element where a bf16 query is just too large for fp16: minus infinity there, which weighs nothing, and a positive score
+    in earnest for half of them."""
+    import torch
+    from embla_metal_b200 import attn
+    rng = np.random.default_rng(2)
+    n, T = 300, 40
+    ctx, pool = attn.Attention(2, 1, attn.BF16, 1, 384), attn.KVPool(1, 1, 3, attn.KV_INT4)
+    rows = rng.standard_normal((2, 1, n, 128))
+    rows[0, ..., 0] = -2.0
+    kb = _bits(rows, "bf16")
+    t = _act(kb, "bf16")
+    table = torch.tensor([[2, 0, 1]], dtype=torch.int32, device="cuda")
+    ctx.kv_append(pool, table, 0, torch.zeros(1, dtype=torch.int32, device="cuda"), t[0], t[1], norm_k=False)
+    k, v = (kv4.values(*kv4.quantise(_val(kb[i, 0], "bf16"))) for i in range(2))
+    assert (k[:, 0] < 0).all()
+    x = np.sign(rng.standard_normal((T, 2, 128))) * 1.0e6
+    x[..., 0] = 2.2e6
+    gt = None
+    if gains:                                              # raw queries of size 1 whose gains make those
+        g = [_bits(np.full(128, 1.0e3 - 1), "bf16"), _bits(np.full(128, 1.1e3 - 1), "bf16")]
+        x = np.sign(x) * np.where(np.arange(128) == 0, 1.0, 0.5)
+        gt = tuple(_act(gb, "bf16") for gb in g)
+    qb = _bits(x, "bf16")
+    q = _val(qb, "bf16")
+    if gains:
+        f = kv4.norm_rows32(q)
+        for gb in g:
+            f = f * (np.float32(1) + _val(gb, "bf16").astype(np.float32))
+        q = _val(_bits(q.astype(np.float32) * f, "bf16"), "bf16")
+    assert (q[..., 0] > 2.1e6).all() and (np.abs(q[..., 1:]) < 2.09e6).all()
+    o = torch.zeros(1, T, 256, dtype=torch.bfloat16, device="cuda")
+    attn.full_prefill(ctx, pool, table, 0, torch.tensor([n - T], dtype=torch.int32, device="cuda"), _act(qb, "bf16").view(1, T, 256), o, gains=gt)
+    ctx.check()
+    got = _out(o, "bf16").reshape(T, 2, 128)
+    seen = np.arange(n)[None] <= n - T + np.arange(T)[:, None]
+    for h in range(2):
+        want, bound = kv4.relu2(q[:, h], k, v, seen, kv4.U16["bf16"], wround=4, dot=2.0 ** -11)
+        _within(got[:, h], want, bound, f"head {h}")
+
+
 # ---- value groups of different sizes, in the decodes -------------------------------------------------------------
 def _group_pages(rng, pool, table, b, lens, Hkv, layer, vf):
     """Pages of sequence b: keys ~ N(0, 1), values ~ N(0, 1) x vf [4] by group; returns their values."""
