@@ -257,6 +257,8 @@ class DecodeStack:
             raise ValueError(f"qkv {tuple(qkv.shape)} / o {tuple(o.shape)} do not fit {len(self.kinds)} layers x {self.batch} sequences")
         if qkv.stride(3) != 1 or o.stride(3) != 1:
             raise ValueError("rows must be contiguous")
+        if pos0.device != self.pos.device or pos0.dtype != torch.int32 or pos0.numel() < b:
+            raise ValueError(f"pos0 {tuple(pos0.shape)} {pos0.dtype} on {pos0.device}: int32, a position for each of {b} sequences, where the stack is")
         if self._shares():
             if self.table.is_cuda and torch.cuda.is_current_stream_capturing():
                 raise ValueError("a chunk over sequences that share blocks (fork) reads its positions: not while a graph is captured")

@@ -194,6 +194,18 @@ def test_a_chunk_from_the_last_row_of_a_shared_block(monkeypatch):
     assert _rows(st, 1, 258) == list(range(255)) + [1260, 1261, 1262]
 
 
+@pytest.mark.parametrize("pos0", [torch.zeros(2), torch.zeros(2, dtype=torch.int64), torch.zeros(1, dtype=torch.int32),
+                                  torch.zeros(2, dtype=torch.int32, device="meta")])
+def test_a_chunk_refuses_positions_that_are_not_the_stack_s(pos0, monkeypatch):
+    st = _stack(2)
+    st.kinds = [stk.FULL]
+    called = []
+    monkeypatch.setattr(stk.attn, "lib", lambda: called.append(1))
+    with pytest.raises(ValueError):
+        st.prefill_chunk(torch.zeros(1, 2, 3, 1), torch.zeros(1, 2, 3, 1), pos0)
+    assert not called and st.pos.tolist() == [0, 0]
+
+
 @pytest.mark.parametrize("seed", range(60))
 def test_random_forks_chunks_and_steps(seed, monkeypatch):
     """Any order of calls: what each sequence's table holds is what that sequence wrote, or has from where it was forked; a call that is refused
