@@ -133,7 +133,7 @@ constexpr float PF4_FULL = 65504.0f;   // a row sum below it has no weight that 
 // One side of a raw 4-bit page -> fp16 in the UMMA layout; rows from `lim` on (behind the last key, or all of a page that is
 // nowhere) become zeros, whatever lies there. 128 converter threads; the lanes of a quarter warp take 8 consecutive rows of one
 // group, so reads and writes are conflict-free. A scale whose products may leave fp16 sets *large; values an eighth of their size with
-// `eighth`. A value group that is not a number becomes zeros, with its position left in nan_from[group] if it is the first (`first`: that of
+// `eighth` (scales below 2^-11 may lose three bits there). A value group that is not a number becomes zeros, with its position left in nan_from[group] if it is the first (`first`: that of
 // the page's row 0): a token that does not see it would have zero times it, a NaN, in its sum.
 __device__ __forceinline__ void convert_side4(const uint8_t* raw, uint8_t* dst, int ctid, int side, int lim, bool eighth, volatile int* large,
                                               int* nan_from, int first) {
@@ -734,11 +734,13 @@ __device__ __forceinline__ void prefill_rows(const PrefillParams& p, const PfSeg
             // weights (S g)^2 where the usual ones are (q.k)^2 2^-10; S = q.k 2^-(the row's exponent), 2^-3 with scales an eighth, whose
             // values are an eighth too
             const int e = (-10 + 2 * reinterpret_cast<const int*>(qsc)[x * BLK + r] + (sh.large ? 6 : 0)) - 2 * (int(__float_as_uint(at.kfac[x * BLK + r]) >> 23) - 127);
-            unit_of = pow2_biased(min(max(127 + e, 1), 204));   // (fp32 then holds the sums; the sink is nothing beside weights of 2^90)
+            // (a unit that is whole here: held where fp32 holds the sums, since the sink is nothing beside weights of 2^90; one whose ranges meet: as it is, and
+            // sums of weights times values that fp32 does not hold become infinite, as in the decode)
+            unit_of = pow2_biased(min(max(127 + e, 1), nparts == 1 ? 204 : 254));
             vunit = sh.large ? 8.0f * unit_of : unit_of;
         }
         if (WIDE) rowsum *= unit_of;
-// O of group cc of the row in usual units; NaN from its first value on that is one
+        // O of group cc of the row in usual units; NaN from its first value on that is one
         auto from_acc = [&](uint32_t a, int cc) {
             if (!KV4) return __uint_as_float(a);
             return __uint_as_float(a) * (at.p0 + pick(t0, x) + r >= sh.nan_from[cc] ? __uint_as_float(0x7fffffffu) : vunit);

@@ -377,8 +377,9 @@ EmblaStatus embla_attn_sliding_prefill(EmblaAttn* ctx, const EmblaRing* ring, co
  * h * 128]; out is token-major, o_dev[b * o_seq_stride + t * o_token_stride + h * 128]. Strides are in
  * elements and must be multiples of 8. Runs on tcgen05 tensor cores with fp32 accumulation in TMEM. Int8 and 4-bit
  * pools; over a 4-bit one q_dev and o_dev must be 16-byte aligned. Over a 4-bit pool a cached key or value that is not a
- * number reaches the tokens from its position on, as in the decode, and none ahead of it; rows of any size are served, scores to 2^48, weights (scores squared) kept to 2^-22; where a score passes 724, a scale 8192 or a query 2e6,
- * the 256 tokens of the head take four times as long. (Int8: scores to 2047, weights to 2^-19.) */
+ * number reaches the tokens from its position on, as in the decode, and none ahead of it; rows of any size are served as far as
+ * fp32 holds sums of weights times values (scores to 2^48 and more), weights (scores squared) kept to 2^-22; where a score passes 724,
+ * a scale 8192 or a query 2e6, the 256 tokens of the head take four times as long. (Int8: scores to 2047, weights to 2^-19.) */
 EmblaStatus embla_attn_full_prefill(EmblaAttn* ctx, const EmblaKVPool* pool, const EmblaKVView* view,
                                     const int32_t* pos0_dev, int32_t n_tokens, const EmblaQuery* q,
                                     int64_t q_token_stride, void* o_dev, int64_t o_token_stride,

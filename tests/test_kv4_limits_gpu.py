@@ -137,6 +137,7 @@ SIZES_BF16 = {
     "queries past fp16": dict(qf=lambda t: 1e8),
     "keys and values past fp16": dict(kf=lambda t, S: 1e5, vf=lambda t, S: 1e5),
     "one value past fp16 in the chunk": dict(vf=lambda t, S: np.where(t == S - 2, 1e5, 1.0)),
+    "scores of 1e16": dict(kf=lambda t, S: 1e5, qf=lambda t: 1e11),
     "all of it": dict(kf=lambda t, S: 1e5, vf=lambda t, S: 1e5, qf=lambda t: 1e6),
 }
 
